@@ -347,6 +347,103 @@ int t2fw_gate_backward(const void *d_f, const void *d_f_key, const void *f, cons
                        void *d_f_logit, void *d_fk_logit,
                        int64_t n_f, int64_t n_fk, int32_t dtype, void *stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * The operators around the recurrences in a training or generation step.  No counterpart in the reference, whose caller writes
+ * them in the framework around it.  Arrays are device memory, dense and of one dtype where nothing else is said, aligned to
+ * their element size; "accumulators' type" is double for T2FW_F64, otherwise float.  No result may overlap an input
+ * unless it is said that it may.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/*
+ * Recurrence with a vector for its state: h_t = f_t h_{t-1} + x_t per channel.  x, f, out [B, T, D]; s0, final_state
+ * [B, D] in the accumulators' type (s0 null: zeros).  `lengths` [B] (int32, or int64 with T2FW_SCAN_LENGTHS64), or null: the steps
+ * of row b from lengths[b] on do not count, whatever they hold; their results are zero and the state passes them as it
+ * is.  `strides`: elements between rows and steps of x and f (x_b, x_t, f_b, f_t), or null for dense arrays; the channels of
+ * a step are next to each other.  T2FW_SCAN_LOGITS: f holds gate logits, the gate is their sigmoid.
+ * `ckpt`: t2fw_gated_scan_checkpoint_bytes for the backward call, or null.
+ */
+#define T2FW_SCAN_LOGITS 1
+#define T2FW_SCAN_LENGTHS64 2
+size_t t2fw_gated_scan_checkpoint_bytes(int64_t B, int64_t T, int64_t D, int32_t dtype);
+size_t t2fw_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, int32_t dtype);
+int t2fw_gated_scan_forward(const void *x, const void *f, const void *s0, const void *lengths,
+                            void *out, void *final_state, void *ckpt,
+                            int64_t B, int64_t T, int64_t D, const int64_t *strides,
+                            int32_t dtype, int32_t flags,
+                            void *workspace, size_t workspace_bytes, void *stream);
+/*
+ * Gradients: d_x_t = G_t, d_f_t = G_t h_{t-1} (of the logits with T2FW_SCAN_LOGITS), d_s0, with G_t = g_out_t + f_{t+1} G_{t+1}
+ * from G_T = g_state (null: zeros).  strides: as above, then g_out's two.  d_s0 may be null.
+ */
+int t2fw_gated_scan_backward(const void *g_out, const void *g_state, const void *x, const void *f,
+                             const void *lengths, const void *ckpt,
+                             void *d_x, void *d_f, void *d_s0,
+                             int64_t B, int64_t T, int64_t D, const int64_t *strides,
+                             int32_t dtype, int32_t flags,
+                             void *workspace, size_t workspace_bytes, void *stream);
+/* One step: x, f, out [B, D]; next_state == s0 (in place) is allowed. */
+int t2fw_gated_scan_step(const void *x, const void *f, const void *s0, void *out, void *next_state,
+                         int64_t B, int64_t D, int32_t dtype, int32_t flags, void *stream);
+
+/*
+ * Residual's addition and root-mean-square norm: stored = x + res, rounded to the stream's type, and of that
+ * y = w stored / sqrt(mean(stored^2) + eps).  x, y [N, D]; res, stored [N, D] of the same type, or float with
+ * T2FW_NORM_STREAM_F32 (for 16-bit x); w [D], float with T2FW_NORM_WEIGHT_F32.  res may be null (stored is x then, and may be null as
+ * well where it is not wanted).
+ * ..._fp8: q [N, D] in float8 e4m3 instead of y, with y = scale q; scale = max |y| / 448 of a row (group 0), scales [N], or of every
+ * `group` columns (a power of two, 8 to 512), scales [N, ceil(D / group)]; 1 where all y are zero.  fp32 / fp16 / bf16.
+ */
+#define T2FW_NORM_STREAM_F32 1
+#define T2FW_NORM_WEIGHT_F32 2
+int t2fw_rms_norm_forward(const void *x, const void *res, const void *w, void *y, void *stored,
+                          int64_t N, int64_t D, double eps, int32_t dtype, int32_t flags, void *stream);
+int t2fw_rms_norm_forward_fp8(const void *x, const void *res, const void *w, void *q, float *scales, void *stored,
+                              int64_t N, int64_t D, int64_t group, double eps,
+                              int32_t dtype, int32_t flags, void *stream);
+/*
+ * Gradients from those of y and of `stored` (g_res, of the stream's type, or null): d_x in x's type, d_res in the stream's (null where that is
+ * x's: the two are one array then), d_w in w's.  Sums over the rows are made in a fixed order.
+ */
+size_t t2fw_rms_norm_backward_workspace_bytes(int64_t N, int64_t D, int32_t dtype);
+int t2fw_rms_norm_backward(const void *g_y, const void *g_res, const void *stored, const void *w,
+                           void *d_x, void *d_res, void *d_w, int64_t N, int64_t D, double eps,
+                           int32_t dtype, int32_t flags, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Clipped policy loss with a KL term, from the logits [N, V] (fp32 / fp16 / bf16) and targets [N] of N tokens.  With
+ * logp = log softmax(logits)[target], r = exp(logp - old_logp), d = ref_logp - logp:
+ *   loss = scale / M  sum over the M tokens of the mask of  -min(r adv, clip(r, low, high) adv) + kl (exp(d) - 1 - d).
+ * old_logp, ref_logp, adv [N] float; mask [N] bytes, or null for all; M is at least 1.  Results: loss [1], logp [N] (of all tokens; 0 for
+ * a token outside the mask whose target is none of the V), and lse, coef [N] for the backward call, all float.  d_logits, if
+ * given: the gradient of the loss, in the logits' type.  A target outside [0, V) inside the mask makes the loss NaN.
+ */
+size_t t2fw_policy_loss_workspace_bytes(int64_t N);
+int t2fw_policy_loss_forward(const void *logits, const int64_t *targets, const float *old_logp, const float *ref_logp,
+                             const float *adv, const void *mask,
+                             float *loss, float *logp, float *lse, float *coef, void *d_logits,
+                             int64_t N, int64_t V, float low, float high, float kl, float scale,
+                             int32_t dtype, void *workspace, size_t workspace_bytes, void *stream);
+/* d_logits for the gradient g_loss [1] of the loss.  T2FW_LOSS_UNLESS_ONE: d_logits is what the forward call wrote, and stays where
+ * g_loss is one. */
+#define T2FW_LOSS_UNLESS_ONE 1
+int t2fw_policy_loss_backward(const void *logits, const int64_t *targets, const float *lse, const float *coef,
+                              const float *g_loss, void *d_logits, int64_t N, int64_t V,
+                              int32_t dtype, int32_t flags, void *stream);
+
+/*
+ * The 2-norm of all arrays together (any of the four types each), to norm [1], and the arrays times
+ * min(1, max_norm / (norm + 1e-6)), each to its dst: its src (in place), another array, or null (not wanted).  `arrays` is host memory.
+ */
+typedef struct t2fw_clip_desc {
+    const void *src;
+    void *dst;
+    int64_t n;
+    int32_t src_dtype, dst_dtype;
+} t2fw_clip_desc;
+size_t t2fw_clip_workspace_bytes(const t2fw_clip_desc *arrays, int64_t count);
+int t2fw_clip_grad_norm(const t2fw_clip_desc *arrays, int64_t count, float max_norm, float *norm,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

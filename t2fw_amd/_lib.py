@@ -36,6 +36,10 @@ class BlockCopyDesc(ctypes.Structure):
                 ("terms", _i64), ("term_stride", _i64)]
 
 
+class ClipDesc(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("n", _i64), ("src_dtype", _i32), ("dst_dtype", _i32)]
+
+
 # name -> (restype, argtypes); mirrors include/t2fw_hip.h one to one
 SIGNATURES = {
     "t2fw_abi_version": (ctypes.c_int, []),
@@ -65,6 +69,20 @@ SIGNATURES = {
     "t2fw_dfw_backward_blocks": (ctypes.c_int, [_vp] * 10 + [_i64] * 4 + [_i32, _i32, _vp]),
     "t2fw_dfw_backward_sums_workspace_bytes": (_sz, [_i64] * 4 + [_i32, _i32]),
     "t2fw_dfw_backward_sums": (ctypes.c_int, [_vp] * 10 + [_i64] * 4 + [_i32, _i32, _vp, _sz, _vp]),
+    "t2fw_gated_scan_checkpoint_bytes": (_sz, [_i64] * 3 + [_i32]),
+    "t2fw_gated_scan_workspace_bytes": (_sz, [_i64] * 3 + [_i32]),
+    "t2fw_gated_scan_forward": (ctypes.c_int, [_vp] * 7 + [_i64] * 3 + [ctypes.POINTER(_i64), _i32, _i32, _vp, _sz, _vp]),
+    "t2fw_gated_scan_backward": (ctypes.c_int, [_vp] * 9 + [_i64] * 3 + [ctypes.POINTER(_i64), _i32, _i32, _vp, _sz, _vp]),
+    "t2fw_gated_scan_step": (ctypes.c_int, [_vp] * 5 + [_i64] * 2 + [_i32, _i32, _vp]),
+    "t2fw_rms_norm_forward": (ctypes.c_int, [_vp] * 5 + [_i64] * 2 + [ctypes.c_double, _i32, _i32, _vp]),
+    "t2fw_rms_norm_forward_fp8": (ctypes.c_int, [_vp] * 6 + [_i64] * 3 + [ctypes.c_double, _i32, _i32, _vp]),
+    "t2fw_rms_norm_backward_workspace_bytes": (_sz, [_i64] * 2 + [_i32]),
+    "t2fw_rms_norm_backward": (ctypes.c_int, [_vp] * 7 + [_i64] * 2 + [ctypes.c_double, _i32, _i32, _vp, _sz, _vp]),
+    "t2fw_policy_loss_workspace_bytes": (_sz, [_i64]),
+    "t2fw_policy_loss_forward": (ctypes.c_int, [_vp] * 11 + [_i64] * 2 + [ctypes.c_float] * 4 + [_i32, _vp, _sz, _vp]),
+    "t2fw_policy_loss_backward": (ctypes.c_int, [_vp] * 6 + [_i64] * 2 + [_i32, _i32, _vp]),
+    "t2fw_clip_workspace_bytes": (_sz, [ctypes.POINTER(ClipDesc), _i64]),
+    "t2fw_clip_grad_norm": (ctypes.c_int, [ctypes.POINTER(ClipDesc), _i64, ctypes.c_float, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

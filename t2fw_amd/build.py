@@ -1,5 +1,5 @@
 """Builds t2fw_amd/lib/libt2fw_hip.so from t2fw_amd/csrc/*.hip with hipcc for gfx950, and
-t2fw_amd/lib/_t2fw_host.so from csrc/host.cpp with g++.
+t2fw_amd/lib/_t2fw_host.so from csrc/host.cpp and csrc/host_ops.cpp with g++.
 
     python -m t2fw_amd.build            # build (always recompiles)
     python -m t2fw_amd.build --if-missing
@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libt2fw_hip.so")
-HOST_SRC = os.path.join(CSRC, "host.cpp")
+HOST_SRCS = [os.path.join(CSRC, "host.cpp"), os.path.join(CSRC, "host_ops.cpp")]
 HOST_PATH = os.path.join(LIB_DIR, "_t2fw_host.so")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 
@@ -44,24 +44,24 @@ def _compile(src):
     return obj, err
 
 
-def _compile_host():
-    """host.cpp, the extension module between torch's tensors and the C ABI (host code only, against torch's headers)"""
+def _compile_host(src):
+    """A source of the extension module between torch's tensors and the C ABI (host code only, against torch's headers)"""
     import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths
-    obj = os.path.join(OBJ_DIR, "host.o")
+    obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-4] + ".cpp.o")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
-           "-I" + sysconfig.get_paths()["include"]] + ["-isystem" + i for i in include_paths()] + ["-c", HOST_SRC, "-o", obj]
+           "-I" + sysconfig.get_paths()["include"]] + ["-isystem" + i for i in include_paths()] + ["-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("g++ failed for %s:\n%s" % (HOST_SRC, r.stderr))
+        raise RuntimeError("g++ failed for %s:\n%s" % (src, r.stderr))
     return obj, r.stderr
 
 
-def _link_host(obj):
+def _link_host(objs):
     from torch.utils.cpp_extension import library_paths
     libs = library_paths()
-    cmd = (["g++", "-shared", obj, "-o", HOST_PATH, "-L" + LIB_DIR, "-l:libt2fw_hip.so", "-Wl,-rpath,$ORIGIN"] + ["-L" + d for d in libs] +
+    cmd = (["g++", "-shared"] + objs + ["-o", HOST_PATH, "-L" + LIB_DIR, "-l:libt2fw_hip.so", "-Wl,-rpath,$ORIGIN"] + ["-L" + d for d in libs] +
            ["-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
@@ -72,10 +72,10 @@ def build(verbose=False):
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = sources()
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        host = ex.submit(_compile_host)
+        host = [ex.submit(_compile_host, src) for src in HOST_SRCS]
         results = list(ex.map(_compile, srcs))
-        host_result = host.result()
-    for obj, err in results + [host_result]:
+        host_results = [h.result() for h in host]
+    for obj, err in results + host_results:
         if verbose and err.strip():
             print(err, file=sys.stderr)
     objs = [o for o, _ in results]
@@ -83,7 +83,7 @@ def build(verbose=False):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("link failed:\n" + r.stderr)
-    _link_host(host_result[0])
+    _link_host([o for o, _ in host_results])
     return LIB_PATH
 
 

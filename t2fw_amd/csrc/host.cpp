@@ -6,62 +6,18 @@
 // 205 / 152 us (of which torch's own hand-over to a Python autograd function and back is 91), one generation step 14.6 / 8.4.
 // Gates, event and block copies with their results in the same step as the launch: a training step on gate logits (8 x 1000 tokens, 12
 // heads, bf16) 181 / 168, of 128-wide heads (24 x 1024, fp16) 260 / 219.
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <ATen/ATen.h>
-
-#include <vector>
-
-#include "../../include/t2fw_hip.h"
+#include "host.hpp"
 
 namespace {
 
-using at::Tensor;
+using namespace t2fw_host;
 
-const Tensor &tensor(PyObject *o) {
-    TORCH_CHECK(THPVariable_Check(o), "t2fw: expected a tensor");
-    return THPVariable_Unpack(o);
-}
-int64_t integer(PyObject *o) {
-    const int64_t v = PyLong_AsLongLong(o);
-    if (v == -1 && PyErr_Occurred()) throw python_error();
-    return v;
-}
-void *address(PyObject *o) {
-    void *v = PyLong_AsVoidPtr(o);
-    if (v == nullptr && PyErr_Occurred()) throw python_error();
-    return v;
-}
-void arguments(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK(n == want, "t2fw: ", n, " arguments, expected ", want); }
-void done(int rc) {
-    TORCH_CHECK_WITH(Error, rc == 0, "t2fw error ", rc, ": ", t2fw_last_error());
-}
-PyObject *wrapped(std::initializer_list<Tensor> ts) {
-    PyObject *t = PyTuple_New((Py_ssize_t)ts.size());
-    if (t == nullptr) throw python_error();
-    Py_ssize_t i = 0;
-    for (const Tensor &v : ts) {
-        PyObject *o = v.defined() ? THPVariable_Wrap(v) : Py_NewRef(Py_None);
-        if (o == nullptr) {
-            Py_DECREF(t);
-            throw python_error();
-        }
-        PyTuple_SET_ITEM(t, i++, o);
-    }
-    return t;
-}
-// The launches run without the interpreter's lock: they wait where the device's queue is full.
-template <typename F> int unlocked(F &&launch) {
-    pybind11::gil_scoped_release release;
-    return launch();
-}
 // torch.empty_like: a tensor subclass has its own
 Tensor empty_like(PyObject *o) {
     if (THPVariable_CheckExact(o)) return at::empty_like(tensor(o));
     const pybind11::object made = pybind11::module_::import("torch").attr("empty_like")(pybind11::handle(o));
     return tensor(made.ptr());
 }
-Tensor bytes_like(const Tensor &t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
 
 // lfw_shape(x, f, q, k, f_key, state, heads) -> (B, T, H, D, K), or None where a call on these is an error
 PyObject *lfw_shape(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -433,4 +389,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_t2fw_host", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__t2fw_host() { return PyModule_Create(&module); }
+using t2fw_host::operator_methods;
+
+PyMODINIT_FUNC PyInit__t2fw_host() {
+    PyObject *const m = PyModule_Create(&module);
+    if (m != nullptr && PyModule_AddFunctions(m, operator_methods) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

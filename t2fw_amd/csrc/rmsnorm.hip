@@ -1,0 +1,407 @@
+// The residual's addition and the root-mean-square norm of what is stored:
+//   h = round(x + res) in the stream's type,  r = 1 / sqrt(mean h^2 + eps),  y = w h r;
+//   backward, from dy and the stream's gradient dres:  u = w dy,  d_x = d_res = r (u - h r^2 mean(u h)) + dres,  d_w = sum over rows of dy h r.
+// The norm is of the rounded h, the one that the backward finds again; sums are carried in 32 bits (64 for double).
+// In 8 bits: y is divided by scale = max |y| / 448 of the row, or of each group of its columns, and rounded to float8 e4m3.
+//
+// A row stays in registers between its sums and its results: a wave (rows of up to 1024 columns) or a workgroup of 4 waves holds
+// it in chunks of 8 columns, CH of them for each lane.  Where the width is no multiple of 8 the last chunk of a row is loaded
+// from 8 columns before its end, and the columns that belong to the chunk before it are left out.
+#include "rmsnorm.hpp"
+#include "vec.hpp"
+
+namespace t2fw {
+namespace {
+
+constexpr int RN_THREADS = 256;
+constexpr int RN_WIDTH = 8;              // columns of a chunk
+constexpr float FP8_LARGEST = 448.0f;
+
+template <typename IO> struct AccT { using type = float; };
+template <> struct AccT<double> { using type = double; };
+
+// Sums over the lanes of a row (one wave, or the four of the workgroup)
+template <int WAVES, typename Acc> __device__ __forceinline__ Acc row_sum(Acc v) {
+    v = group_sum(v, 64);
+    if (WAVES > 1) {
+        __shared__ Acc parts[RN_THREADS / 64];
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) v += parts[i];
+    }
+    return v;
+}
+// max that keeps a NaN
+__device__ __forceinline__ float larger(float a, float b) { return a > b || a != a ? a : b; }
+__device__ __forceinline__ float lanes_max(float v, int lanes) {
+    for (int m = 1; m < lanes; m <<= 1) v = larger(v, __shfl_xor(v, m, 64));
+    return v;
+}
+template <int WAVES> __device__ __forceinline__ float row_max(float v) {
+    v = lanes_max(v, 64);
+    if (WAVES > 1) {
+        __shared__ float parts[RN_THREADS / 64];
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = v;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) v = larger(v, parts[i]);
+    }
+    return v;
+}
+
+// A chunk of a row: its first column, where it is loaded from, how many of the loaded columns are its neighbour's
+struct Chunk {
+    int64_t column, from;
+    int skip;
+    bool there;
+};
+__device__ __forceinline__ Chunk chunk_at(int64_t index, int64_t D) {
+    Chunk c;
+    c.column = index * RN_WIDTH;
+    c.there = c.column < D;
+    c.from = c.column + RN_WIDTH <= D ? c.column : D - RN_WIDTH;
+    c.skip = (int)(c.column - c.from);
+    return c;
+}
+template <typename T> __device__ __forceinline__ void store_chunk(T *row, const Chunk &c, const Vec<T, RN_WIDTH> &v) {
+    if (c.skip == 0) {
+        store_vec(row + c.from, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; ++i)
+            if (i >= c.skip) row[c.from + i] = v.e[i];
+    }
+}
+template <typename Acc, typename T> __device__ __forceinline__ void load_wide(Acc (&o)[RN_WIDTH], const void *row, int64_t from) {
+    const Vec<T, RN_WIDTH> v = load_vec<T, RN_WIDTH>(static_cast<const T *>(row) + from);
+#pragma unroll
+    for (int i = 0; i < RN_WIDTH; ++i) o[i] = widen(v.e[i]);
+}
+template <typename IO, typename Acc> __device__ __forceinline__ void load_weights(Acc (&o)[RN_WIDTH], const NormArgs &a, int64_t from) {
+    if (a.wide_w) load_wide<Acc, float>(o, a.w, from);
+    else load_wide<Acc, IO>(o, a.w, from);
+}
+
+template <typename IO, typename Stream, int WAVES, int CH, bool FP8>
+__global__ __launch_bounds__(RN_THREADS) void norm_forward_kernel(NormArgs a) {
+    using Acc = typename AccT<IO>::type;
+    constexpr int ROWS = RN_THREADS / 64 / WAVES, LANES = 64 * WAVES;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES;
+    if (row >= a.N) return;                              // whole waves; with WAVES > 1 a workgroup has one row
+    const IO *x = static_cast<const IO *>(a.x) + row * a.D;
+    const Stream *res = static_cast<const Stream *>(a.res) + row * a.D;
+    Acc h[CH][RN_WIDTH], sum = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const Chunk k = chunk_at(c * LANES + lane, a.D);
+        if (!k.there) continue;
+        load_wide<Acc, IO>(h[c], x, k.from);
+        Vec<Stream, RN_WIDTH> o;
+        if (a.res != nullptr) {
+            Acc add[RN_WIDTH];
+            load_wide<Acc, Stream>(add, res, k.from);
+#pragma unroll
+            for (int i = 0; i < RN_WIDTH; ++i) h[c][i] += add[i];
+        }
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; ++i) {
+            o.e[i] = narrow<Stream>(h[c][i]);
+            h[c][i] = widen(o.e[i]);
+            sum += i >= k.skip ? h[c][i] * h[c][i] : (Acc)0;
+        }
+        if (a.stored != nullptr) store_chunk(static_cast<Stream *>(a.stored) + row * a.D, k, o);
+    }
+    sum = row_sum<WAVES>(sum);
+    const Acc r = (Acc)1 / sqrt(sum / (Acc)a.D + (Acc)a.eps);
+    if (!FP8) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const Chunk k = chunk_at(c * LANES + lane, a.D);
+            if (!k.there) continue;
+            Acc w[RN_WIDTH];
+            load_weights<IO>(w, a, k.from);
+            Vec<IO, RN_WIDTH> o;
+#pragma unroll
+            for (int i = 0; i < RN_WIDTH; ++i) o.e[i] = narrow<IO>(h[c][i] * r * w[i]);
+            store_chunk(static_cast<IO *>(a.y) + row * a.D, k, o);
+        }
+        return;
+    }
+    float top[CH], all = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const Chunk k = chunk_at(c * LANES + lane, a.D);
+        top[c] = 0;
+        if (!k.there) continue;
+        Acc w[RN_WIDTH];
+        load_weights<IO>(w, a, k.from);
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; ++i) {
+            h[c][i] = h[c][i] * r * w[i];
+            if (i >= k.skip) top[c] = larger(fabsf((float)h[c][i]), top[c]);
+        }
+        all = larger(top[c], all);
+    }
+    const bool by_row = a.groups == 1;
+    if (by_row) all = row_max<WAVES>(all);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const Chunk k = chunk_at(c * LANES + lane, a.D);
+        // a group's chunks are neighbouring lanes of one wave, those past the end of the row among them
+        float scale = (by_row ? all : lanes_max(top[c], (int)(a.group / RN_WIDTH))) / FP8_LARGEST;
+        if (scale == 0.0f) scale = 1.0f;
+        if (!k.there) continue;
+        const int64_t g = by_row ? 0 : k.column / a.group;
+        if (by_row ? lane == 0 && c == 0 : k.column % a.group == 0) a.scales[row * a.groups + g] = scale;
+        // one reciprocal for the chunk; of a scale near the smallest numbers it would overflow
+        const float by = 1.0f / scale;
+        const bool tiny = scale < 1e-35f;
+        uint32_t words[2];
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; i += 4) {
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = tiny ? (float)h[c][i + j] / scale : (float)h[c][i + j] * by;
+            int word = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+            words[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], word, true);
+        }
+        Vec<uint8_t, RN_WIDTH> o;
+        __builtin_memcpy(&o, words, sizeof(o));
+        store_chunk(static_cast<uint8_t *>(a.q) + row * a.D, k, o);
+    }
+}
+
+template <typename IO, typename Stream, int WAVES, int CH>
+__global__ __launch_bounds__(RN_THREADS) void norm_backward_kernel(NormArgs a) {
+    using Acc = typename AccT<IO>::type;
+    constexpr int ROWS = RN_THREADS / 64 / WAVES, LANES = 64 * WAVES;
+    const int lane = threadIdx.x % LANES;
+    Acc dw[CH][RN_WIDTH], w[CH][RN_WIDTH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const Chunk k = chunk_at(c * LANES + lane, a.D);
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; ++i) dw[c][i] = 0;
+        if (k.there) load_weights<IO>(w[c], a, k.from);
+    }
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.N; row += (int64_t)gridDim.x * ROWS) {
+        Acc h[CH][RN_WIDTH], u[CH][RN_WIDTH], squares = 0, dot = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const Chunk k = chunk_at(c * LANES + lane, a.D);
+            if (!k.there) continue;
+            load_wide<Acc, Stream>(h[c], static_cast<const Stream *>(a.stored) + row * a.D, k.from);
+            load_wide<Acc, IO>(u[c], static_cast<const IO *>(a.g_y) + row * a.D, k.from);
+#pragma unroll
+            for (int i = 0; i < RN_WIDTH; ++i) {
+                squares += i >= k.skip ? h[c][i] * h[c][i] : (Acc)0;
+                dot += i >= k.skip ? h[c][i] * u[c][i] * w[c][i] : (Acc)0;
+            }
+        }
+        squares = row_sum<WAVES>(squares);
+        dot = row_sum<WAVES>(dot);
+        const Acc r = (Acc)1 / sqrt(squares / (Acc)a.D + (Acc)a.eps), back = dot * r * r / (Acc)a.D;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const Chunk k = chunk_at(c * LANES + lane, a.D);
+            if (!k.there) continue;
+            Acc g[RN_WIDTH];
+            if (a.g_res != nullptr) {
+                load_wide<Acc, Stream>(g, static_cast<const Stream *>(a.g_res) + row * a.D, k.from);
+            } else {
+#pragma unroll
+                for (int i = 0; i < RN_WIDTH; ++i) g[i] = 0;
+            }
+            Vec<IO, RN_WIDTH> o;
+            Vec<Stream, RN_WIDTH> os;
+#pragma unroll
+            for (int i = 0; i < RN_WIDTH; ++i) {
+                dw[c][i] += u[c][i] * h[c][i] * r;
+                g[i] += r * (u[c][i] * w[c][i] - h[c][i] * back);
+                o.e[i] = narrow<IO>(g[i]);
+                os.e[i] = narrow<Stream>(g[i]);
+            }
+            store_chunk(static_cast<IO *>(a.d_x) + row * a.D, k, o);
+            if (a.d_res != nullptr) store_chunk(static_cast<Stream *>(a.d_res) + row * a.D, k, os);
+        }
+    }
+    // every row-group of every workgroup leaves its share of d_w
+    Acc *part = static_cast<Acc *>(a.partials) + ((int64_t)blockIdx.x * ROWS + threadIdx.x / LANES) * a.D;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const Chunk k = chunk_at(c * LANES + lane, a.D);
+        if (!k.there) continue;
+        Vec<Acc, RN_WIDTH> o;
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; ++i) o.e[i] = dw[c][i];
+        store_chunk(part, k, o);
+    }
+}
+
+// Rows of any width, by one workgroup each: what is stored is read again from memory.  For very wide rows, and those of fewer than 8
+// columns.
+template <typename IO, typename Stream, bool FP8>
+__global__ __launch_bounds__(RN_THREADS) void norm_forward_any_kernel(NormArgs a) {
+    using Acc = typename AccT<IO>::type;
+    const int64_t row = blockIdx.x, base = row * a.D;
+    const IO *x = static_cast<const IO *>(a.x) + base;
+    const Stream *res = static_cast<const Stream *>(a.res);
+    auto value = [&](int64_t i) {
+        Acc h = widen(x[i]);
+        if (res != nullptr) h += (Acc)widen(res[base + i]);
+        return (Acc)widen(narrow<Stream>(h));
+    };
+    auto weight = [&](int64_t i) { return a.wide_w ? (Acc)static_cast<const float *>(a.w)[i] : (Acc)widen(static_cast<const IO *>(a.w)[i]); };
+    Acc sum = 0;
+    for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) {
+        const Acc h = value(i);
+        sum += h * h;
+    }
+    sum = row_sum<RN_THREADS / 64>(sum);
+    const Acc r = (Acc)1 / sqrt(sum / (Acc)a.D + (Acc)a.eps);
+    if (FP8) {
+        const int64_t group = a.groups == 1 ? a.D : a.group;
+        for (int64_t g = 0; g < a.groups; ++g) {
+            const int64_t end = (g + 1) * group < a.D ? (g + 1) * group : a.D;
+            float top = 0;
+            for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS) top = larger(fabsf((float)(value(i) * r * weight(i))), top);
+            float scale = row_max<RN_THREADS / 64>(top) / FP8_LARGEST;
+            if (scale == 0.0f) scale = 1.0f;
+            if (threadIdx.x == 0) a.scales[row * a.groups + g] = scale;
+            for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS)
+                static_cast<uint8_t *>(a.q)[base + i] =
+                    (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32((float)(value(i) * r * weight(i)) / scale, 0.0f, 0, false) & 0xff);
+        }
+    } else {
+        for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) static_cast<IO *>(a.y)[base + i] = narrow<IO>(value(i) * r * weight(i));
+    }
+    if (a.stored != nullptr)
+        for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) static_cast<Stream *>(a.stored)[base + i] = narrow<Stream>(value(i));
+}
+
+template <typename IO, typename Stream> __global__ __launch_bounds__(RN_THREADS) void norm_backward_any_kernel(NormArgs a) {
+    using Acc = typename AccT<IO>::type;
+    Acc *part = static_cast<Acc *>(a.partials) + (int64_t)blockIdx.x * a.D;
+    auto weight = [&](int64_t i) { return a.wide_w ? (Acc)static_cast<const float *>(a.w)[i] : (Acc)widen(static_cast<const IO *>(a.w)[i]); };
+    for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) part[i] = 0;
+    for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+        const Stream *h = static_cast<const Stream *>(a.stored) + row * a.D, *gr = static_cast<const Stream *>(a.g_res);
+        const IO *gy = static_cast<const IO *>(a.g_y) + row * a.D;
+        Acc squares = 0, dot = 0;
+        for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) {
+            const Acc v = widen(h[i]);
+            squares += v * v;
+            dot += v * (Acc)widen(gy[i]) * weight(i);
+        }
+        squares = row_sum<RN_THREADS / 64>(squares);
+        dot = row_sum<RN_THREADS / 64>(dot);
+        const Acc r = (Acc)1 / sqrt(squares / (Acc)a.D + (Acc)a.eps), back = dot * r * r / (Acc)a.D;
+        for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) {
+            const Acc v = widen(h[i]), u = widen(gy[i]);
+            Acc g = r * (u * weight(i) - v * back);
+            if (gr != nullptr) g += (Acc)widen(gr[row * a.D + i]);
+            part[i] += u * v * r;
+            static_cast<IO *>(a.d_x)[row * a.D + i] = narrow<IO>(g);
+            if (a.d_res != nullptr) static_cast<Stream *>(a.d_res)[row * a.D + i] = narrow<Stream>(g);
+        }
+    }
+}
+
+// d_w: the sum of all shares, 32 columns for a workgroup of 8 x 32 threads
+template <typename IO, typename Acc>
+__global__ __launch_bounds__(RN_THREADS) void norm_weights_kernel(NormArgs a, int64_t shares) {
+    __shared__ Acc sums[RN_THREADS / 32][32];
+    const int64_t column = (int64_t)blockIdx.x * 32 + threadIdx.x % 32;
+    const Acc *p = static_cast<const Acc *>(a.partials) + column;
+    Acc s = 0;
+    if (column < a.D)
+        for (int64_t i = threadIdx.x / 32; i < shares; i += RN_THREADS / 32) s += p[i * a.D];
+    sums[threadIdx.x / 32][threadIdx.x % 32] = s;
+    __syncthreads();
+    if (threadIdx.x >= 32 || column >= a.D) return;
+#pragma unroll
+    for (int i = 1; i < RN_THREADS / 32; ++i) s += sums[i][threadIdx.x];
+    if (a.wide_w) static_cast<float *>(a.d_w)[column] = (float)s;
+    else static_cast<IO *>(a.d_w)[column] = narrow<IO>(s);
+}
+
+constexpr int64_t NARROW = 1024, WIDEST = 8192;          // columns of a row of one wave; of any row in registers
+constexpr int64_t BACKWARD_GROUPS = 1024;
+bool in_registers(int64_t D) { return D >= RN_WIDTH && D <= WIDEST; }
+int64_t rows_of_group(int64_t D) { return in_registers(D) && D <= NARROW ? RN_THREADS / 64 : 1; }
+int64_t backward_groups(int64_t N, int64_t D) {
+    const int64_t need = (N + rows_of_group(D) - 1) / rows_of_group(D);
+    return need < BACKWARD_GROUPS ? need : BACKWARD_GROUPS;
+}
+
+template <typename IO, typename Stream, bool FP8> int forward_of(const NormArgs &a, hipStream_t stream) {
+    const int64_t groups = (a.N + rows_of_group(a.D) - 1) / rows_of_group(a.D);
+    if (groups > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "norm: too many rows for one launch");
+    const dim3 grid((unsigned)groups), threads(RN_THREADS);
+#define NORM_RUN(W, C) hipLaunchKernelGGL((norm_forward_kernel<IO, Stream, W, C, FP8>), grid, threads, 0, stream, a)
+    if (!in_registers(a.D)) hipLaunchKernelGGL((norm_forward_any_kernel<IO, Stream, FP8>), grid, threads, 0, stream, a);
+    else if (a.D <= 512) NORM_RUN(1, 1);
+    else if (a.D <= 1024) NORM_RUN(1, 2);
+    else if (a.D <= 2048) NORM_RUN(4, 1);
+    else if (a.D <= 4096) NORM_RUN(4, 2);
+    else NORM_RUN(4, 4);
+#undef NORM_RUN
+    return check_hip(hipGetLastError(), "norm_forward_kernel launch");
+}
+
+template <typename IO, typename Stream> int backward_of(const NormArgs &a, hipStream_t stream) {
+    using Acc = typename AccT<IO>::type;
+    const int64_t groups = backward_groups(a.N, a.D);
+    const dim3 grid((unsigned)groups), threads(RN_THREADS);
+    if (a.N > 0) {
+#define NORM_RUN(W, C) hipLaunchKernelGGL((norm_backward_kernel<IO, Stream, W, C>), grid, threads, 0, stream, a)
+        if (!in_registers(a.D)) hipLaunchKernelGGL((norm_backward_any_kernel<IO, Stream>), grid, threads, 0, stream, a);
+        else if (a.D <= 512) NORM_RUN(1, 1);
+        else if (a.D <= 1024) NORM_RUN(1, 2);
+        else if (a.D <= 2048) NORM_RUN(4, 1);
+        else if (a.D <= 4096) NORM_RUN(4, 2);
+        else NORM_RUN(4, 4);
+#undef NORM_RUN
+        const int rc = check_hip(hipGetLastError(), "norm_backward_kernel launch");
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL((norm_weights_kernel<IO, Acc>), dim3((unsigned)((a.D + 31) / 32)), threads, 0, stream, a, norm_partials(a.N, a.D));
+    return check_hip(hipGetLastError(), "norm_weights_kernel launch");
+}
+
+template <typename IO> int forward_types(const NormArgs &a, hipStream_t stream) {
+    if (a.q != nullptr) return a.wide_stream ? forward_of<IO, float, true>(a, stream) : forward_of<IO, IO, true>(a, stream);
+    return a.wide_stream ? forward_of<IO, float, false>(a, stream) : forward_of<IO, IO, false>(a, stream);
+}
+template <typename IO> int backward_types(const NormArgs &a, hipStream_t stream) {
+    return a.wide_stream ? backward_of<IO, float>(a, stream) : backward_of<IO, IO>(a, stream);
+}
+
+}  // namespace
+
+int64_t norm_partials(int64_t N, int64_t D) { return backward_groups(N, D) * rows_of_group(D); }
+
+int norm_forward(const NormArgs &a, int dtype, hipStream_t stream) {
+    switch (dtype) {
+        case T2FW_F32: return a.q != nullptr ? forward_of<float, float, true>(a, stream) : forward_of<float, float, false>(a, stream);
+        case T2FW_F16: return forward_types<_Float16>(a, stream);
+        case T2FW_BF16: return forward_types<__bf16>(a, stream);
+    }
+    return forward_of<double, double, false>(a, stream);
+}
+
+int norm_backward(const NormArgs &a, int dtype, hipStream_t stream) {
+    switch (dtype) {
+        case T2FW_F32: return backward_of<float, float>(a, stream);
+        case T2FW_F16: return backward_types<_Float16>(a, stream);
+        case T2FW_BF16: return backward_types<__bf16>(a, stream);
+    }
+    return backward_of<double, double>(a, stream);
+}
+
+}  // namespace t2fw
