@@ -34,6 +34,26 @@ template <int WAVES, typename Acc> __device__ __forceinline__ Acc row_sum(Acc v)
     }
     return v;
 }
+// Two of them in one exchange
+template <int WAVES, typename Acc> __device__ __forceinline__ void row_sums(Acc &v, Acc &u) {
+    v = group_sum(v, 64);
+    u = group_sum(u, 64);
+    if (WAVES > 1) {
+        __shared__ Acc parts[2][RN_THREADS / 64];
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) {
+            parts[0][threadIdx.x / 64] = v;
+            parts[1][threadIdx.x / 64] = u;
+        }
+        __syncthreads();
+        v = u = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            v += parts[0][i];
+            u += parts[1][i];
+        }
+    }
+}
 // max that keeps a NaN
 __device__ __forceinline__ float larger(float a, float b) { return a > b || a != a ? a : b; }
 __device__ __forceinline__ float lanes_max(float v, int lanes) {
@@ -190,48 +210,69 @@ __global__ __launch_bounds__(RN_THREADS) void norm_backward_kernel(NormArgs a) {
         if (k.there) load_weights<IO>(w[c], a, k.from);
     }
     for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.N; row += (int64_t)gridDim.x * ROWS) {
-        Acc h[CH][RN_WIDTH], u[CH][RN_WIDTH], squares = 0, dot = 0;
+        // all of the row's loads before its sums
+        Vec<Stream, RN_WIDTH> hv[CH], rv[CH];
+        Vec<IO, RN_WIDTH> uv[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const Chunk k = chunk_at(c * LANES + lane, a.D);
             if (!k.there) continue;
-            load_wide<Acc, Stream>(h[c], static_cast<const Stream *>(a.stored) + row * a.D, k.from);
-            load_wide<Acc, IO>(u[c], static_cast<const IO *>(a.g_y) + row * a.D, k.from);
+            hv[c] = load_vec<Stream, RN_WIDTH>(static_cast<const Stream *>(a.stored) + row * a.D + k.from);
+            uv[c] = load_vec<IO, RN_WIDTH>(static_cast<const IO *>(a.g_y) + row * a.D + k.from);
+            if (a.g_res != nullptr) rv[c] = load_vec<Stream, RN_WIDTH>(static_cast<const Stream *>(a.g_res) + row * a.D + k.from);
+        }
+        Acc squares = 0, dot = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const Chunk k = chunk_at(c * LANES + lane, a.D);
+            if (!k.there) continue;
 #pragma unroll
             for (int i = 0; i < RN_WIDTH; ++i) {
-                squares += i >= k.skip ? h[c][i] * h[c][i] : (Acc)0;
-                dot += i >= k.skip ? h[c][i] * u[c][i] * w[c][i] : (Acc)0;
+                const Acc h = widen(hv[c].e[i]);
+                squares += i >= k.skip ? h * h : (Acc)0;
+                dot += i >= k.skip ? h * (Acc)widen(uv[c].e[i]) * w[c][i] : (Acc)0;
             }
         }
-        squares = row_sum<WAVES>(squares);
-        dot = row_sum<WAVES>(dot);
+        row_sums<WAVES>(squares, dot);
         const Acc r = (Acc)1 / sqrt(squares / (Acc)a.D + (Acc)a.eps), back = dot * r * r / (Acc)a.D;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const Chunk k = chunk_at(c * LANES + lane, a.D);
             if (!k.there) continue;
-            Acc g[RN_WIDTH];
-            if (a.g_res != nullptr) {
-                load_wide<Acc, Stream>(g, static_cast<const Stream *>(a.g_res) + row * a.D, k.from);
-            } else {
-#pragma unroll
-                for (int i = 0; i < RN_WIDTH; ++i) g[i] = 0;
-            }
             Vec<IO, RN_WIDTH> o;
             Vec<Stream, RN_WIDTH> os;
 #pragma unroll
             for (int i = 0; i < RN_WIDTH; ++i) {
-                dw[c][i] += u[c][i] * h[c][i] * r;
-                g[i] += r * (u[c][i] * w[c][i] - h[c][i] * back);
-                o.e[i] = narrow<IO>(g[i]);
-                os.e[i] = narrow<Stream>(g[i]);
+                const Acc h = widen(hv[c].e[i]), u = widen(uv[c].e[i]);
+                dw[c][i] += u * h * r;
+                Acc g = r * (u * w[c][i] - h * back);
+                if (a.g_res != nullptr) g += (Acc)widen(rv[c].e[i]);
+                o.e[i] = narrow<IO>(g);
+                os.e[i] = narrow<Stream>(g);
             }
             store_chunk(static_cast<IO *>(a.d_x) + row * a.D, k, o);
             if (a.d_res != nullptr) store_chunk(static_cast<Stream *>(a.d_res) + row * a.D, k, os);
         }
     }
-    // every row-group of every workgroup leaves its share of d_w
-    Acc *part = static_cast<Acc *>(a.partials) + ((int64_t)blockIdx.x * ROWS + threadIdx.x / LANES) * a.D;
+    // a workgroup's share of d_w: that of its waves, where each had rows of its own, added up in order
+    if (ROWS > 1) {
+        __shared__ Acc sums[ROWS > 1 ? ROWS - 1 : 1][ROWS > 1 ? CH : 1][RN_WIDTH][64];
+        if (threadIdx.x >= 64) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < RN_WIDTH; ++i) sums[threadIdx.x / 64 - 1][c][i][lane] = dw[c][i];
+        }
+        __syncthreads();
+        if (threadIdx.x >= 64) return;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < RN_WIDTH; ++i)
+#pragma unroll
+                for (int r = 0; r < ROWS - 1; ++r) dw[c][i] += sums[r][c][i][lane];
+    }
+    Acc *part = static_cast<Acc *>(a.partials) + (int64_t)blockIdx.x * a.D;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const Chunk k = chunk_at(c * LANES + lane, a.D);
@@ -312,31 +353,35 @@ template <typename IO, typename Stream> __global__ __launch_bounds__(RN_THREADS)
     }
 }
 
-// d_w: the sum of all shares, 32 columns for a workgroup of 8 x 32 threads
+// d_w: the sum of all shares.  A workgroup takes 32 columns with 32 threads each, whose loads do not wait for one another.
+constexpr int RW_THREADS = 1024, RW_COLUMNS = 32, RW_ROWS = RW_THREADS / RW_COLUMNS;
 template <typename IO, typename Acc>
-__global__ __launch_bounds__(RN_THREADS) void norm_weights_kernel(NormArgs a, int64_t shares) {
-    __shared__ Acc sums[RN_THREADS / 32][32];
-    const int64_t column = (int64_t)blockIdx.x * 32 + threadIdx.x % 32;
+__global__ __launch_bounds__(RW_THREADS) void norm_weights_kernel(NormArgs a, int64_t shares) {
+    __shared__ Acc sums[RW_ROWS][RW_COLUMNS];
+    const int64_t column = (int64_t)blockIdx.x * RW_COLUMNS + threadIdx.x % RW_COLUMNS;
     const Acc *p = static_cast<const Acc *>(a.partials) + column;
     Acc s = 0;
-    if (column < a.D)
-        for (int64_t i = threadIdx.x / 32; i < shares; i += RN_THREADS / 32) s += p[i * a.D];
-    sums[threadIdx.x / 32][threadIdx.x % 32] = s;
+    if (column < a.D) {
+#pragma unroll 8
+        for (int64_t i = threadIdx.x / RW_COLUMNS; i < shares; i += RW_ROWS) s += p[i * a.D];
+    }
+    sums[threadIdx.x / RW_COLUMNS][threadIdx.x % RW_COLUMNS] = s;
     __syncthreads();
-    if (threadIdx.x >= 32 || column >= a.D) return;
+    if (threadIdx.x >= RW_COLUMNS || column >= a.D) return;
 #pragma unroll
-    for (int i = 1; i < RN_THREADS / 32; ++i) s += sums[i][threadIdx.x];
+    for (int i = 1; i < RW_ROWS; ++i) s += sums[i][threadIdx.x];
     if (a.wide_w) static_cast<float *>(a.d_w)[column] = (float)s;
     else static_cast<IO *>(a.d_w)[column] = narrow<IO>(s);
 }
 
 constexpr int64_t NARROW = 1024, WIDEST = 8192;          // columns of a row of one wave; of any row in registers
-constexpr int64_t BACKWARD_GROUPS = 1024;
 bool in_registers(int64_t D) { return D >= RN_WIDTH && D <= WIDEST; }
 int64_t rows_of_group(int64_t D) { return in_registers(D) && D <= NARROW ? RN_THREADS / 64 : 1; }
+// Workgroups of the backward: one for each CU before any takes a second row, then as many as are on the chip at once, with four
+// rows of each wave or more, as every workgroup leaves a row of 32-bit sums.
 int64_t backward_groups(int64_t N, int64_t D) {
-    const int64_t need = (N + rows_of_group(D) - 1) / rows_of_group(D);
-    return need < BACKWARD_GROUPS ? need : BACKWARD_GROUPS;
+    const int64_t rows = rows_of_group(D), need = (N + rows - 1) / rows, few = need < 256 ? need : 256, many = need / 4;
+    return many < few ? few : many < 1024 ? many : 1024;
 }
 
 template <typename IO, typename Stream, bool FP8> int forward_of(const NormArgs &a, hipStream_t stream) {
@@ -370,7 +415,8 @@ template <typename IO, typename Stream> int backward_of(const NormArgs &a, hipSt
         const int rc = check_hip(hipGetLastError(), "norm_backward_kernel launch");
         if (rc) return rc;
     }
-    hipLaunchKernelGGL((norm_weights_kernel<IO, Acc>), dim3((unsigned)((a.D + 31) / 32)), threads, 0, stream, a, norm_partials(a.N, a.D));
+    hipLaunchKernelGGL((norm_weights_kernel<IO, Acc>), dim3((unsigned)((a.D + RW_COLUMNS - 1) / RW_COLUMNS)), dim3(RW_THREADS), 0, stream, a,
+                       norm_partials(a.N, a.D));
     return check_hip(hipGetLastError(), "norm_weights_kernel launch");
 }
 
@@ -384,7 +430,7 @@ template <typename IO> int backward_types(const NormArgs &a, hipStream_t stream)
 
 }  // namespace
 
-int64_t norm_partials(int64_t N, int64_t D) { return backward_groups(N, D) * rows_of_group(D); }
+int64_t norm_partials(int64_t N, int64_t D) { return backward_groups(N, D); }
 
 int norm_forward(const NormArgs &a, int dtype, hipStream_t stream) {
     switch (dtype) {

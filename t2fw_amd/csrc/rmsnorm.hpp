@@ -13,7 +13,7 @@ struct NormArgs {
     float *scales;                      // [N, groups]
     void *d_x, *d_res;                  // backward results; d_res is null where it is d_x
     void *d_w;                          // [D] of w's type
-    void *partials;                     // [norm_partials(N, D), D] in the accumulators' type
+    void *partials;                     // [norm_partials(N, D), D], the workgroups' shares of d_w, in the accumulators' type
     int64_t N, D, group, groups;        // group: columns of one scale
     double eps;
     int32_t wide_stream, wide_w;        // the stream / the weights are float32 next to 16-bit tensors
