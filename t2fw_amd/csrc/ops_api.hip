@@ -261,7 +261,7 @@ int t2fw_rms_norm_backward(const void *g_y, const void *g_res, const void *store
     return norm_backward(a, dtype, static_cast<hipStream_t>(stream));
 }
 
-size_t t2fw_policy_loss_workspace_bytes(int64_t N) { return N < 0 ? 0 : ((size_t)N + 1) * sizeof(float); }
+size_t t2fw_policy_loss_workspace_bytes(int64_t N) { return N < 0 ? 0 : (POLICY_SUMS + 1) * sizeof(double); }
 
 int t2fw_policy_loss_forward(const void *logits, const int64_t *targets, const float *old_logp, const float *ref_logp, const float *adv,
                              const void *mask, float *loss, float *logp, float *lse, float *coef, void *d_logits, int64_t N, int64_t V,
@@ -274,13 +274,14 @@ int t2fw_policy_loss_forward(const void *logits, const int64_t *targets, const f
     const bool none = N == 0;
     if ((rc = check_arrays({{"logits", logits, es, none}, {"targets", targets, 8, none}, {"old_logp", old_logp, 4, none},
                             {"ref_logp", ref_logp, 4, none}, {"adv", adv, 4, none}, {"loss", loss, 4, false}, {"logp", logp, 4, none},
-                            {"lse", lse, 4, none}, {"coef", coef, 4, none}, {"d_logits", d_logits, es, true}, {"workspace", workspace, 4, false}})))
+                            {"lse", lse, 4, none}, {"coef", coef, 4, none}, {"d_logits", d_logits, es, true}, {"workspace", workspace, 8, false}})))
         return rc;
     if (workspace_bytes < need) return bad_workspace(need, workspace_bytes);
     PolicyLossArgs a{};
     a.logits = logits; a.targets = targets; a.old_logp = old_logp; a.ref_logp = ref_logp; a.adv = adv;
     a.mask = static_cast<const uint8_t *>(mask);
-    a.loss = loss; a.logp = logp; a.lse = lse; a.coef = coef; a.each = static_cast<float *>(workspace); a.d_logits = d_logits;
+    a.loss = loss; a.logp = logp; a.lse = lse; a.coef = coef; a.tokens = static_cast<int64_t *>(workspace);
+    a.sums = static_cast<double *>(workspace) + 1; a.d_logits = d_logits;
     a.N = N; a.V = V; a.low = low; a.high = high; a.kl = kl; a.scale = scale;
     return policy_loss_forward(a, dtype, static_cast<hipStream_t>(stream));
 }

@@ -10,29 +10,25 @@
 namespace t2fw {
 namespace {
 
-constexpr int PL_THREADS = 1024;
-constexpr int PL_WAVES = PL_THREADS / 64;
-
 // 16-bit logits: the hardware's exponential (2^-21 relative at arguments of -20); 32-bit ones: the library's
 template <typename IO> __device__ __forceinline__ float exp_of(float v) { return sizeof(IO) == 2 ? __expf(v) : expf(v); }
 
-__device__ __forceinline__ float wave_max(float v) {
-    for (int m = 1; m < 64; m <<= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-    return v;
-}
+constexpr int PL_THREADS = 1024;
 
-// number of tokens that count -> 1 / M (M at least 1)
-__global__ __launch_bounds__(PL_THREADS) void policy_count_kernel(const uint8_t *mask, int64_t N, float *inverse) {
-    __shared__ int64_t parts[PL_WAVES];
-    int64_t n = 0;
-    for (int64_t i = threadIdx.x; i < N; i += PL_THREADS) n += mask == nullptr || mask[i] != 0;
-    for (int m = 1; m < 64; m <<= 1) n += __shfl_xor(n, m, 64);
-    if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = n;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < PL_WAVES; ++i) n += parts[i];
-        *inverse = 1.0f / (float)(n > 0 ? n : 1);
-    }
+// A maximum and a sum of exponentials over it; what minus infinity stands for is nothing
+struct Top {
+    float m, s;
+};
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
+template <typename IO> __device__ __forceinline__ Top joined(const Top &a, const Top &b) {
+    // two products and a sum, not a fused form: the lanes of a pair, which see a and b the other way round, get the same bits
+#pragma clang fp contract(off)
+    const float m = fmaxf(a.m, b.m), base = base_of(m);
+    return {m, a.s * exp_of<IO>(a.m - base) + b.s * exp_of<IO>(b.m - base)};
+}
+template <typename IO> __device__ __forceinline__ Top joined_lanes(Top t, int lanes) {
+    for (int m = 1; m < lanes; m <<= 1) t = joined<IO>(t, {__shfl_xor(t.m, m, 64), __shfl_xor(t.s, m, 64)});
+    return t;
 }
 
 struct TokenTerms {
@@ -47,93 +43,205 @@ __device__ __forceinline__ TokenTerms terms_of(const PolicyLossArgs &a, int64_t 
     return {(r != r ? r : -fminf(freely, held)) + a.kl * (em - d), (moves ? -freely : 0.0f) - a.kl * em};
 }
 
-// d z of a row, or its zeros
-template <typename IO>
-__device__ __forceinline__ void write_gradient(const IO *z, IO *dz, int64_t V, float lse, float c, int64_t target) {
-    constexpr int VEC = 16 / sizeof(IO);
-    for (int64_t i = (int64_t)threadIdx.x * VEC; i < V; i += PL_THREADS * VEC) {
-        if (i + VEC <= V) {
-            const Vec<IO, VEC> v = load_vec<IO, VEC>(z + i);
-            Vec<IO, VEC> o;
+// What a workgroup needs besides a row: the number of tokens that count.  Every workgroup counts them itself as long as that is 16 bytes
+// for each thread; a launch of its own does it for more.
+constexpr int64_t COUNTED_BYTES = 16;
+template <int THREADS> __device__ __forceinline__ int64_t counted(const PolicyLossArgs &a) {
+    __shared__ int64_t parts[THREADS / 64];
+    int64_t n = 0;
+    for (int64_t i = (int64_t)threadIdx.x * 8; i < a.N; i += THREADS * 8) {
+        if (i + 8 <= a.N) {
+            const Vec<uint8_t, 8> v = load_vec<uint8_t, 8>(a.mask + i);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float p = c == 0.0f ? 0.0f : -c * exp_of<IO>(widen(v.e[j]) - lse);
-                o.e[j] = narrow<IO>(i + j == target ? p + c : p);
-            }
-            store_vec(dz + i, o);
+            for (int j = 0; j < 8; ++j) n += v.e[j] != 0;
         } else {
-            for (int64_t j = i; j < V; ++j) {
-                const float p = c == 0.0f ? 0.0f : -c * exp_of<IO>(widen(z[j]) - lse);
-                dz[j] = narrow<IO>(j == target ? p + c : p);
-            }
+            for (int64_t j = i; j < a.N; ++j) n += a.mask[j] != 0;
         }
     }
+    for (int m = 1; m < 64; m <<= 1) n += __shfl_xor(n, m, 64);
+    if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = n;
+    __syncthreads();
+    n = 0;
+    for (int i = 0; i < THREADS / 64; ++i) n += parts[i];
+    return n;
+}
+__global__ __launch_bounds__(PL_THREADS) void policy_count_kernel(PolicyLossArgs a) {
+    const int64_t n = counted<PL_THREADS>(a);
+    if (threadIdx.x == 0) *a.tokens = n;
 }
 
-template <typename IO>
-__global__ __launch_bounds__(PL_THREADS) void policy_rows_kernel(PolicyLossArgs a, const float *inverse) {
-    constexpr int VEC = 16 / sizeof(IO);
-    __shared__ float tops[PL_WAVES], sums[PL_WAVES], shared[2];
-    const int64_t row = blockIdx.x;
-    const IO *z = static_cast<const IO *>(a.logits) + row * a.V;
-    float top = -INFINITY, s = 0;
-    for (int64_t i = (int64_t)threadIdx.x * VEC; i < a.V; i += PL_THREADS * VEC) {
-        float v[VEC];
-        if (i + VEC <= a.V) {
-            const Vec<IO, VEC> raw = load_vec<IO, VEC>(z + i);
+// A row in the registers of a workgroup: CH vectors of each thread.  Rows of an odd vocabulary start anywhere, and loads and
+// stores that are not aligned cost a fifth of the rate (8192 x 50257 bfloat16: 388 us, 325 for 50264): the vectors begin at the first aligned
+// element, and the few before them and after the last whole one are one each for the first threads.
+template <typename IO, int THREADS, int CH> struct Row {
+    static constexpr int VEC = 16 / sizeof(IO);
+    Raw16 v[CH];
+    float extra;                        // minus infinity where there is none
+    int head, vectors, rest;            // elements before the vectors, the vectors, elements after them
+    __device__ __forceinline__ static int at(int c) { return c * THREADS + (int)threadIdx.x; }
+    __device__ __forceinline__ int extra_at() const { return (int)threadIdx.x < head ? (int)threadIdx.x : head + vectors * VEC + (int)threadIdx.x - head; }
+    __device__ __forceinline__ bool has_extra() const { return (int)threadIdx.x < head + rest; }
+    __device__ __forceinline__ void load(const IO *z, int64_t V) {
+        const int to_aligned = (int)((16 - reinterpret_cast<uintptr_t>(z) % 16) % 16 / sizeof(IO));
+        head = to_aligned < V ? to_aligned : (int)V;
+        vectors = ((int)V - head) / VEC;
+        rest = (int)V - head - vectors * VEC;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = widen(raw.e[j]);
-        } else {
+        for (int c = 0; c < CH; ++c)
+            if (at(c) < vectors) v[c] = load_raw(z + head + (int64_t)at(c) * VEC);
+        extra = has_extra() ? (float)widen(z[extra_at()]) : -INFINITY;
+    }
+    // The row is held as it came: without this the compiler keeps its 32-bit form from one use to the next, in twice the registers
+    __device__ __forceinline__ void stay_narrow() {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = i + j < a.V ? (float)widen(z[i + j]) : -INFINITY;
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(v[c].w[i]));
+    }
+    __device__ __forceinline__ Top top(int64_t) {
+        float m = extra;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (at(c) < vectors) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) m = fmaxf(m, element<IO>(v[c], j));
+            }
+        const float base = base_of(m);
+        float s = exp_of<IO>(extra - base);
+        stay_narrow();
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (at(c) < vectors) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s += exp_of<IO>(element<IO>(v[c], j) - base);
+            }
+        stay_narrow();
+        return {m, s};
+    }
+    // -c softmax, and at the target, by the thread that has just written there, c more
+    __device__ __forceinline__ void gradient(IO *dz, int64_t V, float lse, float c, int64_t target, float logp) const {
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+            if (at(k) < vectors) {
+                Vec<IO, VEC> o;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o.e[j] = narrow<IO>(-c * exp_of<IO>(element<IO>(v[k], j) - lse));
+                store_vec(dz + head + (int64_t)at(k) * VEC, o);
+            }
+        if (has_extra()) dz[extra_at()] = narrow<IO>(-c * exp_of<IO>(extra - lse));
+        if (target >= 0 && target < V) {
+            const int t = (int)target, in = t - head;
+            const int owner = t < head ? t : in < vectors * VEC ? in / VEC % THREADS : head + in - vectors * VEC;
+            if ((int)threadIdx.x == owner) dz[t] = narrow<IO>(fmaf(-c, exp_of<IO>(logp), c));
         }
-        float m = top;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[j]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        s *= exp_of<IO>(top - base);
-        top = m;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += exp_of<IO>(v[j] - base);
     }
-    const float wm = wave_max(top), wbase = wm == -INFINITY ? 0.0f : wm;
-    s = group_sum(s * exp_of<IO>(top - wbase), 64);
-    if (threadIdx.x % 64 == 0) {
-        tops[threadIdx.x / 64] = wm;
-        sums[threadIdx.x / 64] = s;
+    __device__ __forceinline__ void zeros(IO *dz, int64_t) const {
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+            if (at(k) < vectors) store_vec(dz + head + (int64_t)at(k) * VEC, Vec<IO, VEC>{});
+        if (has_extra()) dz[extra_at()] = (IO)0;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float m = tops[0];
-        for (int i = 1; i < PL_WAVES; ++i) m = fmaxf(m, tops[i]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float total = 0;
-        for (int i = 0; i < PL_WAVES; ++i) total += sums[i] * expf(tops[i] - base);
-        const float lse = base + logf(total);
+};
+
+// The same for a row that does not fit: read twice, the second time from a cache
+template <typename IO, int THREADS> struct Row<IO, THREADS, 0> {
+    static constexpr int VEC = 16 / sizeof(IO);
+    const IO *z;
+    __device__ __forceinline__ void load(const IO *row, int64_t) { z = row; }
+    __device__ __forceinline__ Top top(int64_t V) const {
+        Top t{-INFINITY, 0};
+        for (int64_t i = (int64_t)threadIdx.x * VEC; i < V; i += THREADS * VEC) {
+            float v[VEC], m = t.m;
+            if (i + VEC <= V) {
+                const Vec<IO, VEC> raw = load_vec<IO, VEC>(z + i);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = widen(raw.e[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = i + j < V ? (float)widen(z[i + j]) : -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[j]);
+            const float base = base_of(m);
+            t.s *= exp_of<IO>(t.m - base);
+            t.m = m;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) t.s += exp_of<IO>(v[j] - base);
+        }
+        return t;
+    }
+    __device__ __forceinline__ void gradient(IO *dz, int64_t V, float lse, float c, int64_t target, float logp) const {
+        for (int64_t i = (int64_t)threadIdx.x * VEC; i < V; i += THREADS * VEC) {
+            if (i + VEC <= V) {
+                const Vec<IO, VEC> v = load_vec<IO, VEC>(z + i);
+                Vec<IO, VEC> o;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o.e[j] = narrow<IO>(-c * exp_of<IO>(widen(v.e[j]) - lse));
+                store_vec(dz + i, o);
+            } else {
+                for (int64_t j = i; j < V; ++j) dz[j] = narrow<IO>(-c * exp_of<IO>(widen(z[j]) - lse));
+            }
+            if (target >= i && target < i + VEC && target < V) dz[target] = narrow<IO>(fmaf(-c, exp_of<IO>(logp), c));
+        }
+    }
+    __device__ __forceinline__ void zeros(IO *dz, int64_t V) const {
+        for (int64_t i = (int64_t)threadIdx.x * VEC; i < V; i += THREADS * VEC) {
+            if (i + VEC <= V) store_vec(dz + i, Vec<IO, VEC>{});
+            else
+                for (int64_t j = i; j < V; ++j) dz[j] = (IO)0;
+        }
+    }
+};
+
+// GROUPS workgroups share a CU: what a row's loads and stores leave idle is another's
+template <typename IO, int THREADS, int CH, int GROUPS>
+__global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void policy_rows_kernel(PolicyLossArgs a) {
+    constexpr int WAVES = THREADS / 64;
+    __shared__ Top tops[2][WAVES];
+    const int64_t M = a.mask == nullptr ? a.N : a.N > COUNTED_BYTES * THREADS ? *a.tokens : counted<THREADS>(a);
+    const float share = a.scale / (float)(M > 0 ? M : 1);
+    double sum = 0;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x, turn ^= 1) {
+        const IO *z = static_cast<const IO *>(a.logits) + row * a.V;
         const int64_t t = a.targets[row];
         const bool counts = a.mask == nullptr || a.mask[row] != 0, known = t >= 0 && t < a.V;
-        const float logp = known ? widen(z[t]) - lse : counts ? NAN : 0.0f;
-        const float share = a.scale * *inverse;
-        TokenTerms m2{0, 0};
-        if (counts) m2 = terms_of(a, row, logp);
-        a.logp[row] = logp;
-        a.lse[row] = shared[0] = lse;
-        a.coef[row] = shared[1] = m2.coef * share;
-        a.each[row] = m2.loss * share;
+        const float zt = known ? (float)widen(z[t]) : 0.0f;
+        Row<IO, THREADS, CH> r;
+        r.load(z, a.V);
+        Top top = joined_lanes<IO>(r.top(a.V), 64);
+        if (threadIdx.x % 64 == 0) tops[turn][threadIdx.x / 64] = top;
+        __syncthreads();                                 // (the other half is free again: every wave has read it before this row's barrier)
+        top = joined_lanes<IO>(tops[turn][threadIdx.x % WAVES], WAVES);
+        const float lse = base_of(top.m) + logf(top.s), logp = known ? zt - lse : counts ? NAN : 0.0f;
+        TokenTerms m{0, 0};
+        if (counts) m = terms_of(a, row, logp);
+        if (threadIdx.x == 0) {
+            a.logp[row] = logp;
+            a.lse[row] = lse;
+            a.coef[row] = m.coef * share;
+            sum += (double)(m.loss * share);
+        }
+        if (a.d_logits != nullptr) {
+            IO *const dz = static_cast<IO *>(a.d_logits) + row * a.V;
+            if (counts) r.gradient(dz, a.V, lse, m.coef * share, t, logp);
+            else r.zeros(dz, a.V);
+        }
     }
-    __syncthreads();
-    if (a.d_logits != nullptr) write_gradient(z, static_cast<IO *>(a.d_logits) + row * a.V, a.V, shared[0], shared[1], a.targets[row]);
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = sum;
 }
 
-__global__ __launch_bounds__(PL_THREADS) void policy_sum_kernel(const float *each, int64_t N, float *loss) {
-    __shared__ double parts[PL_WAVES];
+// The loss: the workgroups' sums, in order
+constexpr int PS_THREADS = 1024;
+__global__ __launch_bounds__(PS_THREADS) void policy_sum_kernel(const double *sums, int n, float *loss) {
+    __shared__ double parts[PS_THREADS / 64];
     double s = 0;
-    for (int64_t i = threadIdx.x; i < N; i += PL_THREADS) s += (double)each[i];
+    for (int i = threadIdx.x; i < n; i += PS_THREADS) s += sums[i];
     s = group_sum(s, 64);
     if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < PL_WAVES; ++i) s += parts[i];
+        for (int i = 1; i < PS_THREADS / 64; ++i) s += parts[i];
         *loss = (float)s;
     }
 }
@@ -142,28 +250,59 @@ template <typename IO>
 __global__ __launch_bounds__(PL_THREADS) void policy_gradient_kernel(PolicyLossArgs a) {
     const float g = *a.g_loss;
     if (a.unless_one && g == 1.0f) return;
-    const int64_t row = blockIdx.x;
-    const IO *z = static_cast<const IO *>(a.logits) + row * a.V;
-    write_gradient(z, static_cast<IO *>(a.d_logits) + row * a.V, a.V, a.lse[row], a.coef[row] * g, a.targets[row]);
+    for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+        const IO *z = static_cast<const IO *>(a.logits) + row * a.V;
+        IO *const dz = static_cast<IO *>(a.d_logits) + row * a.V;
+        const int64_t t = a.targets[row];
+        const float lse = a.lse[row], c = a.coef[row] * g;
+        const float logp = t >= 0 && t < a.V ? widen(z[t]) - lse : 0.0f;
+        Row<IO, PL_THREADS, 0> r;
+        r.load(z, a.V);
+        if (c == 0.0f) r.zeros(dz, a.V);
+        else r.gradient(dz, a.V, lse, c, t, logp);
+    }
 }
 
+// Workgroups of a launch over all rows: as many as the chip holds
+int groups_of(int64_t N, int64_t resident) { return (int)(N < resident ? N : resident); }
+
 template <typename IO> int forward_of(const PolicyLossArgs &a, hipStream_t stream) {
-    // 1 / M lies behind the tokens' shares
-    float *const inverse = a.each + a.N;
-    hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(PL_THREADS), 0, stream, a.mask, a.N, inverse);
-    int rc = check_hip(hipGetLastError(), "policy_count_kernel launch");
-    if (rc) return rc;
+    constexpr int VEC = 16 / sizeof(IO);
+    int groups = 0;
+#define POLICY_ROWS(THREADS, CH, GROUPS)                                                                                            \
+    do {                                                                                                                            \
+        groups = groups_of(a.N, 256 * GROUPS);                                                                                      \
+        if (a.mask != nullptr && a.N > COUNTED_BYTES * THREADS)                                                                     \
+            hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(PL_THREADS), 0, stream, a);                                       \
+        hipLaunchKernelGGL((policy_rows_kernel<IO, THREADS, CH, GROUPS>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a);     \
+    } while (0)
     if (a.N > 0) {
-        hipLaunchKernelGGL(policy_rows_kernel<IO>, dim3((unsigned)a.N), dim3(PL_THREADS), 0, stream, a, inverse);
-        if ((rc = check_hip(hipGetLastError(), "policy_rows_kernel launch"))) return rc;
+        const int64_t vectors = a.V / VEC;
+        // A short row leaves most of a large workgroup idle in its exchange, a long one needs the registers of many threads; in between,
+        // several rows on a CU hide each other's loads and stores.  bfloat16, TB/s of logits and gradient (a copy of this size: 5.2):
+        //   16384 x 1000   one wave 2.10, 256 threads 1.49             16384 x 3500   one wave 3.60, 256 threads 3.41, 1024 threads 2
+        //   16384 x 12001  256 threads 4.62, 512 4.13, 1024 3.21       8192 x 32000   2 x 512 threads 5.09, 1024 threads 4.59
+        //   8192 x 50257   1024 threads 5.23, 2 x 512 4.95, 2 x 1024 (64 registers) 4.59, row read twice 3.26
+        if (vectors <= 2 * 64) POLICY_ROWS(64, 2, 32);
+        else if (vectors <= 7 * 64) POLICY_ROWS(64, 7, 16);
+        else if (vectors <= 4 * 256) POLICY_ROWS(256, 4, 8);
+        else if (vectors <= 7 * 256) POLICY_ROWS(256, 7, 6);
+        else if (vectors <= 8 * 512) POLICY_ROWS(512, 8, 3);
+        else if (vectors <= 11 * 512) POLICY_ROWS(512, 11, 2);
+        else if (vectors <= 8 * 1024) POLICY_ROWS(1024, 8, 1);
+        else if (vectors <= 16 * 1024) POLICY_ROWS(1024, 16, 1);
+        else POLICY_ROWS(1024, 0, 2);
+        const int rc = check_hip(hipGetLastError(), "policy_rows_kernel launch");
+        if (rc) return rc;
     }
-    hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(PL_THREADS), 0, stream, a.each, a.N, a.loss);
+#undef POLICY_ROWS
+    hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(PS_THREADS), 0, stream, a.sums, groups, a.loss);
     return check_hip(hipGetLastError(), "policy_sum_kernel launch");
 }
 
 template <typename IO> int backward_of(const PolicyLossArgs &a, hipStream_t stream) {
     if (a.N == 0) return T2FW_OK;
-    hipLaunchKernelGGL(policy_gradient_kernel<IO>, dim3((unsigned)a.N), dim3(PL_THREADS), 0, stream, a);
+    hipLaunchKernelGGL(policy_gradient_kernel<IO>, dim3((unsigned)groups_of(a.N, 512)), dim3(PL_THREADS), 0, stream, a);
     return check_hip(hipGetLastError(), "policy_gradient_kernel launch");
 }
 

@@ -5,13 +5,16 @@
 
 namespace t2fw {
 
+constexpr int POLICY_SUMS = 8192;               // workgroups of a launch, at most
+
 struct PolicyLossArgs {
     const void *logits;                          // [N, V]
     const int64_t *targets;                      // [N]
     const float *old_logp, *ref_logp, *adv;      // [N]
     const uint8_t *mask;                         // [N], or null: every token counts
     float *loss, *logp, *lse, *coef;             // [1]; [N] each: what the backward needs are the last two
-    float *each;                                 // [N] scratch: the tokens' shares of the loss
+    int64_t *tokens;                             // [1] scratch: the tokens that count
+    double *sums;                                // [POLICY_SUMS] scratch: the workgroups' shares of the loss
     void *d_logits;                              // [N, V], or null: no gradient now
     const float *g_loss;                         // backward: the gradient of the loss, one value on the device
     int64_t N, V;

@@ -25,4 +25,23 @@ __device__ __forceinline__ float widen(_Float16 v) { return (float)v; }
 __device__ __forceinline__ float widen(__bf16 v) { return (float)v; }
 template <typename IO, typename Acc> __device__ __forceinline__ IO narrow(Acc v) { return (IO)v; }
 
+// 16 bytes of elements as they came, for what is held long and used several times: as elements of their own, 16-bit ones would take a
+// register each.
+struct Raw16 {
+    uint32_t w[4];
+};
+__device__ __forceinline__ Raw16 load_raw(const void *p) {
+    Raw16 r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <typename IO> __device__ __forceinline__ float element(const Raw16 &r, int j);
+template <> __device__ __forceinline__ float element<float>(const Raw16 &r, int j) { return __uint_as_float(r.w[j]); }
+template <> __device__ __forceinline__ float element<__bf16>(const Raw16 &r, int j) {
+    return __uint_as_float(j % 2 ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
+}
+template <> __device__ __forceinline__ float element<_Float16>(const Raw16 &r, int j) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(j % 2 ? r.w[j / 2] >> 16 : r.w[j / 2]));
+}
+
 }  // namespace t2fw
