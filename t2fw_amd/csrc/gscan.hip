@@ -8,6 +8,14 @@
 // in registers; a workgroup of 256 threads owns CL slots and TG = 256 / CL such stretches in a row, a chunk of
 // C = TG R steps.  Slots are numbered over all rows of the batch, so that narrow rows share a workgroup.  Where the width is no
 // multiple of the vector, a row's last slot starts early and does channels of its neighbour again, to the same bits.
+//
+// Every element is read once: a workgroup makes the map of its chunk, hands it to the chunks after it, and waits for theirs before it.
+// A map travels as one 64-bit word (P, S), written and read atomically at the device's scope, in a place that a launch before has filled with a
+// pattern that no map has; so the word says by itself whether it is there.  Chunks come in groups: the last one of a group
+// also hands on the map of the whole group, and a chunk needs the groups before its own and the chunks before it in its
+// group, about 2 sqrt(chunks) words.  They are composed in a fixed order, so the result does not depend on who is first.
+// Workgroups take their chunk by a ticket: whatever a chunk waits for has been taken by a workgroup that runs already and itself
+// waits for earlier ones only, so every wait ends, in whatever order the hardware starts workgroups.
 #include "gscan.hpp"
 #include "vec.hpp"
 
@@ -47,6 +55,13 @@ template <typename IO> __device__ __forceinline__ double gate_slope(double z) {
     return e * r * r;
 }
 
+// How a call is cut: slots of a row, workgroups side by side, chunks of the sequence, columns of one chunk in the scratch, chunks of a
+// group
+struct GscanGrid {
+    int64_t per_row, blocks, chunks, slots, group;
+};
+constexpr int GS_TICKET = 256;           // bytes before the words
+
 __device__ __forceinline__ int64_t row_length(const GscanArgs &a, int64_t b) {
     if (a.lengths == nullptr) return a.T;
     const int64_t n = a.wide_lengths ? static_cast<const int64_t *>(a.lengths)[b] : static_cast<const int32_t *>(a.lengths)[b];
@@ -62,15 +77,15 @@ template <int VEC, int R> struct Place {
     bool mine;
 };
 template <int VEC, int R>
-__device__ __forceinline__ Place<VEC, R> place_of(const GscanArgs &a, int64_t per_row, int64_t block, int64_t chunk) {
+__device__ __forceinline__ Place<VEC, R> place_of(const GscanArgs &a, const GscanGrid &gr, int64_t block, int64_t chunk) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
     Place<VEC, R> p;
     p.lane = threadIdx.x % CL;
     p.group = threadIdx.x / CL;
     p.slot = block * CL + p.lane;
-    p.mine = p.slot < a.B * per_row;
-    p.b = p.mine ? p.slot / per_row : 0;
-    const int64_t d = (p.slot - p.b * per_row) * VEC;
+    p.mine = p.slot < a.B * gr.per_row;
+    p.b = p.mine ? p.slot / gr.per_row : 0;
+    const int64_t d = (p.slot - p.b * gr.per_row) * VEC;
     p.d = d + VEC <= a.D ? d : a.D - VEC;
     p.t0 = chunk * (TG * R) + (int64_t)p.group * R;
     const int64_t left = p.mine ? a.T - p.t0 : 0, live = p.mine ? row_length(a, p.b) - p.t0 : 0;
@@ -79,210 +94,331 @@ __device__ __forceinline__ Place<VEC, R> place_of(const GscanArgs &a, int64_t pe
     return p;
 }
 
+// A lane's vectors.  16-bit ones are held as they come, two to a register, and put together two at a time.
+template <typename IO, int VEC> struct Held {
+    static constexpr int PAIR = 1;
+    Vec<IO, VEC> d;
+    __device__ __forceinline__ void load(const IO *p) { d = load_vec<IO, VEC>(p); }
+    __device__ __forceinline__ void store(IO *p) const { store_vec(p, d); }
+    __device__ __forceinline__ auto get(int v) const { return widen(d.e[v]); }
+    template <typename Acc> __device__ __forceinline__ void put(int v, const Acc (&x)[1]) { d.e[v] = narrow<IO>(x[0]); }
+};
+template <typename IO> struct Held16 {
+    static constexpr int PAIR = 2;
+    Raw16 d;
+    __device__ __forceinline__ void load(const IO *p) { d = load_raw(p); }
+    __device__ __forceinline__ void store(IO *p) const { __builtin_memcpy(p, &d, sizeof(d)); }
+    __device__ __forceinline__ float get(int v) const { return element<IO>(d, v); }
+    __device__ __forceinline__ void put(int v, const float (&x)[2]) {
+        const IO two[2] = {narrow<IO>(x[0]), narrow<IO>(x[1])};
+        __builtin_memcpy(&d.w[v / 2], two, 4);
+    }
+};
+template <> struct Held<_Float16, 8> : Held16<_Float16> {};
+template <> struct Held<__bf16, 8> : Held16<__bf16> {};
+
 template <typename IO, int VEC, int R>
-__device__ __forceinline__ void load_steps(Vec<IO, VEC> (&v)[R], const void *base, int64_t row, int64_t step, const Place<VEC, R> &p) {
+__device__ __forceinline__ void load_steps(Held<IO, VEC> (&v)[R], const void *base, int64_t row, int64_t step, const Place<VEC, R> &p) {
     const IO *at = static_cast<const IO *>(base) + p.b * row + p.t0 * step + p.d;
 #pragma unroll
     for (int r = 0; r < R; ++r)
-        if (r < p.live) v[r] = load_vec<IO, VEC>(at + r * step);
+        if (r < p.live) v[r].load(at + r * step);
+}
+template <typename IO, int VEC, int R>
+__device__ __forceinline__ void store_steps(void *base, const Held<IO, VEC> (&v)[R], int64_t D, int64_t T, const Place<VEC, R> &p) {
+    IO *at = static_cast<IO *>(base) + (p.b * T + p.t0) * D + p.d;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (r < p.steps) v[r].store(at + r * D);
 }
 
 // What a step beyond the row's length holds does not count, whatever it is: gate one, input nothing
-template <typename IO, typename Acc, int VEC, int R>
-__device__ __forceinline__ void gates_of(Acc (&g)[R][VEC], const Vec<IO, VEC> (&f)[R], const Place<VEC, R> &p, int logits) {
+template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
+__device__ __forceinline__ void gates_of(Acc (&g)[R][VEC], const Held<IO, VEC> (&f)[R], const Place<VEC, R> &p) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const Acc z = widen(f[r].e[v]);
-            g[r][v] = r < p.live ? (logits ? gate_of<IO>(z) : z) : (Acc)1;
+            const Acc z = f[r].get(v);
+            g[r][v] = r < p.live ? (LOGITS ? gate_of<IO>(z) : z) : (Acc)1;
         }
 }
 template <typename IO, typename Acc, int VEC, int R>
-__device__ __forceinline__ Acc value_of(const Vec<IO, VEC> (&x)[R], int r, int v, const Place<VEC, R> &p) {
-    return r < p.live ? (Acc)widen(x[r].e[v]) : (Acc)0;
+__device__ __forceinline__ Acc value_of(const Held<IO, VEC> (&x)[R], int r, int v, const Place<VEC, R> &p) {
+    return r < p.live ? (Acc)x[r].get(v) : (Acc)0;
 }
 
-// The map of every channel over a stretch, forward in time, or of its adjoint, backward
+// The map of a channel over a stretch, forward in time, or of its adjoint, backward
 template <typename IO, typename Acc, int VEC, int R, bool BACK>
-__device__ __forceinline__ void fold_steps(Map<Acc> (&m)[VEC], const Acc (&g)[R][VEC], const Vec<IO, VEC> (&x)[R], const Place<VEC, R> &p) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        Acc pr = 1, s = 0;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int r = BACK ? R - 1 - i : i;
-            const Acc in = value_of<IO, Acc, VEC, R>(x, r, v, p);
-            s = BACK ? g[r][v] * (s + in) : g[r][v] * s + in;
-            pr *= g[r][v];
-        }
-        m[v].p = pr;
-        m[v].s = s;
-    }
-}
-
-// The map of a whole chunk, for what comes after it in the direction of the recurrence
-template <typename IO, typename Acc, int VEC, int R, bool BACK>
-__global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, int64_t per_row, int64_t blocks, int64_t slots) {
-    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
-    __shared__ Map<Acc> maps[TG][GS_CHANNELS];
-    const int64_t block = blockIdx.x % blocks, chunk = blockIdx.x / blocks + (BACK ? 1 : 0);
-    const Place<VEC, R> p = place_of<VEC, R>(a, per_row, block, chunk);
-    Vec<IO, VEC> x[R], f[R];
-    load_steps(f, a.f, a.f_b, a.f_t, p);
-    load_steps(x, BACK ? a.g_out : a.x, BACK ? a.g_b : a.x_b, BACK ? a.g_t : a.x_t, p);
-    Acc g[R][VEC];
-    gates_of<IO, Acc, VEC, R>(g, f, p, a.logits);
-    Map<Acc> m[VEC];
-    fold_steps<IO, Acc, VEC, R, BACK>(m, g, x, p);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = m[v];
-    __syncthreads();
-    if (threadIdx.x >= GS_CHANNELS) return;
+__device__ __forceinline__ Map<Acc> fold_steps(const Acc (&g)[R][VEC], const Held<IO, VEC> (&x)[R], int v, const Place<VEC, R> &p) {
     Acc pr = 1, s = 0;
 #pragma unroll
-    for (int i = 0; i < TG; ++i) {
-        const Map<Acc> m2 = maps[BACK ? TG - 1 - i : i][threadIdx.x];
-        s = m2.p * s + m2.s;
-        pr *= m2.p;
+    for (int i = 0; i < R; ++i) {
+        const int r = BACK ? R - 1 - i : i;
+        const Acc in = value_of<IO, Acc, VEC, R>(x, r, v, p);
+        s = BACK ? g[r][v] * (s + in) : g[r][v] * s + in;
+        pr *= g[r][v];
     }
-    static_cast<Map<Acc> *>(a.words)[chunk * slots + block * GS_CHANNELS + threadIdx.x] = Map<Acc>{pr, s};
+    return {pr, s};
 }
 
 // The channel of a workgroup's thread in [B, D] arrays; whether it is there
-template <int VEC> __device__ __forceinline__ bool channel_of(const GscanArgs &a, int64_t per_row, int64_t block, int64_t *at) {
-    const int64_t slot = block * (GS_CHANNELS / VEC) + threadIdx.x / VEC, b = slot / per_row, d = (slot - b * per_row) * VEC;
-    *at = b * a.D + (d + VEC <= a.D ? d : a.D - VEC) + threadIdx.x % VEC;
-    return slot < a.B * per_row;
+template <int VEC> __device__ __forceinline__ bool channel_of(const GscanArgs &a, const GscanGrid &gr, int64_t block, int thread, int64_t *at) {
+    const int64_t slot = block * (GS_CHANNELS / VEC) + thread / VEC, b = slot / gr.per_row, d = (slot - b * gr.per_row) * VEC;
+    *at = b * a.D + (d + VEC <= a.D ? d : a.D - VEC) + thread % VEC;
+    return slot < a.B * gr.per_row;
 }
 
-template <typename IO, typename Acc, int VEC, int R>
-__global__ __launch_bounds__(GS_THREADS) void gscan_forward_kernel(GscanArgs a, int64_t per_row, int64_t blocks, int64_t chunks, int64_t slots) {
+// ---- maps from chunk to chunk --------------------------------------------------------------------------------------
+constexpr uint64_t EMPTY = ~0ull;                        // a NaN of a pattern that hand_on() gives to nothing
+
+__device__ __forceinline__ void hand_on(uint64_t *word, const Map<float> &m) {
+    uint64_t w = (uint64_t)__float_as_uint(m.s) << 32 | __float_as_uint(m.p);
+    if (w == EMPTY) w = 0x7fc000007fc00000ull;           // another NaN
+    __hip_atomic_store(word, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t look(const uint64_t *word) { return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The maps lo, lo + 1, .. hi - 1 after one another, each waited for
+__device__ __forceinline__ Map<float> wait_for(const uint64_t *words, int64_t lo, int64_t hi, int64_t slots) {
+    constexpr int AHEAD = 8;
+    Map<float> all{1.0f, 0.0f};
+    for (int64_t j = lo; j < hi; j += AHEAD) {
+        uint64_t w[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) w[u] = j + u < hi ? look(words + (j + u) * slots) : 0x000000003f800000ull;      // the map that changes nothing
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            while (w[u] == EMPTY) {
+                __builtin_amdgcn_s_sleep(1);
+                w[u] = look(words + (j + u) * slots);
+            }
+            const float p = __uint_as_float((uint32_t)w[u]), s = __uint_as_float((uint32_t)(w[u] >> 32));
+            all.s = p * all.s + s;
+            all.p *= p;
+        }
+    }
+    return all;
+}
+
+// A chunk's number in the direction of the recurrence, from the ticket (float) or the workgroup's own number (double)
+template <typename Acc> __device__ __forceinline__ int64_t take_chunk(const GscanArgs &a, const GscanGrid &gr) {
+    if (sizeof(Acc) == 8 || gr.chunks == 1) return blockIdx.x;
+    __shared__ uint32_t mine;
+    if (threadIdx.x == 0) mine = __hip_atomic_fetch_add(static_cast<uint32_t *>(a.words), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return mine;
+}
+
+// The recurrence's value before a chunk, in the threads of the first wave: `own` is the chunk's map there, `first` the value before the
+// sequence; all threads of the workgroup call it.
+__device__ __forceinline__ float value_before(const GscanArgs &a, const GscanGrid &gr, int64_t block, int64_t chunk, const Map<float> &own, float first) {
+    if (gr.chunks == 1) return first;
+    __shared__ Map<float> parts[GS_THREADS / 64][GS_CHANNELS];
+    uint64_t *const words = reinterpret_cast<uint64_t *>(static_cast<char *>(a.words) + GS_TICKET) + block * GS_CHANNELS + threadIdx.x % 64;
+    uint64_t *const groups = words + gr.chunks * gr.slots;
+    const int wave = threadIdx.x / 64;
+    if (wave == 0 && chunk < gr.chunks - 1) hand_on(words + chunk * gr.slots, own);
+    // two waves for the groups before this chunk's, two for the chunks before it in its group
+    const int64_t group = chunk / gr.group, start = group * gr.group;
+    const int64_t lo = wave < 2 ? 0 : start, hi = wave < 2 ? group : chunk, half = (lo + hi) / 2;
+    parts[wave][threadIdx.x % 64] = wait_for(wave < 2 ? groups : words, wave % 2 ? half : lo, wave % 2 ? hi : half, gr.slots);
+    __syncthreads();
+    if (wave != 0) return 0.0f;
+    const Map<float> m0 = parts[0][threadIdx.x], m1 = parts[1][threadIdx.x], m2 = parts[2][threadIdx.x], m3 = parts[3][threadIdx.x];
+    if (chunk % gr.group == gr.group - 1 && chunk < gr.chunks - 1) {
+        const float p = m3.p * m2.p, s = m3.p * m2.s + m3.s;
+        hand_on(groups + group * gr.slots, {own.p * p, own.p * s + own.s});
+    }
+    float h = m0.p * first + m0.s;
+    h = m1.p * h + m1.s;
+    h = m2.p * h + m2.s;
+    return m3.p * h + m3.s;
+}
+// double: every map is there from the launch before
+__device__ __forceinline__ double value_before(const GscanArgs &a, const GscanGrid &gr, int64_t block, int64_t chunk, const Map<double> &, double first) {
+    if (threadIdx.x >= GS_CHANNELS) return 0.0;
+    const Map<double> *w = static_cast<const Map<double> *>(a.words) + block * GS_CHANNELS + threadIdx.x;
+    for (int64_t c = 0; c < chunk; ++c) first = w[c * gr.slots].p * first + w[c * gr.slots].s;
+    return first;
+}
+
+// Before a call's main launch: the words empty, the ticket zero
+__global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(void *words, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * GS_THREADS + threadIdx.x;
+    if (i == 0) *static_cast<uint32_t *>(words) = 0;
+    if (i < n) reinterpret_cast<uint64_t *>(static_cast<char *>(words) + GS_TICKET)[i] = EMPTY;
+}
+
+// double: the map of every chunk but the last, for what comes after it in the direction of the recurrence
+template <typename IO, typename Acc, int VEC, int R, bool BACK, bool LOGITS>
+__global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];
-    const int64_t block = blockIdx.x % blocks, chunk = blockIdx.x / blocks;
-    const Place<VEC, R> p = place_of<VEC, R>(a, per_row, block, chunk);
-    Vec<IO, VEC> x[R], f[R];
-    load_steps(f, a.f, a.f_b, a.f_t, p);
-    load_steps(x, a.x, a.x_b, a.x_t, p);
+    const int64_t block = blockIdx.x % gr.blocks, chunk = blockIdx.x / gr.blocks;
+    const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, BACK ? gr.chunks - 1 - chunk : chunk);
+    Held<IO, VEC> x[R], f[R];
+    load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
+    load_steps<IO, VEC, R>(x, BACK ? a.g_out : a.x, BACK ? a.g_b : a.x_b, BACK ? a.g_t : a.x_t, p);
     Acc g[R][VEC];
-    gates_of<IO, Acc, VEC, R>(g, f, p, a.logits);
-    {
-        Map<Acc> m[VEC];
-        fold_steps<IO, Acc, VEC, R, false>(m, g, x, p);
+    gates_of<IO, Acc, VEC, R, LOGITS>(g, f, p);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = m[v];
-    }
+    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, BACK>(g, x, v, p);
     __syncthreads();
-    if (threadIdx.x < GS_CHANNELS) {
-        int64_t at;
-        const bool there = channel_of<VEC>(a, per_row, block, &at);
-        Acc h = there && a.s0 != nullptr ? static_cast<const Acc *>(a.s0)[at] : (Acc)0;
-        const int64_t column = block * GS_CHANNELS + threadIdx.x;
-        const Map<Acc> *w = static_cast<const Map<Acc> *>(a.words) + column;
-        for (int64_t c = 0; c < chunk; ++c) h = w[c * slots].p * h + w[c * slots].s;
-        if (a.ckpt != nullptr) static_cast<Acc *>(a.ckpt)[chunk * slots + column] = h;
+    if (threadIdx.x >= GS_CHANNELS) return;
+    Map<Acc> all{1, 0};
 #pragma unroll
-        for (int i = 0; i < TG; ++i) {
-            const Map<Acc> m2 = maps[i][threadIdx.x];
-            maps[i][threadIdx.x].s = h;                  // the state before this stretch
-            h = m2.p * h + m2.s;
-        }
-        if (there && chunk == chunks - 1) static_cast<Acc *>(a.final_state)[at] = h;
+    for (int i = 0; i < TG; ++i) {
+        const Map<Acc> m = maps[BACK ? TG - 1 - i : i][threadIdx.x];
+        all.s = m.p * all.s + m.s;
+        all.p *= m.p;
     }
-    __syncthreads();
-    Vec<IO, VEC> o[R];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        Acc h = maps[p.group][p.lane * VEC + v].s;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            h = g[r][v] * h + value_of<IO, Acc, VEC, R>(x, r, v, p);
-            o[r].e[v] = r < p.live ? narrow<IO>(h) : narrow<IO>((Acc)0);
-        }
-    }
-    IO *at = static_cast<IO *>(a.out) + (p.b * a.T + p.t0) * a.D + p.d;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-        if (r < p.steps) store_vec(at + r * a.D, o[r]);
+    static_cast<Map<Acc> *>(a.words)[chunk * gr.slots + block * GS_CHANNELS + threadIdx.x] = all;
 }
 
-template <typename IO, typename Acc, int VEC, int R>
-__global__ __launch_bounds__(GS_THREADS) void gscan_backward_kernel(GscanArgs a, int64_t per_row, int64_t blocks, int64_t chunks, int64_t slots) {
-    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
-    __shared__ Map<Acc> maps[TG][GS_CHANNELS];           // states: forward in time
-    __shared__ Acc sums[TG][GS_CHANNELS];                // adjoints: backward, with the same gate products
-    const int64_t block = blockIdx.x % blocks, chunk = chunks - 1 - blockIdx.x / blocks;
-    const Place<VEC, R> p = place_of<VEC, R>(a, per_row, block, chunk);
-    Vec<IO, VEC> x[R], f[R], go[R];
-    load_steps(f, a.f, a.f_b, a.f_t, p);
-    load_steps(go, a.g_out, a.g_b, a.g_t, p);
-    load_steps(x, a.x, a.x_b, a.x_t, p);
+template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
+__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_forward_kernel(GscanArgs a, GscanGrid gr) {
+    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
+    __shared__ Map<Acc> maps[TG][GS_CHANNELS];
+    const int64_t at_grid = take_chunk<Acc>(a, gr), block = at_grid % gr.blocks, chunk = at_grid / gr.blocks;
+    const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
+    Held<IO, VEC> x[R];
     Acc g[R][VEC];
-    gates_of<IO, Acc, VEC, R>(g, f, p, a.logits);
     {
-        Map<Acc> m[VEC], n[VEC];
-        fold_steps<IO, Acc, VEC, R, true>(n, g, go, p);
-        fold_steps<IO, Acc, VEC, R, false>(m, g, x, p);
+        Held<IO, VEC> f[R];
+        load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
+        load_steps<IO, VEC, R>(x, a.x, a.x_b, a.x_t, p);
+        gates_of<IO, Acc, VEC, R, LOGITS>(g, f, p);
+    }
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            maps[p.group][p.lane * VEC + v] = m[v];
-            sums[p.group][p.lane * VEC + v] = n[v].s;
+    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v, p);
+    __syncthreads();
+    Map<Acc> own{1, 0};
+    Acc h = 0;
+    int64_t at = 0;
+    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
+    if (first) {
+#pragma unroll 8
+        for (int i = 0; i < TG; ++i) {
+            const Map<Acc> m = maps[i][threadIdx.x];
+            own.s = m.p * own.s + m.s;
+            own.p *= m.p;
         }
+        if (there && a.s0 != nullptr) h = static_cast<const Acc *>(a.s0)[at];
+    }
+    h = value_before(a, gr, block, chunk, own, h);
+    if (first) {
+        if (a.ckpt != nullptr) static_cast<Acc *>(a.ckpt)[chunk * gr.slots + block * GS_CHANNELS + threadIdx.x] = h;
+#pragma unroll 8
+        for (int i = 0; i < TG; ++i) {
+            const Map<Acc> m = maps[i][threadIdx.x];
+            maps[i][threadIdx.x].s = h;                  // the state before this stretch
+            h = m.p * h + m.s;
+        }
+        if (there && chunk == gr.chunks - 1) static_cast<Acc *>(a.final_state)[at] = h;
     }
     __syncthreads();
-    if (threadIdx.x < GS_CHANNELS) {
-        int64_t at;
-        const bool there = channel_of<VEC>(a, per_row, block, &at);
-        const int64_t column = block * GS_CHANNELS + threadIdx.x;
-        Acc e = there && a.g_state != nullptr ? static_cast<const Acc *>(a.g_state)[at] : (Acc)0;
-        const Map<Acc> *w = static_cast<const Map<Acc> *>(a.words) + column;
-        for (int64_t c = chunks - 1; c > chunk; --c) e = w[c * slots].p * e + w[c * slots].s;
-        Acc h = static_cast<const Acc *>(a.ckpt)[chunk * slots + column];
-        Acc pr[TG];
+    Held<IO, VEC> o[R];
 #pragma unroll
-        for (int i = 0; i < TG; ++i) {
-            const Map<Acc> m2 = maps[i][threadIdx.x];
-            maps[i][threadIdx.x].s = h;
-            pr[i] = m2.p;
-            h = m2.p * h + m2.s;
+    for (int v = 0; v < VEC; v += PAIR) {
+        Acc s[PAIR];
+#pragma unroll
+        for (int j = 0; j < PAIR; ++j) s[j] = maps[p.group][p.lane * VEC + v + j].s;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            Acc out[PAIR];
+#pragma unroll
+            for (int j = 0; j < PAIR; ++j) {
+                s[j] = g[r][v + j] * s[j] + value_of<IO, Acc, VEC, R>(x, r, v + j, p);
+                out[j] = r < p.live ? s[j] : (Acc)0;
+            }
+            o[r].put(v, out);
         }
+    }
+    store_steps<IO, VEC, R>(a.out, o, a.D, a.T, p);
+}
+
+template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
+__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 3) void gscan_backward_kernel(GscanArgs a, GscanGrid gr) {
+    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
+    __shared__ Map<Acc> maps[TG][GS_CHANNELS];           // states: forward in time
+    __shared__ Acc sums[TG][GS_CHANNELS];                // adjoints: backward, with the same gate products
+    const int64_t at_grid = take_chunk<Acc>(a, gr), block = at_grid % gr.blocks, from_end = at_grid / gr.blocks, chunk = gr.chunks - 1 - from_end;
+    const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
+    Held<IO, VEC> x[R], f[R], go[R];
+    load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
+    load_steps<IO, VEC, R>(go, a.g_out, a.g_b, a.g_t, p);
+    load_steps<IO, VEC, R>(x, a.x, a.x_b, a.x_t, p);
+    Acc g[R][VEC];
+    gates_of<IO, Acc, VEC, R, LOGITS>(g, f, p);
 #pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v, p);
+        sums[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, true>(g, go, v, p).s;
+    }
+    __syncthreads();
+    Map<Acc> own{1, 0};
+    Acc e = 0;
+    int64_t at = 0;
+    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
+    if (first) {
+#pragma unroll 8
         for (int i = TG - 1; i >= 0; --i) {
-            const Acc s = sums[i][threadIdx.x];
-            sums[i][threadIdx.x] = e;                    // the adjoint after this stretch
-            e = pr[i] * e + s;
+            const Acc pr = maps[i][threadIdx.x].p;
+            own.s = pr * own.s + sums[i][threadIdx.x];
+            own.p *= pr;
+        }
+        if (there && a.g_state != nullptr) e = static_cast<const Acc *>(a.g_state)[at];
+    }
+    e = value_before(a, gr, block, from_end, own, e);
+    if (first) {
+        Acc h = static_cast<const Acc *>(a.ckpt)[chunk * gr.slots + block * GS_CHANNELS + threadIdx.x];
+#pragma unroll 8
+        for (int i = 0; i < TG; ++i) {
+            const Map<Acc> m = maps[i][threadIdx.x];
+            maps[i][threadIdx.x].s = h;                  // the state before this stretch
+            h = m.p * h + m.s;
+        }
+#pragma unroll 8
+        for (int i = TG - 1; i >= 0; --i) {
+            const Acc pr = maps[i][threadIdx.x].p, s = sums[i][threadIdx.x];
+            sums[i][threadIdx.x] = e;                    // the adjoint after it
+            e = pr * e + s;
         }
         if (there && chunk == 0 && a.d_s0 != nullptr) static_cast<Acc *>(a.d_s0)[at] = e;
     }
     __syncthreads();
-    Vec<IO, VEC> dx[R], df[R];
+    // the results take their inputs' registers
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        Acc h = maps[p.group][p.lane * VEC + v].s, before[R];
+    for (int v = 0; v < VEC; v += PAIR) {
+        Acc before[R][PAIR], after[PAIR];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            before[r] = h;
-            h = g[r][v] * h + value_of<IO, Acc, VEC, R>(x, r, v, p);
+        for (int j = 0; j < PAIR; ++j) {
+            Acc h = maps[p.group][p.lane * VEC + v + j].s;
+            after[j] = sums[p.group][p.lane * VEC + v + j];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                before[r][j] = h;
+                h = g[r][v + j] * h + value_of<IO, Acc, VEC, R>(x, r, v + j, p);
+            }
         }
-        Acc e = sums[p.group][p.lane * VEC + v];
 #pragma unroll
         for (int r = R - 1; r >= 0; --r) {
-            const Acc d = value_of<IO, Acc, VEC, R>(go, r, v, p) + e;
-            e = g[r][v] * d;
-            Acc slope = d * before[r];
-            if (a.logits) slope *= gate_slope<IO>((Acc)widen(f[r].e[v]));
-            dx[r].e[v] = narrow<IO>(r < p.live ? d : (Acc)0);
-            df[r].e[v] = narrow<IO>(r < p.live ? slope : (Acc)0);
+            Acc dx[PAIR], df[PAIR];
+#pragma unroll
+            for (int j = 0; j < PAIR; ++j) {
+                const Acc d = value_of<IO, Acc, VEC, R>(go, r, v + j, p) + after[j];
+                after[j] = g[r][v + j] * d;
+                const Acc slope = LOGITS ? (Acc)gate_slope<IO>((Acc)f[r].get(v + j)) : (Acc)1;
+                dx[j] = r < p.live ? d : (Acc)0;
+                df[j] = r < p.live ? d * before[r][j] * slope : (Acc)0;
+            }
+            go[r].put(v, dx);
+            x[r].put(v, df);
         }
     }
-    const int64_t at = (p.b * a.T + p.t0) * a.D + p.d;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-        if (r < p.steps) {
-            store_vec(static_cast<IO *>(a.d_x) + at + r * a.D, dx[r]);
-            store_vec(static_cast<IO *>(a.d_f) + at + r * a.D, df[r]);
-        }
+    store_steps<IO, VEC, R>(a.d_x, go, a.D, a.T, p);
+    store_steps<IO, VEC, R>(a.d_f, x, a.D, a.T, p);
 }
 
 // One token: x, f, out [B, D], the state in place or not
@@ -315,57 +451,73 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_step_kernel(GscanArgs a, int
     }
 }
 
-template <typename IO, int VEC, int R> int64_t slots_per_row(int64_t D) { return (D + VEC - 1) / VEC; }
+template <typename IO, int VEC, int R> GscanGrid grid_of(int64_t B, int64_t T, int64_t D) {
+    constexpr int CL = GS_CHANNELS / VEC, C = GS_THREADS / CL * R;
+    GscanGrid g;
+    g.per_row = (D + VEC - 1) / VEC;
+    g.blocks = (B * g.per_row + CL - 1) / CL;
+    g.chunks = T <= 0 ? 1 : (T + C - 1) / C;
+    g.slots = g.blocks * GS_CHANNELS;
+    for (g.group = 8; g.group * g.group < g.chunks;) g.group *= 2;
+    return g;
+}
+int64_t words_of(const GscanGrid &g) { return (g.chunks + (g.chunks + g.group - 1) / g.group) * g.slots; }
 
 template <typename IO, int VEC, int R> GscanPlan plan_of(int64_t B, int64_t T, int64_t D) {
-    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
+    const GscanGrid g = grid_of<IO, VEC, R>(B, T, D);
+    const size_t acc = sizeof(typename AccT<IO>::type);
     GscanPlan p;
-    p.chunk = TG * R;
-    p.chunks = T <= 0 ? 1 : (T + p.chunk - 1) / p.chunk;
-    p.slots = (B * slots_per_row<IO, VEC, R>(D) + CL - 1) / CL * GS_CHANNELS;
-    p.acc = sizeof(typename AccT<IO>::type);
+    p.checkpoints = (size_t)(g.chunks * g.slots) * acc;
+    p.workspace = g.chunks == 1 ? 0 : acc == 8 ? (size_t)(g.chunks * g.slots) * 2 * acc : GS_TICKET + (size_t)words_of(g) * sizeof(uint64_t);
     return p;
 }
 
-int too_large() { return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many workgroups for one launch"); }
-
-template <typename IO, int VEC, int R> int forward_of(const GscanArgs &a, hipStream_t stream) {
+// What comes before a call's main launch
+template <typename IO, int VEC, int R, bool BACK, bool LOGITS> int prepare(const GscanArgs &a, const GscanGrid &g, hipStream_t stream) {
     using Acc = typename AccT<IO>::type;
-    const GscanPlan p = plan_of<IO, VEC, R>(a.B, a.T, a.D);
-    const int64_t per_row = slots_per_row<IO, VEC, R>(a.D), blocks = p.slots / GS_CHANNELS;
-    if (blocks > 0x7fffffff / p.chunks) return too_large();
-    if (p.chunks > 1) {
-        hipLaunchKernelGGL((gscan_maps_kernel<IO, Acc, VEC, R, false>), dim3((unsigned)(blocks * (p.chunks - 1))), dim3(GS_THREADS), 0, stream, a,
-                           per_row, blocks, p.slots);
-        const int rc = check_hip(hipGetLastError(), "gscan_maps_kernel launch");
-        if (rc) return rc;
+    if (g.blocks > 0x7fffffff / g.chunks || g.slots > 0x7fffffff * (int64_t)GS_THREADS / (2 * g.chunks))
+        return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many workgroups for one launch");
+    if (g.chunks == 1) return T2FW_OK;
+    if constexpr (sizeof(Acc) == 8) {
+        hipLaunchKernelGGL((gscan_maps_kernel<IO, Acc, VEC, R, BACK, LOGITS>), dim3((unsigned)(g.blocks * (g.chunks - 1))), dim3(GS_THREADS), 0,
+                           stream, a, g);
+        return check_hip(hipGetLastError(), "gscan_maps_kernel launch");
+    } else {
+        const int64_t n = words_of(g);
+        hipLaunchKernelGGL(gscan_empty_kernel, dim3((unsigned)((n + GS_THREADS - 1) / GS_THREADS)), dim3(GS_THREADS), 0, stream, a.words, n);
+        return check_hip(hipGetLastError(), "gscan_empty_kernel launch");
     }
-    hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R>), dim3((unsigned)(blocks * p.chunks)), dim3(GS_THREADS), 0, stream, a, per_row,
-                       blocks, p.chunks, p.slots);
-    return check_hip(hipGetLastError(), "gscan_forward_kernel launch");
 }
 
-template <typename IO, int VEC, int R> int backward_of(const GscanArgs &a, hipStream_t stream) {
+template <typename IO, int VEC, int R, bool LOGITS> int forward_with(const GscanArgs &a, hipStream_t stream) {
     using Acc = typename AccT<IO>::type;
-    const GscanPlan p = plan_of<IO, VEC, R>(a.B, a.T, a.D);
-    const int64_t per_row = slots_per_row<IO, VEC, R>(a.D), blocks = p.slots / GS_CHANNELS;
-    if (blocks > 0x7fffffff / p.chunks) return too_large();
-    if (p.chunks > 1) {
-        hipLaunchKernelGGL((gscan_maps_kernel<IO, Acc, VEC, R, true>), dim3((unsigned)(blocks * (p.chunks - 1))), dim3(GS_THREADS), 0, stream, a,
-                           per_row, blocks, p.slots);
-        const int rc = check_hip(hipGetLastError(), "gscan_maps_kernel launch");
-        if (rc) return rc;
-    }
-    hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R>), dim3((unsigned)(blocks * p.chunks)), dim3(GS_THREADS), 0, stream, a, per_row,
-                       blocks, p.chunks, p.slots);
+    const GscanGrid g = grid_of<IO, VEC, R>(a.B, a.T, a.D);
+    const int rc = prepare<IO, VEC, R, false, LOGITS>(a, g, stream);
+    if (rc) return rc;
+    hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, LOGITS>), dim3((unsigned)(g.blocks * g.chunks)), dim3(GS_THREADS), 0, stream, a, g);
+    return check_hip(hipGetLastError(), "gscan_forward_kernel launch");
+}
+template <typename IO, int VEC, int R> int forward_of(const GscanArgs &a, hipStream_t stream) {
+    return a.logits ? forward_with<IO, VEC, R, true>(a, stream) : forward_with<IO, VEC, R, false>(a, stream);
+}
+
+template <typename IO, int VEC, int R, bool LOGITS> int backward_with(const GscanArgs &a, hipStream_t stream) {
+    using Acc = typename AccT<IO>::type;
+    const GscanGrid g = grid_of<IO, VEC, R>(a.B, a.T, a.D);
+    const int rc = prepare<IO, VEC, R, true, LOGITS>(a, g, stream);
+    if (rc) return rc;
+    hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, LOGITS>), dim3((unsigned)(g.blocks * g.chunks)), dim3(GS_THREADS), 0, stream, a, g);
     return check_hip(hipGetLastError(), "gscan_backward_kernel launch");
+}
+template <typename IO, int VEC, int R> int backward_of(const GscanArgs &a, hipStream_t stream) {
+    return a.logits ? backward_with<IO, VEC, R, true>(a, stream) : backward_with<IO, VEC, R, false>(a, stream);
 }
 
 template <typename IO> int step_of(const GscanArgs &a, hipStream_t stream) {
     using Acc = typename AccT<IO>::type;
     constexpr int VEC = 16 / sizeof(IO);
     const int64_t n = a.B * a.D, groups = (n + (int64_t)GS_THREADS * VEC - 1) / ((int64_t)GS_THREADS * VEC);
-    if (groups > 0x7fffffff) return too_large();
+    if (groups > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many channels for one launch");
     hipLaunchKernelGGL((gscan_step_kernel<IO, Acc, VEC>), dim3((unsigned)groups), dim3(GS_THREADS), 0, stream, a, n);
     return check_hip(hipGetLastError(), "gscan_step_kernel launch");
 }

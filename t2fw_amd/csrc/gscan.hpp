@@ -10,8 +10,8 @@ struct GscanArgs {
     const void *s0, *g_state;           // [B, D] in the accumulators' type
     void *out, *final_state;            // forward: h [B, T, D] dense, the last state [B, D]
     void *d_x, *d_f, *d_s0;             // backward: dense
-    void *ckpt;                         // state before every chunk, [chunks, slots] (gscan.hip), or null
-    void *words;                        // scratch: (gate product, sum) of every chunk, [chunks, slots]
+    void *ckpt;                         // state before every chunk (gscan.hip), or null
+    void *words;                        // scratch: the chunks' maps
     const void *lengths;                // [B] int32 / int64, or null: every row has T steps
     int64_t B, T, D;
     int64_t x_b, x_t, f_b, f_t, g_b, g_t;    // strides of batch rows and steps, in elements
@@ -19,9 +19,7 @@ struct GscanArgs {
 };
 
 struct GscanPlan {
-    int chunk;                          // steps of a chunk
-    int64_t chunks, slots;              // chunks of a row; channels with their padding, all rows together
-    size_t acc;                         // bytes of an accumulator
+    size_t checkpoints, workspace;      // bytes
 };
 
 GscanPlan gscan_plan(int64_t B, int64_t T, int64_t D, int dtype);

@@ -137,14 +137,12 @@ extern "C" {
 
 size_t t2fw_gated_scan_checkpoint_bytes(int64_t B, int64_t T, int64_t D, int32_t dtype) {
     if (check_scan(B, T, D, dtype, 0) || B == 0) return 0;
-    const GscanPlan p = gscan_plan(B, T, D, dtype);
-    return (size_t)(p.chunks * p.slots) * p.acc;
+    return gscan_plan(B, T, D, dtype).checkpoints;
 }
 
 size_t t2fw_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, int32_t dtype) {
     if (check_scan(B, T, D, dtype, 0) || B == 0) return 0;
-    const GscanPlan p = gscan_plan(B, T, D, dtype);
-    return p.chunks == 1 ? 0 : (size_t)(p.chunks * p.slots) * 2 * p.acc;
+    return gscan_plan(B, T, D, dtype).workspace;
 }
 
 int t2fw_gated_scan_forward(const void *x, const void *f, const void *s0, const void *lengths, void *out, void *final_state, void *ckpt,
