@@ -364,6 +364,8 @@ int t2fw_gate_backward(const void *d_f, const void *d_f_key, const void *f, cons
  */
 #define T2FW_SCAN_LOGITS 1
 #define T2FW_SCAN_LENGTHS64 2
+#define T2FW_SCAN_ALONE 4         /* no chunk of a sequence waits for another's result: what is not there is made again from the
+                                     inputs, as it is when a wait takes too long.  Same results, slower: for tests of that way. */
 size_t t2fw_gated_scan_checkpoint_bytes(int64_t B, int64_t T, int64_t D, int32_t dtype);
 size_t t2fw_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, int32_t dtype);
 int t2fw_gated_scan_forward(const void *x, const void *f, const void *s0, const void *lengths,

@@ -14,8 +14,9 @@
 // pattern that no map has; so the word says by itself whether it is there.  Chunks come in groups: the last one of a group
 // also hands on the map of the whole group, and a chunk needs the groups before its own and the chunks before it in its
 // group, about 2 sqrt(chunks) words.  They are composed in a fixed order, so the result does not depend on who is first.
-// Workgroups take their chunk by a ticket: whatever a chunk waits for has been taken by a workgroup that runs already and itself
-// waits for earlier ones only, so every wait ends, in whatever order the hardware starts workgroups.
+// Chunks are numbered so that what a chunk waits for comes earlier in the grid.  Should the hardware not have started that workgroup all the
+// same (another program on the device, say), a wait ends after a number of looks, and the workgroup makes the maps before its own
+// itself from the inputs, by the same operations in the same order: every wait is bounded, and none needs another workgroup to run.
 #include "gscan.hpp"
 #include "vec.hpp"
 
@@ -35,6 +36,19 @@ template <> struct AccT<double> { using type = double; };
 template <typename Acc> struct Map {
     Acc p, s;
 };
+
+__device__ __forceinline__ float fused(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return fma(a, b, c); }
+// m, and then n
+template <typename Acc> __device__ __forceinline__ Map<Acc> after(const Map<Acc> &n, const Map<Acc> &m) {
+    return {n.p * m.p, fused(n.p, m.s, n.s)};
+}
+// ... one step of gate g and input x more: h -> g h + x, or for the adjoint e -> g (e + x)
+// (the same operations wherever it stands: no product of one step fused into the next)
+template <bool BACK, typename Acc> __device__ __forceinline__ Map<Acc> extended(const Map<Acc> &m, Acc g, Acc x) {
+#pragma clang fp contract(off)
+    return {m.p * g, BACK ? g * (m.s + x) : fused(g, m.s, x)};
+}
 
 template <typename IO> __device__ __forceinline__ float gate_of(float z) {
     // 16-bit gates: hardware exponential and reciprocal (2^-21); 32-bit ones: the library's
@@ -58,9 +72,10 @@ template <typename IO> __device__ __forceinline__ double gate_slope(double z) {
 // How a call is cut: slots of a row, workgroups side by side, chunks of the sequence, columns of one chunk in the scratch, chunks of a
 // group
 struct GscanGrid {
-    int64_t per_row, blocks, chunks, slots, group;
+    uint32_t per_row, blocks, chunks, group;
+    int64_t slots;
+    bool fits;
 };
-constexpr int GS_TICKET = 256;           // bytes before the words
 
 __device__ __forceinline__ int64_t row_length(const GscanArgs &a, int64_t b) {
     if (a.lengths == nullptr) return a.T;
@@ -83,12 +98,12 @@ __device__ __forceinline__ Place<VEC, R> place_of(const GscanArgs &a, const Gsca
     p.lane = threadIdx.x % CL;
     p.group = threadIdx.x / CL;
     p.slot = block * CL + p.lane;
-    p.mine = p.slot < a.B * gr.per_row;
-    p.b = p.mine ? p.slot / gr.per_row : 0;
+    p.mine = p.slot < a.B * (int64_t)gr.per_row;
+    p.b = p.mine ? (uint32_t)p.slot / gr.per_row : 0;
     const int64_t d = (p.slot - p.b * gr.per_row) * VEC;
     p.d = d + VEC <= a.D ? d : a.D - VEC;
     p.t0 = chunk * (TG * R) + (int64_t)p.group * R;
-    const int64_t left = p.mine ? a.T - p.t0 : 0, live = p.mine ? row_length(a, p.b) - p.t0 : 0;
+    const int64_t length = row_length(a, p.b), left = p.mine ? a.T - p.t0 : 0, live = p.mine ? length - p.t0 : 0;
     p.steps = left < 0 ? 0 : left < R ? (int)left : R;
     p.live = live < 0 ? 0 : live < R ? (int)live : R;
     return p;
@@ -102,6 +117,10 @@ template <typename IO, int VEC> struct Held {
     __device__ __forceinline__ void store(IO *p) const { store_vec(p, d); }
     __device__ __forceinline__ auto get(int v) const { return widen(d.e[v]); }
     template <typename Acc> __device__ __forceinline__ void put(int v, const Acc (&x)[1]) { d.e[v] = narrow<IO>(x[0]); }
+    __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) d.e[v] = narrow<IO>(x);
+    }
 };
 template <typename IO> struct Held16 {
     static constexpr int PAIR = 2;
@@ -113,141 +132,202 @@ template <typename IO> struct Held16 {
         const IO two[2] = {narrow<IO>(x[0]), narrow<IO>(x[1])};
         __builtin_memcpy(&d.w[v / 2], two, 4);
     }
+    __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+        for (int v = 0; v < 8; v += 2) put(v, {x, x});
+    }
 };
 template <> struct Held<_Float16, 8> : Held16<_Float16> {};
 template <> struct Held<__bf16, 8> : Held16<__bf16> {};
 
+// Every load is made, whether its step counts or not (at a step that is there, or at the array's start), so that no branch stands between
+// them and all are under way at once.
 template <typename IO, int VEC, int R>
 __device__ __forceinline__ void load_steps(Held<IO, VEC> (&v)[R], const void *base, int64_t row, int64_t step, const Place<VEC, R> &p) {
-    const IO *at = static_cast<const IO *>(base) + p.b * row + p.t0 * step + p.d;
+    const IO *at = static_cast<const IO *>(base);
+    if (p.steps > 0) at += p.b * row + p.t0 * step + p.d;
+    const int last = p.steps > 0 ? p.steps - 1 : 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r].load(at + (r < last ? r : last) * step);
+}
+// What a step beyond the row's length holds does not count, whatever it is: it is taken as a gate of one (a logit of plus infinity) or an
+// input of nothing, and its results are stored as zeros
+template <typename IO, int VEC, int R> __device__ __forceinline__ void beyond_end(Held<IO, VEC> (&v)[R], const Place<VEC, R> &p, float with) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-        if (r < p.live) v[r].load(at + r * step);
+        if (r >= p.live) v[r].fill(with);
 }
 template <typename IO, int VEC, int R>
-__device__ __forceinline__ void store_steps(void *base, const Held<IO, VEC> (&v)[R], int64_t D, int64_t T, const Place<VEC, R> &p) {
+__device__ __forceinline__ void store_steps(void *base, Held<IO, VEC> (&v)[R], int64_t D, int64_t T, const Place<VEC, R> &p) {
     IO *at = static_cast<IO *>(base) + (p.b * T + p.t0) * D + p.d;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+        if (r >= p.live) v[r].fill(0.0f);
         if (r < p.steps) v[r].store(at + r * D);
+    }
 }
 
-// What a step beyond the row's length holds does not count, whatever it is: gate one, input nothing
 template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
-__device__ __forceinline__ void gates_of(Acc (&g)[R][VEC], const Held<IO, VEC> (&f)[R], const Place<VEC, R> &p) {
+__device__ __forceinline__ void gates_of(Acc (&g)[R][VEC], const Held<IO, VEC> (&f)[R]) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const Acc z = f[r].get(v);
-            g[r][v] = r < p.live ? (LOGITS ? gate_of<IO>(z) : z) : (Acc)1;
+            g[r][v] = LOGITS ? gate_of<IO>(z) : z;
         }
 }
-template <typename IO, typename Acc, int VEC, int R>
-__device__ __forceinline__ Acc value_of(const Held<IO, VEC> (&x)[R], int r, int v, const Place<VEC, R> &p) {
-    return r < p.live ? (Acc)x[r].get(v) : (Acc)0;
-}
+constexpr float gate_beyond(bool logits) { return logits ? INFINITY : 1.0f; }
 
 // The map of a channel over a stretch, forward in time, or of its adjoint, backward
 template <typename IO, typename Acc, int VEC, int R, bool BACK>
-__device__ __forceinline__ Map<Acc> fold_steps(const Acc (&g)[R][VEC], const Held<IO, VEC> (&x)[R], int v, const Place<VEC, R> &p) {
-    Acc pr = 1, s = 0;
+__device__ __forceinline__ Map<Acc> fold_steps(const Acc (&g)[R][VEC], const Held<IO, VEC> (&x)[R], int v) {
+    Map<Acc> m{1, 0};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int r = BACK ? R - 1 - i : i;
-        const Acc in = value_of<IO, Acc, VEC, R>(x, r, v, p);
-        s = BACK ? g[r][v] * (s + in) : g[r][v] * s + in;
-        pr *= g[r][v];
+        m = extended<BACK>(m, g[r][v], (Acc)x[r].get(v));
     }
-    return {pr, s};
+    return m;
 }
 
 // The channel of a workgroup's thread in [B, D] arrays; whether it is there
 template <int VEC> __device__ __forceinline__ bool channel_of(const GscanArgs &a, const GscanGrid &gr, int64_t block, int thread, int64_t *at) {
-    const int64_t slot = block * (GS_CHANNELS / VEC) + thread / VEC, b = slot / gr.per_row, d = (slot - b * gr.per_row) * VEC;
+    const int64_t slot = block * (GS_CHANNELS / VEC) + thread / VEC, b = (uint32_t)slot / gr.per_row, d = (slot - b * gr.per_row) * VEC;
     *at = b * a.D + (d + VEC <= a.D ? d : a.D - VEC) + thread % VEC;
-    return slot < a.B * gr.per_row;
+    return slot < a.B * (int64_t)gr.per_row;
 }
 
 // ---- maps from chunk to chunk --------------------------------------------------------------------------------------
-constexpr uint64_t EMPTY = ~0ull;                        // a NaN of a pattern that hand_on() gives to nothing
+constexpr uint64_t EMPTY = ~0ull;                        // a NaN of a pattern that word_of() gives to nothing
 
+constexpr uint64_t NOTHING = 0x3f800000ull;              // the map that changes nothing
+__device__ __forceinline__ uint64_t word_of(const Map<float> &m) {
+    const uint64_t w = (uint64_t)__float_as_uint(m.s) << 32 | __float_as_uint(m.p);
+    return w == EMPTY ? 0x7fc000007fc00000ull : w;       // another NaN
+}
+__device__ __forceinline__ Map<float> map_of(uint64_t w) { return {__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))}; }
 __device__ __forceinline__ void hand_on(uint64_t *word, const Map<float> &m) {
-    uint64_t w = (uint64_t)__float_as_uint(m.s) << 32 | __float_as_uint(m.p);
-    if (w == EMPTY) w = 0x7fc000007fc00000ull;           // another NaN
-    __hip_atomic_store(word, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(word, word_of(m), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ uint64_t look(const uint64_t *word) { return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// The maps lo, lo + 1, .. hi - 1 after one another, each waited for
-__device__ __forceinline__ Map<float> wait_for(const uint64_t *words, int64_t lo, int64_t hi, int64_t slots) {
-    constexpr int AHEAD = 8;
+// The map of a whole chunk, by one wave, a channel for each lane: what its workgroup does, without it
+template <typename IO, int VEC, int R, bool BACK, bool LOGITS>
+__device__ __forceinline__ Map<float> map_alone(const GscanArgs &a, const GscanGrid &gr, int64_t block, int64_t chunk) {
+    constexpr int TG = GS_THREADS / (GS_CHANNELS / VEC);
+    const int lane = threadIdx.x % 64;
+    const int64_t slot = block * (GS_CHANNELS / VEC) + lane / VEC;
     Map<float> all{1.0f, 0.0f};
-    for (int64_t j = lo; j < hi; j += AHEAD) {
-        uint64_t w[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) w[u] = j + u < hi ? look(words + (j + u) * slots) : 0x000000003f800000ull;      // the map that changes nothing
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            while (w[u] == EMPTY) {
-                __builtin_amdgcn_s_sleep(1);
-                w[u] = look(words + (j + u) * slots);
-            }
-            const float p = __uint_as_float((uint32_t)w[u]), s = __uint_as_float((uint32_t)(w[u] >> 32));
-            all.s = p * all.s + s;
-            all.p *= p;
+    if (slot >= a.B * (int64_t)gr.per_row) return all;
+    const int64_t b = (uint32_t)slot / gr.per_row, d0 = (slot - b * gr.per_row) * VEC, d = (d0 + VEC <= a.D ? d0 : a.D - VEC) + lane % VEC;
+    const int64_t begin = (BACK ? gr.chunks - 1 - chunk : chunk) * (TG * R), end = row_length(a, b);
+    const IO *f = static_cast<const IO *>(a.f) + b * a.f_b + d;
+    const IO *x = BACK ? static_cast<const IO *>(a.g_out) + b * a.g_b + d : static_cast<const IO *>(a.x) + b * a.x_b + d;
+    const int64_t x_t = BACK ? a.g_t : a.x_t;
+    const auto gate = [&](int64_t t) {
+        const float z = t < end ? (float)widen(f[t * a.f_t]) : 1.0f;
+        return LOGITS && t < end ? gate_of<IO>(z) : z;
+    };
+    for (int i = 0; i < TG; ++i) {
+        const int64_t t0 = begin + (BACK ? TG - 1 - i : i) * R;
+        Map<float> m{1.0f, 0.0f};
+        for (int k = 0; k < R; ++k) {
+            const int64_t t = t0 + (BACK ? R - 1 - k : k);
+            m.s = extended<BACK>(m, gate(t), t < end ? (float)widen(x[t * x_t]) : 0.0f).s;
         }
+        for (int k = 0; k < R; ++k) m.p *= gate(t0 + k);             // (forward in time in either direction: the states' products)
+        all = after(m, all);
     }
     return all;
 }
 
-// A chunk's number in the direction of the recurrence, from the ticket (float) or the workgroup's own number (double)
-template <typename Acc> __device__ __forceinline__ int64_t take_chunk(const GscanArgs &a, const GscanGrid &gr) {
-    if (sizeof(Acc) == 8 || gr.chunks == 1) return blockIdx.x;
-    __shared__ uint32_t mine;
-    if (threadIdx.x == 0) mine = __hip_atomic_fetch_add(static_cast<uint32_t *>(a.words), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    return mine;
+// The maps lo, lo + 1, .. hi - 1 after one another, each waited for.  False: one did not come.
+__device__ __forceinline__ bool wait_for(Map<float> &all, const uint64_t *words, int lo, int hi, int64_t slots, int looks) {
+    constexpr int AHEAD = 8;
+    const uint32_t lane = threadIdx.x % 64;
+    all = {1.0f, 0.0f};
+    for (int j = lo; j < hi; j += AHEAD) {
+        uint64_t w[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) w[u] = j + u < hi ? look(words + (j + u) * slots + lane) : NOTHING;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            int left = looks;
+            while (__any(w[u] == EMPTY)) {
+                if (left-- <= 0) return false;
+                __builtin_amdgcn_s_sleep(1);
+                w[u] = look(words + (j + u) * slots + lane);
+            }
+            all = after(map_of(w[u]), all);
+        }
+    }
+    return true;
 }
 
 // The recurrence's value before a chunk, in the threads of the first wave: `own` is the chunk's map there, `first` the value before the
 // sequence; all threads of the workgroup call it.
-__device__ __forceinline__ float value_before(const GscanArgs &a, const GscanGrid &gr, int64_t block, int64_t chunk, const Map<float> &own, float first) {
+template <typename IO, int VEC, int R, bool BACK, bool LOGITS>
+__device__ __forceinline__ float value_before(const GscanArgs &a, const GscanGrid &gr, uint32_t block, uint32_t chunk, const Map<float> &own,
+                                              float first) {
     if (gr.chunks == 1) return first;
     __shared__ Map<float> parts[GS_THREADS / 64][GS_CHANNELS];
-    uint64_t *const words = reinterpret_cast<uint64_t *>(static_cast<char *>(a.words) + GS_TICKET) + block * GS_CHANNELS + threadIdx.x % 64;
-    uint64_t *const groups = words + gr.chunks * gr.slots;
-    const int wave = threadIdx.x / 64;
-    if (wave == 0 && chunk < gr.chunks - 1) hand_on(words + chunk * gr.slots, own);
+    __shared__ bool missing[GS_THREADS / 64];
+    uint64_t *const words = static_cast<uint64_t *>(a.words) + (int64_t)block * GS_CHANNELS, *const groups = words + gr.chunks * gr.slots;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    if (wave == 0 && chunk < gr.chunks - 1) hand_on(words + chunk * gr.slots + lane, own);
     // two waves for the groups before this chunk's, two for the chunks before it in its group
-    const int64_t group = chunk / gr.group, start = group * gr.group;
-    const int64_t lo = wave < 2 ? 0 : start, hi = wave < 2 ? group : chunk, half = (lo + hi) / 2;
-    parts[wave][threadIdx.x % 64] = wait_for(wave < 2 ? groups : words, wave % 2 ? half : lo, wave % 2 ? hi : half, gr.slots);
+    const int group = chunk / gr.group, start = group * gr.group, half_groups = group / 2, half = (start + (int)chunk) / 2;
+    {
+        const int lo = wave == 0 ? 0 : wave == 1 ? half_groups : wave == 2 ? start : half;
+        const int hi = wave == 0 ? half_groups : wave == 1 ? group : wave == 2 ? half : (int)chunk;
+        Map<float> all;
+        const bool came = wait_for(all, wave < 2 ? groups : words, lo, hi, gr.slots, a.looks);
+        parts[wave][lane] = all;
+        if (lane == 0) missing[wave] = !came;
+    }
     __syncthreads();
     if (wave != 0) return 0.0f;
-    const Map<float> m0 = parts[0][threadIdx.x], m1 = parts[1][threadIdx.x], m2 = parts[2][threadIdx.x], m3 = parts[3][threadIdx.x];
-    if (chunk % gr.group == gr.group - 1 && chunk < gr.chunks - 1) {
-        const float p = m3.p * m2.p, s = m3.p * m2.s + m3.s;
-        hand_on(groups + group * gr.slots, {own.p * p, own.p * s + own.s});
+    if (__builtin_expect(missing[0] || missing[1] || missing[2] || missing[3], 0)) {
+        // all of it from the inputs, put together as its workgroups do
+        Map<float> p[4] = {{1.0f, 0.0f}, {1.0f, 0.0f}, {1.0f, 0.0f}, {1.0f, 0.0f}}, m{1.0f, 0.0f}, n{1.0f, 0.0f};
+        const int size = gr.group, middle = size / 2 - 1;
+        for (int c = 0; c < (int)chunk; ++c) {
+            const Map<float> one = map_alone<IO, VEC, R, BACK, LOGITS>(a, gr, block, c);
+            if (c >= half) p[3] = after(one, p[3]);
+            else if (c >= start) p[2] = after(one, p[2]);
+            else if (c % size < middle) m = after(one, m);
+            else if (c % size < size - 1) n = after(one, n);
+            else {
+                const Map<float> whole = after(one, after(n, m));
+                if (c / size < half_groups) p[0] = after(whole, p[0]);
+                else p[1] = after(whole, p[1]);
+                m = n = {1.0f, 0.0f};
+            }
+        }
+        for (int i = 0; i < 4; ++i) parts[i][lane] = p[i];
     }
-    float h = m0.p * first + m0.s;
-    h = m1.p * h + m1.s;
-    h = m2.p * h + m2.s;
-    return m3.p * h + m3.s;
+    if (chunk == start + gr.group - 1 && chunk < gr.chunks - 1)
+        hand_on(groups + group * gr.slots + lane, after(own, after(parts[3][lane], parts[2][lane])));
+    float h = first;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h = fmaf(parts[i][lane].p, h, parts[i][lane].s);
+    return h;
 }
 // double: every map is there from the launch before
-__device__ __forceinline__ double value_before(const GscanArgs &a, const GscanGrid &gr, int64_t block, int64_t chunk, const Map<double> &, double first) {
+template <typename IO, int VEC, int R, bool BACK, bool LOGITS>
+__device__ __forceinline__ double value_before(const GscanArgs &a, const GscanGrid &gr, uint32_t block, uint32_t chunk, const Map<double> &,
+                                               double first) {
     if (threadIdx.x >= GS_CHANNELS) return 0.0;
-    const Map<double> *w = static_cast<const Map<double> *>(a.words) + block * GS_CHANNELS + threadIdx.x;
-    for (int64_t c = 0; c < chunk; ++c) first = w[c * gr.slots].p * first + w[c * gr.slots].s;
+    const Map<double> *w = static_cast<const Map<double> *>(a.words) + (int64_t)block * GS_CHANNELS + threadIdx.x;
+    for (int64_t c = 0; c < chunk; ++c) first = fma(w[c * gr.slots].p, first, w[c * gr.slots].s);
     return first;
 }
 
-// Before a call's main launch: the words empty, the ticket zero
-__global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(void *words, int64_t n) {
+// Before a call's main launch: the words empty
+__global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(uint64_t *words, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * GS_THREADS + threadIdx.x;
-    if (i == 0) *static_cast<uint32_t *>(words) = 0;
-    if (i < n) reinterpret_cast<uint64_t *>(static_cast<char *>(words) + GS_TICKET)[i] = EMPTY;
+    if (i < n) words[i] = EMPTY;
 }
 
 // double: the map of every chunk but the last, for what comes after it in the direction of the recurrence
@@ -255,60 +335,59 @@ template <typename IO, typename Acc, int VEC, int R, bool BACK, bool LOGITS>
 __global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];
-    const int64_t block = blockIdx.x % gr.blocks, chunk = blockIdx.x / gr.blocks;
+    const uint32_t block = blockIdx.x % gr.blocks, chunk = blockIdx.x / gr.blocks;
     const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, BACK ? gr.chunks - 1 - chunk : chunk);
     Held<IO, VEC> x[R], f[R];
     load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
     load_steps<IO, VEC, R>(x, BACK ? a.g_out : a.x, BACK ? a.g_b : a.x_b, BACK ? a.g_t : a.x_t, p);
+    beyond_end<IO, VEC, R>(f, p, gate_beyond(LOGITS));
+    beyond_end<IO, VEC, R>(x, p, 0.0f);
     Acc g[R][VEC];
-    gates_of<IO, Acc, VEC, R, LOGITS>(g, f, p);
+    gates_of<IO, Acc, VEC, R, LOGITS>(g, f);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, BACK>(g, x, v, p);
+    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, BACK>(g, x, v);
     __syncthreads();
     if (threadIdx.x >= GS_CHANNELS) return;
     Map<Acc> all{1, 0};
 #pragma unroll
     for (int i = 0; i < TG; ++i) {
-        const Map<Acc> m = maps[BACK ? TG - 1 - i : i][threadIdx.x];
-        all.s = m.p * all.s + m.s;
-        all.p *= m.p;
+        all = after(maps[BACK ? TG - 1 - i : i][threadIdx.x], all);
     }
-    static_cast<Map<Acc> *>(a.words)[chunk * gr.slots + block * GS_CHANNELS + threadIdx.x] = all;
+    static_cast<Map<Acc> *>(a.words)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] = all;
 }
 
 template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
 __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_forward_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];
-    const int64_t at_grid = take_chunk<Acc>(a, gr), block = at_grid % gr.blocks, chunk = at_grid / gr.blocks;
+    const uint32_t block = blockIdx.x % gr.blocks, chunk = blockIdx.x / gr.blocks;
     const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
+    int64_t at = 0;
+    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
+    Acc h = there && a.s0 != nullptr ? static_cast<const Acc *>(a.s0)[at] : (Acc)0;
     Held<IO, VEC> x[R];
     Acc g[R][VEC];
     {
         Held<IO, VEC> f[R];
         load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
         load_steps<IO, VEC, R>(x, a.x, a.x_b, a.x_t, p);
-        gates_of<IO, Acc, VEC, R, LOGITS>(g, f, p);
+        beyond_end<IO, VEC, R>(f, p, gate_beyond(LOGITS));
+        beyond_end<IO, VEC, R>(x, p, 0.0f);
+        gates_of<IO, Acc, VEC, R, LOGITS>(g, f);
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v, p);
+    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v);
     __syncthreads();
     Map<Acc> own{1, 0};
-    Acc h = 0;
-    int64_t at = 0;
-    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
     if (first) {
 #pragma unroll 8
         for (int i = 0; i < TG; ++i) {
-            const Map<Acc> m = maps[i][threadIdx.x];
-            own.s = m.p * own.s + m.s;
-            own.p *= m.p;
+            own = after(maps[i][threadIdx.x], own);
         }
-        if (there && a.s0 != nullptr) h = static_cast<const Acc *>(a.s0)[at];
     }
-    h = value_before(a, gr, block, chunk, own, h);
+    h = value_before<IO, VEC, R, false, LOGITS>(a, gr, block, chunk, own, h);
     if (first) {
-        if (a.ckpt != nullptr) static_cast<Acc *>(a.ckpt)[chunk * gr.slots + block * GS_CHANNELS + threadIdx.x] = h;
+        if (a.ckpt != nullptr) static_cast<Acc *>(a.ckpt)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] = h;
 #pragma unroll 8
         for (int i = 0; i < TG; ++i) {
             const Map<Acc> m = maps[i][threadIdx.x];
@@ -329,8 +408,8 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_fo
             Acc out[PAIR];
 #pragma unroll
             for (int j = 0; j < PAIR; ++j) {
-                s[j] = g[r][v + j] * s[j] + value_of<IO, Acc, VEC, R>(x, r, v + j, p);
-                out[j] = r < p.live ? s[j] : (Acc)0;
+                s[j] = g[r][v + j] * s[j] + (Acc)x[r].get(v + j);
+                out[j] = s[j];
             }
             o[r].put(v, out);
         }
@@ -339,40 +418,40 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_fo
 }
 
 template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
-__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 3) void gscan_backward_kernel(GscanArgs a, GscanGrid gr) {
+__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 2) void gscan_backward_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];           // states: forward in time
     __shared__ Acc sums[TG][GS_CHANNELS];                // adjoints: backward, with the same gate products
-    const int64_t at_grid = take_chunk<Acc>(a, gr), block = at_grid % gr.blocks, from_end = at_grid / gr.blocks, chunk = gr.chunks - 1 - from_end;
+    const uint32_t block = blockIdx.x % gr.blocks, from_end = blockIdx.x / gr.blocks, chunk = gr.chunks - 1 - from_end;
     const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
+    int64_t at = 0;
+    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
+    Acc e = there && a.g_state != nullptr ? static_cast<const Acc *>(a.g_state)[at] : (Acc)0;
+    Acc h = first ? static_cast<const Acc *>(a.ckpt)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] : (Acc)0;
     Held<IO, VEC> x[R], f[R], go[R];
     load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
     load_steps<IO, VEC, R>(go, a.g_out, a.g_b, a.g_t, p);
     load_steps<IO, VEC, R>(x, a.x, a.x_b, a.x_t, p);
+    beyond_end<IO, VEC, R>(f, p, gate_beyond(LOGITS));
+    beyond_end<IO, VEC, R>(go, p, 0.0f);
+    beyond_end<IO, VEC, R>(x, p, 0.0f);
     Acc g[R][VEC];
-    gates_of<IO, Acc, VEC, R, LOGITS>(g, f, p);
+    gates_of<IO, Acc, VEC, R, LOGITS>(g, f);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v, p);
-        sums[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, true>(g, go, v, p).s;
+        maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v);
+        sums[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, true>(g, go, v).s;
     }
     __syncthreads();
     Map<Acc> own{1, 0};
-    Acc e = 0;
-    int64_t at = 0;
-    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
     if (first) {
 #pragma unroll 8
         for (int i = TG - 1; i >= 0; --i) {
-            const Acc pr = maps[i][threadIdx.x].p;
-            own.s = pr * own.s + sums[i][threadIdx.x];
-            own.p *= pr;
+            own = after({maps[i][threadIdx.x].p, sums[i][threadIdx.x]}, own);
         }
-        if (there && a.g_state != nullptr) e = static_cast<const Acc *>(a.g_state)[at];
     }
-    e = value_before(a, gr, block, from_end, own, e);
+    e = value_before<IO, VEC, R, true, LOGITS>(a, gr, block, from_end, own, e);
     if (first) {
-        Acc h = static_cast<const Acc *>(a.ckpt)[chunk * gr.slots + block * GS_CHANNELS + threadIdx.x];
 #pragma unroll 8
         for (int i = 0; i < TG; ++i) {
             const Map<Acc> m = maps[i][threadIdx.x];
@@ -399,7 +478,7 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 3) void gscan_ba
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 before[r][j] = h;
-                h = g[r][v + j] * h + value_of<IO, Acc, VEC, R>(x, r, v + j, p);
+                h = g[r][v + j] * h + (Acc)x[r].get(v + j);
             }
         }
 #pragma unroll
@@ -407,11 +486,11 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 3) void gscan_ba
             Acc dx[PAIR], df[PAIR];
 #pragma unroll
             for (int j = 0; j < PAIR; ++j) {
-                const Acc d = value_of<IO, Acc, VEC, R>(go, r, v + j, p) + after[j];
+                const Acc d = (Acc)go[r].get(v + j) + after[j];
                 after[j] = g[r][v + j] * d;
                 const Acc slope = LOGITS ? (Acc)gate_slope<IO>((Acc)f[r].get(v + j)) : (Acc)1;
-                dx[j] = r < p.live ? d : (Acc)0;
-                df[j] = r < p.live ? d * before[r][j] * slope : (Acc)0;
+                dx[j] = d;
+                df[j] = d * before[r][j] * slope;
             }
             go[r].put(v, dx);
             x[r].put(v, df);
@@ -419,6 +498,18 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 3) void gscan_ba
     }
     store_steps<IO, VEC, R>(a.d_x, go, a.D, a.T, p);
     store_steps<IO, VEC, R>(a.d_f, x, a.D, a.T, p);
+}
+
+// No steps: the value before them (zeros where there is none) is that after them
+template <typename Acc> __global__ __launch_bounds__(GS_THREADS) void gscan_pass_kernel(const void *from, void *to, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * GS_THREADS + threadIdx.x;
+    if (i < n) static_cast<Acc *>(to)[i] = from == nullptr ? (Acc)0 : static_cast<const Acc *>(from)[i];
+}
+template <typename Acc> int pass(const void *from, void *to, int64_t n, hipStream_t stream) {
+    if (to == nullptr) return T2FW_OK;
+    if (n > 0x7fffffffll * GS_THREADS) return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many channels for one launch");
+    hipLaunchKernelGGL(gscan_pass_kernel<Acc>, dim3((unsigned)((n + GS_THREADS - 1) / GS_THREADS)), dim3(GS_THREADS), 0, stream, from, to, n);
+    return check_hip(hipGetLastError(), "gscan_pass_kernel launch");
 }
 
 // One token: x, f, out [B, D], the state in place or not
@@ -454,29 +545,32 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_step_kernel(GscanArgs a, int
 template <typename IO, int VEC, int R> GscanGrid grid_of(int64_t B, int64_t T, int64_t D) {
     constexpr int CL = GS_CHANNELS / VEC, C = GS_THREADS / CL * R;
     GscanGrid g;
-    g.per_row = (D + VEC - 1) / VEC;
-    g.blocks = (B * g.per_row + CL - 1) / CL;
-    g.chunks = T <= 0 ? 1 : (T + C - 1) / C;
-    g.slots = g.blocks * GS_CHANNELS;
-    for (g.group = 8; g.group * g.group < g.chunks;) g.group *= 2;
+    // (numbers that do not fit are refused before anything is launched)
+    const int64_t per_row = (D + VEC - 1) / VEC, blocks = (B * per_row + CL - 1) / CL, chunks = T <= 0 ? 1 : (T + C - 1) / C;
+    g.per_row = (uint32_t)per_row;
+    g.blocks = (uint32_t)blocks;
+    g.chunks = (uint32_t)chunks;
+    g.fits = per_row < 0x7fffffff && B * per_row < 0x7fffffff && chunks < 0x7fffffff && blocks * chunks < 0x7fffffff;
+    g.slots = blocks * GS_CHANNELS;
+    for (g.group = 8; (uint64_t)g.group * g.group < (uint64_t)chunks;) g.group *= 2;
     return g;
 }
-int64_t words_of(const GscanGrid &g) { return (g.chunks + (g.chunks + g.group - 1) / g.group) * g.slots; }
+// 64-bit words of the scratch
+int64_t words_of(const GscanGrid &g) { return (g.chunks + (int64_t)(g.chunks + g.group - 1) / g.group) * g.slots; }
 
 template <typename IO, int VEC, int R> GscanPlan plan_of(int64_t B, int64_t T, int64_t D) {
     const GscanGrid g = grid_of<IO, VEC, R>(B, T, D);
     const size_t acc = sizeof(typename AccT<IO>::type);
     GscanPlan p;
     p.checkpoints = (size_t)(g.chunks * g.slots) * acc;
-    p.workspace = g.chunks == 1 ? 0 : acc == 8 ? (size_t)(g.chunks * g.slots) * 2 * acc : GS_TICKET + (size_t)words_of(g) * sizeof(uint64_t);
+    p.workspace = g.chunks == 1 ? 0 : acc == 8 ? (size_t)(g.chunks * g.slots) * 2 * acc : (size_t)words_of(g) * sizeof(uint64_t);
     return p;
 }
 
 // What comes before a call's main launch
 template <typename IO, int VEC, int R, bool BACK, bool LOGITS> int prepare(const GscanArgs &a, const GscanGrid &g, hipStream_t stream) {
     using Acc = typename AccT<IO>::type;
-    if (g.blocks > 0x7fffffff / g.chunks || g.slots > 0x7fffffff * (int64_t)GS_THREADS / (2 * g.chunks))
-        return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many workgroups for one launch");
+    if (!g.fits) return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many workgroups for one launch");
     if (g.chunks == 1) return T2FW_OK;
     if constexpr (sizeof(Acc) == 8) {
         hipLaunchKernelGGL((gscan_maps_kernel<IO, Acc, VEC, R, BACK, LOGITS>), dim3((unsigned)(g.blocks * (g.chunks - 1))), dim3(GS_THREADS), 0,
@@ -484,7 +578,8 @@ template <typename IO, int VEC, int R, bool BACK, bool LOGITS> int prepare(const
         return check_hip(hipGetLastError(), "gscan_maps_kernel launch");
     } else {
         const int64_t n = words_of(g);
-        hipLaunchKernelGGL(gscan_empty_kernel, dim3((unsigned)((n + GS_THREADS - 1) / GS_THREADS)), dim3(GS_THREADS), 0, stream, a.words, n);
+        hipLaunchKernelGGL(gscan_empty_kernel, dim3((unsigned)((n + GS_THREADS - 1) / GS_THREADS)), dim3(GS_THREADS), 0, stream,
+                           static_cast<uint64_t *>(a.words), n);
         return check_hip(hipGetLastError(), "gscan_empty_kernel launch");
     }
 }
@@ -498,6 +593,7 @@ template <typename IO, int VEC, int R, bool LOGITS> int forward_with(const Gscan
     return check_hip(hipGetLastError(), "gscan_forward_kernel launch");
 }
 template <typename IO, int VEC, int R> int forward_of(const GscanArgs &a, hipStream_t stream) {
+    if (a.T == 0) return pass<typename AccT<IO>::type>(a.s0, a.final_state, a.B * a.D, stream);
     return a.logits ? forward_with<IO, VEC, R, true>(a, stream) : forward_with<IO, VEC, R, false>(a, stream);
 }
 
@@ -510,6 +606,7 @@ template <typename IO, int VEC, int R, bool LOGITS> int backward_with(const Gsca
     return check_hip(hipGetLastError(), "gscan_backward_kernel launch");
 }
 template <typename IO, int VEC, int R> int backward_of(const GscanArgs &a, hipStream_t stream) {
+    if (a.T == 0) return pass<typename AccT<IO>::type>(a.g_state, a.d_s0, a.B * a.D, stream);
     return a.logits ? backward_with<IO, VEC, R, true>(a, stream) : backward_with<IO, VEC, R, false>(a, stream);
 }
 

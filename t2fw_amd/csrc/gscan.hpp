@@ -16,6 +16,7 @@ struct GscanArgs {
     int64_t B, T, D;
     int64_t x_b, x_t, f_b, f_t, g_b, g_t;    // strides of batch rows and steps, in elements
     int32_t wide_lengths, logits;       // lengths are int64; f holds gate logits
+    int32_t looks;                      // of a chunk at what another hands on, before it does without
 };
 
 struct GscanPlan {

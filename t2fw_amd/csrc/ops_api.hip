@@ -45,12 +45,15 @@ int check_sizes(std::initializer_list<int64_t> sizes, const char *what) {
     return T2FW_OK;
 }
 
+// A look takes about a microsecond: what is not there after these has not been started, and its workgroup will be long in coming
+constexpr int SCAN_LOOKS = 1 << 14;
+
 int check_scan(int64_t B, int64_t T, int64_t D, int32_t dtype, int32_t flags) {
     if (size_of(dtype) == 0) return bad_dtype(dtype);
     const int rc = check_sizes({B, T, D}, "gated scan");
     if (rc) return rc;
     if (D < 1) return fail(T2FW_ERR_BAD_SHAPE, "gated scan: at least one channel");
-    if (flags & ~(T2FW_SCAN_LOGITS | T2FW_SCAN_LENGTHS64)) return fail(T2FW_ERR_UNSUPPORTED, "gated scan: unknown flags %d", flags);
+    if (flags & ~(T2FW_SCAN_LOGITS | T2FW_SCAN_LENGTHS64 | T2FW_SCAN_ALONE)) return fail(T2FW_ERR_UNSUPPORTED, "gated scan: unknown flags %d", flags);
     return T2FW_OK;
 }
 int scan_strides(GscanArgs &a, const int64_t *strides, bool backward) {
@@ -162,6 +165,7 @@ int t2fw_gated_scan_forward(const void *x, const void *f, const void *s0, const 
     a.B = B; a.T = T; a.D = D;
     a.logits = (flags & T2FW_SCAN_LOGITS) != 0;
     a.wide_lengths = (flags & T2FW_SCAN_LENGTHS64) != 0;
+    a.looks = flags & T2FW_SCAN_ALONE ? 0 : SCAN_LOOKS;
     if ((rc = scan_strides(a, strides, false))) return rc;
     return gscan_forward(a, dtype, static_cast<hipStream_t>(stream));
 }
@@ -184,6 +188,7 @@ int t2fw_gated_scan_backward(const void *g_out, const void *g_state, const void 
     a.B = B; a.T = T; a.D = D;
     a.logits = (flags & T2FW_SCAN_LOGITS) != 0;
     a.wide_lengths = (flags & T2FW_SCAN_LENGTHS64) != 0;
+    a.looks = flags & T2FW_SCAN_ALONE ? 0 : SCAN_LOOKS;
     if ((rc = scan_strides(a, strides, true))) return rc;
     return gscan_backward(a, dtype, static_cast<hipStream_t>(stream));
 }

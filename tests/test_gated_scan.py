@@ -272,6 +272,32 @@ def test_on_another_stream_and_in_a_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape,ragged", [((2, 900, 40), False), ((1, 2600, 7), True), ((3, 1300, 5), False), ((2, 5000, 65), True)], ids=str)
+def test_chunks_that_do_without_one_another(shape, ragged, dtype):
+    """the same bits where no chunk waits for another's map and makes those before it itself"""
+    from t2fw_amd import _lib
+    lib = _lib.load()
+    B, T, D = shape
+    (x, f, s), go, gs = inputs(B, T, D, dtype, True, seed=T)
+    lengths = torch.tensor([T - 130, T, T // 3][:B], device="cuda") if ragged else None
+    code, st = _lib.DTYPE_CODE[dtype], _lib.current_stream_handle(x.device)
+    nc, nw = lib.t2fw_gated_scan_checkpoint_bytes(B, T, D, code), lib.t2fw_gated_scan_workspace_bytes(B, T, D, code)
+    assert nw > 0
+    results = []
+    for flags in (3, 3 | 4):
+        out, last, dx, df, ds = torch.empty_like(x), torch.empty_like(s), torch.empty_like(x), torch.empty_like(x), torch.empty_like(s)
+        ckpt, ws = (torch.empty(n, dtype=torch.uint8, device="cuda") for n in (nc, nw))
+        p = _lib.ptr
+        _lib.check(lib.t2fw_gated_scan_forward(p(x), p(f), p(s), p(lengths), p(out), p(last), p(ckpt), B, T, D, None, code, flags, p(ws), nw, st))
+        _lib.check(lib.t2fw_gated_scan_backward(p(go), p(gs), p(x), p(f), p(lengths), p(ckpt), p(dx), p(df), p(ds), B, T, D, None, code, flags,
+                                                p(ws), nw, st))
+        torch.cuda.synchronize()
+        results.append((out, last, dx, df, ds))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
 def test_refusals():
     import t2fw_amd as t2
     x = torch.zeros(2, 3, 8, device="cuda")
