@@ -330,6 +330,23 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(uint64_t *words
     if (i < n) words[i] = EMPTY;
 }
 
+// Which block of channels and which chunk (in the direction of the recurrence) a workgroup has.  The hardware deals workgroups out to the
+// eight dies in turn, each with a cache of its own: runs of NEAR neighbouring blocks go to one die, so that the lines that neighbours share, as
+// they do where rows start anywhere, are fetched and written once (32 x 4096 bf16, forward: 1021 channels 250 -> 183 us, 1024 190 -> 163).
+constexpr uint32_t DIES = 8, NEAR = 16;
+struct Turn {
+    uint32_t block, chunk;
+};
+__device__ __forceinline__ Turn turn_of(const GscanGrid &gr) {
+    const uint32_t whole = gridDim.x / (DIES * NEAR) * (DIES * NEAR);
+    uint32_t n = blockIdx.x;
+    if (n < whole) {
+        const uint32_t in = n % (DIES * NEAR);
+        n += in % DIES * NEAR + in / DIES - in;
+    }
+    return {n % gr.blocks, n / gr.blocks};
+}
+
 // double: the map of every chunk but the last, for what comes after it in the direction of the recurrence
 template <typename IO, typename Acc, int VEC, int R, bool BACK, bool LOGITS>
 __global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, GscanGrid gr) {
@@ -360,7 +377,8 @@ template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
 __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_forward_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];
-    const uint32_t block = blockIdx.x % gr.blocks, chunk = blockIdx.x / gr.blocks;
+    const Turn turn = turn_of(gr);
+    const uint32_t block = turn.block, chunk = turn.chunk;
     const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
     int64_t at = 0;
     const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
@@ -422,7 +440,8 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 2) void gscan_ba
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];           // states: forward in time
     __shared__ Acc sums[TG][GS_CHANNELS];                // adjoints: backward, with the same gate products
-    const uint32_t block = blockIdx.x % gr.blocks, from_end = blockIdx.x / gr.blocks, chunk = gr.chunks - 1 - from_end;
+    const Turn turn = turn_of(gr);
+    const uint32_t block = turn.block, from_end = turn.chunk, chunk = gr.chunks - 1 - from_end;
     const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
     int64_t at = 0;
     const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
