@@ -4,8 +4,9 @@
 // The norm is of the rounded h, the one that the backward finds again; sums are carried in 32 bits (64 for double).
 // In 8 bits: y is divided by scale = max |y| / 448 of the row, or of each group of its columns, and rounded to float8 e4m3.
 //
-// A row stays in registers between its sums and its results: a wave (rows of up to 1024 columns) or a workgroup of 4 waves holds
-// it in chunks of 8 columns, CH of them for each lane.  Where the width is no multiple of 8 the last chunk of a row is loaded
+// A row stays in registers between its sums and its results: LANES threads hold it in chunks of 8 columns, CH of them each: 16 or 32
+// lanes of a wave for narrow rows, a wave, or 4 to 16 waves.  Every load of a row is made before its sums, without a branch between
+// them, also by lanes that have no columns left.  Where the width is no multiple of 8 the last chunk of a row is loaded
 // from 8 columns before its end, and the columns that belong to the chunk before it are left out.
 #include "rmsnorm.hpp"
 #include "vec.hpp"
@@ -20,26 +21,13 @@ constexpr float FP8_LARGEST = 448.0f;
 template <typename IO> struct AccT { using type = float; };
 template <> struct AccT<double> { using type = double; };
 
-// Sums over the lanes of a row (one wave, or the four of the workgroup)
-template <int WAVES, typename Acc> __device__ __forceinline__ Acc row_sum(Acc v) {
-    v = group_sum(v, 64);
-    if (WAVES > 1) {
-        __shared__ Acc parts[RN_THREADS / 64];
-        __syncthreads();
-        if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = v;
-        __syncthreads();
-        v = 0;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) v += parts[i];
-    }
-    return v;
-}
-// Two of them in one exchange
-template <int WAVES, typename Acc> __device__ __forceinline__ void row_sums(Acc &v, Acc &u) {
-    v = group_sum(v, 64);
-    u = group_sum(u, 64);
-    if (WAVES > 1) {
-        __shared__ Acc parts[2][RN_THREADS / 64];
+// Sums over the LANES threads of a row (part of a wave, one, or a workgroup of several)
+template <int LANES, typename Acc> __device__ __forceinline__ void row_sums(Acc &v, Acc &u) {
+    v = group_sum(v, LANES < 64 ? LANES : 64);
+    u = group_sum(u, LANES < 64 ? LANES : 64);
+    if (LANES > 64) {
+        constexpr int WAVES = LANES > 64 ? LANES / 64 : 1;
+        __shared__ Acc parts[2][WAVES];
         __syncthreads();
         if (threadIdx.x % 64 == 0) {
             parts[0][threadIdx.x / 64] = v;
@@ -54,16 +42,31 @@ template <int WAVES, typename Acc> __device__ __forceinline__ void row_sums(Acc 
         }
     }
 }
+template <int LANES, typename Acc> __device__ __forceinline__ Acc row_sum(Acc v) {
+    v = group_sum(v, LANES < 64 ? LANES : 64);
+    if (LANES > 64) {
+        constexpr int WAVES = LANES > 64 ? LANES / 64 : 1;
+        __shared__ Acc parts[WAVES];
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) v += parts[i];
+    }
+    return v;
+}
 // max that keeps a NaN
 __device__ __forceinline__ float larger(float a, float b) { return a > b || a != a ? a : b; }
 __device__ __forceinline__ float lanes_max(float v, int lanes) {
     for (int m = 1; m < lanes; m <<= 1) v = larger(v, __shfl_xor(v, m, 64));
     return v;
 }
-template <int WAVES> __device__ __forceinline__ float row_max(float v) {
-    v = lanes_max(v, 64);
-    if (WAVES > 1) {
-        __shared__ float parts[RN_THREADS / 64];
+template <int LANES> __device__ __forceinline__ float row_max(float v) {
+    v = lanes_max(v, LANES < 64 ? LANES : 64);
+    if (LANES > 64) {
+        constexpr int WAVES = LANES > 64 ? LANES / 64 : 1;
+        __shared__ float parts[WAVES];
         __syncthreads();
         if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = v;
         __syncthreads();
@@ -73,214 +76,229 @@ template <int WAVES> __device__ __forceinline__ float row_max(float v) {
     return v;
 }
 
-// A chunk of a row: its first column, where it is loaded from, how many of the loaded columns are its neighbour's
-struct Chunk {
-    int64_t column, from;
-    int skip;
-    bool there;
+// 8 columns as they lie in memory
+template <typename T> struct Eight {
+    Raw16 raw[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) raw[i] = load_raw(p + i * (16 / sizeof(T)));
+    }
+    __device__ __forceinline__ float get(int i) const { return element<T>(raw[i / (16 / sizeof(T))], i % (16 / sizeof(T))); }
 };
-__device__ __forceinline__ Chunk chunk_at(int64_t index, int64_t D) {
+template <> struct Eight<double> {
+    Vec<double, RN_WIDTH> v;
+    __device__ __forceinline__ void load(const double *p) { v = load_vec<double, RN_WIDTH>(p); }
+    __device__ __forceinline__ double get(int i) const { return v.e[i]; }
+};
+
+// A chunk of a row: its first column, where it is loaded from, how many of the loaded columns are not its own (8: it is past the end)
+struct Chunk {
+    int column, from, skip;
+    __device__ __forceinline__ bool there() const { return skip < RN_WIDTH; }
+};
+__device__ __forceinline__ Chunk chunk_at(int index, int D) {
     Chunk c;
     c.column = index * RN_WIDTH;
-    c.there = c.column < D;
     c.from = c.column + RN_WIDTH <= D ? c.column : D - RN_WIDTH;
-    c.skip = (int)(c.column - c.from);
+    c.skip = c.column < D ? c.column - c.from : RN_WIDTH;
     return c;
 }
 template <typename T> __device__ __forceinline__ void store_chunk(T *row, const Chunk &c, const Vec<T, RN_WIDTH> &v) {
     if (c.skip == 0) {
         store_vec(row + c.from, v);
-    } else {
+    } else if (c.there()) {
 #pragma unroll
         for (int i = 0; i < RN_WIDTH; ++i)
             if (i >= c.skip) row[c.from + i] = v.e[i];
     }
 }
-template <typename Acc, typename T> __device__ __forceinline__ void load_wide(Acc (&o)[RN_WIDTH], const void *row, int64_t from) {
-    const Vec<T, RN_WIDTH> v = load_vec<T, RN_WIDTH>(static_cast<const T *>(row) + from);
+template <typename IO, typename Acc> __device__ __forceinline__ void load_weights(Acc (&o)[RN_WIDTH], const NormArgs &a, int from) {
+    if (a.wide_w) {
+        const Vec<float, RN_WIDTH> v = load_vec<float, RN_WIDTH>(static_cast<const float *>(a.w) + from);
 #pragma unroll
-    for (int i = 0; i < RN_WIDTH; ++i) o[i] = widen(v.e[i]);
-}
-template <typename IO, typename Acc> __device__ __forceinline__ void load_weights(Acc (&o)[RN_WIDTH], const NormArgs &a, int64_t from) {
-    if (a.wide_w) load_wide<Acc, float>(o, a.w, from);
-    else load_wide<Acc, IO>(o, a.w, from);
+        for (int i = 0; i < RN_WIDTH; ++i) o[i] = v.e[i];
+    } else {
+        Eight<IO> v;
+        v.load(static_cast<const IO *>(a.w) + from);
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; ++i) o[i] = v.get(i);
+    }
 }
 
-template <typename IO, typename Stream, int WAVES, int CH, bool FP8>
-__global__ __launch_bounds__(RN_THREADS) void norm_forward_kernel(NormArgs a) {
+constexpr int threads_of(int lanes) { return lanes < RN_THREADS ? RN_THREADS : lanes; }
+
+template <typename IO, typename Stream, int LANES, int CH, bool FP8>
+__global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArgs a) {
     using Acc = typename AccT<IO>::type;
-    constexpr int ROWS = RN_THREADS / 64 / WAVES, LANES = 64 * WAVES;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
-    const int lane = threadIdx.x % LANES;
-    if (row >= a.N) return;                              // whole waves; with WAVES > 1 a workgroup has one row
-    const IO *x = static_cast<const IO *>(a.x) + row * a.D;
-    const Stream *res = static_cast<const Stream *>(a.res) + row * a.D;
-    Acc h[CH][RN_WIDTH], sum = 0;
+    constexpr int ROWS = threads_of(LANES) / LANES;
+    const int D = (int)a.D, lane = threadIdx.x % LANES;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES, base = (row < a.N ? row : a.N - 1) * a.D;
+    const bool live = row < a.N;                         // (rows past the end compute with the last one, and store nothing)
+    Chunk k[CH];
+    Eight<IO> x[CH];
+    Eight<Stream> res[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const Chunk k = chunk_at(c * LANES + lane, a.D);
-        if (!k.there) continue;
-        load_wide<Acc, IO>(h[c], x, k.from);
-        Vec<Stream, RN_WIDTH> o;
-        if (a.res != nullptr) {
-            Acc add[RN_WIDTH];
-            load_wide<Acc, Stream>(add, res, k.from);
+        k[c] = chunk_at(c * LANES + lane, D);
+        x[c].load(static_cast<const IO *>(a.x) + base + k[c].from);
+    }
+    if (a.res != nullptr) {
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; ++i) h[c][i] += add[i];
-        }
+        for (int c = 0; c < CH; ++c) res[c].load(static_cast<const Stream *>(a.res) + base + k[c].from);
+    }
+    Acc w[CH][RN_WIDTH], h[CH][RN_WIDTH], sum = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) load_weights<IO>(w[c], a, k[c].from);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        Vec<Stream, RN_WIDTH> o;
 #pragma unroll
         for (int i = 0; i < RN_WIDTH; ++i) {
+            h[c][i] = x[c].get(i);
+            if (a.res != nullptr) h[c][i] += res[c].get(i);
             o.e[i] = narrow<Stream>(h[c][i]);
             h[c][i] = widen(o.e[i]);
-            sum += i >= k.skip ? h[c][i] * h[c][i] : (Acc)0;
+            sum += i >= k[c].skip ? h[c][i] * h[c][i] : (Acc)0;
         }
-        if (a.stored != nullptr) store_chunk(static_cast<Stream *>(a.stored) + row * a.D, k, o);
+        if (a.stored != nullptr && live) store_chunk(static_cast<Stream *>(a.stored) + base, k[c], o);
     }
-    sum = row_sum<WAVES>(sum);
+    sum = row_sum<LANES>(sum);
     const Acc r = (Acc)1 / sqrt(sum / (Acc)a.D + (Acc)a.eps);
-    if (!FP8) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < RN_WIDTH; ++i) h[c][i] *= r * w[c][i];
+    if constexpr (!FP8) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const Chunk k = chunk_at(c * LANES + lane, a.D);
-            if (!k.there) continue;
-            Acc w[RN_WIDTH];
-            load_weights<IO>(w, a, k.from);
             Vec<IO, RN_WIDTH> o;
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; ++i) o.e[i] = narrow<IO>(h[c][i] * r * w[i]);
-            store_chunk(static_cast<IO *>(a.y) + row * a.D, k, o);
+            for (int i = 0; i < RN_WIDTH; ++i) o.e[i] = narrow<IO>(h[c][i]);
+            if (live) store_chunk(static_cast<IO *>(a.y) + base, k[c], o);
         }
-        return;
-    }
-    float top[CH], all = 0;
+    } else {
+        float top[CH], all = 0;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const Chunk k = chunk_at(c * LANES + lane, a.D);
-        top[c] = 0;
-        if (!k.there) continue;
-        Acc w[RN_WIDTH];
-        load_weights<IO>(w, a, k.from);
+        for (int c = 0; c < CH; ++c) {
+            top[c] = 0;
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i) {
-            h[c][i] = h[c][i] * r * w[i];
-            if (i >= k.skip) top[c] = larger(fabsf((float)h[c][i]), top[c]);
+            for (int i = 0; i < RN_WIDTH; ++i)
+                if (i >= k[c].skip) top[c] = larger(fabsf(h[c][i]), top[c]);
+            all = larger(top[c], all);
         }
-        all = larger(top[c], all);
-    }
-    const bool by_row = a.groups == 1;
-    if (by_row) all = row_max<WAVES>(all);
+        const bool by_row = a.groups == 1;
+        if (by_row) all = row_max<LANES>(all);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const Chunk k = chunk_at(c * LANES + lane, a.D);
-        // a group's chunks are neighbouring lanes of one wave, those past the end of the row among them
-        float scale = (by_row ? all : lanes_max(top[c], (int)(a.group / RN_WIDTH))) / FP8_LARGEST;
-        if (scale == 0.0f) scale = 1.0f;
-        if (!k.there) continue;
-        const int64_t g = by_row ? 0 : k.column / a.group;
-        if (by_row ? lane == 0 && c == 0 : k.column % a.group == 0) a.scales[row * a.groups + g] = scale;
-        // one reciprocal for the chunk; of a scale near the smallest numbers it would overflow
-        const float by = 1.0f / scale;
-        const bool tiny = scale < 1e-35f;
-        uint32_t words[2];
+        for (int c = 0; c < CH; ++c) {
+            // a group's chunks are neighbouring lanes of one wave, those past the end of the row among them
+            float scale = (by_row ? all : lanes_max(top[c], (int)(a.group / RN_WIDTH))) / FP8_LARGEST;
+            if (scale == 0.0f) scale = 1.0f;
+            if (!live || !k[c].there()) continue;
+            const int64_t g = by_row ? 0 : k[c].column / a.group;
+            if (by_row ? lane == 0 && c == 0 : k[c].column % a.group == 0) a.scales[row * a.groups + g] = scale;
+            // one reciprocal for the chunk; of a scale near the smallest numbers it would overflow
+            const float by = 1.0f / scale;
+            const bool tiny = scale < 1e-35f;
+            uint32_t words[2];
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; i += 4) {
-            float v[4];
+            for (int i = 0; i < RN_WIDTH; i += 4) {
+                float v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = tiny ? (float)h[c][i + j] / scale : (float)h[c][i + j] * by;
-            int word = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-            words[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], word, true);
+                for (int j = 0; j < 4; ++j) v[j] = tiny ? h[c][i + j] / scale : h[c][i + j] * by;
+                const int word = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+                words[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], word, true);
+            }
+            Vec<uint8_t, RN_WIDTH> o;
+            __builtin_memcpy(&o, words, sizeof(o));
+            store_chunk(static_cast<uint8_t *>(a.q) + base, k[c], o);
         }
-        Vec<uint8_t, RN_WIDTH> o;
-        __builtin_memcpy(&o, words, sizeof(o));
-        store_chunk(static_cast<uint8_t *>(a.q) + row * a.D, k, o);
     }
 }
 
-template <typename IO, typename Stream, int WAVES, int CH>
-__global__ __launch_bounds__(RN_THREADS) void norm_backward_kernel(NormArgs a) {
+template <typename IO, typename Stream, int LANES, int CH>
+__global__ __launch_bounds__(threads_of(LANES)) void norm_backward_kernel(NormArgs a) {
     using Acc = typename AccT<IO>::type;
-    constexpr int ROWS = RN_THREADS / 64 / WAVES, LANES = 64 * WAVES;
-    const int lane = threadIdx.x % LANES;
+    constexpr int THREADS = threads_of(LANES), ROWS = THREADS / LANES;
+    const int D = (int)a.D, lane = threadIdx.x % LANES;
     Acc dw[CH][RN_WIDTH], w[CH][RN_WIDTH];
+    Chunk k[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const Chunk k = chunk_at(c * LANES + lane, a.D);
+        k[c] = chunk_at(c * LANES + lane, D);
+        load_weights<IO>(w[c], a, k[c].from);
 #pragma unroll
         for (int i = 0; i < RN_WIDTH; ++i) dw[c][i] = 0;
-        if (k.there) load_weights<IO>(w[c], a, k.from);
     }
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.N; row += (int64_t)gridDim.x * ROWS) {
-        // all of the row's loads before its sums
-        Vec<Stream, RN_WIDTH> hv[CH], rv[CH];
-        Vec<IO, RN_WIDTH> uv[CH];
+    // (all rows of a workgroup go round together)
+    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < a.N; first += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = first + threadIdx.x / LANES, base = (row < a.N ? row : a.N - 1) * a.D;
+        const bool live = row < a.N;
+        Eight<Stream> h[CH], gr[CH];
+        Eight<IO> u[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const Chunk k = chunk_at(c * LANES + lane, a.D);
-            if (!k.there) continue;
-            hv[c] = load_vec<Stream, RN_WIDTH>(static_cast<const Stream *>(a.stored) + row * a.D + k.from);
-            uv[c] = load_vec<IO, RN_WIDTH>(static_cast<const IO *>(a.g_y) + row * a.D + k.from);
-            if (a.g_res != nullptr) rv[c] = load_vec<Stream, RN_WIDTH>(static_cast<const Stream *>(a.g_res) + row * a.D + k.from);
+            h[c].load(static_cast<const Stream *>(a.stored) + base + k[c].from);
+            u[c].load(static_cast<const IO *>(a.g_y) + base + k[c].from);
+        }
+        if (a.g_res != nullptr) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) gr[c].load(static_cast<const Stream *>(a.g_res) + base + k[c].from);
         }
         Acc squares = 0, dot = 0;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const Chunk k = chunk_at(c * LANES + lane, a.D);
-            if (!k.there) continue;
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < RN_WIDTH; ++i) {
-                const Acc h = widen(hv[c].e[i]);
-                squares += i >= k.skip ? h * h : (Acc)0;
-                dot += i >= k.skip ? h * (Acc)widen(uv[c].e[i]) * w[c][i] : (Acc)0;
+                const Acc v = h[c].get(i);
+                squares += i >= k[c].skip ? v * v : (Acc)0;
+                dot += i >= k[c].skip ? v * u[c].get(i) * w[c][i] : (Acc)0;
             }
-        }
-        row_sums<WAVES>(squares, dot);
+        row_sums<LANES>(squares, dot);
         const Acc r = (Acc)1 / sqrt(squares / (Acc)a.D + (Acc)a.eps), back = dot * r * r / (Acc)a.D;
+        const Acc counts = live ? r : (Acc)0;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            const Chunk k = chunk_at(c * LANES + lane, a.D);
-            if (!k.there) continue;
             Vec<IO, RN_WIDTH> o;
             Vec<Stream, RN_WIDTH> os;
 #pragma unroll
             for (int i = 0; i < RN_WIDTH; ++i) {
-                const Acc h = widen(hv[c].e[i]), u = widen(uv[c].e[i]);
-                dw[c][i] += u * h * r;
-                Acc g = r * (u * w[c][i] - h * back);
-                if (a.g_res != nullptr) g += (Acc)widen(rv[c].e[i]);
+                const Acc v = h[c].get(i), t = u[c].get(i);
+                if (live) dw[c][i] += t * v * counts;
+                Acc g = r * (t * w[c][i] - v * back);
+                if (a.g_res != nullptr) g += gr[c].get(i);
                 o.e[i] = narrow<IO>(g);
                 os.e[i] = narrow<Stream>(g);
             }
-            store_chunk(static_cast<IO *>(a.d_x) + row * a.D, k, o);
-            if (a.d_res != nullptr) store_chunk(static_cast<Stream *>(a.d_res) + row * a.D, k, os);
+            if (!live) continue;
+            store_chunk(static_cast<IO *>(a.d_x) + base, k[c], o);
+            if (a.d_res != nullptr) store_chunk(static_cast<Stream *>(a.d_res) + base, k[c], os);
         }
     }
-    // a workgroup's share of d_w: that of its waves, where each had rows of its own, added up in order
-    if (ROWS > 1) {
-        __shared__ Acc sums[ROWS > 1 ? ROWS - 1 : 1][ROWS > 1 ? CH : 1][RN_WIDTH][64];
-        if (threadIdx.x >= 64) {
+    // a workgroup's share of d_w: that of its rows' lanes added up in order
+    if constexpr (ROWS > 1) {
+        __shared__ Acc sums[ROWS - 1][CH * RN_WIDTH][LANES];
+        if (threadIdx.x >= LANES) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < RN_WIDTH; ++i) sums[threadIdx.x / 64 - 1][c][i][lane] = dw[c][i];
+                for (int i = 0; i < RN_WIDTH; ++i) sums[threadIdx.x / LANES - 1][c * RN_WIDTH + i][lane] = dw[c][i];
         }
         __syncthreads();
-        if (threadIdx.x >= 64) return;
+        if (threadIdx.x >= LANES) return;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < RN_WIDTH; ++i)
 #pragma unroll
-                for (int r = 0; r < ROWS - 1; ++r) dw[c][i] += sums[r][c][i][lane];
+                for (int r = 0; r < ROWS - 1; ++r) dw[c][i] += sums[r][c * RN_WIDTH + i][lane];
     }
     Acc *part = static_cast<Acc *>(a.partials) + (int64_t)blockIdx.x * a.D;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const Chunk k = chunk_at(c * LANES + lane, a.D);
-        if (!k.there) continue;
         Vec<Acc, RN_WIDTH> o;
 #pragma unroll
         for (int i = 0; i < RN_WIDTH; ++i) o.e[i] = dw[c][i];
-        store_chunk(part, k, o);
+        store_chunk(part, k[c], o);
     }
 }
 
@@ -303,7 +321,7 @@ __global__ __launch_bounds__(RN_THREADS) void norm_forward_any_kernel(NormArgs a
         const Acc h = value(i);
         sum += h * h;
     }
-    sum = row_sum<RN_THREADS / 64>(sum);
+    sum = row_sum<RN_THREADS>(sum);
     const Acc r = (Acc)1 / sqrt(sum / (Acc)a.D + (Acc)a.eps);
     if (FP8) {
         const int64_t group = a.groups == 1 ? a.D : a.group;
@@ -311,7 +329,7 @@ __global__ __launch_bounds__(RN_THREADS) void norm_forward_any_kernel(NormArgs a
             const int64_t end = (g + 1) * group < a.D ? (g + 1) * group : a.D;
             float top = 0;
             for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS) top = larger(fabsf((float)(value(i) * r * weight(i))), top);
-            float scale = row_max<RN_THREADS / 64>(top) / FP8_LARGEST;
+            float scale = row_max<RN_THREADS>(top) / FP8_LARGEST;
             if (scale == 0.0f) scale = 1.0f;
             if (threadIdx.x == 0) a.scales[row * a.groups + g] = scale;
             for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS)
@@ -339,8 +357,7 @@ template <typename IO, typename Stream> __global__ __launch_bounds__(RN_THREADS)
             squares += v * v;
             dot += v * (Acc)widen(gy[i]) * weight(i);
         }
-        squares = row_sum<RN_THREADS / 64>(squares);
-        dot = row_sum<RN_THREADS / 64>(dot);
+        row_sums<RN_THREADS>(squares, dot);
         const Acc r = (Acc)1 / sqrt(squares / (Acc)a.D + (Acc)a.eps), back = dot * r * r / (Acc)a.D;
         for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) {
             const Acc v = widen(h[i]), u = widen(gy[i]);
@@ -374,27 +391,43 @@ __global__ __launch_bounds__(RW_THREADS) void norm_weights_kernel(NormArgs a, in
     else static_cast<IO *>(a.d_w)[column] = narrow<IO>(s);
 }
 
-constexpr int64_t NARROW = 1024, WIDEST = 8192;          // columns of a row of one wave; of any row in registers
+constexpr int64_t WIDEST = 16384;        // columns of a row in registers
 bool in_registers(int64_t D) { return D >= RN_WIDTH && D <= WIDEST; }
-int64_t rows_of_group(int64_t D) { return in_registers(D) && D <= NARROW ? RN_THREADS / 64 : 1; }
-// Workgroups of the backward: one for each CU before any takes a second row, then as many as are on the chip at once, with four
-// rows of each wave or more, as every workgroup leaves a row of 32-bit sums.
-int64_t backward_groups(int64_t N, int64_t D) {
-    const int64_t rows = rows_of_group(D), need = (N + rows - 1) / rows, few = need < 256 ? need : 256, many = need / 4;
-    return many < few ? few : many < 1024 ? many : 1024;
+// threads of a row (0: the kernels for any width), for chunks of one or two to a thread
+int lanes_of(int64_t D) {
+    return !in_registers(D) ? 0 : D <= 128 ? 16 : D <= 256 ? 32 : D <= 1024 ? 64 : D <= 2048 ? 256 : D <= 8192 ? 512 : 1024;
 }
+int64_t rows_of_group(int64_t D) { return lanes_of(D) == 0 ? 1 : threads_of(lanes_of(D)) / lanes_of(D); }
+// Workgroups of the backward: one for each CU before any takes a second row, then as many as are on the chip at once, with four
+// rows of each thread or more, as every workgroup leaves a row of 32-bit sums.
+int64_t backward_groups(int64_t N, int64_t D) {
+    const int64_t rows = rows_of_group(D), need = (N + rows - 1) / rows, few = need < 256 ? need : 256, many = need / 4;      // (CUs: 256)
+    const int64_t most = 1024 * RN_THREADS / threads_of(lanes_of(D) ? lanes_of(D) : RN_THREADS);
+    return many < few ? few : many < most ? many / 256 * 256 : most;
+}
+// A row's threads and chunks by its width
+#define NORM_BY_WIDTH(RUN, ANY)                                                                                                     \
+    do {                                                                                                                            \
+        const int lanes = lanes_of(a.D);                                                                                            \
+        const bool one = a.D <= (int64_t)lanes * RN_WIDTH;                                                                          \
+        const dim3 threads(lanes == 0 ? RN_THREADS : threads_of(lanes));                                                            \
+        if (lanes == 0) ANY;                                                                                                        \
+        else if (lanes == 16) RUN(16, 1);                                                                                           \
+        else if (lanes == 32) RUN(32, 1);                                                                                           \
+        else if (lanes == 64 && one) RUN(64, 1);                                                                                    \
+        else if (lanes == 64) RUN(64, 2);                                                                                           \
+        else if (lanes == 256) RUN(256, 1);                                                                                         \
+        else if (lanes == 512 && one) RUN(512, 1);                                                                                  \
+        else if (lanes == 512) RUN(512, 2);                                                                                         \
+        else RUN(1024, 2);                                                                                                          \
+    } while (0)
 
 template <typename IO, typename Stream, bool FP8> int forward_of(const NormArgs &a, hipStream_t stream) {
     const int64_t groups = (a.N + rows_of_group(a.D) - 1) / rows_of_group(a.D);
     if (groups > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "norm: too many rows for one launch");
-    const dim3 grid((unsigned)groups), threads(RN_THREADS);
-#define NORM_RUN(W, C) hipLaunchKernelGGL((norm_forward_kernel<IO, Stream, W, C, FP8>), grid, threads, 0, stream, a)
-    if (!in_registers(a.D)) hipLaunchKernelGGL((norm_forward_any_kernel<IO, Stream, FP8>), grid, threads, 0, stream, a);
-    else if (a.D <= 512) NORM_RUN(1, 1);
-    else if (a.D <= 1024) NORM_RUN(1, 2);
-    else if (a.D <= 2048) NORM_RUN(4, 1);
-    else if (a.D <= 4096) NORM_RUN(4, 2);
-    else NORM_RUN(4, 4);
+    const dim3 grid((unsigned)groups);
+#define NORM_RUN(L, C) hipLaunchKernelGGL((norm_forward_kernel<IO, Stream, L, C, FP8>), grid, threads, 0, stream, a)
+    NORM_BY_WIDTH(NORM_RUN, hipLaunchKernelGGL((norm_forward_any_kernel<IO, Stream, FP8>), grid, threads, 0, stream, a));
 #undef NORM_RUN
     return check_hip(hipGetLastError(), "norm_forward_kernel launch");
 }
@@ -402,15 +435,10 @@ template <typename IO, typename Stream, bool FP8> int forward_of(const NormArgs 
 template <typename IO, typename Stream> int backward_of(const NormArgs &a, hipStream_t stream) {
     using Acc = typename AccT<IO>::type;
     const int64_t groups = backward_groups(a.N, a.D);
-    const dim3 grid((unsigned)groups), threads(RN_THREADS);
+    const dim3 grid((unsigned)groups);
     if (a.N > 0) {
-#define NORM_RUN(W, C) hipLaunchKernelGGL((norm_backward_kernel<IO, Stream, W, C>), grid, threads, 0, stream, a)
-        if (!in_registers(a.D)) hipLaunchKernelGGL((norm_backward_any_kernel<IO, Stream>), grid, threads, 0, stream, a);
-        else if (a.D <= 512) NORM_RUN(1, 1);
-        else if (a.D <= 1024) NORM_RUN(1, 2);
-        else if (a.D <= 2048) NORM_RUN(4, 1);
-        else if (a.D <= 4096) NORM_RUN(4, 2);
-        else NORM_RUN(4, 4);
+#define NORM_RUN(L, C) hipLaunchKernelGGL((norm_backward_kernel<IO, Stream, L, C>), grid, threads, 0, stream, a)
+        NORM_BY_WIDTH(NORM_RUN, hipLaunchKernelGGL((norm_backward_any_kernel<IO, Stream>), grid, threads, 0, stream, a));
 #undef NORM_RUN
         const int rc = check_hip(hipGetLastError(), "norm_backward_kernel launch");
         if (rc) return rc;

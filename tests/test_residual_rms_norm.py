@@ -15,7 +15,7 @@ EPS = 1e-5
 TYPES = [(torch.float32,) * 3, (torch.float64,) * 3, (torch.float16,) * 3, (torch.bfloat16,) * 3, (torch.bfloat16, torch.float32, torch.float32),
          (torch.float16, torch.float32, torch.float16), (torch.bfloat16, torch.bfloat16, torch.float32)]
 # rows of less than a chunk, of one wave, of a workgroup, past what stays in registers; odd ones
-SHAPES = [(1, 1), (3, 7), (5, 8), (2, 9), (7, 511), (130, 768), (33, 1021), (1, 1024), (3, 1025), (9, 2047), (2, 4096), (3, 5003), (2, 8192), (2, 8200)]
+SHAPES = [(1, 1), (3, 7), (5, 8), (2, 9), (7, 511), (130, 768), (33, 1021), (1, 1024), (3, 1025), (9, 2047), (2, 4096), (3, 5003), (2, 8192), (2, 8200), (3, 16384), (2, 16390), (9, 100), (65, 256)]
 
 
 def inputs(N, D, types, seed):
@@ -121,7 +121,7 @@ def test_gradients_against_differences():
 @pytest.mark.gpu
 @pytest.mark.parametrize("types", [TYPES[0], TYPES[3], TYPES[5]], ids=str)
 @pytest.mark.parametrize("group", [0, 8, 64, 128, 512])
-@pytest.mark.parametrize("shape", [(1, 8), (3, 5), (4, 100), (5, 768), (3, 1021), (2, 1536), (2, 4100), (2, 9000)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 8), (3, 5), (4, 100), (5, 768), (3, 1021), (2, 1536), (2, 4100), (2, 9000), (2, 16500), (17, 128)], ids=str)
 def test_eight_bits(shape, group, types):
     import t2fw_amd as t2
     (x, res, w), _, _ = inputs(*shape, types, seed=group + shape[1])
