@@ -1,9 +1,9 @@
 // The 2-norm over all gradients of a model, and the gradients scaled to a largest norm:
 //   n = sqrt(sum of g^2),   g <- g min(1, max_norm / (n + 1e-6)).
-// Two launches for up to CLIP_TABLE arrays, whose addresses and sizes travel as kernel arguments.  A workgroup takes chunks of
-// CLIP_CHUNK elements in turn, whichever array they lie in, and leaves one sum; in the second launch every workgroup
-// adds up all sums in the same order, so that the norm does not depend on the order of events.  Squares and sums are
-// carried in double: the conversions and additions hide behind memory, and no square overflows.
+// Two launches for up to CLIP_TABLE arrays, whose addresses and sizes travel as kernel arguments.  The arrays one after the other are cut into
+// equal shares, one for each workgroup (in pieces of CLIP_PIECE elements of one array), which leaves one sum; in the second launch
+// every workgroup adds up all sums in the same order, so that the norm does not depend on the order of events.  Squares and sums
+// are carried in double: the conversions and additions hide behind memory, and no square overflows.
 #include "clip.hpp"
 #include "vec.hpp"
 
@@ -24,79 +24,98 @@ __device__ __forceinline__ double block_sum(double v) {
     return v;
 }
 
-// The array that holds a chunk: the last one whose first chunk is not after it (arrays are not empty)
-__device__ __forceinline__ int array_of(const ClipTable &t, uint32_t chunk) {
+// The array that holds a piece: the last one whose first piece is not after it (arrays are not empty)
+__device__ __forceinline__ int array_of(const ClipTable &t, uint32_t piece) {
     int lo = 0, hi = t.count;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (t.first[mid] <= chunk) lo = mid;
+        if (t.first[mid] <= piece) lo = mid;
         else hi = mid;
     }
     return lo;
 }
 
+// Calls run(array, first element, elements) for what a workgroup's share of the pieces has of each array
+template <typename Run> __device__ __forceinline__ void for_share(const ClipTable &t, uint32_t share, uint32_t shares, const Run &run) {
+    uint32_t piece = (uint32_t)((uint64_t)t.pieces * share / shares);
+    const uint32_t end = (uint32_t)((uint64_t)t.pieces * (share + 1) / shares);
+    if (piece >= end) return;
+    for (int a = array_of(t, piece); piece < end; ++a) {
+        const uint32_t of_array = (t.n[a] + CLIP_PIECE - 1) / CLIP_PIECE, last = t.first[a] + of_array < end ? t.first[a] + of_array : end;
+        const uint32_t from = (piece - t.first[a]) * CLIP_PIECE, to = (last - t.first[a]) * CLIP_PIECE;
+        run(a, from, (to < t.n[a] ? to : t.n[a]) - from);
+        piece = last;
+    }
+}
+
+// Elements 0 .. n - 1 of an array, by the whole workgroup: vectors of VEC, AHEAD of them at a time, and single ones
+template <typename IO, int VEC, int AHEAD, typename Each, typename Single>
+__device__ __forceinline__ void over(const IO *p, uint32_t n, const Each &each, const Single &single) {
+    constexpr uint32_t STEP = CLIP_THREADS * VEC;
+    uint32_t i = 0;
+    for (; i + STEP * AHEAD <= n; i += STEP * AHEAD) {
+        Vec<IO, VEC> v[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) v[u] = load_vec<IO, VEC>(p + i + u * STEP + threadIdx.x * VEC);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) each(i + u * STEP + threadIdx.x * VEC, v[u]);
+    }
+    for (i += threadIdx.x * VEC; i + VEC <= n; i += STEP) each(i, load_vec<IO, VEC>(p + i));
+    // the elements after the last whole vector, which is the one this thread stands at
+    for (; i < n; ++i) single(i, p[i]);
+}
+
 template <typename IO> __device__ __forceinline__ double squares_of(const IO *p, uint32_t n) {
-    constexpr int VEC = 16 / sizeof(IO), U = CLIP_CHUNK / (CLIP_THREADS * VEC);
+    constexpr int VEC = 16 / sizeof(IO);
     double s = 0;
-    if (n == CLIP_CHUNK) {
-        Vec<IO, VEC> v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load_vec<IO, VEC>(p + (u * CLIP_THREADS + threadIdx.x) * VEC);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
+    over<IO, VEC, 8>(
+        p, n,
+        [&](uint32_t, const Vec<IO, VEC> &v) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const double d = (double)widen(v[u].e[i]);
-                s += d * d;
+                const double d = (double)widen(v.e[i]);
+                s = fma(d, d, s);
             }
-        return s;
-    }
-    for (uint32_t i = threadIdx.x; i < n; i += CLIP_THREADS) {
-        const double d = (double)widen(p[i]);
-        s += d * d;
-    }
+        },
+        [&](uint32_t, IO e) {
+            const double d = (double)widen(e);
+            s = fma(d, d, s);
+        });
     return s;
 }
 
 __global__ __launch_bounds__(CLIP_THREADS) void clip_squares_kernel(ClipTable t, double *partials) {
     double s = 0;
-    for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int a = array_of(t, c);
-        const uint32_t at = (c - t.first[a]) * CLIP_CHUNK, left = t.n[a] - at, n = left < CLIP_CHUNK ? left : CLIP_CHUNK;
+    for_share(t, blockIdx.x, gridDim.x, [&](int a, uint32_t from, uint32_t n) {
         switch (t.src_type[a]) {
-            case T2FW_F32: s += squares_of(static_cast<const float *>(t.src[a]) + at, n); break;
-            case T2FW_F16: s += squares_of(static_cast<const _Float16 *>(t.src[a]) + at, n); break;
-            case T2FW_BF16: s += squares_of(static_cast<const __bf16 *>(t.src[a]) + at, n); break;
-            default: s += squares_of(static_cast<const double *>(t.src[a]) + at, n); break;
+            case T2FW_F32: s += squares_of(static_cast<const float *>(t.src[a]) + from, n); break;
+            case T2FW_F16: s += squares_of(static_cast<const _Float16 *>(t.src[a]) + from, n); break;
+            case T2FW_BF16: s += squares_of(static_cast<const __bf16 *>(t.src[a]) + from, n); break;
+            default: s += squares_of(static_cast<const double *>(t.src[a]) + from, n); break;
         }
-    }
+    });
     s = block_sum(s);
     if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-template <typename A, typename B> __device__ __forceinline__ void scale_chunk(const A *src, B *dst, uint32_t n, float by) {
-    constexpr int VEC = 16 / (sizeof(A) > sizeof(B) ? sizeof(A) : sizeof(B)), U = CLIP_CHUNK / (CLIP_THREADS * VEC);
-    if (n == CLIP_CHUNK) {
-        Vec<A, VEC> v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load_vec<A, VEC>(src + (u * CLIP_THREADS + threadIdx.x) * VEC);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
+template <typename A, typename B> __device__ __forceinline__ void scale_share(const A *src, B *dst, uint32_t n, float by) {
+    constexpr int VEC = 16 / (sizeof(A) > sizeof(B) ? sizeof(A) : sizeof(B));
+    over<A, VEC, 8>(
+        src, n,
+        [&](uint32_t i, const Vec<A, VEC> &v) {
             Vec<B, VEC> o;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o.e[i] = narrow<B>(widen(v[u].e[i]) * by);
-            store_vec(dst + (u * CLIP_THREADS + threadIdx.x) * VEC, o);
-        }
-        return;
-    }
-    for (uint32_t i = threadIdx.x; i < n; i += CLIP_THREADS) dst[i] = narrow<B>(widen(src[i]) * by);
+            for (int j = 0; j < VEC; ++j) o.e[j] = narrow<B>(widen(v.e[j]) * by);
+            store_past(dst + i, o);
+        },
+        [&](uint32_t i, A e) { dst[i] = narrow<B>(widen(e) * by); });
 }
 template <typename A> __device__ __forceinline__ void scale_from(const A *src, void *dst, int dst_type, uint32_t at, uint32_t n, float by) {
     switch (dst_type) {
-        case T2FW_F32: scale_chunk(src + at, static_cast<float *>(dst) + at, n, by); break;
-        case T2FW_F16: scale_chunk(src + at, static_cast<_Float16 *>(dst) + at, n, by); break;
-        case T2FW_BF16: scale_chunk(src + at, static_cast<__bf16 *>(dst) + at, n, by); break;
-        default: scale_chunk(src + at, static_cast<double *>(dst) + at, n, by); break;
+        case T2FW_F32: scale_share(src + at, static_cast<float *>(dst) + at, n, by); break;
+        case T2FW_F16: scale_share(src + at, static_cast<_Float16 *>(dst) + at, n, by); break;
+        case T2FW_BF16: scale_share(src + at, static_cast<__bf16 *>(dst) + at, n, by); break;
+        default: scale_share(src + at, static_cast<double *>(dst) + at, n, by); break;
     }
 }
 
@@ -106,18 +125,18 @@ __global__ __launch_bounds__(CLIP_THREADS) void clip_scale_kernel(ClipTable t, c
     const float n = (float)sqrt(block_sum(s));
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
     const float ratio = max_norm / (n + 1e-6f), by = ratio > 1.0f ? 1.0f : ratio;         // a norm that is NaN makes NaN of everything
-    for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int a = array_of(t, c);
+    // From the last array to the first, and with stores that leave the last-level cache alone: it still holds much of what the sums have just
+    // read.  119 M bf16 gradients into float32: 204 us with ordinary stores, 157 so (713 MB at the rate of a copy: 143).
+    for_share(t, gridDim.x - 1 - blockIdx.x, gridDim.x, [&](int a, uint32_t from, uint32_t m) {
         // not wanted; or in place and within the limit: nothing changes
-        if (t.dst[a] == nullptr || (by == 1.0f && t.dst[a] == t.src[a])) continue;
-        const uint32_t at = (c - t.first[a]) * CLIP_CHUNK, left = t.n[a] - at, m = left < CLIP_CHUNK ? left : CLIP_CHUNK;
+        if (t.dst[a] == nullptr || (by == 1.0f && t.dst[a] == t.src[a])) return;
         switch (t.src_type[a]) {
-            case T2FW_F32: scale_from(static_cast<const float *>(t.src[a]), t.dst[a], t.dst_type[a], at, m, by); break;
-            case T2FW_F16: scale_from(static_cast<const _Float16 *>(t.src[a]), t.dst[a], t.dst_type[a], at, m, by); break;
-            case T2FW_BF16: scale_from(static_cast<const __bf16 *>(t.src[a]), t.dst[a], t.dst_type[a], at, m, by); break;
-            default: scale_from(static_cast<const double *>(t.src[a]), t.dst[a], t.dst_type[a], at, m, by); break;
+            case T2FW_F32: scale_from(static_cast<const float *>(t.src[a]), t.dst[a], t.dst_type[a], from, m, by); break;
+            case T2FW_F16: scale_from(static_cast<const _Float16 *>(t.src[a]), t.dst[a], t.dst_type[a], from, m, by); break;
+            case T2FW_BF16: scale_from(static_cast<const __bf16 *>(t.src[a]), t.dst[a], t.dst_type[a], from, m, by); break;
+            default: scale_from(static_cast<const double *>(t.src[a]), t.dst[a], t.dst_type[a], from, m, by); break;
         }
-    }
+    });
 }
 
 }  // namespace

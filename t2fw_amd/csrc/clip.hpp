@@ -6,17 +6,17 @@
 namespace t2fw {
 
 constexpr int CLIP_TABLE = 144;          // arrays of one launch: the table travels as kernel arguments (4 KB)
-constexpr int CLIP_CHUNK = 8192;         // elements that a workgroup takes at a time
-constexpr int CLIP_GROUPS = 2048;        // workgroups of a launch, at most
+constexpr int CLIP_PIECE = 2048;         // elements that are not shared between workgroups: whole vectors for all threads
+constexpr int CLIP_GROUPS = 1024;        // workgroups of a launch, at most
 
 struct ClipTable {
     const void *src[CLIP_TABLE];
     void *dst[CLIP_TABLE];
     uint32_t n[CLIP_TABLE];              // elements (longer arrays take several entries)
-    uint32_t first[CLIP_TABLE];          // chunks before this array
+    uint32_t first[CLIP_TABLE];          // pieces before this array
     uint8_t src_type[CLIP_TABLE], dst_type[CLIP_TABLE];
     int32_t count;
-    uint32_t chunks;
+    uint32_t pieces;
 };
 
 // sums of squares of a table's arrays, one for each workgroup, to partials[0 .. groups)

@@ -102,7 +102,7 @@ int check_loss(int64_t N, int64_t V, int32_t dtype) {
 int clip_tables(std::vector<ClipTable> &tables, const t2fw_clip_desc *arrays, int64_t count) {
     if (count < 0 || count > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "clipping: %lld arrays", (long long)count);
     if (count > 0 && arrays == nullptr) return fail(T2FW_ERR_NULL_POINTER, "null array list");
-    constexpr int64_t MOST = (int64_t)CLIP_CHUNK << 17;              // elements of one entry: 2^30, a whole number of chunks
+    constexpr int64_t MOST = (int64_t)CLIP_PIECE << 19;              // elements of one entry: 2^30, a whole number of pieces
     for (int64_t i = 0; i < count; ++i) {
         const t2fw_clip_desc &d = arrays[i];
         const size_t es = size_of(d.src_dtype), ed = size_of(d.dst_dtype);
@@ -114,22 +114,22 @@ int clip_tables(std::vector<ClipTable> &tables, const t2fw_clip_desc *arrays, in
         if (d.dst == d.src && d.dst != nullptr && d.src_dtype != d.dst_dtype)
             return fail(T2FW_ERR_BAD_DTYPE, "clipping in place: the array has two types");
         for (int64_t at = 0; at < d.n; at += MOST) {
-            if (tables.empty() || tables.back().count == CLIP_TABLE || tables.back().chunks > (1u << 30)) tables.push_back(ClipTable{});
+            if (tables.empty() || tables.back().count == CLIP_TABLE || tables.back().pieces > (1u << 30)) tables.push_back(ClipTable{});
             ClipTable &t = tables.back();
             const int64_t n = d.n - at < MOST ? d.n - at : MOST;
             t.src[t.count] = static_cast<const char *>(d.src) + at * es;
             t.dst[t.count] = d.dst == nullptr ? nullptr : static_cast<char *>(d.dst) + at * ed;
             t.n[t.count] = (uint32_t)n;
-            t.first[t.count] = t.chunks;
+            t.first[t.count] = t.pieces;
             t.src_type[t.count] = (uint8_t)d.src_dtype;
             t.dst_type[t.count] = (uint8_t)d.dst_dtype;
-            t.chunks += (uint32_t)((n + CLIP_CHUNK - 1) / CLIP_CHUNK);
+            t.pieces += (uint32_t)((n + CLIP_PIECE - 1) / CLIP_PIECE);
             ++t.count;
         }
     }
     return T2FW_OK;
 }
-int clip_groups(const ClipTable &t) { return t.chunks < (uint32_t)CLIP_GROUPS ? (int)t.chunks : CLIP_GROUPS; }
+int clip_groups(const ClipTable &t) { return t.pieces < (uint32_t)CLIP_GROUPS ? (int)t.pieces : CLIP_GROUPS; }
 
 }  // namespace
 }  // namespace t2fw

@@ -18,6 +18,15 @@ template <typename IO, int N> __device__ __forceinline__ Vec<IO, N> load_vec(con
 }
 template <typename IO, int N> __device__ __forceinline__ void store_vec(IO *p, const Vec<IO, N> &v) { __builtin_memcpy(p, &v, sizeof(v)); }
 
+// The same past the last-level cache, for results that are not read soon where what is in there still is
+template <typename IO, int N> __device__ __forceinline__ void store_past(IO *p, const Vec<IO, N> &v) {
+    static_assert(sizeof(v) % 4 == 0, "whole words");
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(v) / 4), aligned(sizeof(IO))));
+    Words w;
+    __builtin_memcpy(&w, &v, sizeof(v));
+    __builtin_nontemporal_store(w, reinterpret_cast<Words *>(p));
+}
+
 // Conversions by the hardware's instructions; to 16 bits with rounding to the nearest
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ double widen(double v) { return v; }
