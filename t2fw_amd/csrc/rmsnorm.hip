@@ -4,10 +4,10 @@
 // The norm is of the rounded h, the one that the backward finds again; sums are carried in 32 bits (64 for double).
 // In 8 bits: y is divided by scale = max |y| / 448 of the row, or of each group of its columns, and rounded to float8 e4m3.
 //
-// A row stays in registers between its sums and its results: LANES threads hold it in chunks of 8 columns, CH of them each: 16 or 32
-// lanes of a wave for narrow rows, a wave, or 4 to 16 waves.  Every load of a row is made before its sums, without a branch between
-// them, also by lanes that have no columns left.  Where the width is no multiple of 8 the last chunk of a row is loaded
-// from 8 columns before its end, and the columns that belong to the chunk before it are left out.
+// A row stays in registers between its sums and its results: LANES threads hold it in chunks of 16 bytes of the stream, CH of them each, so that a
+// wave's loads and stores are of whole lines: 16 or 32 lanes of a wave for narrow rows, a wave, or 4 to 16 waves.  Every load of a row is made before its sums, without a branch between
+// them, also by lanes that have no columns left.  Where the width is no multiple of a chunk the last one of a row is loaded
+// from a chunk's width before its end, and the columns that belong to the chunk before it are left out.
 #include "rmsnorm.hpp"
 #include "vec.hpp"
 
@@ -15,7 +15,7 @@ namespace t2fw {
 namespace {
 
 constexpr int RN_THREADS = 256;
-constexpr int RN_WIDTH = 8;              // columns of a chunk
+constexpr int RN_WIDTH = 8;              // columns of a thread, in one chunk or two
 constexpr float FP8_LARGEST = 448.0f;
 
 template <typename IO> struct AccT { using type = float; };
@@ -76,84 +76,81 @@ template <int LANES> __device__ __forceinline__ float row_max(float v) {
     return v;
 }
 
-// 8 columns as they lie in memory
-template <typename T> struct Eight {
-    Raw16 raw[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T *p) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) raw[i] = load_raw(p + i * (16 / sizeof(T)));
-    }
-    __device__ __forceinline__ float get(int i) const { return element<T>(raw[i / (16 / sizeof(T))], i % (16 / sizeof(T))); }
+// W columns as they lie in memory
+template <typename T, int W> struct Piece {
+    uint32_t w[sizeof(T) * W / 4];
+    __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, p, sizeof(w)); }
+    __device__ __forceinline__ float get(int i) const { return element_of<T>(w, i); }
 };
-template <> struct Eight<double> {
-    Vec<double, RN_WIDTH> v;
-    __device__ __forceinline__ void load(const double *p) { v = load_vec<double, RN_WIDTH>(p); }
+template <int W> struct Piece<double, W> {
+    Vec<double, W> v;
+    __device__ __forceinline__ void load(const double *p) { v = load_vec<double, W>(p); }
     __device__ __forceinline__ double get(int i) const { return v.e[i]; }
 };
 
-// A chunk of a row: its first column, where it is loaded from, how many of the loaded columns are not its own (8: it is past the end)
-struct Chunk {
+// A chunk of a row: its first column, where it is loaded from, how many of the loaded columns are not its own (W: it is past the end)
+template <int W> struct Chunk {
     int column, from, skip;
-    __device__ __forceinline__ bool there() const { return skip < RN_WIDTH; }
+    __device__ __forceinline__ bool there() const { return skip < W; }
 };
-__device__ __forceinline__ Chunk chunk_at(int index, int D) {
-    Chunk c;
-    c.column = index * RN_WIDTH;
-    c.from = c.column + RN_WIDTH <= D ? c.column : D - RN_WIDTH;
-    c.skip = c.column < D ? c.column - c.from : RN_WIDTH;
+template <int W> __device__ __forceinline__ Chunk<W> chunk_at(int index, int D) {
+    Chunk<W> c;
+    c.column = index * W;
+    c.from = c.column + W <= D ? c.column : D - W;
+    c.skip = c.column < D ? c.column - c.from : W;
     return c;
 }
-template <typename T> __device__ __forceinline__ void store_chunk(T *row, const Chunk &c, const Vec<T, RN_WIDTH> &v) {
+template <typename T, int W> __device__ __forceinline__ void store_chunk(T *row, const Chunk<W> &c, const Vec<T, W> &v) {
     if (c.skip == 0) {
         store_vec(row + c.from, v);
     } else if (c.there()) {
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i)
+        for (int i = 0; i < W; ++i)
             if (i >= c.skip) row[c.from + i] = v.e[i];
     }
 }
-template <typename IO, typename Acc> __device__ __forceinline__ void load_weights(Acc (&o)[RN_WIDTH], const NormArgs &a, int from) {
+template <typename IO, typename Acc, int W> __device__ __forceinline__ void load_weights(Acc (&o)[W], const NormArgs &a, int from) {
     if (a.wide_w) {
-        const Vec<float, RN_WIDTH> v = load_vec<float, RN_WIDTH>(static_cast<const float *>(a.w) + from);
+        const Vec<float, W> v = load_vec<float, W>(static_cast<const float *>(a.w) + from);
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i) o[i] = v.e[i];
+        for (int i = 0; i < W; ++i) o[i] = v.e[i];
     } else {
-        Eight<IO> v;
+        Piece<IO, W> v;
         v.load(static_cast<const IO *>(a.w) + from);
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i) o[i] = v.get(i);
+        for (int i = 0; i < W; ++i) o[i] = v.get(i);
     }
 }
 
 constexpr int threads_of(int lanes) { return lanes < RN_THREADS ? RN_THREADS : lanes; }
 
-template <typename IO, typename Stream, int LANES, int CH, bool FP8>
+template <typename IO, typename Stream, int LANES, int CH, int W, bool FP8>
 __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArgs a) {
     using Acc = typename AccT<IO>::type;
     constexpr int ROWS = threads_of(LANES) / LANES;
     const int D = (int)a.D, lane = threadIdx.x % LANES;
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES, base = (row < a.N ? row : a.N - 1) * a.D;
     const bool live = row < a.N;                         // (rows past the end compute with the last one, and store nothing)
-    Chunk k[CH];
-    Eight<IO> x[CH];
-    Eight<Stream> res[CH];
+    Chunk<W> k[CH];
+    Piece<IO, W> x[CH];
+    Piece<Stream, W> res[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        k[c] = chunk_at(c * LANES + lane, D);
+        k[c] = chunk_at<W>(c * LANES + lane, D);
         x[c].load(static_cast<const IO *>(a.x) + base + k[c].from);
     }
     if (a.res != nullptr) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) res[c].load(static_cast<const Stream *>(a.res) + base + k[c].from);
     }
-    Acc w[CH][RN_WIDTH], h[CH][RN_WIDTH], sum = 0;
+    Acc w[CH][W], h[CH][W], sum = 0;
 #pragma unroll
-    for (int c = 0; c < CH; ++c) load_weights<IO>(w[c], a, k[c].from);
+    for (int c = 0; c < CH; ++c) load_weights<IO, Acc, W>(w[c], a, k[c].from);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        Vec<Stream, RN_WIDTH> o;
+        Vec<Stream, W> o;
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i) {
+        for (int i = 0; i < W; ++i) {
             h[c][i] = x[c].get(i);
             if (a.res != nullptr) h[c][i] += res[c].get(i);
             o.e[i] = narrow<Stream>(h[c][i]);
@@ -167,13 +164,13 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i) h[c][i] *= r * w[c][i];
+        for (int i = 0; i < W; ++i) h[c][i] *= r * w[c][i];
     if constexpr (!FP8) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            Vec<IO, RN_WIDTH> o;
+            Vec<IO, W> o;
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; ++i) o.e[i] = narrow<IO>(h[c][i]);
+            for (int i = 0; i < W; ++i) o.e[i] = narrow<IO>(h[c][i]);
             if (live) store_chunk(static_cast<IO *>(a.y) + base, k[c], o);
         }
     } else {
@@ -182,7 +179,7 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
         for (int c = 0; c < CH; ++c) {
             top[c] = 0;
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; ++i)
+            for (int i = 0; i < W; ++i)
                 if (i >= k[c].skip) top[c] = larger(fabsf(h[c][i]), top[c]);
             all = larger(top[c], all);
         }
@@ -191,7 +188,7 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             // a group's chunks are neighbouring lanes of one wave, those past the end of the row among them
-            float scale = (by_row ? all : lanes_max(top[c], (int)(a.group / RN_WIDTH))) / FP8_LARGEST;
+            float scale = (by_row ? all : lanes_max(top[c], (int)(a.group / W))) / FP8_LARGEST;
             if (scale == 0.0f) scale = 1.0f;
             if (!live || !k[c].there()) continue;
             const int64_t g = by_row ? 0 : k[c].column / a.group;
@@ -201,40 +198,40 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
             const bool tiny = scale < 1e-35f;
             uint32_t words[2];
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; i += 4) {
+            for (int i = 0; i < W; i += 4) {
                 float v[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = tiny ? h[c][i + j] / scale : h[c][i + j] * by;
                 const int word = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
                 words[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], word, true);
             }
-            Vec<uint8_t, RN_WIDTH> o;
+            Vec<uint8_t, W> o;
             __builtin_memcpy(&o, words, sizeof(o));
             store_chunk(static_cast<uint8_t *>(a.q) + base, k[c], o);
         }
     }
 }
 
-template <typename IO, typename Stream, int LANES, int CH>
+template <typename IO, typename Stream, int LANES, int CH, int W>
 __global__ __launch_bounds__(threads_of(LANES)) void norm_backward_kernel(NormArgs a) {
     using Acc = typename AccT<IO>::type;
     constexpr int THREADS = threads_of(LANES), ROWS = THREADS / LANES;
     const int D = (int)a.D, lane = threadIdx.x % LANES;
-    Acc dw[CH][RN_WIDTH], w[CH][RN_WIDTH];
-    Chunk k[CH];
+    Acc dw[CH][W], w[CH][W];
+    Chunk<W> k[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        k[c] = chunk_at(c * LANES + lane, D);
-        load_weights<IO>(w[c], a, k[c].from);
+        k[c] = chunk_at<W>(c * LANES + lane, D);
+        load_weights<IO, Acc, W>(w[c], a, k[c].from);
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i) dw[c][i] = 0;
+        for (int i = 0; i < W; ++i) dw[c][i] = 0;
     }
     // (all rows of a workgroup go round together)
     for (int64_t first = (int64_t)blockIdx.x * ROWS; first < a.N; first += (int64_t)gridDim.x * ROWS) {
         const int64_t row = first + threadIdx.x / LANES, base = (row < a.N ? row : a.N - 1) * a.D;
         const bool live = row < a.N;
-        Eight<Stream> h[CH], gr[CH];
-        Eight<IO> u[CH];
+        Piece<Stream, W> h[CH], gr[CH];
+        Piece<IO, W> u[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             h[c].load(static_cast<const Stream *>(a.stored) + base + k[c].from);
@@ -248,7 +245,7 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_backward_kernel(NormAr
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; ++i) {
+            for (int i = 0; i < W; ++i) {
                 const Acc v = h[c].get(i);
                 squares += i >= k[c].skip ? v * v : (Acc)0;
                 dot += i >= k[c].skip ? v * u[c].get(i) * w[c][i] : (Acc)0;
@@ -258,10 +255,10 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_backward_kernel(NormAr
         const Acc counts = live ? r : (Acc)0;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            Vec<IO, RN_WIDTH> o;
-            Vec<Stream, RN_WIDTH> os;
+            Vec<IO, W> o;
+            Vec<Stream, W> os;
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; ++i) {
+            for (int i = 0; i < W; ++i) {
                 const Acc v = h[c].get(i), t = u[c].get(i);
                 if (live) dw[c][i] += t * v * counts;
                 Acc g = r * (t * w[c][i] - v * back);
@@ -276,28 +273,28 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_backward_kernel(NormAr
     }
     // a workgroup's share of d_w: that of its rows' lanes added up in order
     if constexpr (ROWS > 1) {
-        __shared__ Acc sums[ROWS - 1][CH * RN_WIDTH][LANES];
+        __shared__ Acc sums[ROWS - 1][CH * W][LANES];
         if (threadIdx.x >= LANES) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < RN_WIDTH; ++i) sums[threadIdx.x / LANES - 1][c * RN_WIDTH + i][lane] = dw[c][i];
+                for (int i = 0; i < W; ++i) sums[threadIdx.x / LANES - 1][c * W + i][lane] = dw[c][i];
         }
         __syncthreads();
         if (threadIdx.x >= LANES) return;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int i = 0; i < RN_WIDTH; ++i)
+            for (int i = 0; i < W; ++i)
 #pragma unroll
-                for (int r = 0; r < ROWS - 1; ++r) dw[c][i] += sums[r][c * RN_WIDTH + i][lane];
+                for (int r = 0; r < ROWS - 1; ++r) dw[c][i] += sums[r][c * W + i][lane];
     }
     Acc *part = static_cast<Acc *>(a.partials) + (int64_t)blockIdx.x * a.D;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        Vec<Acc, RN_WIDTH> o;
+        Vec<Acc, W> o;
 #pragma unroll
-        for (int i = 0; i < RN_WIDTH; ++i) o.e[i] = dw[c][i];
+        for (int i = 0; i < W; ++i) o.e[i] = dw[c][i];
         store_chunk(part, k[c], o);
     }
 }
@@ -391,6 +388,7 @@ __global__ __launch_bounds__(RW_THREADS) void norm_weights_kernel(NormArgs a, in
     else static_cast<IO *>(a.d_w)[column] = narrow<IO>(s);
 }
 
+template <typename Stream> constexpr int chunk_of() { return sizeof(Stream) == 2 ? 8 : 4; }
 constexpr int64_t WIDEST = 16384;        // columns of a row in registers
 bool in_registers(int64_t D) { return D >= RN_WIDTH && D <= WIDEST; }
 // threads of a row (0: the kernels for any width), for chunks of one or two to a thread
@@ -398,12 +396,14 @@ int lanes_of(int64_t D) {
     return !in_registers(D) ? 0 : D <= 128 ? 16 : D <= 256 ? 32 : D <= 1024 ? 64 : D <= 2048 ? 256 : D <= 8192 ? 512 : 1024;
 }
 int64_t rows_of_group(int64_t D) { return lanes_of(D) == 0 ? 1 : threads_of(lanes_of(D)) / lanes_of(D); }
-// Workgroups of the backward: one for each CU before any takes a second row, then as many as are on the chip at once, with four
-// rows of each thread or more, as every workgroup leaves a row of 32-bit sums.
+// Workgroups of the backward: one for each of the 256 CUs before any takes a second round of rows, then as many as are on the chip at
+// once, with at least four rounds each, as every workgroup leaves a row of 32-bit sums; all with the same number of rounds.
 int64_t backward_groups(int64_t N, int64_t D) {
-    const int64_t rows = rows_of_group(D), need = (N + rows - 1) / rows, few = need < 256 ? need : 256, many = need / 4;      // (CUs: 256)
+    const int64_t rows = rows_of_group(D), rounds = (N + rows - 1) / rows;
     const int64_t most = 1024 * RN_THREADS / threads_of(lanes_of(D) ? lanes_of(D) : RN_THREADS);
-    return many < few ? few : many < most ? many / 256 * 256 : most;
+    if (rounds <= 1024) return rounds < 256 ? rounds : 256;
+    const int64_t each = rounds <= 4 * most ? 4 : (rounds + most - 1) / most;
+    return (rounds + each - 1) / each;
 }
 // A row's threads and chunks by its width
 #define NORM_BY_WIDTH(RUN, ANY)                                                                                                     \
@@ -426,7 +426,9 @@ template <typename IO, typename Stream, bool FP8> int forward_of(const NormArgs 
     const int64_t groups = (a.N + rows_of_group(a.D) - 1) / rows_of_group(a.D);
     if (groups > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "norm: too many rows for one launch");
     const dim3 grid((unsigned)groups);
-#define NORM_RUN(L, C) hipLaunchKernelGGL((norm_forward_kernel<IO, Stream, L, C, FP8>), grid, threads, 0, stream, a)
+    // 8 bits: a chunk is 8 columns in every type, as a group's chunks have to be in one wave
+    constexpr int W = FP8 ? RN_WIDTH : chunk_of<Stream>(), PER = RN_WIDTH / W;
+#define NORM_RUN(L, C) hipLaunchKernelGGL((norm_forward_kernel<IO, Stream, L, C * PER, W, FP8>), grid, threads, 0, stream, a)
     NORM_BY_WIDTH(NORM_RUN, hipLaunchKernelGGL((norm_forward_any_kernel<IO, Stream, FP8>), grid, threads, 0, stream, a));
 #undef NORM_RUN
     return check_hip(hipGetLastError(), "norm_forward_kernel launch");
@@ -437,7 +439,8 @@ template <typename IO, typename Stream> int backward_of(const NormArgs &a, hipSt
     const int64_t groups = backward_groups(a.N, a.D);
     const dim3 grid((unsigned)groups);
     if (a.N > 0) {
-#define NORM_RUN(L, C) hipLaunchKernelGGL((norm_backward_kernel<IO, Stream, L, C>), grid, threads, 0, stream, a)
+    constexpr int W = chunk_of<Stream>(), PER = RN_WIDTH / W;
+#define NORM_RUN(L, C) hipLaunchKernelGGL((norm_backward_kernel<IO, Stream, L, C * PER, W>), grid, threads, 0, stream, a)
         NORM_BY_WIDTH(NORM_RUN, hipLaunchKernelGGL((norm_backward_any_kernel<IO, Stream>), grid, threads, 0, stream, a));
 #undef NORM_RUN
         const int rc = check_hip(hipGetLastError(), "norm_backward_kernel launch");

@@ -44,13 +44,14 @@ __device__ __forceinline__ Raw16 load_raw(const void *p) {
     __builtin_memcpy(&r, p, sizeof(r));
     return r;
 }
-template <typename IO> __device__ __forceinline__ float element(const Raw16 &r, int j);
-template <> __device__ __forceinline__ float element<float>(const Raw16 &r, int j) { return __uint_as_float(r.w[j]); }
-template <> __device__ __forceinline__ float element<__bf16>(const Raw16 &r, int j) {
-    return __uint_as_float(j % 2 ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
+template <typename IO> __device__ __forceinline__ float element_of(const uint32_t *w, int j);
+template <> __device__ __forceinline__ float element_of<float>(const uint32_t *w, int j) { return __uint_as_float(w[j]); }
+template <> __device__ __forceinline__ float element_of<__bf16>(const uint32_t *w, int j) {
+    return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
 }
-template <> __device__ __forceinline__ float element<_Float16>(const Raw16 &r, int j) {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)(j % 2 ? r.w[j / 2] >> 16 : r.w[j / 2]));
+template <> __device__ __forceinline__ float element_of<_Float16>(const uint32_t *w, int j) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(j % 2 ? w[j / 2] >> 16 : w[j / 2]));
 }
+template <typename IO> __device__ __forceinline__ float element(const Raw16 &r, int j) { return element_of<IO>(r.w, j); }
 
 }  // namespace t2fw
