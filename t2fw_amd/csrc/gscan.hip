@@ -121,6 +121,7 @@ template <typename IO, int VEC> struct Held {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) d.e[v] = narrow<IO>(x);
     }
+    __device__ __forceinline__ void as_it_came() {}      // 32-bit numbers take no more once they are made
 };
 template <typename IO> struct Held16 {
     static constexpr int PAIR = 2;
@@ -135,6 +136,12 @@ template <typename IO> struct Held16 {
     __device__ __forceinline__ void fill(float x) {
 #pragma unroll
         for (int v = 0; v < 8; v += 2) put(v, {x, x});
+    }
+    // What has been made of it (32-bit numbers, gates) is made again from here on, rather than kept in two or four times the registers:
+    // more workgroups on a CU, whose waits overlap (32 x 4096 x 1024 bf16 with logits: backward 311 us with the gates kept, 273 so).
+    __device__ __forceinline__ void as_it_came() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(d.w[i]));
     }
 };
 template <> struct Held<_Float16, 8> : Held16<_Float16> {};
@@ -167,26 +174,20 @@ __device__ __forceinline__ void store_steps(void *base, Held<IO, VEC> (&v)[R], i
     }
 }
 
-template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
-__device__ __forceinline__ void gates_of(Acc (&g)[R][VEC], const Held<IO, VEC> (&f)[R]) {
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const Acc z = f[r].get(v);
-            g[r][v] = LOGITS ? gate_of<IO>(z) : z;
-        }
+template <typename IO, typename Acc, bool LOGITS, int VEC> __device__ __forceinline__ Acc gate_at(const Held<IO, VEC> &f, int v) {
+    const Acc z = f.get(v);
+    return LOGITS ? gate_of<IO>(z) : z;
 }
 constexpr float gate_beyond(bool logits) { return logits ? INFINITY : 1.0f; }
 
-// The map of a channel over a stretch, forward in time, or of its adjoint, backward
+// The map of a channel over a stretch of gates g, forward in time, or of its adjoint, backward
 template <typename IO, typename Acc, int VEC, int R, bool BACK>
-__device__ __forceinline__ Map<Acc> fold_steps(const Acc (&g)[R][VEC], const Held<IO, VEC> (&x)[R], int v) {
+__device__ __forceinline__ Map<Acc> fold_steps(const Acc (&g)[R], const Held<IO, VEC> (&x)[R], int v) {
     Map<Acc> m{1, 0};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int r = BACK ? R - 1 - i : i;
-        m = extended<BACK>(m, g[r][v], (Acc)x[r].get(v));
+        m = extended<BACK>(m, g[r], (Acc)x[r].get(v));
     }
     return m;
 }
@@ -359,10 +360,13 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, Gsc
     load_steps<IO, VEC, R>(x, BACK ? a.g_out : a.x, BACK ? a.g_b : a.x_b, BACK ? a.g_t : a.x_t, p);
     beyond_end<IO, VEC, R>(f, p, gate_beyond(LOGITS));
     beyond_end<IO, VEC, R>(x, p, 0.0f);
-    Acc g[R][VEC];
-    gates_of<IO, Acc, VEC, R, LOGITS>(g, f);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, BACK>(g, x, v);
+    for (int v = 0; v < VEC; ++v) {
+        Acc g[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) g[r] = gate_at<IO, Acc, LOGITS>(f[r], v);
+        maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, BACK>(g, x, v);
+    }
     __syncthreads();
     if (threadIdx.x >= GS_CHANNELS) return;
     Map<Acc> all{1, 0};
@@ -374,7 +378,7 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, Gsc
 }
 
 template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
-__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_forward_kernel(GscanArgs a, GscanGrid gr) {
+__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 ? 5 : 4) void gscan_forward_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];
     const Turn turn = turn_of(gr);
@@ -383,18 +387,23 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_fo
     int64_t at = 0;
     const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
     Acc h = there && a.s0 != nullptr ? static_cast<const Acc *>(a.s0)[at] : (Acc)0;
-    Held<IO, VEC> x[R];
-    Acc g[R][VEC];
-    {
-        Held<IO, VEC> f[R];
-        load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
-        load_steps<IO, VEC, R>(x, a.x, a.x_b, a.x_t, p);
-        beyond_end<IO, VEC, R>(f, p, gate_beyond(LOGITS));
-        beyond_end<IO, VEC, R>(x, p, 0.0f);
-        gates_of<IO, Acc, VEC, R, LOGITS>(g, f);
+    Held<IO, VEC> x[R], f[R];
+    load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
+    load_steps<IO, VEC, R>(x, a.x, a.x_b, a.x_t, p);
+    beyond_end<IO, VEC, R>(f, p, gate_beyond(LOGITS));
+    beyond_end<IO, VEC, R>(x, p, 0.0f);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        Acc g[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) g[r] = gate_at<IO, Acc, LOGITS>(f[r], v);
+        maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v);
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v);
+    for (int r = 0; r < R; ++r) {
+        x[r].as_it_came();
+        f[r].as_it_came();
+    }
     __syncthreads();
     Map<Acc> own{1, 0};
     if (first) {
@@ -415,7 +424,7 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_fo
         if (there && chunk == gr.chunks - 1) static_cast<Acc *>(a.final_state)[at] = h;
     }
     __syncthreads();
-    Held<IO, VEC> o[R];
+    // the results take their inputs' registers
 #pragma unroll
     for (int v = 0; v < VEC; v += PAIR) {
         Acc s[PAIR];
@@ -426,17 +435,17 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 4) void gscan_fo
             Acc out[PAIR];
 #pragma unroll
             for (int j = 0; j < PAIR; ++j) {
-                s[j] = g[r][v + j] * s[j] + (Acc)x[r].get(v + j);
+                s[j] = fused(gate_at<IO, Acc, LOGITS>(f[r], v + j), s[j], (Acc)x[r].get(v + j));
                 out[j] = s[j];
             }
-            o[r].put(v, out);
+            x[r].put(v, out);
         }
     }
-    store_steps<IO, VEC, R>(a.out, o, a.D, a.T, p);
+    store_steps<IO, VEC, R>(a.out, x, a.D, a.T, p);
 }
 
 template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
-__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 2) void gscan_backward_kernel(GscanArgs a, GscanGrid gr) {
+__global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 ? 4 : 2) void gscan_backward_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];           // states: forward in time
     __shared__ Acc sums[TG][GS_CHANNELS];                // adjoints: backward, with the same gate products
@@ -454,12 +463,19 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 2) void gscan_ba
     beyond_end<IO, VEC, R>(f, p, gate_beyond(LOGITS));
     beyond_end<IO, VEC, R>(go, p, 0.0f);
     beyond_end<IO, VEC, R>(x, p, 0.0f);
-    Acc g[R][VEC];
-    gates_of<IO, Acc, VEC, R, LOGITS>(g, f);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
+        Acc g[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) g[r] = gate_at<IO, Acc, LOGITS>(f[r], v);
         maps[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, false>(g, x, v);
         sums[p.group][p.lane * VEC + v] = fold_steps<IO, Acc, VEC, R, true>(g, go, v).s;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        x[r].as_it_came();
+        f[r].as_it_came();
+        go[r].as_it_came();
     }
     __syncthreads();
     Map<Acc> own{1, 0};
@@ -489,15 +505,16 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 2) void gscan_ba
     // the results take their inputs' registers
 #pragma unroll
     for (int v = 0; v < VEC; v += PAIR) {
-        Acc before[R][PAIR], after[PAIR];
+        Acc before[R][PAIR], g[R][PAIR], later[PAIR];
 #pragma unroll
         for (int j = 0; j < PAIR; ++j) {
             Acc h = maps[p.group][p.lane * VEC + v + j].s;
-            after[j] = sums[p.group][p.lane * VEC + v + j];
+            later[j] = sums[p.group][p.lane * VEC + v + j];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+                g[r][j] = gate_at<IO, Acc, LOGITS>(f[r], v + j);
                 before[r][j] = h;
-                h = g[r][v + j] * h + (Acc)x[r].get(v + j);
+                h = fused(g[r][j], h, (Acc)x[r].get(v + j));
             }
         }
 #pragma unroll
@@ -505,8 +522,8 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : 2) void gscan_ba
             Acc dx[PAIR], df[PAIR];
 #pragma unroll
             for (int j = 0; j < PAIR; ++j) {
-                const Acc d = (Acc)go[r].get(v + j) + after[j];
-                after[j] = g[r][v + j] * d;
+                const Acc d = (Acc)go[r].get(v + j) + later[j];
+                later[j] = g[r][j] * d;
                 const Acc slope = LOGITS ? (Acc)gate_slope<IO>((Acc)f[r].get(v + j)) : (Acc)1;
                 dx[j] = d;
                 df[j] = d * before[r][j] * slope;
