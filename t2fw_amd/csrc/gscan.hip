@@ -71,6 +71,7 @@ template <typename IO> __device__ __forceinline__ double gate_slope(double z) {
 
 // How a call is cut: slots of a row, workgroups side by side, chunks of the sequence, columns of one chunk in the scratch, chunks of a
 // group
+constexpr int ALL_AT_ONCE = 2048;        // workgroups: less than two rounds of the chip
 struct GscanGrid {
     uint32_t per_row, blocks, chunks, group;
     int64_t slots;
@@ -277,13 +278,14 @@ __device__ __forceinline__ float value_before(const GscanArgs &a, const GscanGri
     uint64_t *const words = static_cast<uint64_t *>(a.words) + (int64_t)block * GS_CHANNELS, *const groups = words + gr.chunks * gr.slots;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     if (wave == 0 && chunk < gr.chunks - 1) hand_on(words + chunk * gr.slots + lane, own);
-    // two waves for the groups before this chunk's, two for the chunks before it in its group
-    const int group = chunk / gr.group, start = group * gr.group, half_groups = group / 2, half = (start + (int)chunk) / 2;
+    // in the first group, four waves for the chunks before this one; later, two for the groups before this chunk's and two for the chunks
+    // before it in its group
+    const int group = chunk / gr.group, start = group * gr.group, c = (int)chunk;
     {
-        const int lo = wave == 0 ? 0 : wave == 1 ? half_groups : wave == 2 ? start : half;
-        const int hi = wave == 0 ? half_groups : wave == 1 ? group : wave == 2 ? half : (int)chunk;
+        const int lo = group == 0 ? c * wave / 4 : wave == 0 ? 0 : wave == 1 ? group / 2 : wave == 2 ? start : (start + c) / 2;
+        const int hi = group == 0 ? c * (wave + 1) / 4 : wave == 0 ? group / 2 : wave == 1 ? group : wave == 2 ? (start + c) / 2 : c;
         Map<float> all;
-        const bool came = wait_for(all, wave < 2 ? groups : words, lo, hi, gr.slots, a.looks);
+        const bool came = wait_for(all, group != 0 && wave < 2 ? groups : words, lo, hi, gr.slots, a.looks);
         parts[wave][lane] = all;
         if (lane == 0) missing[wave] = !came;
     }
@@ -291,25 +293,31 @@ __device__ __forceinline__ float value_before(const GscanArgs &a, const GscanGri
     if (wave != 0) return 0.0f;
     if (__builtin_expect(missing[0] || missing[1] || missing[2] || missing[3], 0)) {
         // all of it from the inputs, put together as its workgroups do
-        Map<float> p[4] = {{1.0f, 0.0f}, {1.0f, 0.0f}, {1.0f, 0.0f}, {1.0f, 0.0f}}, m{1.0f, 0.0f}, n{1.0f, 0.0f};
-        const int size = gr.group, middle = size / 2 - 1;
-        for (int c = 0; c < (int)chunk; ++c) {
-            const Map<float> one = map_alone<IO, VEC, R, BACK, LOGITS>(a, gr, block, c);
-            if (c >= half) p[3] = after(one, p[3]);
-            else if (c >= start) p[2] = after(one, p[2]);
-            else if (c % size < middle) m = after(one, m);
-            else if (c % size < size - 1) n = after(one, n);
-            else {
-                const Map<float> whole = after(one, after(n, m));
-                if (c / size < half_groups) p[0] = after(whole, p[0]);
+        const Map<float> none{1.0f, 0.0f};
+        Map<float> p[4] = {none, none, none, none}, q[4] = {none, none, none, none};
+        const int last = gr.group - 1;
+        for (int i = 0; i < c; ++i) {
+            const Map<float> one = map_alone<IO, VEC, R, BACK, LOGITS>(a, gr, block, i);
+            const int of = i / (int)gr.group, in = i - of * (int)gr.group, n = of == group ? c - start : last;       // chunks of its group that are put together
+            const int part = of == 0 ? (in >= n / 4) + (in >= n * 2 / 4) + (in >= n * 3 / 4) : in < n / 2 ? 2 : 3;
+            if (of < group && in == last) {
+                const Map<float> whole = after(one, of == 0 ? after(q[3], after(q[2], after(q[1], q[0]))) : after(q[3], q[2]));
+                if (of < group / 2) p[0] = after(whole, p[0]);
                 else p[1] = after(whole, p[1]);
-                m = n = {1.0f, 0.0f};
+                q[0] = q[1] = q[2] = q[3] = none;
+                continue;
             }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (part == k) (of == group ? p : q)[k] = after(one, (of == group ? p : q)[k]);
         }
-        for (int i = 0; i < 4; ++i) parts[i][lane] = p[i];
+        for (int k = 0; k < 4; ++k) parts[k][lane] = p[k];
     }
-    if (chunk == start + gr.group - 1 && chunk < gr.chunks - 1)
-        hand_on(groups + group * gr.slots + lane, after(own, after(parts[3][lane], parts[2][lane])));
+    if (c == start + (int)gr.group - 1 && chunk < gr.chunks - 1) {
+        Map<float> before = after(parts[3][lane], parts[2][lane]);
+        if (group == 0) before = after(parts[3][lane], after(parts[2][lane], after(parts[1][lane], parts[0][lane])));
+        hand_on(groups + group * gr.slots + lane, after(own, before));
+    }
     float h = first;
 #pragma unroll
     for (int i = 0; i < 4; ++i) h = fmaf(parts[i][lane].p, h, parts[i][lane].s);
@@ -332,18 +340,18 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(uint64_t *words
 }
 
 // Which block of channels and which chunk (in the direction of the recurrence) a workgroup has.  The hardware deals workgroups out to the
-// eight dies in turn, each with a cache of its own: runs of NEAR neighbouring blocks go to one die, so that the lines that neighbours share, as
+// eight dies in turn, each with a cache of its own: runs of 16 neighbouring blocks go to one die (of 4, where all workgroups are on the chip at once), so that the lines that neighbours share, as
 // they do where rows start anywhere, are fetched and written once (32 x 4096 bf16, forward: 1021 channels 250 -> 183 us, 1024 190 -> 163).
-constexpr uint32_t DIES = 8, NEAR = 16;
+constexpr uint32_t DIES = 8;
 struct Turn {
     uint32_t block, chunk;
 };
 __device__ __forceinline__ Turn turn_of(const GscanGrid &gr) {
-    const uint32_t whole = gridDim.x / (DIES * NEAR) * (DIES * NEAR);
+    const uint32_t near = gridDim.x < ALL_AT_ONCE ? 4 : 16, round = DIES * near;
     uint32_t n = blockIdx.x;
-    if (n < whole) {
-        const uint32_t in = n % (DIES * NEAR);
-        n += in % DIES * NEAR + in / DIES - in;
+    if (n < gridDim.x / round * round) {
+        const uint32_t in = n % round;
+        n += in % DIES * near + in / DIES - in;
     }
     return {n % gr.blocks, n / gr.blocks};
 }
@@ -588,7 +596,12 @@ template <typename IO, int VEC, int R> GscanGrid grid_of(int64_t B, int64_t T, i
     g.chunks = (uint32_t)chunks;
     g.fits = per_row < 0x7fffffff && B * per_row < 0x7fffffff && chunks < 0x7fffffff && blocks * chunks < 0x7fffffff;
     g.slots = blocks * GS_CHANNELS;
-    for (g.group = 8; (uint64_t)g.group * g.group < (uint64_t)chunks;) g.group *= 2;
+    // Where all workgroups are on the chip at once, the time is that of the wait: one group, so that nothing waits for a map made of
+    // maps (1 x 8191 x 768 bf16 forward, 64 chunks: 15.3 us, in groups of 8 20.2).  Otherwise the words read are what costs (2 x 32768 x
+    // 1024 bf16 backward, 256 chunks: groups of 16 156 us, 32 161, 64 171, 128 185).
+    g.group = 8;
+    if (chunks <= 128 && blocks * chunks < ALL_AT_ONCE) g.group = 128;
+    while ((uint64_t)g.group * g.group < (uint64_t)chunks) g.group *= 2;
     return g;
 }
 // 64-bit words of the scratch
