@@ -24,7 +24,8 @@ namespace t2fw {
 namespace {
 
 constexpr int GS_THREADS = 256;
-constexpr int GS_CHANNELS = 64;          // channels of a workgroup
+constexpr int FEW_STEPS = 1024;
+constexpr int GS_CHANNELS = 64;          // channels of a workgroup (CHN below: more of them where there are few steps)
 
 // elements of a lane: 32 in all, whatever the type
 template <typename IO> struct Tile {
@@ -73,7 +74,7 @@ template <typename IO> __device__ __forceinline__ double gate_slope(double z) {
 // group
 constexpr int ALL_AT_ONCE = 2048;        // workgroups: less than two rounds of the chip
 struct GscanGrid {
-    uint32_t per_row, blocks, chunks, group;
+    uint32_t per_row, blocks, chunks, group, channels;
     int64_t slots;
     bool fits;
 };
@@ -92,9 +93,9 @@ template <int VEC, int R> struct Place {
     int lane, group;             // slot within the workgroup, stretch within the chunk
     bool mine;
 };
-template <int VEC, int R>
+template <int VEC, int R, int CHN>
 __device__ __forceinline__ Place<VEC, R> place_of(const GscanArgs &a, const GscanGrid &gr, int64_t block, int64_t chunk) {
-    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
+    constexpr int CL = CHN / VEC, TG = GS_THREADS / CL;
     Place<VEC, R> p;
     p.lane = threadIdx.x % CL;
     p.group = threadIdx.x / CL;
@@ -193,9 +194,9 @@ __device__ __forceinline__ Map<Acc> fold_steps(const Acc (&g)[R], const Held<IO,
     return m;
 }
 
-// The channel of a workgroup's thread in [B, D] arrays; whether it is there
-template <int VEC> __device__ __forceinline__ bool channel_of(const GscanArgs &a, const GscanGrid &gr, int64_t block, int thread, int64_t *at) {
-    const int64_t slot = block * (GS_CHANNELS / VEC) + thread / VEC, b = (uint32_t)slot / gr.per_row, d = (slot - b * gr.per_row) * VEC;
+// Where a workgroup's channel is in [B, D] arrays; whether it is there
+template <int VEC, int CHN> __device__ __forceinline__ bool channel_of(const GscanArgs &a, const GscanGrid &gr, int64_t block, int thread, int64_t *at) {
+    const int64_t slot = block * (CHN / VEC) + thread / VEC, b = (uint32_t)slot / gr.per_row, d = (slot - b * gr.per_row) * VEC;
     *at = b * a.D + (d + VEC <= a.D ? d : a.D - VEC) + thread % VEC;
     return slot < a.B * (int64_t)gr.per_row;
 }
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, Gsc
     constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL;
     __shared__ Map<Acc> maps[TG][GS_CHANNELS];
     const uint32_t block = blockIdx.x % gr.blocks, chunk = blockIdx.x / gr.blocks;
-    const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, BACK ? gr.chunks - 1 - chunk : chunk);
+    const Place<VEC, R> p = place_of<VEC, R, GS_CHANNELS>(a, gr, block, BACK ? gr.chunks - 1 - chunk : chunk);
     Held<IO, VEC> x[R], f[R];
     load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
     load_steps<IO, VEC, R>(x, BACK ? a.g_out : a.x, BACK ? a.g_b : a.x_b, BACK ? a.g_t : a.x_t, p);
@@ -385,15 +386,15 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, Gsc
     static_cast<Map<Acc> *>(a.words)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] = all;
 }
 
-template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
+template <typename IO, typename Acc, int VEC, int R, int CHN, bool LOGITS>
 __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 ? 5 : 4) void gscan_forward_kernel(GscanArgs a, GscanGrid gr) {
-    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
-    __shared__ Map<Acc> maps[TG][GS_CHANNELS];
+    constexpr int CL = CHN / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
+    __shared__ Map<Acc> maps[TG][CHN];
     const Turn turn = turn_of(gr);
     const uint32_t block = turn.block, chunk = turn.chunk;
-    const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
+    const Place<VEC, R> p = place_of<VEC, R, CHN>(a, gr, block, chunk);
     int64_t at = 0;
-    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
+    const bool first = CHN == GS_CHANNELS && threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC, CHN>(a, gr, block, threadIdx.x, &at);
     Acc h = there && a.s0 != nullptr ? static_cast<const Acc *>(a.s0)[at] : (Acc)0;
     Held<IO, VEC> x[R], f[R];
     load_steps<IO, VEC, R>(f, a.f, a.f_b, a.f_t, p);
@@ -413,23 +414,39 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
         f[r].as_it_came();
     }
     __syncthreads();
-    Map<Acc> own{1, 0};
-    if (first) {
+    if constexpr (CHN == GS_CHANNELS) {
+        Map<Acc> own{1, 0};
+        if (first) {
 #pragma unroll 8
-        for (int i = 0; i < TG; ++i) {
-            own = after(maps[i][threadIdx.x], own);
+            for (int i = 0; i < TG; ++i) {
+                own = after(maps[i][threadIdx.x], own);
+            }
         }
-    }
-    h = value_before<IO, VEC, R, false, LOGITS>(a, gr, block, chunk, own, h);
-    if (first) {
-        if (a.ckpt != nullptr) static_cast<Acc *>(a.ckpt)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] = h;
+        h = value_before<IO, VEC, R, false, LOGITS>(a, gr, block, chunk, own, h);
+        if (first) {
+            if (a.ckpt != nullptr) static_cast<Acc *>(a.ckpt)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] = h;
 #pragma unroll 8
-        for (int i = 0; i < TG; ++i) {
-            const Map<Acc> m = maps[i][threadIdx.x];
-            maps[i][threadIdx.x].s = h;                  // the state before this stretch
-            h = m.p * h + m.s;
+            for (int i = 0; i < TG; ++i) {
+                const Map<Acc> m = maps[i][threadIdx.x];
+                maps[i][threadIdx.x].s = h;                  // the state before this stretch
+                h = m.p * h + m.s;
+            }
+            if (there && chunk == gr.chunks - 1) static_cast<Acc *>(a.final_state)[at] = h;
         }
-        if (there && chunk == gr.chunks - 1) static_cast<Acc *>(a.final_state)[at] = h;
+    } else {
+        // a chunk that is the whole sequence
+        for (int column = threadIdx.x; column < CHN; column += GS_THREADS) {
+            const bool is = channel_of<VEC, CHN>(a, gr, block, column, &at);
+            Acc h = is && a.s0 != nullptr ? static_cast<const Acc *>(a.s0)[at] : (Acc)0;
+            if (a.ckpt != nullptr) static_cast<Acc *>(a.ckpt)[(int64_t)block * CHN + column] = h;
+#pragma unroll
+            for (int i = 0; i < TG; ++i) {
+                const Map<Acc> m = maps[i][column];
+                maps[i][column].s = h;
+                h = m.p * h + m.s;
+            }
+            if (is) static_cast<Acc *>(a.final_state)[at] = h;
+        }
     }
     __syncthreads();
     // the results take their inputs' registers
@@ -452,16 +469,16 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
     store_steps<IO, VEC, R>(a.out, x, a.D, a.T, p);
 }
 
-template <typename IO, typename Acc, int VEC, int R, bool LOGITS>
+template <typename IO, typename Acc, int VEC, int R, int CHN, bool LOGITS>
 __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 ? 4 : 2) void gscan_backward_kernel(GscanArgs a, GscanGrid gr) {
-    constexpr int CL = GS_CHANNELS / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
-    __shared__ Map<Acc> maps[TG][GS_CHANNELS];           // states: forward in time
-    __shared__ Acc sums[TG][GS_CHANNELS];                // adjoints: backward, with the same gate products
+    constexpr int CL = CHN / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
+    __shared__ Map<Acc> maps[TG][CHN];           // states: forward in time
+    __shared__ Acc sums[TG][CHN];                // adjoints: backward, with the same gate products
     const Turn turn = turn_of(gr);
     const uint32_t block = turn.block, from_end = turn.chunk, chunk = gr.chunks - 1 - from_end;
-    const Place<VEC, R> p = place_of<VEC, R>(a, gr, block, chunk);
+    const Place<VEC, R> p = place_of<VEC, R, CHN>(a, gr, block, chunk);
     int64_t at = 0;
-    const bool first = threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC>(a, gr, block, threadIdx.x, &at);
+    const bool first = CHN == GS_CHANNELS && threadIdx.x < GS_CHANNELS, there = first && channel_of<VEC, CHN>(a, gr, block, threadIdx.x, &at);
     Acc e = there && a.g_state != nullptr ? static_cast<const Acc *>(a.g_state)[at] : (Acc)0;
     Acc h = first ? static_cast<const Acc *>(a.ckpt)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] : (Acc)0;
     Held<IO, VEC> x[R], f[R], go[R];
@@ -486,28 +503,49 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
         go[r].as_it_came();
     }
     __syncthreads();
-    Map<Acc> own{1, 0};
-    if (first) {
+    if constexpr (CHN == GS_CHANNELS) {
+        Map<Acc> own{1, 0};
+        if (first) {
 #pragma unroll 8
-        for (int i = TG - 1; i >= 0; --i) {
-            own = after({maps[i][threadIdx.x].p, sums[i][threadIdx.x]}, own);
+            for (int i = TG - 1; i >= 0; --i) {
+                own = after({maps[i][threadIdx.x].p, sums[i][threadIdx.x]}, own);
+            }
         }
-    }
-    e = value_before<IO, VEC, R, true, LOGITS>(a, gr, block, from_end, own, e);
-    if (first) {
+        e = value_before<IO, VEC, R, true, LOGITS>(a, gr, block, from_end, own, e);
+        if (first) {
 #pragma unroll 8
-        for (int i = 0; i < TG; ++i) {
-            const Map<Acc> m = maps[i][threadIdx.x];
-            maps[i][threadIdx.x].s = h;                  // the state before this stretch
-            h = m.p * h + m.s;
-        }
+            for (int i = 0; i < TG; ++i) {
+                const Map<Acc> m = maps[i][threadIdx.x];
+                maps[i][threadIdx.x].s = h;                  // the state before this stretch
+                h = m.p * h + m.s;
+            }
 #pragma unroll 8
-        for (int i = TG - 1; i >= 0; --i) {
-            const Acc pr = maps[i][threadIdx.x].p, s = sums[i][threadIdx.x];
-            sums[i][threadIdx.x] = e;                    // the adjoint after it
-            e = pr * e + s;
+            for (int i = TG - 1; i >= 0; --i) {
+                const Acc pr = maps[i][threadIdx.x].p, s = sums[i][threadIdx.x];
+                sums[i][threadIdx.x] = e;                    // the adjoint after it
+                e = pr * e + s;
+            }
+            if (there && chunk == 0 && a.d_s0 != nullptr) static_cast<Acc *>(a.d_s0)[at] = e;
         }
-        if (there && chunk == 0 && a.d_s0 != nullptr) static_cast<Acc *>(a.d_s0)[at] = e;
+    } else {
+        for (int column = threadIdx.x; column < CHN; column += GS_THREADS) {
+            const bool is = channel_of<VEC, CHN>(a, gr, block, column, &at);
+            Acc e = is && a.g_state != nullptr ? static_cast<const Acc *>(a.g_state)[at] : (Acc)0;
+            Acc h = static_cast<const Acc *>(a.ckpt)[(int64_t)block * CHN + column];
+#pragma unroll
+            for (int i = 0; i < TG; ++i) {
+                const Map<Acc> m = maps[i][column];
+                maps[i][column].s = h;
+                h = m.p * h + m.s;
+            }
+#pragma unroll
+            for (int i = TG - 1; i >= 0; --i) {
+                const Acc pr = maps[i][column].p, s = sums[i][column];
+                sums[i][column] = e;
+                e = pr * e + s;
+            }
+            if (is && a.d_s0 != nullptr) static_cast<Acc *>(a.d_s0)[at] = e;
+        }
     }
     __syncthreads();
     // the results take their inputs' registers
@@ -586,16 +624,26 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_step_kernel(GscanArgs a, int
     }
 }
 
+// Channels of a workgroup: as few steps as fit, as long as there is a workgroup for every CU (4096 x 16 x 768 bf16 with logits, forward and
+// backward: 303 and 497 us with 64 channels, 81 and 148 with 256; 8192 x 8 x 768: 546 and 932, 71 and 114 with 1024).
+template <int VEC, int R> constexpr int64_t steps_of(int chn) { return GS_THREADS / (chn / VEC) * R; }
+template <int VEC, int R> int channels_of(int64_t B, int64_t T, int64_t D) {
+    const int64_t per_row = (D + VEC - 1) / VEC * VEC;
+    for (int chn : {FEW_STEPS, 256})
+        if (GS_THREADS >= chn / VEC && T <= steps_of<VEC, R>(chn) && B * per_row >= (int64_t)256 * chn) return chn;
+    return GS_CHANNELS;
+}
 template <typename IO, int VEC, int R> GscanGrid grid_of(int64_t B, int64_t T, int64_t D) {
-    constexpr int CL = GS_CHANNELS / VEC, C = GS_THREADS / CL * R;
     GscanGrid g;
+    g.channels = channels_of<VEC, R>(B, T, D);
+    const int64_t CL = g.channels / VEC, C = steps_of<VEC, R>(g.channels);
     // (numbers that do not fit are refused before anything is launched)
     const int64_t per_row = (D + VEC - 1) / VEC, blocks = (B * per_row + CL - 1) / CL, chunks = T <= 0 ? 1 : (T + C - 1) / C;
     g.per_row = (uint32_t)per_row;
     g.blocks = (uint32_t)blocks;
     g.chunks = (uint32_t)chunks;
     g.fits = per_row < 0x7fffffff && B * per_row < 0x7fffffff && chunks < 0x7fffffff && blocks * chunks < 0x7fffffff;
-    g.slots = blocks * GS_CHANNELS;
+    g.slots = blocks * g.channels;
     // Where all workgroups are on the chip at once, the time is that of the wait: one group, so that nothing waits for a map made of
     // maps (1 x 8191 x 768 bf16 forward, 64 chunks: 15.3 us, in groups of 8 20.2).  Otherwise the words read are what costs (2 x 32768 x
     // 1024 bf16 backward, 256 chunks: groups of 16 156 us, 32 161, 64 171, 128 185).
@@ -638,7 +686,12 @@ template <typename IO, int VEC, int R, bool LOGITS> int forward_with(const Gscan
     const GscanGrid g = grid_of<IO, VEC, R>(a.B, a.T, a.D);
     const int rc = prepare<IO, VEC, R, false, LOGITS>(a, g, stream);
     if (rc) return rc;
-    hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, LOGITS>), dim3((unsigned)(g.blocks * g.chunks)), dim3(GS_THREADS), 0, stream, a, g);
+    const dim3 grid(g.blocks * g.chunks), threads(GS_THREADS);
+    if (g.channels == GS_CHANNELS) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, GS_CHANNELS, LOGITS>), grid, threads, 0, stream, a, g);
+    if constexpr (GS_THREADS >= 256 / VEC)
+        if (g.channels == 256) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, 256, LOGITS>), grid, threads, 0, stream, a, g);
+    if constexpr (GS_THREADS >= FEW_STEPS / VEC)
+        if (g.channels == FEW_STEPS) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, FEW_STEPS, LOGITS>), grid, threads, 0, stream, a, g);
     return check_hip(hipGetLastError(), "gscan_forward_kernel launch");
 }
 template <typename IO, int VEC, int R> int forward_of(const GscanArgs &a, hipStream_t stream) {
@@ -651,7 +704,12 @@ template <typename IO, int VEC, int R, bool LOGITS> int backward_with(const Gsca
     const GscanGrid g = grid_of<IO, VEC, R>(a.B, a.T, a.D);
     const int rc = prepare<IO, VEC, R, true, LOGITS>(a, g, stream);
     if (rc) return rc;
-    hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, LOGITS>), dim3((unsigned)(g.blocks * g.chunks)), dim3(GS_THREADS), 0, stream, a, g);
+    const dim3 grid(g.blocks * g.chunks), threads(GS_THREADS);
+    if (g.channels == GS_CHANNELS) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, GS_CHANNELS, LOGITS>), grid, threads, 0, stream, a, g);
+    if constexpr (GS_THREADS >= 256 / VEC)
+        if (g.channels == 256) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, 256, LOGITS>), grid, threads, 0, stream, a, g);
+    if constexpr (GS_THREADS >= FEW_STEPS / VEC)
+        if (g.channels == FEW_STEPS) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, FEW_STEPS, LOGITS>), grid, threads, 0, stream, a, g);
     return check_hip(hipGetLastError(), "gscan_backward_kernel launch");
 }
 template <typename IO, int VEC, int R> int backward_of(const GscanArgs &a, hipStream_t stream) {

@@ -108,6 +108,19 @@ def test_values_and_gradients(shape, logits, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(3000, 7, 90), (2901, 1, 97), (700, 20, 100), (667, 32, 103), (66000, 3, 5)], ids=str)
+def test_few_steps_of_many_rows(shape, dtype):
+    """more channels to a workgroup, which has the whole sequence; ragged"""
+    ins, go, gs = inputs(*shape, dtype, True, seed=sum(shape))
+    lengths = torch.randint(0, shape[1] + 1, (shape[0],), generator=torch.Generator().manual_seed(1))
+    got = run(ins, lengths.cuda(), True, go, gs)
+    ref = reference(*ins, lengths, True, unit(dtype, True), go, gs)
+    for n in ref:
+        check(n, got[n], ref[n])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [torch.int64, torch.int32], ids=str)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("T,D", [(5, 16), (300, 24), (513, 65)])
