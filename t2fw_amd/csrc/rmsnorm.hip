@@ -58,8 +58,13 @@ template <int LANES, typename Acc> __device__ __forceinline__ Acc row_sum(Acc v)
 }
 // max that keeps a NaN
 __device__ __forceinline__ float larger(float a, float b) { return a > b || a != a ? a : b; }
-__device__ __forceinline__ float lanes_max(float v, int lanes) {
-    for (int m = 1; m < lanes; m <<= 1) v = larger(v, __shfl_xor(v, m, 64));
+__device__ __forceinline__ float lanes_max(float v, int lanes) {          // of groups of 1 to 64 neighbouring lanes, as group_sum
+    if (lanes >= 2) v = larger(v, dpp_move<DPP_QUAD_XOR1>(v));
+    if (lanes >= 4) v = larger(v, dpp_move<DPP_QUAD_XOR2>(v));
+    if (lanes >= 8) v = larger(v, dpp_move<DPP_ROW_HALF_MIRROR>(v));
+    if (lanes >= 16) v = larger(v, dpp_move<DPP_ROW_MIRROR>(v));
+    if (lanes >= 32) v = larger(v, __shfl_xor(v, 16, 64));
+    if (lanes >= 64) v = larger(v, __shfl_xor(v, 32, 64));
     return v;
 }
 template <int LANES> __device__ __forceinline__ float row_max(float v) {
@@ -195,15 +200,18 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
             if (by_row ? lane == 0 && c == 0 : k[c].column % a.group == 0) a.scales[row * a.groups + g] = scale;
             // one reciprocal for the chunk; of a scale near the smallest numbers it would overflow
             const float by = 1.0f / scale;
-            const bool tiny = scale < 1e-35f;
+            float v[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = h[c][i] * by;
+            if (__builtin_expect(scale < 1e-35f, 0)) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] = h[c][i] / scale;
+            }
             uint32_t words[2];
 #pragma unroll
             for (int i = 0; i < W; i += 4) {
-                float v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = tiny ? h[c][i + j] / scale : h[c][i + j] * by;
-                const int word = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-                words[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], word, true);
+                const int word = __builtin_amdgcn_cvt_pk_fp8_f32(v[i], v[i + 1], 0, false);
+                words[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[i + 2], v[i + 3], word, true);
             }
             Vec<uint8_t, W> o;
             __builtin_memcpy(&o, words, sizeof(o));
