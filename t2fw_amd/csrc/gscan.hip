@@ -17,6 +17,12 @@
 // Chunks are numbered so that what a chunk waits for comes earlier in the grid.  Should the hardware not have started that workgroup all the
 // same (another program on the device, say), a wait ends after a number of looks, and the workgroup makes the maps before its own
 // itself from the inputs, by the same operations in the same order: every wait is bounded, and none needs another workgroup to run.
+//
+// Bound by memory where there is enough of it to move: 2 x 32768 x 1024 float32, GPU time, forward 149 us (805 MB, 5.4 TB/s), backward
+// 243 us (1.34 GB, 5.5 TB/s; a copy of that size 5.0 to 5.4); 32 x 4096 x 1024 bf16 with logits 164 and 273 us (4.9 TB/s).  Two passes over the
+// data, the chunks' maps first, took 338 and 805 us for the former.  Small calls are bound by the chain launch, load, hand on, wait, store:
+// 1 x 8191 x 768 bf16 forward 14.8 us (11.4 in a variant that did not wait), 8 x 1024 x 768 forward 14.0, backward 16.1, and 2 for
+// the launch that empties the words.
 #include "gscan.hpp"
 #include "vec.hpp"
 
@@ -594,7 +600,7 @@ template <typename Acc> int pass(const void *from, void *to, int64_t n, hipStrea
     return check_hip(hipGetLastError(), "gscan_pass_kernel launch");
 }
 
-// One token: x, f, out [B, D], the state in place or not
+// One token: x, f, out [B, D], the state in place or not.  A launch and a round to memory: 64 x 768 bf16 2.5 us.
 template <typename IO, typename Acc, int VEC>
 __global__ __launch_bounds__(GS_THREADS) void gscan_step_kernel(GscanArgs a, int64_t n) {
     const int64_t i = ((int64_t)blockIdx.x * GS_THREADS + threadIdx.x) * VEC;

@@ -4,6 +4,10 @@
 //   d loss / d z = c (onehot(t) - softmax(z)),  c = scale / M (-r A [not held by the clip] - kl (exp(d) - 1)).
 // The coefficient c of a row depends on nothing but the row and M, so that the launch that reads a row for its log-sum-exp
 // writes its gradient too, for a gradient of the loss of one; the backward has nothing left to do then but to look at that value.
+//
+// Bound by memory: 8192 x 50257 bf16, loss and gradient, 315 us (1.65 GB of logits and gradient, 5.2 TB/s, as a copy); with the gradient in a pass
+// of its own the logits would be read twice.  Few rows are bound by the chain load, exchange, exponentials, store: 333 x 8000
+// float32 13.5 us, 4 for the sum of the tokens' shares and 2 for the backward's look.
 #include "policy_loss.hpp"
 #include "vec.hpp"
 

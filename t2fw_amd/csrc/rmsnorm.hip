@@ -8,6 +8,11 @@
 // wave's loads and stores are of whole lines: 16 or 32 lanes of a wave for narrow rows, a wave, or 4 to 16 waves.  Every load of a row is made before its sums, without a branch between
 // them, also by lanes that have no columns left.  Where the width is no multiple of a chunk the last one of a row is loaded
 // from a chunk's width before its end, and the columns that belong to the chunk before it are left out.
+//
+// Bound by memory: 65536 x 1024 bf16 forward 111 us, backward 112 us with the weights' gradient (4.8 TB/s of four arrays each), 32768 x 4096
+// in 8 bits 182 us (5.2 TB/s; a copy 5.0 to 5.4).  Rows of an odd width lose a fifth in 16-bit types, whose vectors are then
+// not aligned (65536 x 1021: 130 and 126 us); aligned ones would start at another column in every row, and the backward's
+// sums over the rows are per column.  64 x 768 in 8 bits: 4.9 us, one chain of loads, two sums over a wave and stores.
 #include "rmsnorm.hpp"
 #include "vec.hpp"
 
