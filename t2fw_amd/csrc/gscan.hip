@@ -14,9 +14,10 @@
 // pattern that no map has; so the word says by itself whether it is there.  Chunks come in groups: the last one of a group
 // also hands on the map of the whole group, and a chunk needs the groups before its own and the chunks before it in its
 // group, about 2 sqrt(chunks) words.  They are composed in a fixed order, so the result does not depend on who is first.
-// Chunks are numbered so that what a chunk waits for comes earlier in the grid.  Should the hardware not have started that workgroup all the
-// same (another program on the device, say), a wait ends after a number of looks, and the workgroup makes the maps before its own
-// itself from the inputs, by the same operations in the same order: every wait is bounded, and none needs another workgroup to run.
+// Chunks are numbered so that what a chunk waits for comes earlier in the grid, or among the same 128 workgroups.  Should the hardware not have
+// started that workgroup all the same (another program on the device, say), a wait ends after a number of looks, and the workgroup makes
+// the maps before its own itself from the inputs, by the same operations in the same order: every wait is bounded, and none needs
+// another workgroup to run.
 //
 // Bound by memory where there is enough of it to move: 2 x 32768 x 1024 float32, GPU time, forward 149 us (805 MB, 5.4 TB/s), backward
 // 243 us (1.34 GB, 5.5 TB/s; a copy of that size 5.0 to 5.4); 32 x 4096 x 1024 bf16 with logits 164 and 273 us (4.9 TB/s).  Two passes over the
@@ -30,8 +31,9 @@ namespace t2fw {
 namespace {
 
 constexpr int GS_THREADS = 256;
+constexpr int GS_CHANNELS = 64;          // channels of a workgroup (CHN below: 256 or FEW_STEPS of them where there are few steps)
 constexpr int FEW_STEPS = 1024;
-constexpr int GS_CHANNELS = 64;          // channels of a workgroup (CHN below: more of them where there are few steps)
+constexpr int ALL_AT_ONCE = 2048;        // workgroups: less than two rounds of the chip
 
 // elements of a lane: 32 in all, whatever the type
 template <typename IO> struct Tile {
@@ -77,8 +79,7 @@ template <typename IO> __device__ __forceinline__ double gate_slope(double z) {
 }
 
 // How a call is cut: slots of a row, workgroups side by side, chunks of the sequence, columns of one chunk in the scratch, chunks of a
-// group
-constexpr int ALL_AT_ONCE = 2048;        // workgroups: less than two rounds of the chip
+// group, channels of a workgroup
 struct GscanGrid {
     uint32_t per_row, blocks, chunks, group, channels;
     int64_t slots;
@@ -209,7 +210,6 @@ template <int VEC, int CHN> __device__ __forceinline__ bool channel_of(const Gsc
 
 // ---- maps from chunk to chunk --------------------------------------------------------------------------------------
 constexpr uint64_t EMPTY = ~0ull;                        // a NaN of a pattern that word_of() gives to nothing
-
 constexpr uint64_t NOTHING = 0x3f800000ull;              // the map that changes nothing
 __device__ __forceinline__ uint64_t word_of(const Map<float> &m) {
     const uint64_t w = (uint64_t)__float_as_uint(m.s) << 32 | __float_as_uint(m.p);
@@ -330,6 +330,7 @@ __device__ __forceinline__ float value_before(const GscanArgs &a, const GscanGri
     for (int i = 0; i < 4; ++i) h = fmaf(parts[i][lane].p, h, parts[i][lane].s);
     return h;
 }
+
 // double: every map is there from the launch before
 template <typename IO, int VEC, int R, bool BACK, bool LOGITS>
 __device__ __forceinline__ double value_before(const GscanArgs &a, const GscanGrid &gr, uint32_t block, uint32_t chunk, const Map<double> &,
@@ -347,8 +348,9 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(uint64_t *words
 }
 
 // Which block of channels and which chunk (in the direction of the recurrence) a workgroup has.  The hardware deals workgroups out to the
-// eight dies in turn, each with a cache of its own: runs of 16 neighbouring blocks go to one die (of 4, where all workgroups are on the chip at once), so that the lines that neighbours share, as
-// they do where rows start anywhere, are fetched and written once (32 x 4096 bf16, forward: 1021 channels 250 -> 183 us, 1024 190 -> 163).
+// eight dies in turn, each with a cache of its own: runs of 16 neighbouring blocks go to one die, so that the lines that neighbours share,
+// as they do where rows start anywhere, are fetched and written once (32 x 4096 bf16, forward: 1021 channels 250 -> 183 us, 1024
+// 190 -> 163).  Runs of 4 where all workgroups are on the chip at once (8 x 1024 x 768, backward: 15.9 us, of 16 18.3).
 constexpr uint32_t DIES = 8;
 struct Turn {
     uint32_t block, chunk;
@@ -386,9 +388,7 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_maps_kernel(GscanArgs a, Gsc
     if (threadIdx.x >= GS_CHANNELS) return;
     Map<Acc> all{1, 0};
 #pragma unroll
-    for (int i = 0; i < TG; ++i) {
-        all = after(maps[BACK ? TG - 1 - i : i][threadIdx.x], all);
-    }
+    for (int i = 0; i < TG; ++i) all = after(maps[BACK ? TG - 1 - i : i][threadIdx.x], all);
     static_cast<Map<Acc> *>(a.words)[chunk * gr.slots + (int64_t)block * GS_CHANNELS + threadIdx.x] = all;
 }
 
@@ -424,9 +424,7 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
         Map<Acc> own{1, 0};
         if (first) {
 #pragma unroll 8
-            for (int i = 0; i < TG; ++i) {
-                own = after(maps[i][threadIdx.x], own);
-            }
+            for (int i = 0; i < TG; ++i) own = after(maps[i][threadIdx.x], own);
         }
         h = value_before<IO, VEC, R, false, LOGITS>(a, gr, block, chunk, own, h);
         if (first) {
@@ -434,7 +432,7 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
 #pragma unroll 8
             for (int i = 0; i < TG; ++i) {
                 const Map<Acc> m = maps[i][threadIdx.x];
-                maps[i][threadIdx.x].s = h;                  // the state before this stretch
+                maps[i][threadIdx.x].s = h;              // the state before this stretch
                 h = m.p * h + m.s;
             }
             if (there && chunk == gr.chunks - 1) static_cast<Acc *>(a.final_state)[at] = h;
@@ -478,8 +476,8 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
 template <typename IO, typename Acc, int VEC, int R, int CHN, bool LOGITS>
 __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 ? 4 : 2) void gscan_backward_kernel(GscanArgs a, GscanGrid gr) {
     constexpr int CL = CHN / VEC, TG = GS_THREADS / CL, PAIR = Held<IO, VEC>::PAIR;
-    __shared__ Map<Acc> maps[TG][CHN];           // states: forward in time
-    __shared__ Acc sums[TG][CHN];                // adjoints: backward, with the same gate products
+    __shared__ Map<Acc> maps[TG][CHN];                   // states: forward in time
+    __shared__ Acc sums[TG][CHN];                        // adjoints: backward, with the same gate products
     const Turn turn = turn_of(gr);
     const uint32_t block = turn.block, from_end = turn.chunk, chunk = gr.chunks - 1 - from_end;
     const Place<VEC, R> p = place_of<VEC, R, CHN>(a, gr, block, chunk);
@@ -513,22 +511,20 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
         Map<Acc> own{1, 0};
         if (first) {
 #pragma unroll 8
-            for (int i = TG - 1; i >= 0; --i) {
-                own = after({maps[i][threadIdx.x].p, sums[i][threadIdx.x]}, own);
-            }
+            for (int i = TG - 1; i >= 0; --i) own = after({maps[i][threadIdx.x].p, sums[i][threadIdx.x]}, own);
         }
         e = value_before<IO, VEC, R, true, LOGITS>(a, gr, block, from_end, own, e);
         if (first) {
 #pragma unroll 8
             for (int i = 0; i < TG; ++i) {
                 const Map<Acc> m = maps[i][threadIdx.x];
-                maps[i][threadIdx.x].s = h;                  // the state before this stretch
+                maps[i][threadIdx.x].s = h;              // the state before this stretch
                 h = m.p * h + m.s;
             }
 #pragma unroll 8
             for (int i = TG - 1; i >= 0; --i) {
                 const Acc pr = maps[i][threadIdx.x].p, s = sums[i][threadIdx.x];
-                sums[i][threadIdx.x] = e;                    // the adjoint after it
+                sums[i][threadIdx.x] = e;                // the adjoint after it
                 e = pr * e + s;
             }
             if (there && chunk == 0 && a.d_s0 != nullptr) static_cast<Acc *>(a.d_s0)[at] = e;

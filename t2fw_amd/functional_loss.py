@@ -17,7 +17,8 @@ def policy_loss(logits, targets, old_logp, ref_logp, advantages, mask=None, clip
     outside the mask (``logp`` is 0 there); inside it makes the loss NaN.
 
     Float32 and bfloat16 logits: the forward writes their gradient in the pass that reads them, for a loss that is
-    differentiated with a gradient of one, and the backward recomputes it for another.  So pass the factor of an accumulated
+    differentiated with a gradient of one (an array of the logits' size, held until the backward takes it), and the backward recomputes
+    it for another.  So pass the factor of an accumulated
     or scaled loss as ``scale`` rather than multiply the loss.  Float16: the backward makes the gradient, whatever the loss is multiplied by."""
     low, high = clip
     return _lib.host().policy_loss(logits, targets, old_logp, ref_logp, advantages, mask, 1.0 - low, 1.0 + high, kl_coef, scale,

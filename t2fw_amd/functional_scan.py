@@ -20,7 +20,8 @@ def gated_scan(x, f, state=None, lengths=None, logits=False):
     ``x, f: [B, T, D]`` (float32, float16, bfloat16 or float64; one type), with their channels next to each other in memory and any
     strides between rows and steps: parts of a projection need not be copied.  ``state: [B, D]``, the state before the first step
     (``None``: zeros), and the last state are float32 (float64 for float64 tensors) whatever the type of ``x``: a state
-    that takes up thousands of steps is not rounded between calls.  ``logits=True``: ``f`` holds gate logits, the gate is their
+    that takes up thousands of steps is not rounded between calls.  Gates may be any numbers, but their products over the steps of a sequence
+    have to stay finite: stretches are put together by them, and an infinite one makes NaN even of a state of zero.  ``logits=True``: ``f`` holds gate logits, the gate is their
     sigmoid, and the gradient that comes back is the logits'.
 
     ``lengths: [B]`` (int32 or int64, on the device), for rows that are padded at their end: steps from ``lengths[b]`` on do not count,
