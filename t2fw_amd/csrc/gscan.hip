@@ -31,7 +31,7 @@ namespace t2fw {
 namespace {
 
 constexpr int GS_THREADS = 256;
-constexpr int GS_CHANNELS = 64;          // channels of a workgroup (CHN below: 256 or FEW_STEPS of them where there are few steps)
+constexpr int GS_CHANNELS = 64;          // channels of a workgroup (CHN below: 128 to FEW_STEPS of them where there are few steps)
 constexpr int FEW_STEPS = 1024;
 constexpr int ALL_AT_ONCE = 2048;        // workgroups: less than two rounds of the chip
 
@@ -627,11 +627,11 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_step_kernel(GscanArgs a, int
 }
 
 // Channels of a workgroup: as few steps as fit, as long as there is a workgroup for every CU (4096 x 16 x 768 bf16 with logits, forward and
-// backward: 303 and 497 us with 64 channels, 81 and 148 with 256; 8192 x 8 x 768: 546 and 932, 71 and 114 with 1024).
+// backward: 303 and 497 us with 64 channels, 64 and 105 with 512; 8192 x 8 x 768: 546 and 932, 71 and 114 with 1024).
 template <int VEC, int R> constexpr int64_t steps_of(int chn) { return GS_THREADS / (chn / VEC) * R; }
 template <int VEC, int R> int channels_of(int64_t B, int64_t T, int64_t D) {
     const int64_t per_row = (D + VEC - 1) / VEC * VEC;
-    for (int chn : {FEW_STEPS, 256})
+    for (int chn : {FEW_STEPS, 512, 256, 128})
         if (GS_THREADS >= chn / VEC && T <= steps_of<VEC, R>(chn) && B * per_row >= (int64_t)256 * chn) return chn;
     return GS_CHANNELS;
 }
@@ -690,8 +690,11 @@ template <typename IO, int VEC, int R, bool LOGITS> int forward_with(const Gscan
     if (rc) return rc;
     const dim3 grid(g.blocks * g.chunks), threads(GS_THREADS);
     if (g.channels == GS_CHANNELS) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, GS_CHANNELS, LOGITS>), grid, threads, 0, stream, a, g);
+    if (g.channels == 128) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, 128, LOGITS>), grid, threads, 0, stream, a, g);
     if constexpr (GS_THREADS >= 256 / VEC)
         if (g.channels == 256) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, 256, LOGITS>), grid, threads, 0, stream, a, g);
+    if constexpr (GS_THREADS >= 512 / VEC)
+        if (g.channels == 512) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, 512, LOGITS>), grid, threads, 0, stream, a, g);
     if constexpr (GS_THREADS >= FEW_STEPS / VEC)
         if (g.channels == FEW_STEPS) hipLaunchKernelGGL((gscan_forward_kernel<IO, Acc, VEC, R, FEW_STEPS, LOGITS>), grid, threads, 0, stream, a, g);
     return check_hip(hipGetLastError(), "gscan_forward_kernel launch");
@@ -708,8 +711,11 @@ template <typename IO, int VEC, int R, bool LOGITS> int backward_with(const Gsca
     if (rc) return rc;
     const dim3 grid(g.blocks * g.chunks), threads(GS_THREADS);
     if (g.channels == GS_CHANNELS) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, GS_CHANNELS, LOGITS>), grid, threads, 0, stream, a, g);
+    if (g.channels == 128) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, 128, LOGITS>), grid, threads, 0, stream, a, g);
     if constexpr (GS_THREADS >= 256 / VEC)
         if (g.channels == 256) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, 256, LOGITS>), grid, threads, 0, stream, a, g);
+    if constexpr (GS_THREADS >= 512 / VEC)
+        if (g.channels == 512) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, 512, LOGITS>), grid, threads, 0, stream, a, g);
     if constexpr (GS_THREADS >= FEW_STEPS / VEC)
         if (g.channels == FEW_STEPS) hipLaunchKernelGGL((gscan_backward_kernel<IO, Acc, VEC, R, FEW_STEPS, LOGITS>), grid, threads, 0, stream, a, g);
     return check_hip(hipGetLastError(), "gscan_backward_kernel launch");

@@ -109,7 +109,7 @@ def test_values_and_gradients(shape, logits, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("shape", [(3000, 7, 90), (2901, 1, 97), (700, 20, 100), (667, 32, 103), (66000, 3, 5)], ids=str)
+@pytest.mark.parametrize("shape", [(3000, 7, 90), (2901, 1, 97), (700, 20, 100), (667, 32, 103), (66000, 3, 5), (1400, 13, 96), (341, 60, 97), (5000, 16, 3)], ids=str)
 def test_few_steps_of_many_rows(shape, dtype):
     """more channels to a workgroup, which has the whole sequence; ragged"""
     ins, go, gs = inputs(*shape, dtype, True, seed=sum(shape))
