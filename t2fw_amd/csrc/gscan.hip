@@ -648,10 +648,13 @@ template <typename IO, int VEC, int R> GscanGrid grid_of(int64_t B, int64_t T, i
     g.slots = blocks * g.channels;
     // Where all workgroups are on the chip at once, the time is that of the wait: one group, so that nothing waits for a map made of
     // maps (1 x 8191 x 768 bf16 forward, 64 chunks: 15.3 us, in groups of 8 20.2).  Otherwise the words read are what costs (2 x 32768 x
-    // 1024 bf16 backward, 256 chunks: groups of 16 156 us, 32 161, 64 171, 128 185).
+    // 1024 bf16 backward, 256 chunks: groups of 16 156 us, 32 161, 64 171, 128 185).  One or two workgroups side by side are between the
+    // two, few words and long waits: groups twice as large (1 x 131072 x 128 bf16 forward and backward: 44 and 56 us, without 60 and 77;
+    // of four workgroups side by side, 2 x 65536 x 128, the same either way).
     g.group = 8;
     if (chunks <= 128 && blocks * chunks < ALL_AT_ONCE) g.group = 128;
     while ((uint64_t)g.group * g.group < (uint64_t)chunks) g.group *= 2;
+    if (blocks <= 2 && chunks > 128) g.group *= 2;
     return g;
 }
 // 64-bit words of the scratch

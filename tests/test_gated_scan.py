@@ -121,6 +121,19 @@ def test_few_steps_of_many_rows(shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("D", [24, 70, 130])
+def test_many_chunks(D, dtype):
+    """several groups of chunks, one to three workgroups side by side"""
+    ins, go, gs = inputs(1, 17001, D, dtype, True, seed=D, mean=5.0)
+    lengths = torch.tensor([16890])
+    got = run(ins, lengths.cuda(), True, go, gs)
+    ref = reference(*ins, lengths, True, unit(dtype, True), go, gs)
+    for n in ref:
+        check(n, got[n], ref[n])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [torch.int64, torch.int32], ids=str)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("T,D", [(5, 16), (300, 24), (513, 65)])
@@ -286,7 +299,7 @@ def test_on_another_stream_and_in_a_graph():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
-@pytest.mark.parametrize("shape,ragged", [((2, 900, 40), False), ((1, 2600, 7), True), ((3, 1300, 5), False), ((2, 5000, 65), True)], ids=str)
+@pytest.mark.parametrize("shape,ragged", [((2, 900, 40), False), ((1, 2600, 7), True), ((3, 1300, 5), False), ((2, 5000, 65), True), ((1, 17001, 24), False)], ids=str)
 def test_chunks_that_do_without_one_another(shape, ragged, dtype):
     """the same bits where no chunk waits for another's map and makes those before it itself"""
     from t2fw_amd import _lib
