@@ -2,7 +2,9 @@
 //   h = round(x + res) in the stream's type,  r = 1 / sqrt(mean h^2 + eps),  y = w h r;
 //   backward, from dy and the stream's gradient dres:  u = w dy,  d_x = d_res = r (u - h r^2 mean(u h)) + dres,  d_w = sum over rows of dy h r.
 // The norm is of the rounded h, the one that the backward finds again; sums are carried in 32 bits (64 for double).
-// In 8 bits: y is divided by scale = max |y| / 448 of the row, or of each group of its columns, and rounded to float8 e4m3.
+// In 8 bits: y is divided by scale = max |y| / 448 of the row, or of each group of its columns, and rounded to float8 e4m3.  r is in both and
+// goes out: with p = (h 2^e) w, r = 2^e rest, 1 <= rest < 2, which a product of 16-bit numbers gives exactly, the code is that of
+// 448 p / max |p|, rounded once, and scale = max |p| rest / 448.
 //
 // A row stays in registers between its sums and its results: LANES threads hold it in chunks of 16 bytes of the stream, CH of them each, so that a
 // wave's loads and stores are of whole lines: 16 or 32 lanes of a wave for narrow rows, a wave, or 4 to 16 waves.  Every load of a row is made before its sums, without a branch between
@@ -134,6 +136,31 @@ template <typename IO, typename Acc, int W> __device__ __forceinline__ void load
 
 constexpr int threads_of(int lanes) { return lanes < RN_THREADS ? RN_THREADS : lanes; }
 
+// r = power * rest with a power of two; a NaN stays in rest
+__device__ __forceinline__ void parts_of(float r, float *power, float *rest) {
+    const uint32_t bits = __float_as_uint(r);
+    *power = __uint_as_float(bits & 0x7f800000u);
+    *rest = r != r ? r : __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+}
+__device__ __forceinline__ float scale_of(float top, float rest) {
+    const float scale = top * rest / FP8_LARGEST;
+    return scale == 0.0f ? 1.0f : scale;
+}
+// 448 p / top for W numbers: a product with the reciprocal and one correction of it, which leaves the rounded quotient.  For numbers
+// whose reciprocal or remainder 32 bits do not hold, those that are not finite among them, y / scale.
+template <int W> __device__ __forceinline__ void codes_of(float (&v)[W], const float (&p)[W], float top, float rest, float scale) {
+    const float by = 1.0f / top;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const float n = p[i] * FP8_LARGEST, q = n * by;
+        v[i] = fmaf(fmaf(-q, top, n), by, q);
+    }
+    if (__builtin_expect(!(scale >= 1e-33f && scale != 1.0f && top <= 1e35f), 0)) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = p[i] * rest / scale;
+    }
+}
+
 template <typename IO, typename Stream, int LANES, int CH, int W, bool FP8>
 __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArgs a) {
     using Acc = typename AccT<IO>::type;
@@ -171,26 +198,25 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
     }
     sum = row_sum<LANES>(sum);
     const Acc r = (Acc)1 / sqrt(sum / (Acc)a.D + (Acc)a.eps);
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int i = 0; i < W; ++i) h[c][i] *= r * w[c][i];
     if constexpr (!FP8) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             Vec<IO, W> o;
 #pragma unroll
-            for (int i = 0; i < W; ++i) o.e[i] = narrow<IO>(h[c][i]);
+            for (int i = 0; i < W; ++i) o.e[i] = narrow<IO>(h[c][i] * (r * w[c][i]));
             if (live) store_chunk(static_cast<IO *>(a.y) + base, k[c], o);
         }
     } else {
-        float top[CH], all = 0;
+        float top[CH], all = 0, power, rest;
+        parts_of(r, &power, &rest);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             top[c] = 0;
 #pragma unroll
-            for (int i = 0; i < W; ++i)
+            for (int i = 0; i < W; ++i) {
+                h[c][i] = h[c][i] * power * w[c][i];
                 if (i >= k[c].skip) top[c] = larger(fabsf(h[c][i]), top[c]);
+            }
             all = larger(top[c], all);
         }
         const bool by_row = a.groups == 1;
@@ -198,20 +224,12 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             // a group's chunks are neighbouring lanes of one wave, those past the end of the row among them
-            float scale = (by_row ? all : lanes_max(top[c], (int)(a.group / W))) / FP8_LARGEST;
-            if (scale == 0.0f) scale = 1.0f;
+            const float largest = by_row ? all : lanes_max(top[c], (int)(a.group / W)), scale = scale_of(largest, rest);
             if (!live || !k[c].there()) continue;
             const int64_t g = by_row ? 0 : k[c].column / a.group;
             if (by_row ? lane == 0 && c == 0 : k[c].column % a.group == 0) a.scales[row * a.groups + g] = scale;
-            // one reciprocal for the chunk; of a scale near the smallest numbers it would overflow
-            const float by = 1.0f / scale;
             float v[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = h[c][i] * by;
-            if (__builtin_expect(scale < 1e-35f, 0)) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) v[i] = h[c][i] / scale;
-            }
+            codes_of<W>(v, h[c], largest, rest, scale);
             uint32_t words[2];
 #pragma unroll
             for (int i = 0; i < W; i += 4) {
@@ -335,16 +353,22 @@ __global__ __launch_bounds__(RN_THREADS) void norm_forward_any_kernel(NormArgs a
     const Acc r = (Acc)1 / sqrt(sum / (Acc)a.D + (Acc)a.eps);
     if (FP8) {
         const int64_t group = a.groups == 1 ? a.D : a.group;
+        float power, rest;
+        parts_of((float)r, &power, &rest);
         for (int64_t g = 0; g < a.groups; ++g) {
             const int64_t end = (g + 1) * group < a.D ? (g + 1) * group : a.D;
             float top = 0;
-            for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS) top = larger(fabsf((float)(value(i) * r * weight(i))), top);
-            float scale = row_max<RN_THREADS>(top) / FP8_LARGEST;
-            if (scale == 0.0f) scale = 1.0f;
-            if (threadIdx.x == 0) a.scales[row * a.groups + g] = scale;
             for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS)
-                static_cast<uint8_t *>(a.q)[base + i] =
-                    (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32((float)(value(i) * r * weight(i)) / scale, 0.0f, 0, false) & 0xff);
+                top = larger(fabsf((float)value(i) * power * (float)weight(i)), top);
+            top = row_max<RN_THREADS>(top);
+            const float scale = scale_of(top, rest);
+            if (threadIdx.x == 0) a.scales[row * a.groups + g] = scale;
+            for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS) {
+                const float p[1] = {(float)value(i) * power * (float)weight(i)};
+                float v[1];
+                codes_of<1>(v, p, top, rest, scale);
+                static_cast<uint8_t *>(a.q)[base + i] = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], 0.0f, 0, false) & 0xff);
+            }
         }
     } else {
         for (int64_t i = threadIdx.x; i < a.D; i += RN_THREADS) static_cast<IO *>(a.y)[base + i] = narrow<IO>(value(i) * r * weight(i));

@@ -150,6 +150,22 @@ def test_eight_bits(shape, group, types):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape,group", [((500, 768), 0), ((300, 1021), 0), ((40, 4096), 128), ((6, 9000), 0), ((300, 5), 0)], ids=str)
+def test_eight_bits_are_those_of_the_exact_quotient(shape, group, dtype):
+    """of 16-bit numbers: the products h w are exact in 32 bits, and no quotient of two of them is nearer to the middle between two
+    8-bit numbers than 32 bits tell apart"""
+    import t2fw_amd as t2
+    (x, res, w), _, _ = inputs(*shape, (dtype,) * 3, seed=shape[1])
+    q, _, stored = t2.residual_rms_norm_fp8(x, res, w, eps=EPS, group=group)
+    D, width = shape[1], group or shape[1]
+    p = stored.double().cpu() * w.double().cpu()
+    top = torch.nn.functional.pad(p, (0, -D % width)).view(shape[0], -1, width).abs().amax(-1).repeat_interleave(width, 1)[:, :D]
+    want = (448 * p / top).float().to(torch.float8_e4m3fn)
+    assert torch.equal(q.cpu().double(), want.double())
+
+
+@pytest.mark.gpu
 def test_small_large_and_not_finite_rows():
     import t2fw_amd as t2
     w = torch.ones(256, device="cuda")
