@@ -417,19 +417,20 @@ int t2fw_rms_norm_backward(const void *g_y, const void *g_res, const void *store
  * logp = log softmax(logits)[target], r = exp(logp - old_logp), d = ref_logp - logp:
  *   loss = scale / M  sum over the M tokens of the mask of  -min(r adv, clip(r, low, high) adv) + kl (exp(d) - 1 - d).
  * old_logp, ref_logp, adv [N] float; mask [N] bytes, or null for all; M is at least 1.  Results: loss [1], logp [N] (of all tokens; 0 for
- * a token outside the mask whose target is none of the V), and lse, coef [N] for the backward call, all float.  d_logits, if
- * given: the gradient of the loss, in the logits' type.  A target outside [0, V) inside the mask makes the loss NaN.
+ * a token outside the mask whose target is none of the V), and for the backward call tops [N, 2], a row's largest logit and the sum of
+ * exp(logit - largest), and coef [N], all float.  d_logits, if given: the gradient of the loss, in the logits' type.  A target outside
+ * [0, V) inside the mask makes the loss NaN.
  */
 size_t t2fw_policy_loss_workspace_bytes(int64_t N);
 int t2fw_policy_loss_forward(const void *logits, const int64_t *targets, const float *old_logp, const float *ref_logp,
                              const float *adv, const void *mask,
-                             float *loss, float *logp, float *lse, float *coef, void *d_logits,
+                             float *loss, float *logp, float *tops, float *coef, void *d_logits,
                              int64_t N, int64_t V, float low, float high, float kl, float scale,
                              int32_t dtype, void *workspace, size_t workspace_bytes, void *stream);
 /* d_logits for the gradient g_loss [1] of the loss.  T2FW_LOSS_UNLESS_ONE: d_logits is what the forward call wrote, and stays where
  * g_loss is one. */
 #define T2FW_LOSS_UNLESS_ONE 1
-int t2fw_policy_loss_backward(const void *logits, const int64_t *targets, const float *lse, const float *coef,
+int t2fw_policy_loss_backward(const void *logits, const int64_t *targets, const float *tops, const float *coef,
                               const float *g_loss, void *d_logits, int64_t N, int64_t V,
                               int32_t dtype, int32_t flags, void *stream);
 

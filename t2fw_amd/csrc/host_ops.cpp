@@ -331,7 +331,7 @@ struct LossCall {
     double low, high, kl, scale;
 };
 struct LossResult {
-    Tensor loss, logp, lse, coef;
+    Tensor loss, logp, tops, coef;
 };
 LossResult loss_forward(const Tensor &logits, const Tensor &targets, const Tensor &old_logp, const Tensor &ref_logp, const Tensor &adv,
                         const Tensor &mask, const Tensor &d_logits, const LossCall &c, void *stream) {
@@ -340,14 +340,14 @@ LossResult loss_forward(const Tensor &logits, const Tensor &targets, const Tenso
     LossResult r;
     r.loss = at::empty({}, options);
     r.logp = at::empty(targets.sizes(), options);
-    // the log-sum-exps, the coefficients of the rows, and the call's scratch
+    // the largest logits and sums, the coefficients of the rows, and the call's scratch
     const size_t bytes = t2fw_policy_loss_workspace_bytes(N);
-    const Tensor both = at::empty({2, N}, options), ws = bytes_like(logits, (int64_t)bytes);
-    r.lse = both.select(0, 0);
-    r.coef = both.select(0, 1);
+    const Tensor all = at::empty({3, N}, options), ws = bytes_like(logits, (int64_t)bytes);
+    r.tops = all.narrow(0, 0, 2);
+    r.coef = all.select(0, 2);
     done(t2fw_policy_loss_forward(logits.data_ptr(), (const int64_t *)targets.data_ptr(), (const float *)old_logp.data_ptr(),
                                   (const float *)ref_logp.data_ptr(), (const float *)adv.data_ptr(), data(mask), (float *)r.loss.data_ptr(),
-                                  (float *)r.logp.data_ptr(), (float *)r.lse.data_ptr(), (float *)r.coef.data_ptr(), data(d_logits), N, V,
+                                  (float *)r.logp.data_ptr(), (float *)r.tops.data_ptr(), (float *)r.coef.data_ptr(), data(d_logits), N, V,
                                   (float)c.low, (float)c.high, (float)c.kl, (float)c.scale, dtype_code(logits, "logits"), ws.data_ptr(), bytes,
                                   stream));
     return r;
@@ -363,7 +363,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         if (logits.scalar_type() != at::kHalf) made = at::empty(logits.sizes(), logits.options());
         const LossResult r = loss_forward(logits, targets, old_logp, ref_logp, adv, mask, made, {low, high, kl, scale},
                                           reinterpret_cast<void *>((uintptr_t)stream));
-        ctx->save_for_backward({logits, targets, r.lse, r.coef});
+        ctx->save_for_backward({logits, targets, r.tops, r.coef});
         if (made.defined()) ctx->saved_data["made"] = made;
         ctx->saved_data["stream"] = stream;
         ctx->mark_non_differentiable({r.logp});
@@ -372,7 +372,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         once("policy_loss");
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &logits = saved[0], &targets = saved[1], &lse = saved[2], &coef = saved[3];
+        const Tensor &logits = saved[0], &targets = saved[1], &tops = saved[2], &coef = saved[3];
         const c10::DeviceGuard guard(logits.device());
         const Tensor g = grads[0].contiguous();
         Tensor d;
@@ -385,7 +385,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         } else {
             d = at::empty(logits.sizes(), logits.options());
         }
-        done(t2fw_policy_loss_backward(logits.data_ptr(), (const int64_t *)targets.data_ptr(), (const float *)lse.data_ptr(),
+        done(t2fw_policy_loss_backward(logits.data_ptr(), (const int64_t *)targets.data_ptr(), (const float *)tops.data_ptr(),
                                        (const float *)coef.data_ptr(), (const float *)g.data_ptr(), d.data_ptr(), targets.numel(), logits.size(-1),
                                        dtype_code(logits, "logits"), flags, as_address(ctx->saved_data["stream"])));
         return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};

@@ -267,7 +267,7 @@ int t2fw_rms_norm_backward(const void *g_y, const void *g_res, const void *store
 size_t t2fw_policy_loss_workspace_bytes(int64_t N) { return N < 0 ? 0 : (POLICY_SUMS + 1) * sizeof(double); }
 
 int t2fw_policy_loss_forward(const void *logits, const int64_t *targets, const float *old_logp, const float *ref_logp, const float *adv,
-                             const void *mask, float *loss, float *logp, float *lse, float *coef, void *d_logits, int64_t N, int64_t V,
+                             const void *mask, float *loss, float *logp, float *tops, float *coef, void *d_logits, int64_t N, int64_t V,
                              float low, float high, float kl, float scale, int32_t dtype, void *workspace, size_t workspace_bytes,
                              void *stream) {
     int rc = check_loss(N, V, dtype);
@@ -277,30 +277,30 @@ int t2fw_policy_loss_forward(const void *logits, const int64_t *targets, const f
     const bool none = N == 0;
     if ((rc = check_arrays({{"logits", logits, es, none}, {"targets", targets, 8, none}, {"old_logp", old_logp, 4, none},
                             {"ref_logp", ref_logp, 4, none}, {"adv", adv, 4, none}, {"loss", loss, 4, false}, {"logp", logp, 4, none},
-                            {"lse", lse, 4, none}, {"coef", coef, 4, none}, {"d_logits", d_logits, es, true}, {"workspace", workspace, 8, false}})))
+                            {"tops", tops, 4, none}, {"coef", coef, 4, none}, {"d_logits", d_logits, es, true}, {"workspace", workspace, 8, false}})))
         return rc;
     if (workspace_bytes < need) return bad_workspace(need, workspace_bytes);
     PolicyLossArgs a{};
     a.logits = logits; a.targets = targets; a.old_logp = old_logp; a.ref_logp = ref_logp; a.adv = adv;
     a.mask = static_cast<const uint8_t *>(mask);
-    a.loss = loss; a.logp = logp; a.lse = lse; a.coef = coef; a.tokens = static_cast<int64_t *>(workspace);
+    a.loss = loss; a.logp = logp; a.tops = tops; a.coef = coef; a.tokens = static_cast<int64_t *>(workspace);
     a.sums = static_cast<double *>(workspace) + 1; a.d_logits = d_logits;
     a.N = N; a.V = V; a.low = low; a.high = high; a.kl = kl; a.scale = scale;
     return policy_loss_forward(a, dtype, static_cast<hipStream_t>(stream));
 }
 
-int t2fw_policy_loss_backward(const void *logits, const int64_t *targets, const float *lse, const float *coef, const float *g_loss,
+int t2fw_policy_loss_backward(const void *logits, const int64_t *targets, const float *tops, const float *coef, const float *g_loss,
                               void *d_logits, int64_t N, int64_t V, int32_t dtype, int32_t flags, void *stream) {
     int rc = check_loss(N, V, dtype);
     if (rc) return rc;
     if (flags & ~T2FW_LOSS_UNLESS_ONE) return fail(T2FW_ERR_UNSUPPORTED, "policy loss: unknown flags %d", flags);
     if (N == 0) return T2FW_OK;
     const size_t es = size_of(dtype);
-    if ((rc = check_arrays({{"logits", logits, es, false}, {"targets", targets, 8, false}, {"lse", lse, 4, false}, {"coef", coef, 4, false},
+    if ((rc = check_arrays({{"logits", logits, es, false}, {"targets", targets, 8, false}, {"tops", tops, 4, false}, {"coef", coef, 4, false},
                             {"g_loss", g_loss, 4, false}, {"d_logits", d_logits, es, false}})))
         return rc;
     PolicyLossArgs a{};
-    a.logits = logits; a.targets = targets; a.lse = const_cast<float *>(lse); a.coef = const_cast<float *>(coef); a.g_loss = g_loss;
+    a.logits = logits; a.targets = targets; a.tops = const_cast<float *>(tops); a.coef = const_cast<float *>(coef); a.g_loss = g_loss;
     a.d_logits = d_logits;
     a.N = N; a.V = V;
     a.unless_one = (flags & T2FW_LOSS_UNLESS_ONE) != 0;

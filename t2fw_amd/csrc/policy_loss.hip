@@ -4,6 +4,8 @@
 //   d loss / d z = c (onehot(t) - softmax(z)),  c = scale / M (-r A [not held by the clip] - kl (exp(d) - 1)).
 // The coefficient c of a row depends on nothing but the row and M, so that the launch that reads a row for its log-sum-exp
 // writes its gradient too, for a gradient of the loss of one; the backward has nothing left to do then but to look at that value.
+// The log-sum-exp is never one number: with m the largest logit and s = sum exp(z - m), logp = (z_t - m) - log s and softmax = exp(z - m) / s,
+// so that logits with a common offset lose nothing to it.
 //
 // Bound by memory: 8192 x 50257 bf16, loss and gradient, 315 us (1.65 GB of logits and gradient, 5.2 TB/s, as a copy); with the gradient in a pass
 // of its own the logits would be read twice.  Few rows are bound by the chain load, exchange, exponentials, store: 333 x 8000
@@ -122,17 +124,17 @@ template <typename IO, int THREADS, int CH> struct Row {
         stay_narrow();
         return {m, s};
     }
-    // -c softmax, and at the target, by the thread that has just written there, c more
-    __device__ __forceinline__ void gradient(IO *dz, int64_t V, float lse, float c, int64_t target, float logp) const {
+    // -c softmax = -per exp(z - base), and at the target, by the thread that has just written there, c more
+    __device__ __forceinline__ void gradient(IO *dz, int64_t V, float base, float per, float c, int64_t target, float logp) const {
 #pragma unroll
         for (int k = 0; k < CH; ++k)
             if (at(k) < vectors) {
                 Vec<IO, VEC> o;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o.e[j] = narrow<IO>(-c * exp_of<IO>(element<IO>(v[k], j) - lse));
+                for (int j = 0; j < VEC; ++j) o.e[j] = narrow<IO>(-per * exp_of<IO>(element<IO>(v[k], j) - base));
                 store_vec(dz + head + (int64_t)at(k) * VEC, o);
             }
-        if (has_extra()) dz[extra_at()] = narrow<IO>(-c * exp_of<IO>(extra - lse));
+        if (has_extra()) dz[extra_at()] = narrow<IO>(-per * exp_of<IO>(extra - base));
         if (target >= 0 && target < V) {
             const int t = (int)target, in = t - head;
             const int owner = t < head ? t : in < vectors * VEC ? in / VEC % THREADS : head + in - vectors * VEC;
@@ -174,16 +176,16 @@ template <typename IO, int THREADS> struct Row<IO, THREADS, 0> {
         }
         return t;
     }
-    __device__ __forceinline__ void gradient(IO *dz, int64_t V, float lse, float c, int64_t target, float logp) const {
+    __device__ __forceinline__ void gradient(IO *dz, int64_t V, float base, float per, float c, int64_t target, float logp) const {
         for (int64_t i = (int64_t)threadIdx.x * VEC; i < V; i += THREADS * VEC) {
             if (i + VEC <= V) {
                 const Vec<IO, VEC> v = load_vec<IO, VEC>(z + i);
                 Vec<IO, VEC> o;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o.e[j] = narrow<IO>(-c * exp_of<IO>(widen(v.e[j]) - lse));
+                for (int j = 0; j < VEC; ++j) o.e[j] = narrow<IO>(-per * exp_of<IO>(widen(v.e[j]) - base));
                 store_vec(dz + i, o);
             } else {
-                for (int64_t j = i; j < V; ++j) dz[j] = narrow<IO>(-c * exp_of<IO>(widen(z[j]) - lse));
+                for (int64_t j = i; j < V; ++j) dz[j] = narrow<IO>(-per * exp_of<IO>(widen(z[j]) - base));
             }
             if (target >= i && target < i + VEC && target < V) dz[target] = narrow<IO>(fmaf(-c, exp_of<IO>(logp), c));
         }
@@ -217,18 +219,19 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void policy_rows_k
         if (threadIdx.x % 64 == 0) tops[turn][threadIdx.x / 64] = top;
         __syncthreads();                                 // (the other half is free again: every wave has read it before this row's barrier)
         top = joined_lanes<IO>(tops[turn][threadIdx.x % WAVES], WAVES);
-        const float lse = base_of(top.m) + logf(top.s), logp = known ? zt - lse : counts ? NAN : 0.0f;
+        const float base = base_of(top.m), logp = known ? zt - base - logf(top.s) : counts ? NAN : 0.0f;
         TokenTerms m{0, 0};
         if (counts) m = terms_of(a, row, logp);
         if (threadIdx.x == 0) {
             a.logp[row] = logp;
-            a.lse[row] = lse;
+            a.tops[2 * row] = base;
+            a.tops[2 * row + 1] = top.s;
             a.coef[row] = m.coef * share;
             sum += (double)(m.loss * share);
         }
         if (a.d_logits != nullptr) {
             IO *const dz = static_cast<IO *>(a.d_logits) + row * a.V;
-            if (counts) r.gradient(dz, a.V, lse, m.coef * share, t, logp);
+            if (counts) r.gradient(dz, a.V, base, m.coef * share / top.s, m.coef * share, t, logp);
             else r.zeros(dz, a.V);
         }
     }
@@ -258,12 +261,12 @@ __global__ __launch_bounds__(PL_THREADS) void policy_gradient_kernel(PolicyLossA
         const IO *z = static_cast<const IO *>(a.logits) + row * a.V;
         IO *const dz = static_cast<IO *>(a.d_logits) + row * a.V;
         const int64_t t = a.targets[row];
-        const float lse = a.lse[row], c = a.coef[row] * g;
-        const float logp = t >= 0 && t < a.V ? widen(z[t]) - lse : 0.0f;
+        const float base = a.tops[2 * row], s = a.tops[2 * row + 1], c = a.coef[row] * g;
+        const float logp = t >= 0 && t < a.V ? widen(z[t]) - base - logf(s) : 0.0f;
         Row<IO, PL_THREADS, 0> r;
         r.load(z, a.V);
         if (c == 0.0f) r.zeros(dz, a.V);
-        else r.gradient(dz, a.V, lse, c, t, logp);
+        else r.gradient(dz, a.V, base, c / s, c, t, logp);
     }
 }
 

@@ -12,7 +12,7 @@ struct PolicyLossArgs {
     const int64_t *targets;                      // [N]
     const float *old_logp, *ref_logp, *adv;      // [N]
     const uint8_t *mask;                         // [N], or null: every token counts
-    float *loss, *logp, *lse, *coef;             // [1]; [N] each: what the backward needs are the last two
+    float *loss, *logp, *tops, *coef;            // [1], [N], [N, 2], [N]: what the backward needs are the last two
     int64_t *tokens;                             // [1] scratch: the tokens that count
     double *sums;                                // [POLICY_SUMS] scratch: the workgroups' shares of the loss
     void *d_logits;                              // [N, V], or null: no gradient now

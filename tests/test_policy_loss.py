@@ -90,6 +90,19 @@ def test_values_and_gradients(shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(7, 300), (40, 8000), (3, 140000)], ids=str)
+def test_a_common_offset_of_the_logits_changes_no_bit(shape):
+    """32-bit logits in steps of 1/64, 4096 more of each: nothing is rounded in the addition, nor in a difference of two"""
+    ins = inputs(*shape, torch.float32, seed=11)
+    results = []
+    for offset in (0.0, 4096.0):
+        z = ((ins[0] * 64).round() / 64 + offset).requires_grad_(True)
+        loss, logp = call([z] + ins[1:])
+        results.append((loss, logp, torch.autograd.grad(loss, z, retain_graph=True)[0], torch.autograd.grad(3 * loss, z)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_any_factor_of_the_loss(dtype):
     """a factor as `scale`, one that the loss is multiplied by, and a second backward of one forward"""
