@@ -3,8 +3,10 @@
 //   backward, from dy and the stream's gradient dres:  u = w dy,  d_x = d_res = r (u - h r^2 mean(u h)) + dres,  d_w = sum over rows of dy h r.
 // The norm is of the rounded h, the one that the backward finds again; sums are carried in 32 bits (64 for double).
 // In 8 bits: y is divided by scale = max |y| / 448 of the row, or of each group of its columns, and rounded to float8 e4m3.  r is in both and
-// goes out: with p = (h 2^e) w, r = 2^e rest, 1 <= rest < 2, which a product of 16-bit numbers gives exactly, the code is that of
-// 448 p / max |p|, rounded once, and scale = max |p| rest / 448.
+// goes out: with p = (h 2^e) w, r = 2^e rest, 1 <= rest < 2, the code is that of 448 p / max |p|, rounded once, and
+// scale = max |p| rest / 448.  A product of 16-bit numbers is exact in 32 bits.  What the rounding of others leaves out is carried for a stream of
+// 32 bits, whose time it does not change (16384 x 8192: 325 us, without 322); next to a 16-bit stream, weights of 32 bits leave one
+// code in a million at the other side of a middle (carried, 32768 x 4096 would take 233 us for 193).
 //
 // A row stays in registers between its sums and its results: LANES threads hold it in chunks of 16 bytes of the stream, CH of them each, so that a
 // wave's loads and stores are of whole lines: 16 or 32 lanes of a wave for narrow rows, a wave, or 4 to 16 waves.  Every load of a row is made before its sums, without a branch between
@@ -146,18 +148,26 @@ __device__ __forceinline__ float scale_of(float top, float rest) {
     const float scale = top * rest / FP8_LARGEST;
     return scale == 0.0f ? 1.0f : scale;
 }
-// 448 p / top for W numbers: a product with the reciprocal and one correction of it, which leaves the rounded quotient.  For numbers
-// whose reciprocal or remainder 32 bits do not hold, those that are not finite among them, y / scale.
-template <int W> __device__ __forceinline__ void codes_of(float (&v)[W], const float (&p)[W], float top, float rest, float scale) {
-    const float by = 1.0f / top;
+// What the product of the largest lost in its rounding, of its absolute value; minus infinity from the others
+__device__ __forceinline__ float lost_of(float h, float w, float top) {
+    const float p = h * w, lost = fmaf(h, w, -p);
+    return fabsf(p) == top ? p < 0 ? -lost : lost : -INFINITY;
+}
+// 448 h w / (top + lost), or 448 h / top, for W numbers: a product with the reciprocal, and from the remainder what it is off by.  For numbers whose
+// reciprocal or remainder 32 bits do not hold, those that are not finite among them, y / scale.
+template <int W, bool CARRIED>
+__device__ __forceinline__ void codes_of(float (&v)[W], const float (&h)[W], const float (&w)[W], float top, float lost, float rest, float scale) {
+    const float by = 1.0f / top, by448 = by * FP8_LARGEST;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float n = p[i] * FP8_LARGEST, q = n * by;
-        v[i] = fmaf(fmaf(-q, top, n), by, q);
+        const float p = CARRIED ? h[i] * w[i] : h[i], q = p * by;
+        float left = fmaf(-q, top, p);
+        if (CARRIED) left = fmaf(-q, lost, left + fmaf(h[i], w[i], -p));
+        v[i] = fmaf(q, FP8_LARGEST, left * by448);
     }
     if (__builtin_expect(!(scale >= 1e-33f && scale != 1.0f && top <= 1e35f), 0)) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = p[i] * rest / scale;
+        for (int i = 0; i < W; ++i) v[i] = (CARRIED ? h[i] * w[i] : h[i]) * rest / scale;
     }
 }
 
@@ -207,6 +217,7 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
             if (live) store_chunk(static_cast<IO *>(a.y) + base, k[c], o);
         }
     } else {
+        constexpr bool CARRIED = sizeof(Stream) > 2;     // else h becomes the product
         float top[CH], all = 0, power, rest;
         parts_of(r, &power, &rest);
 #pragma unroll
@@ -214,22 +225,37 @@ __global__ __launch_bounds__(threads_of(LANES)) void norm_forward_kernel(NormArg
             top[c] = 0;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                h[c][i] = h[c][i] * power * w[c][i];
-                if (i >= k[c].skip) top[c] = larger(fabsf(h[c][i]), top[c]);
+                h[c][i] *= power;
+                if (!CARRIED) h[c][i] *= w[c][i];
+                if (i >= k[c].skip) top[c] = larger(fabsf(CARRIED ? h[c][i] * w[c][i] : h[c][i]), top[c]);
             }
             all = larger(top[c], all);
         }
         const bool by_row = a.groups == 1;
         if (by_row) all = row_max<LANES>(all);
+        float lost[CH], lost_all = -INFINITY;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            // a group's chunks are neighbouring lanes of one wave, those past the end of the row among them
-            const float largest = by_row ? all : lanes_max(top[c], (int)(a.group / W)), scale = scale_of(largest, rest);
+            // (a group's chunks are neighbouring lanes of one wave, those past the end of the row among them)
+            if (!by_row) top[c] = lanes_max(top[c], (int)(a.group / W));
+            lost[c] = 0;
+            if (!CARRIED) continue;
+            lost[c] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (i >= k[c].skip) lost[c] = fmaxf(lost[c], lost_of(h[c][i], w[c][i], by_row ? all : top[c]));
+            lost_all = fmaxf(lost_all, lost[c]);
+            if (!by_row) lost[c] = lanes_max(lost[c], (int)(a.group / W));
+        }
+        if (CARRIED && by_row) lost_all = row_max<LANES>(lost_all);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const float largest = by_row ? all : top[c], scale = scale_of(largest, rest);
             if (!live || !k[c].there()) continue;
             const int64_t g = by_row ? 0 : k[c].column / a.group;
             if (by_row ? lane == 0 && c == 0 : k[c].column % a.group == 0) a.scales[row * a.groups + g] = scale;
             float v[W];
-            codes_of<W>(v, h[c], largest, rest, scale);
+            codes_of<W, CARRIED>(v, h[c], w[c], largest, by_row ? lost_all : lost[c], rest, scale);
             uint32_t words[2];
 #pragma unroll
             for (int i = 0; i < W; i += 4) {
@@ -361,12 +387,16 @@ __global__ __launch_bounds__(RN_THREADS) void norm_forward_any_kernel(NormArgs a
             for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS)
                 top = larger(fabsf((float)value(i) * power * (float)weight(i)), top);
             top = row_max<RN_THREADS>(top);
+            float lost = -INFINITY;
+            for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS)
+                lost = fmaxf(lost, lost_of((float)value(i) * power, (float)weight(i), top));
+            lost = row_max<RN_THREADS>(lost);
             const float scale = scale_of(top, rest);
             if (threadIdx.x == 0) a.scales[row * a.groups + g] = scale;
             for (int64_t i = g * group + threadIdx.x; i < end; i += RN_THREADS) {
-                const float p[1] = {(float)value(i) * power * (float)weight(i)};
+                const float h[1] = {(float)value(i) * power}, w[1] = {(float)weight(i)};
                 float v[1];
-                codes_of<1>(v, p, top, rest, scale);
+                codes_of<1, true>(v, h, w, top, lost, rest, scale);
                 static_cast<uint8_t *>(a.q)[base + i] = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], 0.0f, 0, false) & 0xff);
             }
         }
