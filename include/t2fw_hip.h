@@ -416,7 +416,7 @@ int t2fw_rms_norm_backward(const void *g_y, const void *g_res, const void *store
  * Clipped policy loss with a KL term, from the logits [N, V] (fp32 / fp16 / bf16) and targets [N] of N tokens.  With
  * logp = log softmax(logits)[target], r = exp(logp - old_logp), d = ref_logp - logp:
  *   loss = scale / M  sum over the M tokens of the mask of  -min(r adv, clip(r, low, high) adv) + kl (exp(d) - 1 - d).
- * old_logp, ref_logp, adv [N] float; mask [N] bytes, or null for all; M is at least 1.  Results: loss [1], logp [N] (of all tokens; 0 for
+ * old_logp, ref_logp, adv [N] float (ref_logp is not read where kl is 0); mask [N] bytes, or null for all; M is at least 1.  Results: loss [1], logp [N] (of all tokens; 0 for
  * a token outside the mask whose target is none of the V), and for the backward call tops [N, 2], a row's largest logit and the sum of
  * exp(logit - largest), and coef [N], all float.  d_logits, if given: the gradient of the loss, in the logits' type.  A target outside
  * [0, V) inside the mask makes the loss NaN.

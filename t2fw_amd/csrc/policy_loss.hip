@@ -42,11 +42,15 @@ struct TokenTerms {
 };
 // one token's share of the loss and its row's coefficient, both without scale / M
 __device__ __forceinline__ TokenTerms terms_of(const PolicyLossArgs &a, int64_t row, float logp) {
-    const float adv = a.adv[row], r = expf(logp - a.old_logp[row]), d = a.ref_logp[row] - logp, em = expm1f(d);
+    const float adv = a.adv[row], r = expf(logp - a.old_logp[row]);
     const float freely = r * adv, held = fminf(fmaxf(r, a.low), a.high) * adv;
     const bool moves = freely < held || (r >= a.low && r <= a.high) || r != r;
     // the clip's comparisons drop a NaN that the sums keep
-    return {(r != r ? r : -fminf(freely, held)) + a.kl * (em - d), (moves ? -freely : 0.0f) - a.kl * em};
+    const TokenTerms clipped{r != r ? r : -fminf(freely, held), moves ? -freely : 0.0f};
+    // left out rather than multiplied by zero: without a reference its log probabilities are anything, and exp(ref - logp) may be infinite
+    if (a.kl == 0.0f) return clipped;
+    const float d = a.ref_logp[row] - logp, em = expm1f(d);
+    return {clipped.loss + a.kl * (em - d), clipped.coef - a.kl * em};
 }
 
 // What a workgroup needs besides a row: the number of tokens that count.  Every workgroup counts them itself as long as that is 16 bytes

@@ -13,7 +13,8 @@ def policy_loss(logits, targets, old_logp, ref_logp, advantages, mask=None, clip
         loss = scale * mean over the mask's tokens of  -min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef (exp(d) - 1 - d)
 
     ``logits: [..., V]`` float32, float16 or bfloat16; ``targets`` int64, ``old_logp, ref_logp, advantages`` float32 and ``mask`` bool,
-    each of the shape of the tokens.  No token in the mask: the loss is zero.  A target outside the vocabulary is for tokens
+    each of the shape of the tokens.  With ``kl_coef=0`` the values of ``ref_logp`` are not looked at: any tensor of that shape will do.
+    No token in the mask: the loss is zero.  A target outside the vocabulary is for tokens
     outside the mask (``logp`` is 0 there); inside it makes the loss NaN.
 
     Float32 and bfloat16 logits: the forward writes their gradient in the pass that reads them, for a loss that is
