@@ -437,6 +437,8 @@ int t2fw_policy_loss_backward(const void *logits, const int64_t *targets, const 
 /*
  * The 2-norm of all arrays together (any of the four types each), to norm [1], and the arrays times
  * min(1, max_norm / (norm + 1e-6)), each to its dst: its src (in place), another array, or null (not wanted).  `arrays` is host memory.
+ * Norm and factor are computed in double; a norm above the largest float is infinite in `norm` only.  ..._f64: the same with max_norm
+ * in double, which arrays of T2FW_F64 tell apart.
  */
 typedef struct t2fw_clip_desc {
     const void *src;
@@ -447,6 +449,8 @@ typedef struct t2fw_clip_desc {
 size_t t2fw_clip_workspace_bytes(const t2fw_clip_desc *arrays, int64_t count);
 int t2fw_clip_grad_norm(const t2fw_clip_desc *arrays, int64_t count, float max_norm, float *norm,
                         void *workspace, size_t workspace_bytes, void *stream);
+int t2fw_clip_grad_norm_f64(const t2fw_clip_desc *arrays, int64_t count, double max_norm, float *norm,
+                            void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -83,6 +83,7 @@ SIGNATURES = {
     "t2fw_policy_loss_backward": (ctypes.c_int, [_vp] * 6 + [_i64] * 2 + [_i32, _i32, _vp]),
     "t2fw_clip_workspace_bytes": (_sz, [ctypes.POINTER(ClipDesc), _i64]),
     "t2fw_clip_grad_norm": (ctypes.c_int, [ctypes.POINTER(ClipDesc), _i64, ctypes.c_float, _vp, _vp, _sz, _vp]),
+    "t2fw_clip_grad_norm_f64": (ctypes.c_int, [ctypes.POINTER(ClipDesc), _i64, ctypes.c_double, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

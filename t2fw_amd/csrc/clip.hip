@@ -98,19 +98,24 @@ __global__ __launch_bounds__(CLIP_THREADS) void clip_squares_kernel(ClipTable t,
     if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-template <typename A, typename B> __device__ __forceinline__ void scale_share(const A *src, B *dst, uint32_t n, float by) {
+// A product in double, whatever the types: a norm above float32's largest has a factor that 32 bits do not hold, and 64-bit gradients keep
+// theirs.  16-bit results go by way of 32 bits.
+template <typename B> __device__ __forceinline__ B scaled(double v, double by) {
+    return sizeof(B) == 2 ? narrow<B>((float)(v * by)) : narrow<B>(v * by);
+}
+template <typename A, typename B> __device__ __forceinline__ void scale_share(const A *src, B *dst, uint32_t n, double by) {
     constexpr int VEC = 16 / (sizeof(A) > sizeof(B) ? sizeof(A) : sizeof(B));
     over<A, VEC, 8>(
         src, n,
         [&](uint32_t i, const Vec<A, VEC> &v) {
             Vec<B, VEC> o;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o.e[j] = narrow<B>(widen(v.e[j]) * by);
+            for (int j = 0; j < VEC; ++j) o.e[j] = scaled<B>(widen(v.e[j]), by);
             store_past(dst + i, o);
         },
-        [&](uint32_t i, A e) { dst[i] = narrow<B>(widen(e) * by); });
+        [&](uint32_t i, A e) { dst[i] = scaled<B>(widen(e), by); });
 }
-template <typename A> __device__ __forceinline__ void scale_from(const A *src, void *dst, int dst_type, uint32_t at, uint32_t n, float by) {
+template <typename A> __device__ __forceinline__ void scale_from(const A *src, void *dst, int dst_type, uint32_t at, uint32_t n, double by) {
     switch (dst_type) {
         case T2FW_F32: scale_share(src + at, static_cast<float *>(dst) + at, n, by); break;
         case T2FW_F16: scale_share(src + at, static_cast<_Float16 *>(dst) + at, n, by); break;
@@ -119,17 +124,17 @@ template <typename A> __device__ __forceinline__ void scale_from(const A *src, v
     }
 }
 
-__global__ __launch_bounds__(CLIP_THREADS) void clip_scale_kernel(ClipTable t, const double *partials, int total, float max_norm, float *norm) {
+__global__ __launch_bounds__(CLIP_THREADS) void clip_scale_kernel(ClipTable t, const double *partials, int total, double max_norm, float *norm) {
     double s = 0;
     for (int i = threadIdx.x; i < total; i += CLIP_THREADS) s += partials[i];
-    const float n = (float)sqrt(block_sum(s));
-    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
-    const float ratio = max_norm / (n + 1e-6f), by = ratio > 1.0f ? 1.0f : ratio;         // a norm that is NaN makes NaN of everything
+    const double n = sqrt(block_sum(s));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    const double ratio = max_norm / (n + 1e-6), by = ratio > 1.0 ? 1.0 : ratio;           // a norm that is NaN makes NaN of everything
     // From the last array to the first, and with stores that leave the last-level cache alone: it still holds much of what the sums have just
     // read.  119 M bf16 gradients into float32: 204 us with ordinary stores, 157 so (713 MB at the rate of a copy: 143).
     for_share(t, gridDim.x - 1 - blockIdx.x, gridDim.x, [&](int a, uint32_t from, uint32_t m) {
         // not wanted; or in place and within the limit: nothing changes
-        if (t.dst[a] == nullptr || (by == 1.0f && t.dst[a] == t.src[a])) return;
+        if (t.dst[a] == nullptr || (by == 1.0 && t.dst[a] == t.src[a])) return;
         switch (t.src_type[a]) {
             case T2FW_F32: scale_from(static_cast<const float *>(t.src[a]), t.dst[a], t.dst_type[a], from, m, by); break;
             case T2FW_F16: scale_from(static_cast<const _Float16 *>(t.src[a]), t.dst[a], t.dst_type[a], from, m, by); break;
@@ -146,7 +151,7 @@ int clip_squares(const ClipTable &t, int groups, double *partials, hipStream_t s
     return check_hip(hipGetLastError(), "clip_squares_kernel launch");
 }
 
-int clip_scale(const ClipTable &t, int groups, const double *partials, int total, float max_norm, float *norm, hipStream_t stream) {
+int clip_scale(const ClipTable &t, int groups, const double *partials, int total, double max_norm, float *norm, hipStream_t stream) {
     hipLaunchKernelGGL(clip_scale_kernel, dim3(groups), dim3(CLIP_THREADS), 0, stream, t, partials, total, max_norm, norm);
     return check_hip(hipGetLastError(), "clip_scale_kernel launch");
 }

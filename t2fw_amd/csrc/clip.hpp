@@ -22,6 +22,6 @@ struct ClipTable {
 // sums of squares of a table's arrays, one for each workgroup, to partials[0 .. groups)
 int clip_squares(const ClipTable &t, int groups, double *partials, hipStream_t stream);
 // norm = sqrt of the sum of all `total` partials; arrays times min(1, max_norm / (norm + 1e-6)), to dst
-int clip_scale(const ClipTable &t, int groups, const double *partials, int total, float max_norm, float *norm, hipStream_t stream);
+int clip_scale(const ClipTable &t, int groups, const double *partials, int total, double max_norm, float *norm, hipStream_t stream);
 
 }  // namespace t2fw

@@ -478,7 +478,7 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const size_t bytes = t2fw_clip_workspace_bytes(d.data(), count);
     const Tensor norm = at::empty({}, first.options().dtype(at::kFloat)), ws = bytes_like(first, (int64_t)bytes);
     done(unlocked([&] {
-        return t2fw_clip_grad_norm(d.data(), count, (float)most, (float *)norm.data_ptr(), ws.data_ptr(), bytes, stream);
+        return t2fw_clip_grad_norm_f64(d.data(), count, most, (float *)norm.data_ptr(), ws.data_ptr(), bytes, stream);
     }));
     if (!alone)
         for (Py_ssize_t i = 0; i < count; ++i) {

@@ -318,11 +318,16 @@ size_t t2fw_clip_workspace_bytes(const t2fw_clip_desc *arrays, int64_t count) tr
 }
 
 int t2fw_clip_grad_norm(const t2fw_clip_desc *arrays, int64_t count, float max_norm, float *norm, void *workspace, size_t workspace_bytes,
-                        void *stream) try {
+                        void *stream) {
+    return t2fw_clip_grad_norm_f64(arrays, count, max_norm, norm, workspace, workspace_bytes, stream);
+}
+
+int t2fw_clip_grad_norm_f64(const t2fw_clip_desc *arrays, int64_t count, double max_norm, float *norm, void *workspace, size_t workspace_bytes,
+                            void *stream) try {
     std::vector<ClipTable> tables;
     int rc = clip_tables(tables, arrays, count);
     if (rc) return rc;
-    if (!(max_norm >= 0)) return fail(T2FW_ERR_BAD_SHAPE, "clipping: a largest norm of %g", (double)max_norm);
+    if (!(max_norm >= 0)) return fail(T2FW_ERR_BAD_SHAPE, "clipping: a largest norm of %g", max_norm);
     if ((rc = check_arrays({{"norm", norm, 4, false}, {"workspace", workspace, 8, false}}))) return rc;
     int total = 0;
     for (const ClipTable &t : tables) total += clip_groups(t);
