@@ -3,6 +3,7 @@
 // autograd function costs 44 to 91 (host.cpp).  A backward runs on the stream of its forward, as torch runs every node.
 #include "host.hpp"
 
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 namespace t2fw_host {
@@ -58,6 +59,11 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     for (const Tensor &t : ts)
         if (t.defined() && t.requires_grad()) return true;
     return false;
+}
+// Forward-mode derivatives: there are none, and a result without its tangent would pass for one whose tangent is zero
+void no_tangents(std::initializer_list<Tensor> ts, const char *what) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor &t : ts) TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "t2fw: ", what, " has no forward-mode derivatives");
 }
 // The gradients are results of kernels that torch knows nothing of
 void once(const char *what) { TORCH_CHECK(!at::GradMode::is_enabled(), "t2fw: ", what, " can be differentiated once only (create_graph)"); }
@@ -140,6 +146,7 @@ PyObject *gated_scan(PyObject *, PyObject *const *a, Py_ssize_t n) {
     arguments(n, 6);
     const Tensor x = tensor(a[0]), f = tensor(a[1]), state = optional_tensor(a[2]), lengths = optional_tensor(a[3]);
     check_on(x, x, "x");
+    no_tangents({x, f, state}, "gated_scan");
     check_on(f, x, "f");
     TORCH_CHECK(x.dim() == 3 && x.size(2) >= 1, "t2fw: expected x, f [B, T, D] with at least one channel, x is ", x.sizes());
     check_sizes(f, x.sizes(), "f");
@@ -184,6 +191,7 @@ PyObject *gated_scan_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
     check_type(state, accumulators_type(x), "state");
     TORCH_CHECK(!wants_grad({x, f, state}), "t2fw: gated_scan_step has no gradients: call gated_scan, or this under torch.no_grad()");
     Tensor out = optional_tensor(a[3]);
+    no_tangents({x, f, state, out}, "gated_scan_step");
     if (out.defined()) {
         check_contiguous(out, x, "out");
         check_sizes(out, x.sizes(), "out");
@@ -285,6 +293,7 @@ PyObject *residual_rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     arguments(n, 5);
     const Tensor x = tensor(a[0]), res = optional_tensor(a[1]), w = tensor(a[2]);
     const NormCall c = check_norm(x, res, w);
+    no_tangents({x, res, w}, "residual_rms_norm");
     const double eps = real(a[3]);
     void *const stream = address(a[4]);
     const c10::DeviceGuard guard(x.device());
@@ -309,6 +318,7 @@ PyObject *residual_rms_norm_fp8(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor &x = tensor(a[0]), res = optional_tensor(a[1]), &w = tensor(a[2]);
     const NormCall c = check_norm(x, res, w);
     TORCH_CHECK(!wants_grad({x, res, w}), "t2fw: residual_rms_norm_fp8 has no gradients: call it under torch.no_grad()");
+    no_tangents({x, res, w}, "residual_rms_norm_fp8");
     const double eps = real(a[3]);
     const int64_t group = integer(a[4]);
     void *const stream = address(a[5]);
@@ -399,6 +409,7 @@ PyObject *policy_loss(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor logits = tensor(a[0]), targets = tensor(a[1]), mask = optional_tensor(a[5]);
     const Tensor per[3] = {tensor(a[2]), tensor(a[3]), tensor(a[4])};
     check_contiguous(logits, logits, "logits");
+    no_tangents({logits, per[0], per[1], per[2]}, "policy_loss");
     TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1, "t2fw: expected logits [..., V] with V of at least one, they are ", logits.sizes());
     TORCH_CHECK(dtype_code(logits, "logits") != T2FW_F64, "t2fw: unsupported dtype ", logits.scalar_type(), " of logits");
     const at::IntArrayRef tokens = logits.sizes().slice(0, logits.dim() - 1);
@@ -460,6 +471,7 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     for (Py_ssize_t i = 0; i < count; ++i) {
         const Tensor &g = tensor(PySequence_Fast_GET_ITEM(grads.ptr(), i));
         check_dense(g, first, "every gradient");
+        no_tangents({g}, "clip_grad_norm");
         d[i].src = g.data_ptr();
         d[i].dst = inplace ? g.data_ptr() : nullptr;
         d[i].n = g.numel();
@@ -467,6 +479,7 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (!outs) continue;
         const Tensor &o = tensor(PySequence_Fast_GET_ITEM(outs.ptr(), i));
         check_dense(o, first, "every result");
+        no_tangents({o}, "clip_grad_norm");
         check_sizes(o, g.sizes(), "a result");
         TORCH_CHECK(o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous()), "t2fw: a result is laid out otherwise than its gradient");
         d[i].dst = o.data_ptr();
