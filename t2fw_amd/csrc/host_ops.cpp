@@ -68,6 +68,15 @@ void no_tangents(std::initializer_list<Tensor> ts, const char *what) {
 // The gradients are results of kernels that torch knows nothing of
 void once(const char *what) { TORCH_CHECK(!at::GradMode::is_enabled(), "t2fw: ", what, " can be differentiated once only (create_graph)"); }
 
+// What a node has saved, dense and of the type and number of elements that its kernels take: hooks on saved tensors may bring it back in
+// another order of memory
+Tensor restored(const Tensor &t, const Tensor &like, at::ScalarType type, int64_t numel) {
+    check_on(t, like, "a saved tensor");
+    check_type(t, type, "a saved tensor");
+    TORCH_CHECK(t.numel() == numel, "t2fw: a saved tensor has ", t.numel(), " elements, expected ", numel);
+    return t.contiguous();
+}
+
 // An address in a node's saved data
 int64_t as_integer(void *p) { return (int64_t)(uintptr_t)p; }
 void *as_address(const c10::IValue &v) { return reinterpret_cast<void *>((uintptr_t)v.toInt()); }
@@ -112,13 +121,27 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         once("gated_scan");
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &f = saved[1], &lengths = saved[2], &ckpt = saved[3];
-        const c10::DeviceGuard guard(x.device());
+        check_on(saved[0], saved[0], "a saved tensor");
+        check_on(saved[1], saved[0], "a saved tensor");
+        TORCH_CHECK(saved[0].dim() == 3, "t2fw: a saved tensor has ", saved[0].dim(), " axes, expected 3");
+        check_type(saved[1], saved[0].scalar_type(), "a saved tensor");
+        check_sizes(saved[1], saved[0].sizes(), "a saved tensor");
+        const c10::DeviceGuard guard(saved[0].device());
+        const Tensor x = dense_channels(saved[0]), f = dense_channels(saved[1]);
         const int64_t B = x.size(0), T = x.size(1), D = x.size(2);
         const int32_t dtype = dtype_code(x, "x");
+        const Tensor ckpt = restored(saved[3], x, at::kByte, (int64_t)t2fw_gated_scan_checkpoint_bytes(B, T, D, dtype));
+        const bool wide = (ctx->saved_data["flags"].toInt() & T2FW_SCAN_LENGTHS64) != 0;
+        const Tensor lengths = saved[2].defined() ? restored(saved[2], x, wide ? at::kLong : at::kInt, B) : Tensor();
         // a result that nothing depends on has no gradient
         const Tensor go = grads[0].defined() ? dense_channels(grads[0]) : at::zeros({1}, x.options()).expand({B, T, D}).contiguous();
         const Tensor gs = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        check_type(go, x.scalar_type(), "the gradient");
+        check_sizes(go, x.sizes(), "the gradient");
+        if (gs.defined()) {
+            check_type(gs, accumulators_type(x), "the state's gradient");
+            check_sizes(gs, {B, D}, "the state's gradient");
+        }
         const Tensor dx = at::empty({B, T, D}, x.options()), df = at::empty({B, T, D}, f.options());
         Tensor ds, ws;
         if (ctx->saved_data["state"].toBool()) ds = at::empty({B, D}, x.options().dtype(accumulators_type(x)));
@@ -265,12 +288,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         once("residual_rms_norm");
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &stored = saved[0], &w = saved[1];
-        const c10::DeviceGuard guard(stored.device());
+        const c10::DeviceGuard guard(saved[0].device());
         const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
         const int64_t N = ctx->saved_data["N"].toInt(), D = ctx->saved_data["D"].toInt();
         const int32_t dtype = (int32_t)ctx->saved_data["dtype"].toInt(), flags = (int32_t)ctx->saved_data["flags"].toInt();
         const bool residual = ctx->saved_data["residual"].toBool(), wide = (flags & T2FW_NORM_STREAM_F32) != 0;
+        const Tensor stored = restored(saved[0], saved[0], wide ? at::kFloat : type, N * D);
+        const Tensor w = restored(saved[1], stored, (flags & T2FW_NORM_WEIGHT_F32) != 0 ? at::kFloat : type, D);
         const auto options = stored.options().dtype(type);
         const Tensor gy = grads[0].defined() ? grads[0].contiguous() : at::zeros(stored.sizes(), options);
         const Tensor gres = residual && grads[1].defined() ? grads[1].contiguous() : Tensor();
@@ -375,6 +399,9 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
                                           reinterpret_cast<void *>((uintptr_t)stream));
         ctx->save_for_backward({logits, targets, r.tops, r.coef});
         if (made.defined()) ctx->saved_data["made"] = made;
+        ctx->saved_data["N"] = targets.numel();
+        ctx->saved_data["V"] = logits.size(-1);
+        ctx->saved_data["type"] = (int64_t)logits.scalar_type();
         ctx->saved_data["stream"] = stream;
         ctx->mark_non_differentiable({r.logp});
         return {r.loss, r.logp};
@@ -382,8 +409,11 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         once("policy_loss");
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &logits = saved[0], &targets = saved[1], &tops = saved[2], &coef = saved[3];
-        const c10::DeviceGuard guard(logits.device());
+        const c10::DeviceGuard guard(saved[0].device());
+        const int64_t N = ctx->saved_data["N"].toInt(), V = ctx->saved_data["V"].toInt();
+        const Tensor logits = restored(saved[0], saved[0], (at::ScalarType)ctx->saved_data["type"].toInt(), N * V);
+        const Tensor targets = restored(saved[1], logits, at::kLong, N), tops = restored(saved[2], logits, at::kFloat, 2 * N);
+        const Tensor coef = restored(saved[3], logits, at::kFloat, N);
         const Tensor g = grads[0].contiguous();
         Tensor d;
         int32_t flags = 0;
@@ -396,7 +426,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
             d = at::empty(logits.sizes(), logits.options());
         }
         done(t2fw_policy_loss_backward(logits.data_ptr(), (const int64_t *)targets.data_ptr(), (const float *)tops.data_ptr(),
-                                       (const float *)coef.data_ptr(), (const float *)g.data_ptr(), d.data_ptr(), targets.numel(), logits.size(-1),
+                                       (const float *)coef.data_ptr(), (const float *)g.data_ptr(), d.data_ptr(), N, V,
                                        dtype_code(logits, "logits"), flags, as_address(ctx->saved_data["stream"])));
         return {d, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
