@@ -6,6 +6,8 @@
 #include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 
+#include <algorithm>
+
 namespace t2fw_host {
 namespace {
 
@@ -480,6 +482,28 @@ void check_dense(const Tensor &t, const Tensor &like, const char *name) {
     TORCH_CHECK(t.is_non_overlapping_and_dense(), name, " must be dense");
 }
 
+// Many workgroups write the results at once: none may share memory with another, nor with a gradient, but its own in place.
+void check_apart(const std::vector<t2fw_clip_desc> &d, const std::vector<int64_t> &sizes) {
+    struct Span {
+        uintptr_t begin, end;
+        bool operator<(const Span &o) const { return begin < o.begin; }
+    };
+    std::vector<Span> to;
+    to.reserve(d.size());
+    const auto span = [](const void *p, int64_t bytes) { return Span{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes}; };
+    for (size_t i = 0; i < d.size(); ++i)
+        if (d[i].dst != nullptr && d[i].n > 0) to.push_back(span(d[i].dst, d[i].n * sizes[2 * i + 1]));
+    if (!std::is_sorted(to.begin(), to.end())) std::sort(to.begin(), to.end());
+    for (size_t i = 1; i < to.size(); ++i) TORCH_CHECK(to[i - 1].end <= to[i].begin, "t2fw: two results of clip_grad_norm share memory");
+    for (size_t i = 0; i < d.size(); ++i) {
+        if (to.empty() || d[i].n == 0 || (d[i].src == d[i].dst && d[i].src_dtype == d[i].dst_dtype)) continue;
+        const Span s = span(d[i].src, d[i].n * sizes[2 * i]);
+        // the first result that begins at the gradient's end or later; the one before it is the last that could reach into the gradient
+        const auto next = std::lower_bound(to.begin(), to.end(), Span{s.end, s.end});
+        TORCH_CHECK(next == to.begin() || (next - 1)->end <= s.begin, "t2fw: a result of clip_grad_norm shares memory with a gradient");
+    }
+}
+
 // clip_grad_norm(sequence of tensors, largest norm, sequence of results, None for in place, False for the norm alone, stream) -> norm
 PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -498,6 +522,7 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor first = tensor(PySequence_Fast_GET_ITEM(grads.ptr(), 0));
     check_on(first, first, "gradients");
     std::vector<t2fw_clip_desc> d((size_t)count);
+    std::vector<int64_t> sizes((size_t)count * 2);       // of an element of each gradient and of its result
     for (Py_ssize_t i = 0; i < count; ++i) {
         const Tensor &g = tensor(PySequence_Fast_GET_ITEM(grads.ptr(), i));
         check_dense(g, first, "every gradient");
@@ -506,6 +531,7 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
         d[i].dst = inplace ? g.data_ptr() : nullptr;
         d[i].n = g.numel();
         d[i].src_dtype = d[i].dst_dtype = dtype_code(g, "a gradient");
+        sizes[2 * i] = sizes[2 * i + 1] = g.element_size();
         if (!outs) continue;
         const Tensor &o = tensor(PySequence_Fast_GET_ITEM(outs.ptr(), i));
         check_dense(o, first, "every result");
@@ -514,7 +540,9 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
         TORCH_CHECK(o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous()), "t2fw: a result is laid out otherwise than its gradient");
         d[i].dst = o.data_ptr();
         d[i].dst_dtype = dtype_code(o, "a result");
+        sizes[2 * i + 1] = o.element_size();
     }
+    check_apart(d, sizes);
     const double most = real(a[1]);
     void *const stream = address(a[3]);
     const c10::DeviceGuard guard(first.device());

@@ -15,7 +15,8 @@ def clip_grad_norm(grads, max_norm, out=None):
     """Multiplies ``grads`` (a list of tensors, ``[p.grad for p in model.parameters() if p.grad is not None]``) by
     ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being the 2-norm of all of them together, and returns the norm as it was before, a
     float32 scalar on the device.  In place, or into ``out``, a list of tensors of the same shapes and any type (float32
-    gradients for the optimizer from 16-bit ones).  Types may be mixed.  Within the limit gradients in place are not touched.  Norm and factor
+    gradients for the optimizer from 16-bit ones).  Types may be mixed.  What is written may share memory with nothing else of the call: a tensor that is
+    in the list twice is refused.  Within the limit gradients in place are not touched.  Norm and factor
     are computed in float64: gradients whose norm is above the largest float32 are scaled as others are, while the norm returned is
     infinite.  An infinite gradient (or squares beyond float64) makes zeros of the finite ones and NaN of the infinite ones, a NaN makes NaN of
     all of them."""
