@@ -489,32 +489,51 @@ int64_t backward_groups(int64_t N, int64_t D) {
         else RUN(1024, 2);                                                                                                          \
     } while (0)
 
-template <typename IO, typename Stream, bool FP8> int forward_of(const NormArgs &a, hipStream_t stream) {
-    const int64_t groups = (a.N + rows_of_group(a.D) - 1) / rows_of_group(a.D);
-    if (groups > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "norm: too many rows for one launch");
-    const dim3 grid((unsigned)groups);
+// Rows `at` and the `n - 1` after them
+template <typename IO, typename Stream> NormArgs rows_of(const NormArgs &a, int64_t at, int64_t n) {
+    const auto moved = [](auto p, int64_t bytes) { return p == nullptr ? p : decltype(p)((uintptr_t)p + bytes); };
+    NormArgs r = a;
+    r.N = n;
+    r.x = moved(a.x, at * a.D * sizeof(IO));
+    r.res = moved(a.res, at * a.D * sizeof(Stream));
+    r.y = moved(a.y, at * a.D * sizeof(IO));
+    r.stored = moved(a.stored, at * a.D * sizeof(Stream));
+    r.q = moved(a.q, at * a.D);
+    r.scales = moved(a.scales, at * a.groups * sizeof(float));
+    return r;
+}
+
+template <typename IO, typename Stream, bool FP8> int forward_of(const NormArgs &all, hipStream_t stream) {
+    // A grid has less than 2^32 threads along an axis; of more the hardware starts the remainder, and no error comes.
+    const int64_t per_group = rows_of_group(all.D), most = per_group * ((1ll << 31) / (lanes_of(all.D) ? threads_of(lanes_of(all.D)) : RN_THREADS));
     // 8 bits: a chunk is 8 columns in every type, as a group's chunks have to be in one wave
     constexpr int W = FP8 ? RN_WIDTH : chunk_of<Stream>(), PER = RN_WIDTH / W;
+    for (int64_t at = 0; at < all.N; at += most) {
+        const NormArgs a = rows_of<IO, Stream>(all, at, all.N - at < most ? all.N - at : most);
+        const dim3 grid((unsigned)((a.N + per_group - 1) / per_group));
 #define NORM_RUN(L, C) hipLaunchKernelGGL((norm_forward_kernel<IO, Stream, L, C * PER, W, FP8>), grid, threads, 0, stream, a)
-    NORM_BY_WIDTH(NORM_RUN, hipLaunchKernelGGL((norm_forward_any_kernel<IO, Stream, FP8>), grid, threads, 0, stream, a));
+        NORM_BY_WIDTH(NORM_RUN, hipLaunchKernelGGL((norm_forward_any_kernel<IO, Stream, FP8>), grid, threads, 0, stream, a));
 #undef NORM_RUN
-    return check_hip(hipGetLastError(), "norm_forward_kernel launch");
+        const int rc = check_hip(hipGetLastError(), "norm_forward_kernel launch");
+        if (rc) return rc;
+    }
+    return T2FW_OK;
 }
 
 template <typename IO, typename Stream> int backward_of(const NormArgs &a, hipStream_t stream) {
     using Acc = typename AccT<IO>::type;
-    const int64_t groups = backward_groups(a.N, a.D);
+    const int64_t groups = backward_groups(a.N, a.D), columns = (a.D + RW_COLUMNS - 1) / RW_COLUMNS;
+    if (columns * RW_THREADS > 0xffffffffll) return fail(T2FW_ERR_BAD_SHAPE, "norm: too many columns for one launch of the weights' gradient");
     const dim3 grid((unsigned)groups);
     if (a.N > 0) {
-    constexpr int W = chunk_of<Stream>(), PER = RN_WIDTH / W;
+        constexpr int W = chunk_of<Stream>(), PER = RN_WIDTH / W;
 #define NORM_RUN(L, C) hipLaunchKernelGGL((norm_backward_kernel<IO, Stream, L, C * PER, W>), grid, threads, 0, stream, a)
         NORM_BY_WIDTH(NORM_RUN, hipLaunchKernelGGL((norm_backward_any_kernel<IO, Stream>), grid, threads, 0, stream, a));
 #undef NORM_RUN
         const int rc = check_hip(hipGetLastError(), "norm_backward_kernel launch");
         if (rc) return rc;
     }
-    hipLaunchKernelGGL((norm_weights_kernel<IO, Acc>), dim3((unsigned)((a.D + RW_COLUMNS - 1) / RW_COLUMNS)), dim3(RW_THREADS), 0, stream, a,
-                       norm_partials(a.N, a.D));
+    hipLaunchKernelGGL((norm_weights_kernel<IO, Acc>), dim3((unsigned)columns), dim3(RW_THREADS), 0, stream, a, norm_partials(a.N, a.D));
     return check_hip(hipGetLastError(), "norm_weights_kernel launch");
 }
 
