@@ -33,6 +33,8 @@ namespace {
 constexpr int GS_THREADS = 256;
 constexpr int GS_CHANNELS = 64;          // channels of a workgroup (CHN below: 128 to FEW_STEPS of them where there are few steps)
 constexpr int FEW_STEPS = 1024;
+// A grid has less than 2^32 threads along an axis; of more the hardware starts the remainder, and no error comes
+constexpr int64_t MOST_GROUPS = (1ll << 32) / GS_THREADS - 1;
 constexpr int ALL_AT_ONCE = 2048;        // workgroups: less than two rounds of the chip
 
 // elements of a lane: 32 in all, whatever the type
@@ -586,13 +588,13 @@ __global__ __launch_bounds__(GS_THREADS, sizeof(Acc) == 8 ? 1 : sizeof(IO) == 2 
 
 // No steps: the value before them (zeros where there is none) is that after them
 template <typename Acc> __global__ __launch_bounds__(GS_THREADS) void gscan_pass_kernel(const void *from, void *to, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * GS_THREADS + threadIdx.x;
-    if (i < n) static_cast<Acc *>(to)[i] = from == nullptr ? (Acc)0 : static_cast<const Acc *>(from)[i];
+    for (int64_t i = (int64_t)blockIdx.x * GS_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * GS_THREADS)
+        static_cast<Acc *>(to)[i] = from == nullptr ? (Acc)0 : static_cast<const Acc *>(from)[i];
 }
 template <typename Acc> int pass(const void *from, void *to, int64_t n, hipStream_t stream) {
     if (to == nullptr) return T2FW_OK;
-    if (n > 0x7fffffffll * GS_THREADS) return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many channels for one launch");
-    hipLaunchKernelGGL(gscan_pass_kernel<Acc>, dim3((unsigned)((n + GS_THREADS - 1) / GS_THREADS)), dim3(GS_THREADS), 0, stream, from, to, n);
+    const int64_t groups = (n + GS_THREADS - 1) / GS_THREADS;
+    hipLaunchKernelGGL(gscan_pass_kernel<Acc>, dim3((unsigned)(groups < MOST_GROUPS ? groups : MOST_GROUPS)), dim3(GS_THREADS), 0, stream, from, to, n);
     return check_hip(hipGetLastError(), "gscan_pass_kernel launch");
 }
 
@@ -644,7 +646,7 @@ template <typename IO, int VEC, int R> GscanGrid grid_of(int64_t B, int64_t T, i
     g.per_row = (uint32_t)per_row;
     g.blocks = (uint32_t)blocks;
     g.chunks = (uint32_t)chunks;
-    g.fits = per_row < 0x7fffffff && B * per_row < 0x7fffffff && chunks < 0x7fffffff && blocks * chunks < 0x7fffffff;
+    g.fits = per_row < 0x7fffffff && B * per_row < 0x7fffffff && chunks <= MOST_GROUPS && blocks * chunks <= MOST_GROUPS;
     g.slots = blocks * g.channels;
     // Where all workgroups are on the chip at once, the time is that of the wait: one group, so that nothing waits for a map made of
     // maps (1 x 8191 x 768 bf16 forward, 64 chunks: 15.3 us, in groups of 8 20.2).  Otherwise the words read are what costs (2 x 32768 x
@@ -732,7 +734,7 @@ template <typename IO> int step_of(const GscanArgs &a, hipStream_t stream) {
     using Acc = typename AccT<IO>::type;
     constexpr int VEC = 16 / sizeof(IO);
     const int64_t n = a.B * a.D, groups = (n + (int64_t)GS_THREADS * VEC - 1) / ((int64_t)GS_THREADS * VEC);
-    if (groups > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many channels for one launch");
+    if (groups > MOST_GROUPS) return fail(T2FW_ERR_BAD_SHAPE, "gated scan: too many channels for one launch");
     hipLaunchKernelGGL((gscan_step_kernel<IO, Acc, VEC>), dim3((unsigned)groups), dim3(GS_THREADS), 0, stream, a, n);
     return check_hip(hipGetLastError(), "gscan_step_kernel launch");
 }
