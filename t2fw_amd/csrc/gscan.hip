@@ -62,7 +62,9 @@ template <bool BACK, typename Acc> __device__ __forceinline__ Map<Acc> extended(
 }
 
 template <typename IO> __device__ __forceinline__ float gate_of(float z) {
-    // 16-bit gates: hardware exponential and reciprocal (2^-21); 32-bit ones: the library's
+    // From 16-bit logits: hardware exponential, off by |z| 1.25 2^-24 (its argument is rounded to 32 bits once multiplied by log2 e) and 2^-22, and
+    // reciprocal, 2^-22: 2^-20 at z = -8, 2^-18 at -40.  The logit's own rounding to 16 bits is worth |z| 2^-12 or 2^-9.  From 32-bit ones: the library's,
+    // with which 32 x 4096 x 1024 bf16 would take 258 and 401 us for 176 and 273.
     return sizeof(IO) == 2 ? __builtin_amdgcn_rcpf(1.0f + __expf(-z)) : 1.0f / (1.0f + expf(-z));
 }
 template <typename IO> __device__ __forceinline__ double gate_of(double z) { return 1.0 / (1.0 + exp(-z)); }

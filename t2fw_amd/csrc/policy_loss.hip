@@ -16,7 +16,9 @@
 namespace t2fw {
 namespace {
 
-// 16-bit logits: the hardware's exponential (2^-21 relative at arguments of -20); 32-bit ones: the library's
+// 16-bit logits: the hardware's exponential, off by |v| 1.25 2^-24 (the argument is rounded to 32 bits once multiplied by log2 e) and 2^-22: 2^-19
+// at a logit 20 below the largest, whose term is 2^-29 of the largest's; the logits' own rounding is worth 2^-12 or 2^-9 of them.  32-bit ones: the library's, with
+// which 8192 x 50257 bf16 would take 493 us for 325.
 template <typename IO> __device__ __forceinline__ float exp_of(float v) { return sizeof(IO) == 2 ? __expf(v) : expf(v); }
 
 constexpr int PL_THREADS = 1024;
