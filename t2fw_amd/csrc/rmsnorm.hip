@@ -458,7 +458,12 @@ __global__ __launch_bounds__(RW_THREADS) void norm_weights_kernel(NormArgs a, in
 template <typename Stream> constexpr int chunk_of() { return sizeof(Stream) == 2 ? 8 : 4; }
 constexpr int64_t WIDEST = 16384;        // columns of a row in registers
 bool in_registers(int64_t D) { return D >= RN_WIDTH && D <= WIDEST; }
-// threads of a row (0: the kernels for any width), for chunks of one or two to a thread
+// Threads of a row (0: the kernels for any width), with chunks of one or two for each: lanes that have no columns cost as others do, and two
+// chunks a thread are slower backward than one of twice as many threads.  bf16, forward and backward in us, the threads taken first:
+//   65536 x 64    16: 10.2, 14.9   32: 14.8, 21.1            16384 x 1024   64: 26.5, 29.3   256: 26.9, 38.6
+//   65536 x 128   16: 17.1, 16.5   32: 16.6, 20.7            16384 x 2048   256: 57.4, 59.2   512: 64.6, 72.1
+//   32768 x 256   32: 16.6, 16.8   16: 15.9, 17.3   64: 16.6, 20.8   8192 x 4096   512: 55.2, 54.4   256: 55.6, 60.9   1024: 62.2, 83.3
+//   32768 x 512   64: 27.5, 27.4   32: 26.3, 28.4            8192 x 8192    512: 106, 108   1024: 107, 122
 int lanes_of(int64_t D) {
     return !in_registers(D) ? 0 : D <= 128 ? 16 : D <= 256 ? 32 : D <= 1024 ? 64 : D <= 2048 ? 256 : D <= 8192 ? 512 : 1024;
 }
