@@ -44,6 +44,9 @@ at::ScalarType accumulators_type(const Tensor &t) { return t.scalar_type() == at
 
 void check_on(const Tensor &t, const Tensor &like, const char *name) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.layout() == at::kStrided, name, " must be a dense tensor");
+    // (its memory holds the other sign)
+    TORCH_CHECK(!t.is_neg(), name, " is a negated view: call resolve_neg()");
     TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", not on ", like.device());
 }
 void check_contiguous(const Tensor &t, const Tensor &like, const char *name) {
@@ -84,9 +87,10 @@ int64_t as_integer(void *p) { return (int64_t)(uintptr_t)p; }
 void *as_address(const c10::IValue &v) { return reinterpret_cast<void *>((uintptr_t)v.toInt()); }
 
 // ---- gated_scan ---------------------------------------------------------------------------------------------------
+// (a gradient may be a view that torch negates when it reads it)
 // x, f [B, T, D] with dense channels; anything else is copied (gradients that are expanded scalars, say)
 Tensor dense_channels(const Tensor &t) {
-    return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous();
+    return t.size(2) <= 1 || t.stride(2) == 1 ? t.resolve_neg() : t.contiguous().resolve_neg();
 }
 
 struct ScanResult {
@@ -137,7 +141,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
         const Tensor lengths = saved[2].defined() ? restored(saved[2], x, wide ? at::kLong : at::kInt, B) : Tensor();
         // a result that nothing depends on has no gradient
         const Tensor go = grads[0].defined() ? dense_channels(grads[0]) : at::zeros({1}, x.options()).expand({B, T, D}).contiguous();
-        const Tensor gs = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor gs = grads[1].defined() ? grads[1].contiguous().resolve_neg() : Tensor();
         check_type(go, x.scalar_type(), "the gradient");
         check_sizes(go, x.sizes(), "the gradient");
         if (gs.defined()) {
@@ -298,8 +302,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor stored = restored(saved[0], saved[0], wide ? at::kFloat : type, N * D);
         const Tensor w = restored(saved[1], stored, (flags & T2FW_NORM_WEIGHT_F32) != 0 ? at::kFloat : type, D);
         const auto options = stored.options().dtype(type);
-        const Tensor gy = grads[0].defined() ? grads[0].contiguous() : at::zeros(stored.sizes(), options);
-        const Tensor gres = residual && grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor gy = grads[0].defined() ? grads[0].contiguous().resolve_neg() : at::zeros(stored.sizes(), options);
+        const Tensor gres = residual && grads[1].defined() ? grads[1].contiguous().resolve_neg() : Tensor();
         const Tensor dx = at::empty(stored.sizes(), options), dw = at::empty(w.sizes(), w.options());
         const Tensor dres = wide ? at::empty(stored.sizes(), stored.options()) : Tensor();
         const size_t bytes = t2fw_rms_norm_backward_workspace_bytes(N, D, dtype);
@@ -416,7 +420,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const Tensor logits = restored(saved[0], saved[0], (at::ScalarType)ctx->saved_data["type"].toInt(), N * V);
         const Tensor targets = restored(saved[1], logits, at::kLong, N), tops = restored(saved[2], logits, at::kFloat, 2 * N);
         const Tensor coef = restored(saved[3], logits, at::kFloat, N);
-        const Tensor g = grads[0].contiguous();
+        const Tensor g = grads[0].contiguous().resolve_neg();
         Tensor d;
         int32_t flags = 0;
         const auto made = ctx->saved_data.find("made");
