@@ -360,7 +360,7 @@ int t2fw_gate_backward(const void *d_f, const void *d_f_key, const void *f, cons
  * of row b from lengths[b] on do not count, whatever they hold; their results are zero and the state passes them as it
  * is.  `strides`: elements between rows and steps of x and f (x_b, x_t, f_b, f_t), or null for dense arrays; the channels of
  * a step are next to each other.  The products of a row's gates have to stay finite (of gates in [-1, 1] they always
- * do).  T2FW_SCAN_LOGITS: f holds gate logits, the gate is their sigmoid.
+ * do); next to infinite values, which they multiply, one that underflows makes NaN.  T2FW_SCAN_LOGITS: f holds gate logits, the gate is their sigmoid.
  * `ckpt`: t2fw_gated_scan_checkpoint_bytes for the backward call, or null.
  */
 #define T2FW_SCAN_LOGITS 1

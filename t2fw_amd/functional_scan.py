@@ -21,8 +21,9 @@ def gated_scan(x, f, state=None, lengths=None, logits=False):
     strides between rows and steps: parts of a projection need not be copied.  ``state: [B, D]``, the state before the first step
     (``None``: zeros), and the last state are float32 (float64 for float64 tensors) whatever the type of ``x``: a state
     that takes up thousands of steps is not rounded between calls.  Gates may be any numbers, but their products over the steps of a sequence
-    have to stay finite: stretches are put together by them, and an infinite one makes NaN even of a state of zero.  ``logits=True``: ``f`` holds gate logits, the gate is their
-    sigmoid, and the gradient that comes back is the logits'.
+    have to stay finite: stretches are put together by them, and an infinite one makes NaN even of a state of zero.  So does, next to an
+    infinite state or step, a product too small for the accumulators' type, where the recurrence step by step would stay infinite.
+    ``logits=True``: ``f`` holds gate logits, the gate is their sigmoid, and the gradient that comes back is the logits'.
 
     ``lengths: [B]`` (int32 or int64, on the device), for rows that are padded at their end: steps from ``lengths[b]`` on do not count,
     whatever they hold, NaN included.  Their outputs and gradients are zero, and the last state of the row is that after its last
