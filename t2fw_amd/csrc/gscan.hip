@@ -35,7 +35,7 @@ constexpr int GS_CHANNELS = 64;          // channels of a workgroup (CHN below: 
 constexpr int FEW_STEPS = 1024;
 // A grid has less than 2^32 threads along an axis; of more the hardware starts the remainder, and no error comes
 constexpr int64_t MOST_GROUPS = (1ll << 32) / GS_THREADS - 1;
-constexpr int ALL_AT_ONCE = 2048;        // workgroups: less than two rounds of the chip
+constexpr int FEW_GROUPS = 2048;         // workgroups (the chip holds 512 to 1280 of them, by type and direction)
 
 // elements of a lane: 32 in all, whatever the type
 template <typename IO> struct Tile {
@@ -354,13 +354,15 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(uint64_t *words
 // Which block of channels and which chunk (in the direction of the recurrence) a workgroup has.  The hardware deals workgroups out to the
 // eight dies in turn, each with a cache of its own: runs of 16 neighbouring blocks go to one die, so that the lines that neighbours share,
 // as they do where rows start anywhere, are fetched and written once (32 x 4096 bf16, forward: 1021 channels 250 -> 183 us, 1024
-// 190 -> 163).  Runs of 4 where all workgroups are on the chip at once (8 x 1024 x 768, backward: 15.9 us, of 16 18.3).
+// 190 -> 163; in runs of 4 the backward of 32 x 4096 x 1024 takes 296 us, of 16 273).  Runs of 4 for few workgroups: a backward right after its
+// forward finds more of the inputs in its die's cache (8 x 1024 x 768: 15.9 us, of 16 18.3; by itself the same either way, while
+// 1 x 12000 x 1021 loses by it, 36.5 and 34.2).
 constexpr uint32_t DIES = 8;
 struct Turn {
     uint32_t block, chunk;
 };
 __device__ __forceinline__ Turn turn_of(const GscanGrid &gr) {
-    const uint32_t near = gridDim.x < ALL_AT_ONCE ? 4 : 16, round = DIES * near;
+    const uint32_t near = gridDim.x < FEW_GROUPS ? 4 : 16, round = DIES * near;
     uint32_t n = blockIdx.x;
     if (n < gridDim.x / round * round) {
         const uint32_t in = n % round;
@@ -650,13 +652,15 @@ template <typename IO, int VEC, int R> GscanGrid grid_of(int64_t B, int64_t T, i
     g.chunks = (uint32_t)chunks;
     g.fits = per_row < 0x7fffffff && B * per_row < 0x7fffffff && chunks <= MOST_GROUPS && blocks * chunks <= MOST_GROUPS;
     g.slots = blocks * g.channels;
-    // Where all workgroups are on the chip at once, the time is that of the wait: one group, so that nothing waits for a map made of
-    // maps (1 x 8191 x 768 bf16 forward, 64 chunks: 15.3 us, in groups of 8 20.2).  Otherwise the words read are what costs (2 x 32768 x
-    // 1024 bf16 backward, 256 chunks: groups of 16 156 us, 32 161, 64 171, 128 185).  One or two workgroups side by side are between the
+    // With few workgroups the time is largely that of the wait: one group, so that nothing waits for a map made of maps (forward and backward
+    // with the emptying launch: 1 x 8191 x 768 bf16, 768 workgroups, 18.3 and 22.0 us, in groups of 8 23.4 and 26.1; 2 x 8191 x 768, 1536 of
+    // them, 24.7 and 33.1, 26.5 and 33.0; only 1 x 16384 x 768, 1536 of 128 chunks, loses by it: 28.7 and 36.8, in groups of 16 27.7 and
+    // 34.5).  Otherwise the words read are what costs (1 x 16384 x 1024, 2048 workgroups: in groups of 16 30.1 and 46.1, one group 33.9 and 52.8;
+    // 2 x 32768 x 1024 backward, 256 chunks: groups of 16 156, 32 161, 64 171, 128 185).  One or two workgroups side by side are between the
     // two, few words and long waits: groups twice as large (1 x 131072 x 128 bf16 forward and backward: 44 and 56 us, without 60 and 77;
     // of four workgroups side by side, 2 x 65536 x 128, the same either way).
     g.group = 8;
-    if (chunks <= 128 && blocks * chunks < ALL_AT_ONCE) g.group = 128;
+    if (chunks <= 128 && blocks * chunks < FEW_GROUPS) g.group = 128;
     while ((uint64_t)g.group * g.group < (uint64_t)chunks) g.group *= 2;
     if (blocks <= 2 && chunks > 128) g.group *= 2;
     return g;
