@@ -355,8 +355,8 @@ __global__ __launch_bounds__(GS_THREADS) void gscan_empty_kernel(uint64_t *words
 // eight dies in turn, each with a cache of its own: runs of 16 neighbouring blocks go to one die, so that the lines that neighbours share,
 // as they do where rows start anywhere, are fetched and written once (32 x 4096 bf16, forward: 1021 channels 250 -> 183 us, 1024
 // 190 -> 163; in runs of 4 the backward of 32 x 4096 x 1024 takes 296 us, of 16 273).  Runs of 4 for few workgroups: a backward right after its
-// forward finds more of the inputs in its die's cache (8 x 1024 x 768: 15.9 us, of 16 18.3; by itself the same either way, while
-// 1 x 12000 x 1021 loses by it, 36.5 and 34.2).
+// forward, 8 x 1024 x 768, 15.9 us, of 16 18.3 (the same backward over and over does not tell them apart; 1 x 12000 x 1021 loses by it, 36.5 and
+// 34.2).
 constexpr uint32_t DIES = 8;
 struct Turn {
     uint32_t block, chunk;
