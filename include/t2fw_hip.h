@@ -452,6 +452,60 @@ int t2fw_clip_grad_norm(const t2fw_clip_desc *arrays, int64_t count, float max_n
 int t2fw_clip_grad_norm_f64(const t2fw_clip_desc *arrays, int64_t count, double max_norm, float *norm,
                             void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * A selective state space layer, and beam search over recurrent states.  As above: no counterpart in the reference.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/*
+ * Causal convolution of `taps` (2 to 8) steps per channel: z_t = bias + sum_j w[d, j] xs_{t+j}, xs being s0 [B, taps - 1, D] (null: zeros), the
+ * inputs before the first, oldest first, and then x [B, T, D]; y = z, or z sigmoid(z) with T2FW_CONV_SILU.  fp32 / fp16 / bf16; w [D, taps] and bias [D]
+ * (or null) of that type, or float with T2FW_CONV_WEIGHT_F32.  `last` [B, taps - 1, D]: the inputs before the next sequence.
+ * `lengths` [B] (int32, or int64 with T2FW_CONV_LENGTHS64), or null: steps of row b from lengths[b] on do not count,
+ * whatever they hold; y is zero there, and `last` is what precedes them.  `strides`: elements between rows and steps of x, or null for a dense array; the channels of a
+ * step are next to each other.
+ */
+#define T2FW_CONV_SILU 1
+#define T2FW_CONV_LENGTHS64 2
+#define T2FW_CONV_WEIGHT_F32 4
+int t2fw_short_conv_forward(const void *x, const void *w, const void *bias, const void *s0, const void *lengths,
+                            void *y, void *last, int64_t B, int64_t T, int64_t D, int64_t taps,
+                            const int64_t *strides, int32_t dtype, int32_t flags, void *stream);
+/*
+ * Gradients from those of y and of `last` (g_last, or null): d_x, d_w, d_bias and d_s0 (null where they are not wanted) in the types of what they belong to.
+ * strides: as above, then g_y's two.  Sums over rows and steps are made in float, in a fixed order.
+ */
+size_t t2fw_short_conv_backward_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t taps, int32_t dtype);
+int t2fw_short_conv_backward(const void *g_y, const void *g_last, const void *x, const void *w, const void *bias,
+                             const void *s0, const void *lengths, void *d_x, void *d_w, void *d_bias, void *d_s0,
+                             int64_t B, int64_t T, int64_t D, int64_t taps, const int64_t *strides,
+                             int32_t dtype, int32_t flags, void *workspace, size_t workspace_bytes, void *stream);
+/* One step: x [B, D] with x_stride elements between its rows, y [B, D]; next_state == s0 (in place) is allowed. */
+int t2fw_short_conv_step(const void *x, const void *w, const void *bias, const void *s0, void *y, void *next_state,
+                         int64_t B, int64_t D, int64_t taps, int64_t x_stride, int32_t dtype, int32_t flags, void *stream);
+
+/*
+ * The n (1 to 128) best of the K V candidates of each of B requests, best first: candidate (k, v) has the score scores[k] + log softmax(logits[k])[v].
+ * logits [B, K, V] fp32 / fp16 / bf16, K at most 256; scores [B, K] float; results [B, n].  Of equal scores the lower k V + v is the better one; scores are compared in double, with sums of
+ * float exponentials.  `finished` [B, K] bytes, or null: a beam that has ended has one candidate, the token `pad`, with its own score.  A
+ * candidate that cannot be (a logit of minus infinity, a score of minus infinity or NaN, another token of an ended beam, a beam with a NaN or plus infinity among
+ * its logits) has a score of minus infinity; which tokens of a beam with NaN come is not said.
+ */
+size_t t2fw_beam_select_workspace_bytes(int64_t B, int64_t K, int64_t V, int64_t n, int32_t dtype);
+int t2fw_beam_select(const void *logits, const float *scores, const void *finished,
+                     float *out_scores, int64_t *out_beams, int64_t *out_tokens,
+                     int64_t B, int64_t K, int64_t V, int64_t n, int64_t pad, int32_t dtype,
+                     void *workspace, size_t workspace_bytes, void *stream);
+/*
+ * What belongs to beams, moved to the beams that go on from them: dst[b, k] = src[b, beams[b, k]], rows of row_bytes, for K (1 to 64) beams of each of B
+ * requests.  dst == src (in place) is allowed, another overlap is not, nor one with beams [B, K].  An index that is no beam stands for k.  `arrays` is host memory.
+ */
+typedef struct t2fw_reorder_desc {
+    const void *src;
+    void *dst;
+    int64_t row_bytes;
+} t2fw_reorder_desc;
+int t2fw_beam_reorder(const t2fw_reorder_desc *arrays, int64_t count, const int64_t *beams, int64_t B, int64_t K, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,10 @@ class BlockCopyDesc(ctypes.Structure):
                 ("terms", _i64), ("term_stride", _i64)]
 
 
+class ReorderDesc(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("row_bytes", _i64)]
+
+
 class ClipDesc(ctypes.Structure):
     _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("n", _i64), ("src_dtype", _i32), ("dst_dtype", _i32)]
 
@@ -84,6 +88,13 @@ SIGNATURES = {
     "t2fw_clip_workspace_bytes": (_sz, [ctypes.POINTER(ClipDesc), _i64]),
     "t2fw_clip_grad_norm": (ctypes.c_int, [ctypes.POINTER(ClipDesc), _i64, ctypes.c_float, _vp, _vp, _sz, _vp]),
     "t2fw_clip_grad_norm_f64": (ctypes.c_int, [ctypes.POINTER(ClipDesc), _i64, ctypes.c_double, _vp, _vp, _sz, _vp]),
+    "t2fw_short_conv_forward": (ctypes.c_int, [_vp] * 7 + [_i64] * 4 + [ctypes.POINTER(_i64), _i32, _i32, _vp]),
+    "t2fw_short_conv_backward_workspace_bytes": (_sz, [_i64] * 4 + [_i32]),
+    "t2fw_short_conv_backward": (ctypes.c_int, [_vp] * 11 + [_i64] * 4 + [ctypes.POINTER(_i64), _i32, _i32, _vp, _sz, _vp]),
+    "t2fw_short_conv_step": (ctypes.c_int, [_vp] * 6 + [_i64] * 4 + [_i32, _i32, _vp]),
+    "t2fw_beam_select_workspace_bytes": (_sz, [_i64] * 4 + [_i32]),
+    "t2fw_beam_select": (ctypes.c_int, [_vp] * 6 + [_i64] * 5 + [_i32, _vp, _sz, _vp]),
+    "t2fw_beam_reorder": (ctypes.c_int, [ctypes.POINTER(ReorderDesc), _i64, _vp, _i64, _i64, _vp]),
 }
 
 _lib = None

@@ -1,5 +1,5 @@
 """Builds t2fw_amd/lib/libt2fw_hip.so from t2fw_amd/csrc/*.hip with hipcc for gfx950, and
-t2fw_amd/lib/_t2fw_host.so from csrc/host.cpp and csrc/host_ops.cpp with g++.
+t2fw_amd/lib/_t2fw_host.so from csrc/host*.cpp with g++.
 
     python -m t2fw_amd.build            # build (always recompiles)
     python -m t2fw_amd.build --if-missing
@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libt2fw_hip.so")
-HOST_SRCS = [os.path.join(CSRC, "host.cpp"), os.path.join(CSRC, "host_ops.cpp")]
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_ops.cpp", "host_layers.cpp")]
 HOST_PATH = os.path.join(LIB_DIR, "_t2fw_host.so")
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 

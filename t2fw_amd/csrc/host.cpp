@@ -389,11 +389,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_t2fw_host", nullptr, -1, methods,
 
 }  // namespace
 
+using t2fw_host::layer_methods;
 using t2fw_host::operator_methods;
 
 PyMODINIT_FUNC PyInit__t2fw_host() {
     PyObject *const m = PyModule_Create(&module);
-    if (m != nullptr && PyModule_AddFunctions(m, operator_methods) != 0) {
+    if (m != nullptr && (PyModule_AddFunctions(m, operator_methods) != 0 || PyModule_AddFunctions(m, layer_methods) != 0)) {
         Py_DECREF(m);
         return nullptr;
     }

@@ -53,5 +53,7 @@ inline Tensor bytes_like(const Tensor &t, int64_t n) { return at::empty({n}, t.o
 
 // the operators around the recurrences (host_ops.cpp)
 extern PyMethodDef operator_methods[];
+// the selective state space layer and beam search (host_layers.cpp)
+extern PyMethodDef layer_methods[];
 
 }  // namespace t2fw_host

@@ -14,6 +14,7 @@ Inputs are already gated, as for ``LFWFunction`` (t2fw/functional_lfw.py:25-30).
 """
 import torch
 
+from .beam import reorder_beams
 from .functional_lfw import LFWFunction, lfw_step
 
 
@@ -79,6 +80,16 @@ class FastWeightState(torch.nn.Module):
         super()._apply(fn, *args, **kwargs)
         if self.state is not None:
             self.state = fn(self.state.detach())
+        return self
+
+    @torch.no_grad()
+    def reorder(self, beams):
+        """Beam search: ``beams: [requests, K]``, the beam that each of the K goes on from; the rows are those of ``requests * K``
+        beams, or of their heads, heads innermost."""
+        if self.state is not None:
+            if self.state.grad_fn is not None or self.state.requires_grad:
+                self.state = self.state.detach().clone()         # (a recorded graph may read it: as in forward)
+            reorder_beams([self.state], beams)
         return self
 
     def detach_state(self):
