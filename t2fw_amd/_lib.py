@@ -92,6 +92,12 @@ SIGNATURES = {
     "t2fw_short_conv_backward_workspace_bytes": (_sz, [_i64] * 4 + [_i32]),
     "t2fw_short_conv_backward": (ctypes.c_int, [_vp] * 11 + [_i64] * 4 + [ctypes.POINTER(_i64), _i32, _i32, _vp, _sz, _vp]),
     "t2fw_short_conv_step": (ctypes.c_int, [_vp] * 6 + [_i64] * 4 + [_i32, _i32, _vp]),
+    "t2fw_selective_scan_checkpoint_bytes": (_sz, [_i64] * 4),
+    "t2fw_selective_scan_workspace_bytes": (_sz, [_i64] * 4),
+    "t2fw_selective_scan_forward": (ctypes.c_int, [_vp] * 13 + [_i64] * 4 + [ctypes.POINTER(_i64), _i32, _i32, _vp, _sz, _vp]),
+    "t2fw_selective_scan_backward_workspace_bytes": (_sz, [_i64] * 4),
+    "t2fw_selective_scan_backward": (ctypes.c_int, [_vp] * 21 + [_i64] * 4 + [ctypes.POINTER(_i64), _i32, _i32, _vp, _sz, _vp]),
+    "t2fw_selective_scan_step": (ctypes.c_int, [_vp] * 11 + [_i64] * 3 + [ctypes.POINTER(_i64), _i32, _i32, _vp]),
     "t2fw_beam_select_workspace_bytes": (_sz, [_i64] * 4 + [_i32]),
     "t2fw_beam_select": (ctypes.c_int, [_vp] * 6 + [_i64] * 5 + [_i32, _vp, _sz, _vp]),
     "t2fw_beam_reorder": (ctypes.c_int, [ctypes.POINTER(ReorderDesc), _i64, _vp, _i64, _i64, _vp]),

@@ -190,6 +190,203 @@ PyObject *short_conv_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- selective_scan -----------------------------------------------------------------------------------------------
+// x, dt, a, b, c, state, skip, gate, dt_bias, lengths, as the entry points have them; those that may be missing are undefined then
+struct SelectInputs {
+    Tensor x, dt, a, b, c, state, skip, gate, dt_bias, lengths;
+};
+struct SelectResult {
+    Tensor y, last, ckpt;
+};
+SelectResult select_forward(const SelectInputs &i, int32_t flags, bool need_grad, void *stream) {
+    const int64_t B = i.x.size(0), T = i.x.size(1), D = i.x.size(2), N = i.a.size(1);
+    SelectResult r;
+    r.y = at::empty({B, T, D}, i.x.options());
+    r.last = at::empty({B, D, N}, i.a.options());
+    if (need_grad) r.ckpt = bytes_like(i.x, (int64_t)t2fw_selective_scan_checkpoint_bytes(B, T, D, N));
+    const size_t bytes = t2fw_selective_scan_workspace_bytes(B, T, D, N);
+    Tensor ws;
+    if (bytes > 0) ws = bytes_like(i.x, (int64_t)bytes);
+    const bool gated = i.gate.defined();
+    const int64_t strides[10] = {i.x.stride(0), i.x.stride(1), i.dt.stride(0), i.dt.stride(1), i.b.stride(0), i.b.stride(1), i.c.stride(0), i.c.stride(1),
+                                 gated ? i.gate.stride(0) : 0, gated ? i.gate.stride(1) : 0};
+    done(t2fw_selective_scan_forward(i.x.data_ptr(), i.dt.data_ptr(), (const float *)i.a.data_ptr(), i.b.data_ptr(), i.c.data_ptr(),
+                                     (const float *)data(i.skip), data(i.gate), (const float *)data(i.dt_bias), (const float *)data(i.state),
+                                     data(i.lengths), r.y.data_ptr(), (float *)r.last.data_ptr(), r.ckpt.defined() && r.ckpt.numel() > 0 ? r.ckpt.data_ptr() : nullptr,
+                                     B, T, D, N, strides, dtype_code(i.x, "x"), flags, data(ws), bytes, stream));
+    return r;
+}
+
+struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &dt, const Tensor &a, const Tensor &b, const Tensor &c,
+                                 const Maybe &state, const Maybe &skip, const Maybe &gate, const Maybe &dt_bias, const Maybe &lengths, int64_t flags,
+                                 int64_t stream) {
+        const SelectInputs i{x, dt, a, b, c, of(state), of(skip), of(gate), of(dt_bias), of(lengths)};
+        const SelectResult r = select_forward(i, (int32_t)flags, true, reinterpret_cast<void *>((uintptr_t)stream));
+        ctx->save_for_backward({x, dt, a, b, c, i.skip, i.gate, i.dt_bias, i.lengths, r.ckpt});
+        ctx->saved_data["flags"] = flags;
+        ctx->saved_data["stream"] = stream;
+        ctx->saved_data["state"] = i.state.defined();
+        ctx->saved_data["type"] = (int64_t)x.scalar_type();
+        ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), x.size(1), x.size(2), a.size(1)};
+        ctx->set_materialize_grads(false);
+        return {r.y, r.last};
+    }
+    // a saved tensor of steps, as its sizes have to be
+    static Tensor steps(const Tensor &t, const Tensor &like, at::ScalarType type, at::IntArrayRef sizes) {
+        check_on(t, like, "a saved tensor");
+        check_type(t, type, "a saved tensor");
+        check_sizes(t, sizes, "a saved tensor");
+        return dense_channels(t);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        once("selective_scan");
+        const variable_list saved = ctx->get_saved_variables();
+        const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();
+        const int64_t B = n[0], T = n[1], D = n[2], N = n[3];
+        const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        const c10::DeviceGuard guard(saved[0].device());
+        const Tensor x = steps(saved[0], saved[0], type, {B, T, D}), dt = steps(saved[1], x, type, {B, T, D});
+        const Tensor a = restored(saved[2], x, at::kFloat, D * N), b = steps(saved[3], x, type, {B, T, N}), c = steps(saved[4], x, type, {B, T, N});
+        const Tensor skip = saved[5].defined() ? restored(saved[5], x, at::kFloat, D) : Tensor();
+        const Tensor gate = saved[6].defined() ? steps(saved[6], x, type, {B, T, D}) : Tensor();
+        const Tensor bias = saved[7].defined() ? restored(saved[7], x, at::kFloat, D) : Tensor();
+        const int32_t flags = (int32_t)ctx->saved_data["flags"].toInt(), dtype = lowp_code(x, "x");
+        const Tensor lengths = saved[8].defined() ? restored(saved[8], x, flags & T2FW_SELECT_LENGTHS64 ? at::kLong : at::kInt, B) : Tensor();
+        const Tensor ckpt = restored(saved[9], x, at::kByte, (int64_t)t2fw_selective_scan_checkpoint_bytes(B, T, D, N));
+        // a result that nothing depends on has no gradient
+        const Tensor gy = grads[0].defined() ? dense_channels(grads[0]) : at::zeros({1}, x.options()).expand({B, T, D}).contiguous();
+        const Tensor gs = grads[1].defined() ? grads[1].contiguous().resolve_neg() : Tensor();
+        check_type(gy, type, "the gradient");
+        check_sizes(gy, {B, T, D}, "the gradient");
+        if (gs.defined()) {
+            check_type(gs, at::kFloat, "the state's gradient");
+            check_sizes(gs, {B, D, N}, "the state's gradient");
+        }
+        const auto wide = x.options().dtype(at::kFloat);
+        const Tensor dx = at::empty({B, T, D}, x.options()), ddt = at::empty({B, T, D}, x.options()), da = at::empty({D, N}, wide);
+        const Tensor db = at::empty({B, T, N}, x.options()), dc = at::empty({B, T, N}, x.options());
+        const Tensor dskip = skip.defined() ? at::empty({D}, wide) : Tensor(), dgate = gate.defined() ? at::empty({B, T, D}, x.options()) : Tensor();
+        const Tensor dbias = bias.defined() ? at::empty({D}, wide) : Tensor(), ds = ctx->saved_data["state"].toBool() ? at::empty({B, D, N}, wide) : Tensor();
+        const size_t bytes = t2fw_selective_scan_backward_workspace_bytes(B, T, D, N);
+        Tensor ws;
+        if (bytes > 0) ws = bytes_like(x, (int64_t)bytes);
+        const bool gated = gate.defined();
+        const int64_t strides[12] = {x.stride(0), x.stride(1), dt.stride(0), dt.stride(1), b.stride(0), b.stride(1), c.stride(0), c.stride(1),
+                                     gated ? gate.stride(0) : 0, gated ? gate.stride(1) : 0, gy.stride(0), gy.stride(1)};
+        done(t2fw_selective_scan_backward(gy.data_ptr(), (const float *)data(gs), x.data_ptr(), dt.data_ptr(), (const float *)a.data_ptr(), b.data_ptr(),
+                                          c.data_ptr(), (const float *)data(skip), data(gate), (const float *)data(bias), data(lengths),
+                                          ckpt.numel() > 0 ? ckpt.data_ptr() : nullptr, dx.data_ptr(), ddt.data_ptr(), (float *)da.data_ptr(),
+                                          db.data_ptr(), dc.data_ptr(), (float *)data(dskip), data(dgate), (float *)data(dbias), (float *)data(ds), B, T, D,
+                                          N, strides, dtype, flags, data(ws), bytes, as_address(ctx->saved_data["stream"])));
+        return {dx, ddt, da, db, dc, ds, dskip, dgate, dbias, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// Tensors of one call, of whole sequences (`axes` 3) or of a token (2)
+void check_select(const SelectInputs &i, int64_t axes) {
+    const char *const shape = axes == 3 ? "[B, T, D]" : "[B, D]";
+    check_on(i.x, i.x, "x");
+    TORCH_CHECK(i.x.dim() == axes && i.x.size(-1) >= 1, "t2fw: expected x ", shape, " with at least one channel, it is ", i.x.sizes());
+    lowp_code(i.x, "x");
+    check_rows(i.x, i.x, "x");
+    const auto like_x = [&](const Tensor &t, const char *name) {
+        check_rows(t, i.x, name);
+        check_sizes(t, i.x.sizes(), name);
+        check_type(t, i.x.scalar_type(), name);
+    };
+    like_x(i.dt, "dt");
+    if (i.gate.defined()) like_x(i.gate, "gate");
+    const int64_t B = i.x.size(0), D = i.x.size(-1);
+    check_contiguous(i.a, i.x, "a");
+    check_type(i.a, at::kFloat, "a");
+    TORCH_CHECK(i.a.dim() == 2 && i.a.size(0) == D && i.a.size(1) >= 1 && i.a.size(1) <= 64, "t2fw: expected a [D, N] of ", D, " channels and 1 to 64 states, it is ", i.a.sizes());
+    const int64_t N = i.a.size(1);
+    std::vector<int64_t> per_step(i.x.sizes().begin(), i.x.sizes().end());
+    per_step.back() = N;
+    const Tensor *const rows[2] = {&i.b, &i.c};
+    const char *const names[2] = {"b", "c"};
+    for (int k = 0; k < 2; ++k) {
+        check_on(*rows[k], i.x, names[k]);
+        check_sizes(*rows[k], per_step, names[k]);
+        check_rows(*rows[k], i.x, names[k]);
+        check_type(*rows[k], i.x.scalar_type(), names[k]);
+    }
+    const auto per_channel = [&](const Tensor &t, at::IntArrayRef sizes, const char *name) {
+        if (!t.defined()) return;
+        check_contiguous(t, i.x, name);
+        check_sizes(t, sizes, name);
+        check_type(t, at::kFloat, name);
+    };
+    per_channel(i.state, {B, D, N}, "state");
+    per_channel(i.skip, {D}, "skip");
+    per_channel(i.dt_bias, {D}, "dt_bias");
+}
+
+// selective_scan(x, dt, a, b, c, state, skip, gate, dt_bias, lengths (five: or None), softplus, stream) -> (y, last state)
+PyObject *selective_scan(PyObject *, PyObject *const *p, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 12);
+    const SelectInputs i{tensor(p[0]), tensor(p[1]), tensor(p[2]), tensor(p[3]), tensor(p[4]), optional_tensor(p[5]), optional_tensor(p[6]),
+                         optional_tensor(p[7]), optional_tensor(p[8]), optional_tensor(p[9])};
+    check_select(i, 3);
+    check_lengths(i.lengths, i.x);
+    no_tangents({i.x, i.dt, i.a, i.b, i.c, i.state, i.skip, i.gate, i.dt_bias}, "selective_scan");
+    const int64_t flags = (truth(p[10]) ? T2FW_SELECT_SOFTPLUS : 0) |
+                          (i.lengths.defined() && i.lengths.scalar_type() == at::kLong ? T2FW_SELECT_LENGTHS64 : 0);
+    void *const stream = address(p[11]);
+    const c10::DeviceGuard guard(i.x.device());
+    pybind11::gil_scoped_release release;
+    if (!wants_grad({i.x, i.dt, i.a, i.b, i.c, i.state, i.skip, i.gate, i.dt_bias})) {
+        const SelectResult r = select_forward(i, (int32_t)flags, false, stream);
+        pybind11::gil_scoped_acquire acquire;
+        return wrapped({r.y, r.last});
+    }
+    const variable_list r = SelectiveScan::apply(i.x, i.dt, i.a, i.b, i.c, maybe(i.state), maybe(i.skip), maybe(i.gate), maybe(i.dt_bias), maybe(i.lengths),
+                                                 flags, as_integer(stream));
+    pybind11::gil_scoped_acquire acquire;
+    return wrapped({r[0], r[1]});
+    END_HANDLE_TH_ERRORS
+}
+
+// selective_scan_step(x, dt, a, b, c, state, skip, gate, dt_bias (three: or None), softplus, out or None, inplace, stream) -> (y, state)
+PyObject *selective_scan_step(PyObject *, PyObject *const *p, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 13);
+    const SelectInputs i{tensor(p[0]), tensor(p[1]), tensor(p[2]), tensor(p[3]), tensor(p[4]), tensor(p[5]), optional_tensor(p[6]), optional_tensor(p[7]),
+                         optional_tensor(p[8]), Tensor()};
+    Tensor out = optional_tensor(p[10]);
+    check_select(i, 2);
+    no_tangents({i.x, i.dt, i.a, i.b, i.c, i.state, i.skip, i.gate, i.dt_bias, out}, "selective_scan_step");
+    TORCH_CHECK(!wants_grad({i.x, i.dt, i.a, i.b, i.c, i.state, i.skip, i.gate, i.dt_bias, out}),
+                "t2fw: selective_scan_step has no gradients: call selective_scan, or this under torch.no_grad()");
+    const bool inplace = truth(p[11]);
+    if (inplace) check_apart(i.state, {i.x, i.dt, i.a, i.b, i.c, i.skip, i.gate, i.dt_bias, out}, "state");
+    if (out.defined()) {
+        check_contiguous(out, i.x, "out");
+        check_sizes(out, i.x.sizes(), "out");
+        check_type(out, i.x.scalar_type(), "out");
+        check_apart(out, {i.x, i.dt, i.a, i.b, i.c, i.state, i.skip, i.gate, i.dt_bias}, "out");
+    }
+    const c10::DeviceGuard guard(i.x.device());
+    if (!out.defined()) out = at::empty(i.x.sizes(), i.x.options());
+    const Tensor next = inplace ? i.state : at::empty(i.state.sizes(), i.state.options());
+    const int32_t flags = truth(p[9]) ? T2FW_SELECT_SOFTPLUS : 0;
+    void *const stream = address(p[12]);
+    const int64_t strides[5] = {i.x.stride(0), i.dt.stride(0), i.b.stride(0), i.c.stride(0), i.gate.defined() ? i.gate.stride(0) : 0};
+    done(unlocked([&] {
+        return t2fw_selective_scan_step(i.x.data_ptr(), i.dt.data_ptr(), (const float *)i.a.data_ptr(), i.b.data_ptr(), i.c.data_ptr(),
+                                        (const float *)data(i.skip), data(i.gate), (const float *)data(i.dt_bias), (const float *)i.state.data_ptr(),
+                                        out.data_ptr(), (float *)next.data_ptr(), i.x.size(0), i.x.size(1), i.a.size(1), strides, dtype_code(i.x, "x"),
+                                        flags, stream);
+    }));
+    // written behind torch's back
+    if (inplace) bump(i.state);
+    if (p[10] != Py_None) bump(out);
+    return wrapped({out, next});
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- beam search --------------------------------------------------------------------------------------------------
 // beam_select(logits, scores, count or None, finished or None, pad, stream) -> (scores, beams, tokens)
 PyObject *beam_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -299,6 +496,6 @@ PyObject *reorder_beams(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }  // namespace
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef layer_methods[] = {METHOD(short_conv), METHOD(short_conv_step), METHOD(beam_select), METHOD(reorder_beams), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef layer_methods[] = {METHOD(short_conv), METHOD(short_conv_step), METHOD(selective_scan), METHOD(selective_scan_step), METHOD(beam_select), METHOD(reorder_beams), {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace t2fw_host

@@ -1,6 +1,7 @@
 // C ABI of the selective state space layer and of beam search (include/t2fw_hip.h): argument validation, and what a call needs laid out.
 #include "checks.hpp"
 #include "beam.hpp"
+#include "select.hpp"
 #include "short_conv.hpp"
 
 #include <exception>
@@ -43,6 +44,30 @@ int conv_args(ConvArgs &a, int64_t B, int64_t T, int64_t D, int64_t taps, const 
 }
 size_t conv_weight_size(int32_t dtype, int32_t flags) { return flags & T2FW_CONV_WEIGHT_F32 ? 4 : size_of(dtype); }
 size_t lengths_size(bool wide) { return wide ? 8 : 4; }
+
+int check_select(int64_t B, int64_t T, int64_t D, int64_t N, int32_t dtype, int32_t flags) {
+    int rc = check_lowp(dtype, "selective scan");
+    if (rc || (rc = check_sizes({B, T, D, 2 * SELECT_STATES}, "selective scan"))) return rc;
+    if (D < 1) return fail(T2FW_ERR_BAD_SHAPE, "selective scan: at least one channel");
+    if (N < 1 || N > SELECT_STATES) return fail(T2FW_ERR_BAD_SHAPE, "selective scan: 1 to %d states of a channel, not %lld", SELECT_STATES, (long long)N);
+    if (flags & ~(T2FW_SELECT_SOFTPLUS | T2FW_SELECT_LENGTHS64)) return fail(T2FW_ERR_UNSUPPORTED, "selective scan: unknown flags %d", flags);
+    return T2FW_OK;
+}
+// rows and steps of x, dt, b, c, gate and, backward, g_y
+int select_args(SelectArgs &s, int64_t B, int64_t T, int64_t D, int64_t N, const int64_t *strides, bool backward, int32_t flags) {
+    s.B = B; s.T = T; s.D = D; s.N = N;
+    s.softplus = (flags & T2FW_SELECT_SOFTPLUS) != 0;
+    s.wide_lengths = (flags & T2FW_SELECT_LENGTHS64) != 0;
+    int64_t *const to[12] = {&s.x_b, &s.x_t, &s.dt_b, &s.dt_t, &s.b_b, &s.b_t, &s.c_b, &s.c_t, &s.z_b, &s.z_t, &s.g_b, &s.g_t};
+    for (int i = 0; i < 12; ++i) {
+        const int64_t width = i >= 4 && i < 8 ? N : D;
+        *to[i] = i % 2 == 0 ? T * width : width;
+        if (strides == nullptr || (i >= 10 && !backward) || (i / 2 == 4 && s.gate == nullptr)) continue;
+        if (strides[i] < 0) return fail(T2FW_ERR_BAD_SHAPE, "selective scan: strides must be non-negative");
+        *to[i] = strides[i];
+    }
+    return T2FW_OK;
+}
 
 struct BeamLayout {
     int64_t pieces, shares;                  // bytes of the first array of the scratch
@@ -127,6 +152,82 @@ int t2fw_short_conv_step(const void *x, const void *w, const void *bias, const v
     a.x = x; a.w = w; a.bias = bias; a.state = s0; a.y = y; a.last = next_state;
     a.x_b = x_stride;
     return conv_step(a, dtype, static_cast<hipStream_t>(stream));
+}
+
+size_t t2fw_selective_scan_checkpoint_bytes(int64_t B, int64_t T, int64_t D, int64_t N) {
+    return check_select(B, T, D, N, T2FW_F32, 0) ? 0 : select_plan(B, T, D, N).checkpoints;
+}
+size_t t2fw_selective_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t N) {
+    return check_select(B, T, D, N, T2FW_F32, 0) ? 0 : select_plan(B, T, D, N).forward;
+}
+size_t t2fw_selective_scan_backward_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t N) {
+    return check_select(B, T, D, N, T2FW_F32, 0) ? 0 : select_plan(B, T, D, N).backward;
+}
+
+int t2fw_selective_scan_forward(const void *x, const void *dt, const float *a, const void *b, const void *c, const float *skip, const void *gate,
+                                const float *dt_bias, const float *s0, const void *lengths, void *y, float *last, void *ckpt, int64_t B, int64_t T,
+                                int64_t D, int64_t N, const int64_t *strides, int32_t dtype, int32_t flags, void *workspace, size_t workspace_bytes,
+                                void *stream) {
+    int rc = check_select(B, T, D, N, dtype, flags);
+    if (rc) return rc;
+    if (B == 0) return T2FW_OK;
+    const size_t es = size_of(dtype), need = t2fw_selective_scan_workspace_bytes(B, T, D, N);
+    const bool none = T == 0;
+    if ((rc = check_arrays({{"x", x, es, none}, {"dt", dt, es, none}, {"a", a, 4, false}, {"b", b, es, none}, {"c", c, es, none}, {"skip", skip, 4, true},
+                            {"gate", gate, es, true}, {"dt_bias", dt_bias, 4, true}, {"s0", s0, 4, true},
+                            {"lengths", lengths, lengths_size(flags & T2FW_SELECT_LENGTHS64), true}, {"y", y, es, none}, {"last", last, 4, false},
+                            {"ckpt", ckpt, 16, true}, {"workspace", workspace, 16, need == 0}})))
+        return rc;
+    if (workspace_bytes < need) return bad_workspace(need, workspace_bytes);
+    SelectArgs s{};
+    s.x = x; s.dt = dt; s.a = a; s.b = b; s.c = c; s.skip = skip; s.gate = gate; s.dt_bias = dt_bias; s.s0 = s0; s.lengths = lengths;
+    s.y = y; s.last = last; s.ckpt = static_cast<float *>(ckpt); s.maps = static_cast<float *>(workspace);
+    if ((rc = select_args(s, B, T, D, N, strides, false, flags))) return rc;
+    return select_forward(s, dtype, static_cast<hipStream_t>(stream));
+}
+
+int t2fw_selective_scan_backward(const void *g_y, const float *g_last, const void *x, const void *dt, const float *a, const void *b, const void *c,
+                                 const float *skip, const void *gate, const float *dt_bias, const void *lengths, const void *ckpt, void *d_x, void *d_dt,
+                                 float *d_a, void *d_b, void *d_c, float *d_skip, void *d_gate, float *d_bias, float *d_s0, int64_t B, int64_t T,
+                                 int64_t D, int64_t N, const int64_t *strides, int32_t dtype, int32_t flags, void *workspace, size_t workspace_bytes,
+                                 void *stream) {
+    int rc = check_select(B, T, D, N, dtype, flags);
+    if (rc) return rc;
+    const size_t es = size_of(dtype), need = t2fw_selective_scan_backward_workspace_bytes(B, T, D, N);
+    const bool none = B == 0 || T == 0;
+    if ((rc = check_arrays({{"g_y", g_y, es, none}, {"g_last", g_last, 4, true}, {"x", x, es, none}, {"dt", dt, es, none}, {"a", a, 4, false},
+                            {"b", b, es, none}, {"c", c, es, none}, {"skip", skip, 4, true}, {"gate", gate, es, true}, {"dt_bias", dt_bias, 4, true},
+                            {"lengths", lengths, lengths_size(flags & T2FW_SELECT_LENGTHS64), true}, {"ckpt", ckpt, 16, none}, {"d_x", d_x, es, none},
+                            {"d_dt", d_dt, es, none}, {"d_a", d_a, 4, false}, {"d_b", d_b, es, none}, {"d_c", d_c, es, none}, {"d_skip", d_skip, 4, true},
+                            {"d_gate", d_gate, es, gate == nullptr || none}, {"d_bias", d_bias, 4, true}, {"d_s0", d_s0, 4, true},
+                            {"workspace", workspace, 16, need == 0}})))
+        return rc;
+    if (workspace_bytes < need) return bad_workspace(need, workspace_bytes);
+    SelectArgs s{};
+    s.g_y = g_y; s.g_state = g_last; s.x = x; s.dt = dt; s.a = a; s.b = b; s.c = c; s.skip = skip; s.gate = gate; s.dt_bias = dt_bias; s.lengths = lengths;
+    s.ckpt = static_cast<float *>(const_cast<void *>(ckpt)); s.maps = static_cast<float *>(workspace);
+    s.d_x = d_x; s.d_dt = d_dt; s.d_a = d_a; s.d_b = d_b; s.d_c = d_c; s.d_skip = d_skip; s.d_gate = d_gate; s.d_bias = d_bias; s.d_s0 = d_s0;
+    if ((rc = select_args(s, B, T, D, N, strides, true, flags))) return rc;
+    return select_backward(s, dtype, static_cast<hipStream_t>(stream));
+}
+
+int t2fw_selective_scan_step(const void *x, const void *dt, const float *a, const void *b, const void *c, const float *skip, const void *gate,
+                             const float *dt_bias, const float *s0, void *y, float *next_state, int64_t B, int64_t D, int64_t N, const int64_t *strides,
+                             int32_t dtype, int32_t flags, void *stream) {
+    int rc = check_select(B, 1, D, N, dtype, flags & ~T2FW_SELECT_LENGTHS64);
+    if (rc) return rc;
+    if (B == 0) return T2FW_OK;
+    const size_t es = size_of(dtype);
+    if ((rc = check_arrays({{"x", x, es, false}, {"dt", dt, es, false}, {"a", a, 4, false}, {"b", b, es, false}, {"c", c, es, false},
+                            {"skip", skip, 4, true}, {"gate", gate, es, true}, {"dt_bias", dt_bias, 4, true}, {"s0", s0, 4, false}, {"y", y, es, false},
+                            {"next_state", next_state, 4, false}})))
+        return rc;
+    SelectArgs s{};
+    s.x = x; s.dt = dt; s.a = a; s.b = b; s.c = c; s.skip = skip; s.gate = gate; s.dt_bias = dt_bias; s.s0 = s0; s.y = y; s.last = next_state;
+    int64_t both[10];
+    for (int i = 0; strides != nullptr && i < 10; ++i) both[i] = strides[i / 2];         // (there is one step)
+    if ((rc = select_args(s, B, 1, D, N, strides == nullptr ? nullptr : both, false, flags))) return rc;
+    return select_step(s, dtype, static_cast<hipStream_t>(stream));
 }
 
 size_t t2fw_beam_select_workspace_bytes(int64_t B, int64_t K, int64_t V, int64_t n, int32_t dtype) {

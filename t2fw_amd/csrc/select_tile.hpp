@@ -1,0 +1,337 @@
+// What the selective scan's kernels share (select_fwd.hip, select_bwd.hip).
+//
+// h_t = exp(dt_t a) h_{t-1} + dt_t x_t b_t for every channel and state, y_t = <c_t, h_t> + skip x_t, out = y silu(gate).
+//
+// Layout: a lane owns four states of a channel, G = ceil(N / 4) lanes (a power of two) a channel, a workgroup of 256 threads 256 / G channels of one
+// row and a chunk of its steps, which it goes through one by one with the states in registers.  What a step needs per channel (the step's length by the
+// softplus, its product with the input, the gate) is made once, by one of the up to four lanes of a quad for each of as many steps, and
+// handed to the others by the cross-lane moves that an instruction's operand can have.  b and c, the same for all channels, go through
+// shared memory, 16 steps at a time.  Sums over a channel's lanes are made for as many steps as the quad has lanes at once.
+//
+// A stretch of steps is an affine map of the state before it, h -> exp(a sum dt) h + S: its decay needs no more than the sum of its steps' lengths.  So a
+// sequence is cut in chunks where there are too few channels for the chip: one launch for the chunks' maps, and another in which a
+// chunk puts those before it together and goes through its steps.  It costs a chunk's decays twice.
+//
+// Bound by the vector units: a state and step is a product, an exponential (which takes two instructions' time), a product and two
+// multiply-adds forward.
+#pragma once
+#include "activation.hpp"
+#include "select.hpp"
+#include "vec.hpp"
+
+namespace t2fw {
+namespace select_ns {
+
+constexpr int THREADS = 256, S = 4, TILE = SELECT_TILE;
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int64_t MOST_GROUPS = (1ll << 32) / THREADS - 1;      // a grid has less than 2^32 threads along an axis
+
+// How a call is cut: channels of a workgroup are side by side, then rows, then chunks of `steps`
+struct Grid {
+    uint32_t blocks, chunks, tiles;      // tiles: of a whole row
+    int64_t steps;
+    bool fits;
+};
+
+// ---- a channel's lanes ---------------------------------------------------------------------------------------------
+// steps that the lanes of a channel share out
+template <int G> constexpr int share() { return G < 4 ? G : 4; }
+
+// The value of the lane that has step j of a round
+template <int G, int J> __device__ __forceinline__ float of_step(float v) {
+    if constexpr (G == 1) return v;
+    else if constexpr (G == 2) return dpp_move<J == 0 ? 0xA0 : 0xF5>(v);         // quad_perm [0,0,2,2], [1,1,3,3]
+    else return dpp_move<J * 0x55>(v);                                           // quad_perm [J,J,J,J]
+}
+constexpr int DPP_ROW_SHL4 = 0x104, DPP_ROW_SHL8 = 0x108;
+
+// Sums over the lanes of a channel, of one value per step of a round: the first lanes get that of their step each
+template <int G> __device__ __forceinline__ float sum_steps(const float (&v)[share<G>()]) {
+    if constexpr (G == 1) return v[0];
+    const bool odd = threadIdx.x & 1;
+    if constexpr (G == 2) {
+        return (odd ? v[1] : v[0]) + dpp_move<DPP_QUAD_XOR1>(odd ? v[0] : v[1]);
+    } else if constexpr (G >= 4) {
+        const bool upper = threadIdx.x & 2;
+        const float p = (odd ? v[1] : v[0]) + dpp_move<DPP_QUAD_XOR1>(odd ? v[0] : v[1]);
+        const float q = (odd ? v[3] : v[2]) + dpp_move<DPP_QUAD_XOR1>(odd ? v[2] : v[3]);
+        float r = (upper ? q : p) + dpp_move<DPP_QUAD_XOR2>(upper ? p : q);
+        if constexpr (G >= 16) r += dpp_move<DPP_ROW_SHL8>(r);
+        if constexpr (G >= 8) r += dpp_move<DPP_ROW_SHL4>(r);
+        return r;
+    }
+}
+// A sum over the steps of a round and all of them: over the lanes that have a step each
+template <int G> __device__ __forceinline__ float sum_share(float v) { return group_sum(v, share<G>()); }
+
+// ---- scalars of a step ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v|, and log(1 + e) = 2 artanh(r), r = e / (2 + e) <= 1/3: r + r^3 / 3 + ..., its seven terms off by 2^-26
+// of it.  Relative accuracy for steps of any length, which a logarithm of a sum does not have.
+struct Softplus {
+    float value, slope;
+};
+template <bool SLOPE> __device__ __forceinline__ Softplus softplus_of(float v) {
+    const float e = exp2_of(-fabsf(v) * LOG2E), r = e * __builtin_amdgcn_rcpf(2.0f + e), q = r * r;
+    float p = 1.0f / 13.0f;
+    p = fmaf(p, q, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    p = fmaf(p * q, r, r);
+    Softplus s;
+    s.value = fmaf(2.0f, p, fmaxf(v, 0.0f));
+    s.slope = SLOPE ? (v >= 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(1.0f + e) : 0.0f;
+    return s;
+}
+
+__device__ __forceinline__ int64_t row_length(const SelectArgs &a, int64_t b) {
+    if (a.lengths == nullptr) return a.T;
+    const int64_t n = a.wide_lengths ? static_cast<const int64_t *>(a.lengths)[b] : static_cast<const int32_t *>(a.lengths)[b];
+    return n < 0 ? 0 : n < a.T ? n : a.T;
+}
+
+// Where a thread is
+struct Place {
+    int64_t b, d, begin, end, live;      // row, channel, first step of the chunk and the one after its last; ... after the last that counts
+    int ng, n0;                          // lane of the channel, its first state
+    uint32_t block, chunk;
+    bool mine;                           // the channel exists (else it is the last one, and nothing of it is stored)
+};
+template <int G> __device__ __forceinline__ Place place_of(const SelectArgs &a, const Grid &g) {
+    Place p;
+    p.block = blockIdx.x % g.blocks;
+    const uint32_t rest = blockIdx.x / g.blocks;
+    p.b = rest % (uint32_t)a.B;
+    p.chunk = rest / (uint32_t)a.B;
+    p.ng = threadIdx.x % G;
+    p.n0 = p.ng * S;
+    p.d = (int64_t)p.block * (THREADS / G) + threadIdx.x / G;
+    p.mine = p.d < a.D;
+    if (!p.mine) p.d = a.D - 1;
+    p.begin = p.chunk * g.steps;
+    p.end = p.begin + g.steps < a.T ? p.begin + g.steps : a.T;
+    const int64_t n = row_length(a, p.b);
+    p.live = n < p.begin ? p.begin : n < p.end ? n : p.end;
+    return p;
+}
+
+// A lane's states of [.., N] arrays; of those beyond N nothing
+__device__ __forceinline__ void load_states(float (&v)[S], const float *at, int n0, int64_t N) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) v[s] = n0 + s < N ? at[n0 + s] : 0.0f;
+}
+__device__ __forceinline__ void store_states(float *at, const float (&v)[S], int n0, int64_t N) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (n0 + s < N) at[n0 + s] = v[s];
+}
+__device__ __forceinline__ void load_padded(float (&v)[S], const float *at) {
+    const Vec<float, S> x = load_vec<float, S>(at);
+#pragma unroll
+    for (int s = 0; s < S; ++s) v[s] = x.e[s];
+}
+__device__ __forceinline__ void store_padded(float *at, const float (&v)[S]) { store_vec(at, Vec<float, S>{{v[0], v[1], v[2], v[3]}}); }
+
+// The decays' exponents per unit of step, for the hardware's exponential, which is that of two
+__device__ __forceinline__ void load_rates(float (&v)[S], const SelectArgs &a, const Place &p) {
+    load_states(v, a.a + p.d * a.N, p.n0, a.N);
+#pragma unroll
+    for (int s = 0; s < S; ++s) v[s] *= LOG2E;
+}
+
+// What a tile needs of the arrays, on its way: a lane's steps of those per channel ...
+template <typename IO, int G> struct PerChannel {
+    static constexpr int ROUNDS = TILE / share<G>();
+    IO v[ROUNDS];
+    __device__ __forceinline__ void load(const void *base, int64_t row, int64_t step, const SelectArgs &a, const Place &p, int64_t t0) {
+        const IO *const at = static_cast<const IO *>(base) + p.b * row + p.d;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const int64_t t = t0 + r * share<G>() + p.ng % share<G>();
+            v[r] = at[(t < a.T ? t : a.T - 1) * step];
+        }
+    }
+};
+// ... and elements of b or c, which go to shared memory
+template <typename IO, int G> struct PerStep {
+    static constexpr int NP = G * S, EACH = (TILE * NP + THREADS - 1) / THREADS;
+    IO v[EACH];
+    __device__ __forceinline__ void load(const void *base, int64_t row, int64_t step, const SelectArgs &a, const Place &p, int64_t t0) {
+        const IO *const at = static_cast<const IO *>(base) + p.b * row;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int j = i * THREADS + threadIdx.x, n = j % NP;
+            const int64_t t = t0 + j / NP;
+            v[i] = at[(t < a.T ? t : a.T - 1) * step + (n < a.N ? n : 0)];
+        }
+    }
+    // zeros for states that are none, and for steps that do not count, whatever they hold
+    __device__ __forceinline__ void store(float *to, const SelectArgs &a, const Place &p, int64_t t0) const {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int j = i * THREADS + threadIdx.x;
+            if (j < TILE * NP) to[j] = j % NP < a.N && t0 + j / NP < p.live ? widen(v[i]) : 0.0f;
+        }
+    }
+};
+
+// The state (BACK: the adjoint) at a chunk's start (end): the maps of the chunks before (after) it, from `first`
+template <int G, bool BACK> __device__ __forceinline__ void through_maps(float (&h)[S], const SelectArgs &a, const Grid &g, const Place &p, const float (&rate)[S]) {
+    constexpr int NP = G * S, AHEAD = 4;
+    const int n = BACK ? (int)(g.chunks - 1 - p.chunk) : (int)p.chunk;
+    const float *const maps = a.maps, *const lengths = a.maps + (int64_t)g.chunks * a.B * a.D * NP;
+    for (int i = 0; i < n; i += AHEAD) {
+        float v[AHEAD][S], sum[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int j = i + u < n ? i + u : n - 1, chunk = BACK ? (int)g.chunks - 1 - j : j;
+            const int64_t at = ((int64_t)chunk * a.B + p.b) * a.D + p.d;
+            load_padded(v[u], maps + at * NP + p.n0);
+            sum[u] = lengths[at];
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (i + u < n) {
+#pragma unroll
+                for (int s = 0; s < S; ++s) h[s] = fmaf(exp2_of(rate[s] * sum[u]), h[s], v[u][s]);
+            }
+    }
+}
+
+// A step's length, and its product with the input
+template <bool SLOPE> struct StepLength {
+    float dt, slope;
+};
+template <bool SLOPE> __device__ __forceinline__ StepLength<SLOPE> length_of(const SelectArgs &a, float raw) {
+    if (!a.softplus) return {raw, 1.0f};
+    const Softplus s = softplus_of<SLOPE>(raw);
+    return {s.value, s.slope};
+}
+
+// The map of a chunk (BACK: of its adjoint): what it makes of a state of zero, and the sum of its steps' lengths
+template <typename IO, int G, bool BACK> __global__ __launch_bounds__(THREADS) void select_maps_kernel(SelectArgs a, Grid g) {
+    constexpr int NP = G * S, Q = share<G>(), ROUNDS = TILE / Q;
+    constexpr bool FAST = sizeof(IO) == 2;
+    __shared__ float rows[2][TILE][NP];
+    // forward every chunk but the last, backward every one but the first
+    Place p = place_of<G>(a, g);
+    if (BACK) {
+        p.chunk += 1;
+        p.begin += g.steps;
+        p.end = p.begin + g.steps < a.T ? p.begin + g.steps : a.T;
+        const int64_t n = row_length(a, p.b);
+        p.live = n < p.begin ? p.begin : n < p.end ? n : p.end;
+    }
+    float rate[S], h[S] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f;
+    load_rates(rate, a, p);
+    const float bias = a.dt_bias == nullptr ? 0.0f : a.dt_bias[p.d];
+    const int tiles = (int)((p.live - p.begin + TILE - 1) / TILE);
+    PerChannel<IO, G> in, dt, gate;
+    PerStep<IO, G> row;
+    const auto load = [&](int k) {
+        const int64_t t0 = p.begin + (int64_t)(BACK ? tiles - 1 - k : k) * TILE;
+        in.load(BACK ? a.g_y : a.x, BACK ? a.g_b : a.x_b, BACK ? a.g_t : a.x_t, a, p, t0);
+        dt.load(a.dt, a.dt_b, a.dt_t, a, p, t0);
+        if (BACK && a.gate != nullptr) gate.load(a.gate, a.z_b, a.z_t, a, p, t0);
+        row.load(BACK ? a.c : a.b, BACK ? a.c_b : a.b_b, BACK ? a.c_t : a.b_t, a, p, t0);
+    };
+    if (tiles > 0) load(0);
+    for (int k = 0; k < tiles; ++k) {
+        const int64_t t0 = p.begin + (int64_t)(BACK ? tiles - 1 - k : k) * TILE;
+        float (&here)[TILE][NP] = rows[k % 2];
+        row.store(&here[0][0], a, p, t0);
+        float length[ROUNDS], push[ROUNDS];
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const bool counts = t0 + r * Q + p.ng % Q < p.live;
+            const float raw = widen(dt.v[r]) + bias, one = length_of<false>(a, raw).dt;
+            length[r] = counts ? one : 0.0f;
+            float v = widen(in.v[r]);
+            if (BACK && a.gate != nullptr) v *= silu_of<FAST>(widen(gate.v[r]));
+            push[r] = counts ? (BACK ? v : one * v) : 0.0f;
+            total += length[r];
+        }
+        __syncthreads();
+        if (k + 1 < tiles) load(k + 1);
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+            const int r = BACK ? ROUNDS - 1 - i : i;
+            const auto step = [&](auto J) {
+                constexpr int j = decltype(J)::value;
+                const float l = of_step<G, j>(length[r]), u = of_step<G, j>(push[r]);
+                float row_v[S];
+                load_padded(row_v, &here[r * Q + j][p.n0]);
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    const float decay = exp2_of(l * rate[s]);
+                    h[s] = BACK ? decay * fmaf(u, row_v[s], h[s]) : fmaf(decay, h[s], u * row_v[s]);
+                }
+            };
+            if constexpr (BACK) {
+                if constexpr (Q == 4) { step(std::integral_constant<int, 3>{}); step(std::integral_constant<int, 2>{}); }
+                if constexpr (Q >= 2) step(std::integral_constant<int, 1>{});
+                step(std::integral_constant<int, 0>{});
+            } else {
+                step(std::integral_constant<int, 0>{});
+                if constexpr (Q >= 2) step(std::integral_constant<int, 1>{});
+                if constexpr (Q == 4) { step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 3>{}); }
+            }
+        }
+    }
+    total = sum_share<G>(total);
+    if (!p.mine) return;
+    const int64_t at = ((int64_t)p.chunk * a.B + p.b) * a.D + p.d;
+    store_padded(a.maps + at * NP + p.n0, h);
+    if (p.ng == 0) (a.maps + (int64_t)g.chunks * a.B * a.D * NP)[at] = total;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+inline int lanes_of(int64_t N) {
+    int g = 1;
+    while (g * S < N) g *= 2;
+    return g;
+}
+// `want` workgroups, or as many as there are chunks of no less than `least` tiles
+inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N, int64_t want, int64_t least) {
+    Grid g{};
+    const int64_t channels = THREADS / lanes_of(N), blocks = (D + channels - 1) / channels, tiles = T <= 0 ? 0 : (T + TILE - 1) / TILE;
+    const long double rows = (long double)blocks * B;
+    int64_t chunks = 1;
+    if (rows > 0 && rows < want) chunks = (int64_t)((want + rows - 1) / rows);
+    if (chunks > tiles / least) chunks = tiles / least;
+    if (chunks < 1) chunks = 1;
+    const int64_t each = tiles == 0 ? 1 : (tiles + chunks - 1) / chunks;
+    g.steps = each * TILE;
+    g.chunks = (uint32_t)(tiles == 0 ? 1 : (tiles + each - 1) / each);
+    g.blocks = (uint32_t)blocks;
+    g.fits = blocks < 0x7fffffff && B < 0x7fffffff && tiles < 0x7fffffff && rows * g.chunks < MOST_GROUPS;
+    g.tiles = (uint32_t)tiles;
+    return g;
+}
+Grid forward_grid(int64_t B, int64_t T, int64_t D, int64_t N);
+Grid backward_grid(int64_t B, int64_t T, int64_t D, int64_t N);
+inline size_t maps_bytes(const Grid &g, int64_t B, int64_t D, int64_t N) {
+    return g.chunks == 1 ? 0 : (size_t)g.chunks * B * D * (lanes_of(N) * S + 1) * sizeof(float);
+}
+inline int too_many() { return fail(T2FW_ERR_BAD_SHAPE, "selective scan: too many workgroups for one launch"); }
+
+#define SELECT_LANES(what, IO, lanes, ...)                                  \
+    switch (lanes) {                                                        \
+        case 1: return what<IO, 1>(__VA_ARGS__);                            \
+        case 2: return what<IO, 2>(__VA_ARGS__);                            \
+        case 4: return what<IO, 4>(__VA_ARGS__);                            \
+        case 8: return what<IO, 8>(__VA_ARGS__);                            \
+        default: return what<IO, 16>(__VA_ARGS__);                          \
+    }
+#define SELECT_OF(what, dtype, lanes, ...)                                  \
+    switch (dtype) {                                                        \
+        case T2FW_F32: SELECT_LANES(what, float, lanes, __VA_ARGS__)        \
+        case T2FW_F16: SELECT_LANES(what, _Float16, lanes, __VA_ARGS__)     \
+        default: SELECT_LANES(what, __bf16, lanes, __VA_ARGS__)             \
+    }
+
+}  // namespace select_ns
+}  // namespace t2fw
