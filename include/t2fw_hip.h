@@ -488,7 +488,7 @@ int t2fw_short_conv_step(const void *x, const void *w, const void *bias, const v
  * z sigmoid(z) of the gate z where there is one.  x, dt, gate (or null), y [B, T, D], b, c [B, T, N] fp32 / fp16 / bf16; a [D, N], skip, dt_bias [D]
  * (or null), s0 (null: zeros), last [B, D, N] float.  dt_bias is added to dt, and T2FW_SELECT_SOFTPLUS takes log(1 + e^dt) of that.  `lengths`: as for
  * t2fw_gated_scan_forward (T2FW_SELECT_LENGTHS64).  `strides`: elements between rows and steps of x, dt, b, c and gate (ten numbers; gate's are not looked at without one), or
- * null for dense arrays; the channels (states) of a step are next to each other.  The products of a channel's decays over the steps of a row have to
+ * null for dense arrays; the channels (states) of a step are next to each other, and 16 steps within 4 GB.  The products of a channel's decays over the steps of a row have to
  * stay finite (of dt a <= 0 they always do).  `ckpt`: t2fw_selective_scan_checkpoint_bytes for the backward call, or null.  The workspaces need no
  * initialisation and are not read across calls.
  */

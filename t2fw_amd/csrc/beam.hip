@@ -1,7 +1,7 @@
 // Beam search: the best continuations over all beams of a request and the vocabulary, and the states of its beams moved to where they go on.
 //
 // Selection.  A candidate (k, v) has the score score_k + z_kv - lse_k.  Within a beam the logit alone orders candidates, so a workgroup reads a
-// piece of 8192 logits of one beam once, for its part of the log-sum-exp and for its n best; a second launch puts the parts together, in
+// piece of 2048 to 16384 logits of one beam once, for its part of the log-sum-exp and for its n best; a second launch puts the parts together, in
 // double, and takes the n best of all lists.  No two candidates are equal: of equal scores the lower index is the better one.
 //   The n best of what 256 threads hold: n of the threads' largest are no smaller than the n-th largest of those, so nothing smaller can be among the n
 //   best.  What is not smaller (most often little more than n, at most what n threads hold) goes to a list, where each counts those above it: its place.
@@ -16,7 +16,7 @@
 namespace t2fw {
 namespace {
 
-constexpr int THREADS = 256, EACH = BEAM_PIECE / THREADS;
+constexpr int THREADS = 256;
 constexpr int64_t MOST_GROUPS = (1ll << 32) / THREADS - 1;      // a grid has less than 2^32 threads along an axis
 
 // ---- keys ---------------------------------------------------------------------------------------------------------
@@ -56,26 +56,81 @@ template <typename T, typename Op> __device__ __forceinline__ T over_group(T v, 
     return v;
 }
 
+__device__ __forceinline__ uint64_t shuffled(uint64_t v, int m) { return __shfl_xor(v, m, 64); }
+__device__ __forceinline__ Candidate shuffled(const Candidate &v, int m) { return {__shfl_xor(v.key, m, 64), __shfl_xor(v.at, m, 64)}; }
+
 struct Share {
     float top;
     uint32_t unused;
     double sum;
 };
 
-template <typename IO> __global__ __launch_bounds__(THREADS) void beam_piece_kernel(BeamArgs a) {
+// Groups of threads that the n best are looked for among: few, as each is compared with all, but some times n, or most groups are not below the n-th
+__host__ __device__ constexpr int groups_of(int n) { return n <= 16 ? 64 : n <= 48 ? 128 : THREADS; }
+// The best of a thread's group
+template <typename Key, typename Above> __device__ __forceinline__ Key of_group(Key mine, int n, Above above) {
+    if (n <= 48) {
+        const Key o = shuffled(mine, 1);
+        if (above(o, mine)) mine = o;
+    }
+    if (n <= 16) {
+        const Key o = shuffled(mine, 2);
+        if (above(o, mine)) mine = o;
+    }
+    return mine;
+}
+// The n-th largest of the groups' best, `mine`: all are distinct
+template <typename Key, typename Above> __device__ __forceinline__ Key nth_best(const Key &mine, Key (&best)[THREADS], Key &least, int n, Above above) {
+    const int groups = groups_of(n), per = THREADS / groups;
+    if (threadIdx.x % per == 0) best[threadIdx.x / per] = mine;
+    __syncthreads();
+    if ((int)threadIdx.x < groups) {                     // (of 64 groups: one wave)
+        const Key one = best[threadIdx.x];
+        int place = 0;
+#pragma unroll 16
+        for (int i = 0; i < groups; ++i) place += above(best[i], one);
+        if (place == n - 1) least = one;
+    }
+    __syncthreads();
+    return least;
+}
+
+template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam_piece_kernel(BeamArgs a) {
     constexpr int VEC = 16 / sizeof(IO), VECS = EACH / VEC;
     __shared__ float tops[THREADS / 64];
     __shared__ double sums[THREADS / 64];
     __shared__ uint64_t best[THREADS], least;
     __shared__ int found;
-    extern __shared__ uint64_t list[];                    // EACH n
+    extern __shared__ uint64_t list[];                    // what the groups of threads that are not below the n-th hold
     const int64_t row = blockIdx.x / a.pieces;
     const int piece = blockIdx.x % a.pieces;
-    const int64_t begin = (int64_t)piece * BEAM_PIECE;
-    const int here = a.V - begin < BEAM_PIECE ? (int)(a.V - begin) : BEAM_PIECE;
+    const int64_t begin = (int64_t)piece * a.piece;
+    const int here = a.V - begin < a.piece ? (int)(a.V - begin) : a.piece;
     const IO *const z = static_cast<const IO *>(a.logits) + row * a.V + begin;
-    const bool ended = a.finished != nullptr && a.finished[row] != 0, never = !(a.scores[row] > -INFINITY);
+    // all loads at once, of what is not there of the first logits; the last vector of the piece, where it is no whole one, by its elements
+    Vec<IO, VEC> raw[VECS];
+    if (here >= VEC) {
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+            const int at = (i * THREADS + threadIdx.x) * VEC;
+            raw[i] = load_vec<IO, VEC>(z + (at + VEC <= here ? at : 0));
+        }
+    }
     float v[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int at = (i / VEC * THREADS + threadIdx.x) * VEC;
+        v[i] = at + VEC <= here ? widen(raw[i / VEC].e[i % VEC]) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+        const int at = (i * THREADS + threadIdx.x) * VEC;
+        if (at < here && at + VEC > here) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[i * VEC + e] = at + e < here ? widen(z[at + e]) : -INFINITY;
+        }
+    }
+    const bool ended = a.finished != nullptr && a.finished[row] != 0, never = !(a.scores[row] > -INFINITY);
     if (ended || never) {
         // an ended beam has one candidate, the token for that; one that cannot be has none
 #pragma unroll
@@ -83,56 +138,41 @@ template <typename IO> __global__ __launch_bounds__(THREADS) void beam_piece_ker
             const int at = (i / VEC * THREADS + threadIdx.x) * VEC + i % VEC;
             v[i] = ended && begin + at == a.pad ? 0.0f : -INFINITY;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VECS; ++i) {
-            const int at = (i * THREADS + threadIdx.x) * VEC;
-            if (at + VEC <= here) {
-                const Vec<IO, VEC> x = load_vec<IO, VEC>(z + at);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[i * VEC + e] = widen(x.e[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[i * VEC + e] = at + e < here ? widen(z[at + e]) : -INFINITY;
-            }
-        }
     }
     if (threadIdx.x == 0) found = 0;
-    float top = -INFINITY;
+    // a thread's largest, the first of equal ones
+    float mine_z = -INFINITY;
+    int mine_i = 0;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) top = fmaxf(top, v[i]);
-    top = over_group(top, tops, [](float x, float y) { return fmaxf(x, y); });
+    for (int i = 0; i < EACH; ++i) {
+        const bool more = v[i] > mine_z;
+        mine_z = more ? v[i] : mine_z;
+        mine_i = more ? i : mine_i;
+    }
+    const float top = over_group(mine_z, tops, [](float x, float y) { return fmaxf(x, y); });
+    // Exponentials by the hardware, as powers of two: off by 2^-22, and by |z - top| 2^-23 for the exponent's rounding where e^(z - top) is the smaller.  Of
+    // nothing above minus infinity the sum is zero, or NaN where there is one, which the largest does not show.
     float sum = 0.0f;
     if (top > -INFINITY) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) sum += expf(v[i] - top);
+        for (int i = 0; i < EACH; ++i) sum += __builtin_amdgcn_exp2f((v[i] - top) * 1.44269504088896340736f);
     } else {
-        // nothing above minus infinity: nothing, or NaN that the largest does not show
 #pragma unroll
         for (int i = 0; i < EACH; ++i) sum += v[i] == v[i] ? 0.0f : v[i];
     }
     const double all = over_group((double)sum, sums, [](double x, double y) { return x + y; });
     if (threadIdx.x == 0) static_cast<Share *>(a.partial)[blockIdx.x] = {top, 0, all};
-    // the threads' best, and the n-th of those
-    uint64_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int at = (i / VEC * THREADS + threadIdx.x) * VEC + i % VEC;
-        const uint64_t k = at < here ? packed(v[i], (uint32_t)(begin + at)) : 0;
-        mine = k > mine ? k : mine;
-    }
-    best[threadIdx.x] = mine;
-    __syncthreads();
-    // (threads that hold nothing are told apart by their numbers)
-    int above = 0;
-#pragma unroll 16
-    for (int i = 0; i < THREADS; ++i) above += best[i] > mine || (best[i] == mine && i < (int)threadIdx.x);
-    if (above == a.n - 1) least = mine;
-    __syncthreads();
-    const uint64_t limit = least > 0 ? least : 1;
+    const int mine_at = (mine_i / VEC * THREADS + threadIdx.x) * VEC + mine_i % VEC;
+    // (threads that hold nothing are told apart by small numbers)
+    const uint64_t mine = mine_at < here ? packed(mine_z, (uint32_t)(begin + mine_at)) : THREADS - threadIdx.x;
+    const auto more = [](uint64_t x, uint64_t y) { return x > y; };
+    uint64_t limit = nth_best(of_group(mine, a.n, more), best, least, a.n, more);
+    if (limit <= THREADS) limit = THREADS + 1;
     if (mine >= limit) {
+        const float limit_z = logit_of(limit);
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
+            if (v[i] < limit_z) continue;                // (NaN is not: it counts as the lowest)
             const int at = (i / VEC * THREADS + threadIdx.x) * VEC + i % VEC;
             const uint64_t k = at < here ? packed(v[i], (uint32_t)(begin + at)) : 0;
             if (k >= limit) list[atomicAdd(&found, 1)] = k;
@@ -144,6 +184,7 @@ template <typename IO> __global__ __launch_bounds__(THREADS) void beam_piece_ker
     for (int j = threadIdx.x; j < m; j += THREADS) {
         const uint64_t k = list[j];
         int place = 0;
+#pragma unroll 8
         for (int i = 0; i < m; ++i) place += list[i] > k;
         if (place < a.n) to[place] = k;
     }
@@ -151,72 +192,91 @@ template <typename IO> __global__ __launch_bounds__(THREADS) void beam_piece_ker
 }
 
 // A request: the n best of its lists, in rounds of ROUND candidates, each with the n best so far
-constexpr int HOLD = 8, ROUND = THREADS * HOLD;
-__global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a) {
-    __shared__ double lse[BEAM_ROWS];                     // (the largest logit and the logarithm of the sum apart, as they are added)
-    __shared__ float tops[BEAM_ROWS];
+constexpr int HOLD = 4, ROUND = THREADS * HOLD;
+__global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lanes) {
+    __shared__ double sums[BEAM_ROWS];                    // logarithms of the sums; the largest logits stay apart
+    __shared__ float tops[BEAM_ROWS], scores[BEAM_ROWS];
+    __shared__ bool ended[BEAM_ROWS];
     __shared__ Candidate best[THREADS], least;
     __shared__ int found;
-    extern __shared__ uint64_t memory[];                  // (HOLD + 1) n candidates, and n of the rounds before
-    Candidate *const list = reinterpret_cast<Candidate *>(memory), *const kept = list + (HOLD + 1) * a.n;
+    extern __shared__ uint64_t memory[];                  // what the groups of threads hold, and the n of the rounds before
+    Candidate *const kept = reinterpret_cast<Candidate *>(memory), *const list = kept + a.n;
     const int64_t b = blockIdx.x;
     const uint32_t per_beam = (uint32_t)a.pieces * a.n, total = (uint32_t)a.K * per_beam;
-    for (int k = threadIdx.x; k < a.K; k += THREADS) {
-        const Share *const s = static_cast<const Share *>(a.partial) + (b * a.K + k) * a.pieces;
-        float top = -INFINITY;
-        for (int p = 0; p < a.pieces; ++p) top = fmaxf(top, s[p].top);
-        double sum = 0.0;
-        for (int p = 0; p < a.pieces; ++p) sum += s[p].top > -INFINITY ? s[p].sum * exp((double)s[p].top - (double)top) : s[p].sum;
-        tops[k] = top;
-        lse[k] = log(sum);
-    }
-    for (int j = threadIdx.x; j < a.n; j += THREADS) kept[j] = {0, 0xffffffffu};
-    __syncthreads();
-    for (uint32_t from = 0; from < total; from += ROUND) {
-        if (threadIdx.x == 0) found = 0;
-        // those of the rounds before are with the first n threads
-        uint64_t key[HOLD + 1];
-        uint32_t at[HOLD + 1];
-        Candidate mine{0, 0xffffffffu};
-        if ((int)threadIdx.x < a.n) mine = kept[threadIdx.x];
-        key[HOLD] = mine.key;
-        at[HOLD] = mine.at;
-        uint64_t p[HOLD];
+    uint64_t p[HOLD];
+    const auto load = [&](uint32_t from) {
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
             const uint32_t j = from + i * THREADS + threadIdx.x;
             p[i] = j < total ? a.lists[b * total + j] : 0;
         }
+    };
+    load(0);
+    // `lanes` threads for a beam's pieces
+    for (int k = threadIdx.x / lanes; k < a.K; k += THREADS / lanes) {
+        const Share *const s = static_cast<const Share *>(a.partial) + (b * a.K + k) * a.pieces;
+        const int in = threadIdx.x % lanes;
+        float top = -INFINITY, most = -INFINITY;
+        double sum = 0.0;
+        if (in < a.pieces) {
+            top = most = s[in].top;
+            sum = s[in].sum;
+        }
+        for (int q = in + lanes; q < a.pieces; q += lanes) {
+            const float t = s[q].top;
+            most = fmaxf(top, t);
+            sum = (top > -INFINITY ? sum * exp((double)top - (double)most) : sum) + (t > -INFINITY ? s[q].sum * exp((double)t - (double)most) : s[q].sum);
+            top = most;
+        }
+        for (int m = 1; m < lanes; m <<= 1) most = fmaxf(most, __shfl_xor(most, m, 64));
+        if (top > -INFINITY) sum *= exp((double)top - (double)most);
+        for (int m = 1; m < lanes; m <<= 1) sum += __shfl_xor(sum, m, 64);
+        if (in == 0) {
+            tops[k] = most;
+            sums[k] = log(sum);
+            scores[k] = a.scores[b * a.K + k];
+            ended[k] = a.finished != nullptr && a.finished[b * a.K + k] != 0;
+        }
+    }
+    for (int j = threadIdx.x; j < a.n; j += THREADS) kept[j] = {0, 0xffffffffu - j};
+    __syncthreads();
+    for (uint32_t from = 0; from < total; from += ROUND) {
+        if (from > 0) load(from);
+        if (threadIdx.x == 0) found = 0;
+        // those of the rounds before are with the first n threads; threads that hold nothing are told apart by their places
+        uint64_t key[HOLD + 1];
+        uint32_t at[HOLD + 1];
+        Candidate mine{0, 0xfffffeffu - threadIdx.x};
+        if ((int)threadIdx.x < a.n) mine = kept[threadIdx.x];
+        key[HOLD] = mine.key;
+        at[HOLD] = mine.at;
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
             const uint32_t j = from + i * THREADS + threadIdx.x, k = p[i] != 0 ? j / per_beam : 0;
-            const float score = a.scores[b * a.K + k], z = logit_of(p[i]);
+            const float score = scores[k], z = logit_of(p[i]);
             double s = -(double)INFINITY;
-            if (a.finished != nullptr && a.finished[b * a.K + k] != 0) s = z == 0.0f && token_of(p[i]) == (uint32_t)a.pad ? (double)score : s;
-            else if (z > -INFINITY && score > -INFINITY) s = (double)score + (((double)z - (double)tops[k]) - lse[k]);
+            if (ended[k]) s = z == 0.0f && token_of(p[i]) == (uint32_t)a.pad ? (double)score : s;
+            else if (z > -INFINITY && score > -INFINITY) s = (double)score + (((double)z - (double)tops[k]) - sums[k]);
             key[i] = p[i] != 0 ? ordered(s) : 0;
-            at[i] = p[i] != 0 ? k * (uint32_t)a.V + token_of(p[i]) : 0xffffffffu;
+            at[i] = p[i] != 0 ? k * (uint32_t)a.V + token_of(p[i]) : 0;
             const Candidate one{key[i], at[i]};
-            if (one.above(mine)) mine = one;
+            if (key[i] != 0 && one.above(mine)) mine = one;
         }
-        best[threadIdx.x] = mine;
-        __syncthreads();
-        int above = 0;
-#pragma unroll 8
-        for (int i = 0; i < THREADS; ++i) above += best[i].above(mine) || (!mine.above(best[i]) && i < (int)threadIdx.x);
-        if (above == a.n - 1) least = mine;
-        __syncthreads();
-        const Candidate limit = least;
+        const auto more = [](const Candidate &x, const Candidate &y) { return x.above(y); };
+        const Candidate limit = nth_best(of_group(mine, a.n, more), best, least, a.n, more);
+        if (!limit.above(mine)) {
 #pragma unroll
-        for (int i = 0; i <= HOLD; ++i) {
-            const Candidate one{key[i], at[i]};
-            if (one.key != 0 && !limit.above(one)) list[atomicAdd(&found, 1)] = one;
+            for (int i = 0; i <= HOLD; ++i) {
+                const Candidate one{key[i], at[i]};
+                if (one.key != 0 && !limit.above(one)) list[atomicAdd(&found, 1)] = one;
+            }
         }
         __syncthreads();
         const int m = found;
         for (int j = threadIdx.x; j < m; j += THREADS) {
             const Candidate one = list[j];
             int place = 0;
+#pragma unroll 4
             for (int i = 0; i < m; ++i) place += list[i].above(one);
             if (place < a.n) kept[place] = one;
         }
@@ -295,17 +355,39 @@ template <int K, typename Word> int launch_reorder(const ReorderTable &t, const 
 
 }  // namespace
 
+// Logits of a thread: 64 where there are workgroups enough all the same, as what a workgroup does for its n best takes as long as 30 of a thread's logits;
+// of few logits 8 (a request of 4 x 8000: PIECE_US)
+int beam_each(int64_t rows, int64_t V) {
+    const auto pieces = [&](int each) { return (V + each * THREADS - 1) / (each * THREADS); };
+    if (rows * pieces(64) >= 512) return 64;
+    return V <= 64 * THREADS && rows * pieces(32) < 256 ? 8 : 32;
+}
+BeamPieces beam_pieces(int64_t B, int64_t K, int64_t V) {
+    const int64_t most = (int64_t)beam_each(B * K, V) * THREADS, n = (V + most - 1) / most;
+    return {(int32_t)n, (int32_t)(((V + n - 1) / n + 7) / 8 * 8)};       // of nearly equal size, and no more than `most`, which is whole eights
+}
+
+template <typename IO> int launch_pieces(const BeamArgs &a, unsigned groups, size_t held, hipStream_t stream) {
+    const int each = beam_each(a.B * a.K, a.V);
+    const unsigned list = (unsigned)(each * held * sizeof(uint64_t));
+    if (each == 64) hipLaunchKernelGGL((beam_piece_kernel<IO, 64>), dim3(groups), dim3(THREADS), list, stream, a);
+    else if (each == 32) hipLaunchKernelGGL((beam_piece_kernel<IO, 32>), dim3(groups), dim3(THREADS), list, stream, a);
+    else hipLaunchKernelGGL((beam_piece_kernel<IO, 8>), dim3(groups), dim3(THREADS), list, stream, a);
+    return check_hip(hipGetLastError(), "beam_piece_kernel launch");
+}
+
 int beam_select(const BeamArgs &a, int dtype, hipStream_t stream) {
     const int64_t groups = a.B * a.K * a.pieces;
     if (groups > MOST_GROUPS || a.B > MOST_GROUPS) return fail(T2FW_ERR_BAD_SHAPE, "beam selection: too many workgroups for one launch");
-    const dim3 grid((unsigned)groups), threads(THREADS);
-    const unsigned list = (unsigned)(EACH * a.n * sizeof(uint64_t)), merge = (unsigned)((HOLD + 2) * a.n * sizeof(Candidate));
-    if (dtype == T2FW_F32) hipLaunchKernelGGL(beam_piece_kernel<float>, grid, threads, list, stream, a);
-    else if (dtype == T2FW_F16) hipLaunchKernelGGL(beam_piece_kernel<_Float16>, grid, threads, list, stream, a);
-    else hipLaunchKernelGGL(beam_piece_kernel<__bf16>, grid, threads, list, stream, a);
-    int rc = check_hip(hipGetLastError(), "beam_piece_kernel launch");
+    // threads of the n groups that are not below the n-th
+    const int held = a.n * (THREADS / groups_of(a.n));
+    const unsigned merge = (unsigned)(((HOLD + 1) * held + a.n) * sizeof(Candidate));
+    int lanes = 1;
+    while (lanes < a.pieces && lanes < 64) lanes *= 2;
+    const int rc = dtype == T2FW_F32 ? launch_pieces<float>(a, (unsigned)groups, held, stream) : dtype == T2FW_F16 ? launch_pieces<_Float16>(a, (unsigned)groups, held, stream) :
+                   launch_pieces<__bf16>(a, (unsigned)groups, held, stream);
     if (rc) return rc;
-    hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)a.B), threads, merge, stream, a);
+    hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes);
     return check_hip(hipGetLastError(), "beam_merge_kernel launch");
 }
 

@@ -7,7 +7,6 @@ namespace t2fw {
 
 constexpr int BEAM_COUNT = 128;         // candidates of a call, at most
 constexpr int BEAM_ROWS = 256;          // beams of a request, at most
-constexpr int BEAM_PIECE = 8192;        // logits of a workgroup
 
 struct BeamArgs {
     const void *logits;                 // [B, K, V] dense
@@ -18,8 +17,12 @@ struct BeamArgs {
     void *partial;                      // scratch: [B, K, pieces] largest logits and sums
     uint64_t *lists;                    // scratch: [B, K, pieces, n] best of a piece
     int64_t B, K, V;
-    int32_t n, pieces, pad;
+    int32_t n, pieces, piece, pad;      // piece: logits of a workgroup
 };
+struct BeamPieces {
+    int32_t pieces, piece;
+};
+BeamPieces beam_pieces(int64_t B, int64_t K, int64_t V);
 int beam_select(const BeamArgs &a, int dtype, hipStream_t stream);
 
 constexpr int REORDER_TABLE = 96;       // arrays of a launch

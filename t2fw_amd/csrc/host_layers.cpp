@@ -198,7 +198,13 @@ struct SelectInputs {
 struct SelectResult {
     Tensor y, last, ckpt;
 };
-SelectResult select_forward(const SelectInputs &i, int32_t flags, bool need_grad, void *stream) {
+// Steps further apart than the kernels address are brought together
+Tensor near_steps(const Tensor &t) {
+    return t.defined() && t.size(1) > 1 && t.stride(1) > (int64_t)(0xffffffffu / (16 * t.element_size())) ? t.contiguous() : t;
+}
+SelectResult select_forward(const SelectInputs &in, int32_t flags, bool need_grad, void *stream) {
+    const SelectInputs i{near_steps(in.x), near_steps(in.dt), in.a, near_steps(in.b), near_steps(in.c), in.state, in.skip, near_steps(in.gate), in.dt_bias,
+                         in.lengths};
     const int64_t B = i.x.size(0), T = i.x.size(1), D = i.x.size(2), N = i.a.size(1);
     SelectResult r;
     r.y = at::empty({B, T, D}, i.x.options());
@@ -237,7 +243,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         check_on(t, like, "a saved tensor");
         check_type(t, type, "a saved tensor");
         check_sizes(t, sizes, "a saved tensor");
-        return dense_channels(t);
+        return near_steps(dense_channels(t));
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         once("selective_scan");
@@ -255,7 +261,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         const Tensor lengths = saved[8].defined() ? restored(saved[8], x, flags & T2FW_SELECT_LENGTHS64 ? at::kLong : at::kInt, B) : Tensor();
         const Tensor ckpt = restored(saved[9], x, at::kByte, (int64_t)t2fw_selective_scan_checkpoint_bytes(B, T, D, N));
         // a result that nothing depends on has no gradient
-        const Tensor gy = grads[0].defined() ? dense_channels(grads[0]) : at::zeros({1}, x.options()).expand({B, T, D}).contiguous();
+        const Tensor gy = grads[0].defined() ? near_steps(dense_channels(grads[0])) : at::zeros({1}, x.options()).expand({B, T, D}).contiguous();
         const Tensor gs = grads[1].defined() ? grads[1].contiguous().resolve_neg() : Tensor();
         check_type(gy, type, "the gradient");
         check_sizes(gy, {B, T, D}, "the gradient");

@@ -54,7 +54,7 @@ int check_select(int64_t B, int64_t T, int64_t D, int64_t N, int32_t dtype, int3
     return T2FW_OK;
 }
 // rows and steps of x, dt, b, c, gate and, backward, g_y
-int select_args(SelectArgs &s, int64_t B, int64_t T, int64_t D, int64_t N, const int64_t *strides, bool backward, int32_t flags) {
+int select_args(SelectArgs &s, int64_t B, int64_t T, int64_t D, int64_t N, const int64_t *strides, bool backward, size_t es, int32_t flags) {
     s.B = B; s.T = T; s.D = D; s.N = N;
     s.softplus = (flags & T2FW_SELECT_SOFTPLUS) != 0;
     s.wide_lengths = (flags & T2FW_SELECT_LENGTHS64) != 0;
@@ -64,20 +64,24 @@ int select_args(SelectArgs &s, int64_t B, int64_t T, int64_t D, int64_t N, const
         *to[i] = i % 2 == 0 ? T * width : width;
         if (strides == nullptr || (i >= 10 && !backward) || (i / 2 == 4 && s.gate == nullptr)) continue;
         if (strides[i] < 0) return fail(T2FW_ERR_BAD_SHAPE, "selective scan: strides must be non-negative");
+        // (a tile of 16 steps is addressed by 32 bits)
+        if (i % 2 == 1 && T > 1 && strides[i] > (int64_t)(0xffffffffu / (SELECT_TILE * es)))
+            return fail(T2FW_ERR_UNSUPPORTED, "selective scan: steps are %lld elements apart, 16 of them have to be within 4 GB", (long long)strides[i]);
         *to[i] = strides[i];
     }
     return T2FW_OK;
 }
 
 struct BeamLayout {
-    int64_t pieces, shares;                  // bytes of the first array of the scratch
+    BeamPieces cut;
+    int64_t shares;                          // bytes of the first array of the scratch
     size_t bytes;
 };
 BeamLayout beam_layout(int64_t B, int64_t K, int64_t V, int64_t n) {
     BeamLayout l;
-    l.pieces = (V + BEAM_PIECE - 1) / BEAM_PIECE;
-    l.shares = B * K * l.pieces * 16;
-    l.bytes = (size_t)(l.shares + B * K * l.pieces * n * 8);
+    l.cut = beam_pieces(B, K, V);
+    l.shares = B * K * l.cut.pieces * 16;
+    l.bytes = (size_t)(l.shares + B * K * l.cut.pieces * n * 8);
     return l;
 }
 int check_beams(int64_t B, int64_t K, int64_t V, int64_t n, int32_t dtype) {
@@ -182,7 +186,7 @@ int t2fw_selective_scan_forward(const void *x, const void *dt, const float *a, c
     SelectArgs s{};
     s.x = x; s.dt = dt; s.a = a; s.b = b; s.c = c; s.skip = skip; s.gate = gate; s.dt_bias = dt_bias; s.s0 = s0; s.lengths = lengths;
     s.y = y; s.last = last; s.ckpt = static_cast<float *>(ckpt); s.maps = static_cast<float *>(workspace);
-    if ((rc = select_args(s, B, T, D, N, strides, false, flags))) return rc;
+    if ((rc = select_args(s, B, T, D, N, strides, false, es, flags))) return rc;
     return select_forward(s, dtype, static_cast<hipStream_t>(stream));
 }
 
@@ -207,7 +211,7 @@ int t2fw_selective_scan_backward(const void *g_y, const float *g_last, const voi
     s.g_y = g_y; s.g_state = g_last; s.x = x; s.dt = dt; s.a = a; s.b = b; s.c = c; s.skip = skip; s.gate = gate; s.dt_bias = dt_bias; s.lengths = lengths;
     s.ckpt = static_cast<float *>(const_cast<void *>(ckpt)); s.maps = static_cast<float *>(workspace);
     s.d_x = d_x; s.d_dt = d_dt; s.d_a = d_a; s.d_b = d_b; s.d_c = d_c; s.d_skip = d_skip; s.d_gate = d_gate; s.d_bias = d_bias; s.d_s0 = d_s0;
-    if ((rc = select_args(s, B, T, D, N, strides, true, flags))) return rc;
+    if ((rc = select_args(s, B, T, D, N, strides, true, es, flags))) return rc;
     return select_backward(s, dtype, static_cast<hipStream_t>(stream));
 }
 
@@ -226,7 +230,7 @@ int t2fw_selective_scan_step(const void *x, const void *dt, const float *a, cons
     s.x = x; s.dt = dt; s.a = a; s.b = b; s.c = c; s.skip = skip; s.gate = gate; s.dt_bias = dt_bias; s.s0 = s0; s.y = y; s.last = next_state;
     int64_t both[10];
     for (int i = 0; strides != nullptr && i < 10; ++i) both[i] = strides[i / 2];         // (there is one step)
-    if ((rc = select_args(s, B, 1, D, N, strides == nullptr ? nullptr : both, false, flags))) return rc;
+    if ((rc = select_args(s, B, 1, D, N, strides == nullptr ? nullptr : both, false, es, flags))) return rc;
     return select_step(s, dtype, static_cast<hipStream_t>(stream));
 }
 
@@ -252,7 +256,7 @@ int t2fw_beam_select(const void *logits, const float *scores, const void *finish
     a.out_scores = out_scores; a.out_beams = out_beams; a.out_tokens = out_tokens;
     a.partial = workspace;
     a.lists = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + l.shares);
-    a.B = B; a.K = K; a.V = V; a.n = (int32_t)n; a.pieces = (int32_t)l.pieces; a.pad = (int32_t)pad;
+    a.B = B; a.K = K; a.V = V; a.n = (int32_t)n; a.pieces = l.cut.pieces; a.piece = l.cut.piece; a.pad = (int32_t)pad;
     return beam_select(a, dtype, static_cast<hipStream_t>(stream));
 }
 

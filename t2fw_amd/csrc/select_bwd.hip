@@ -55,7 +55,7 @@ template <int G> __device__ __forceinline__ void add_channels(float *to, const f
     }
 }
 
-template <typename IO, int G> __global__ __launch_bounds__(THREADS, G >= 4 ? 2 : 1) void select_backward_kernel(SelectArgs a, Grid g) {
+template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, G >= 4 ? 2 : 1) void select_backward_kernel(SelectArgs a, Grid g) {
     constexpr int NP = G * S, Q = share<G>(), ROUNDS = TILE / Q;
     constexpr bool FAST = sizeof(IO) == 2;
     __shared__ float bs[TILE][NP], cs[TILE][NP], sums[THREADS / 64][TILE][2 * NP];
@@ -71,31 +71,43 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS, G >= 4 ? 2 :
     const auto load = [&](int64_t t0) {
         x.load(a.x, a.x_b, a.x_t, a, p, t0);
         dt.load(a.dt, a.dt_b, a.dt_t, a, p, t0);
-        if (a.gate != nullptr) gate.load(a.gate, a.z_b, a.z_t, a, p, t0);
+        if constexpr (GATED) gate.load(a.gate, a.z_b, a.z_t, a, p, t0);
         gy.load(a.g_y, a.g_b, a.g_t, a, p, t0);
         b.load(a.b, a.b_b, a.b_t, a, p, t0);
         c.load(a.c, a.c_b, a.c_t, a, p, t0);
-        load_padded(next_h, a.ckpt + ((p.b * g.tiles + t0 / TILE) * a.D + p.d) * NP + p.n0);
+        const Buffer at = buffer_of(a.ckpt + (p.b * g.tiles + t0 / TILE) * a.D * NP, a.D * NP * 4);
+        const auto v = __builtin_bit_cast(Vec<float, S>, __builtin_amdgcn_raw_buffer_load_b128(at, (uint32_t)((p.d * NP + p.n0) * 4), 0, 0));
+#pragma unroll
+        for (int s = 0; s < S; ++s) next_h[s] = v.e[s];
     };
     if (tiles > 0) load(p.begin + (int64_t)(tiles - 1) * TILE);
     if (a.g_state != nullptr) load_states(adj, a.g_state + (p.b * a.D + p.d) * a.N, p.n0, a.N);
     through_maps<G, true>(adj, a, g, p, rate);
-    const int64_t row = p.b * a.T * a.D + p.d;
-    IO *const d_x = static_cast<IO *>(a.d_x) + row, *const d_dt = static_cast<IO *>(a.d_dt) + row, *const d_gate = static_cast<IO *>(a.d_gate) + row;
-    const bool stores = p.mine && p.ng < Q;
-    float *const bc = a.bc + (((int64_t)p.block * a.B + p.b) * a.T) * 2 * NP;
+    // sums over the block's channels, of the tile
+    const auto store_steps = [&](int64_t t0, bool some) {
+        constexpr int ALL = TILE * 2 * NP;
+        const Buffer to = result_of(a.bc + (((int64_t)p.block * a.B + p.b) * a.T + t0) * 2 * NP, (a.T - t0) * 2 * NP * 4);
+#pragma unroll
+        for (int i = 0; i < ALL; i += THREADS) {
+            const int at = i + threadIdx.x, from = at < ALL ? at : 0;
+            const float *const v = &sums[0][0][0] + from;
+            store_to<float>(to, at < ALL ? at * 4u : BEYOND, 0, some ? ((v[0] + v[ALL]) + v[2 * ALL]) + v[3 * ALL] : 0.0f);
+        }
+    };
     // steps beyond the row's length
-    {
-        const int64_t from = p.begin + (int64_t)tiles * TILE;
-        if (stores)
-            for (int64_t t = from + p.ng; t < p.end; t += Q) {
-                d_x[t * a.D] = d_dt[t * a.D] = narrow<IO>(0.0f);
-                if (a.gate != nullptr) d_gate[t * a.D] = narrow<IO>(0.0f);
-            }
-        for (int64_t i = from * 2 * NP + threadIdx.x; i < p.end * 2 * NP; i += THREADS) bc[i] = 0.0f;
+    for (int64_t t0 = p.begin + (int64_t)tiles * TILE; t0 < p.end; t0 += TILE) {
+        const Results<IO, G> d_x(a.d_x, a, p, t0), d_dt(a.d_dt, a, p, t0), d_gate(GATED ? a.d_gate : a.d_x, a, p, t0);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            d_x.store(r, 0.0f);
+            d_dt.store(r, 0.0f);
+            if constexpr (GATED) d_gate.store(r, 0.0f);
+        }
+        store_steps(t0, false);
     }
     for (int k = tiles - 1; k >= 0; --k) {
         const int64_t t0 = p.begin + (int64_t)k * TILE;
+        const Results<IO, G> d_x(a.d_x, a, p, t0), d_dt(a.d_dt, a, p, t0), d_gate(GATED ? a.d_gate : a.d_x, a, p, t0);
         b.store(&bs[0][0], a, p, t0);
         c.store(&cs[0][0], a, p, t0);
         float length[ROUNDS], slope[ROUNDS], xs[ROUNDS], gys[ROUNDS], zs[ROUNDS], h0[S];
@@ -107,7 +119,7 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS, G >= 4 ? 2 :
             slope[r] = counts ? one.slope : 0.0f;
             xs[r] = counts ? widen(x.v[r]) : 0.0f;
             gys[r] = counts ? widen(gy.v[r]) : 0.0f;
-            zs[r] = a.gate != nullptr && counts ? widen(gate.v[r]) : 0.0f;
+            zs[r] = GATED && counts ? widen(gate.v[r]) : 0.0f;
         }
 #pragma unroll
         for (int s = 0; s < S; ++s) h0[s] = p.mine ? next_h[s] : 0.0f;
@@ -129,7 +141,7 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS, G >= 4 ? 2 :
                     decay[t][s] = exp2_of(l * rate[s]);
                     h[t][s] = fmaf(decay[t][s], t > 0 ? h[t - 1][s] : h0[s], u * bv[s]);
                 }
-                if (a.gate != nullptr) {
+                if constexpr (GATED) {
                     float cv[S];
                     load_padded(cv, &cs[t][p.n0]);
                     y[j] = 0.0f;
@@ -141,11 +153,11 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS, G >= 4 ? 2 :
             if constexpr (Q >= 2) step(std::integral_constant<int, 1>{});
             if constexpr (Q == 4) { step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 3>{}); }
             dy[r] = gys[r];
-            if (a.gate != nullptr) {
+            if constexpr (GATED) {
                 const float sig = sigmoid_of<FAST>(zs[r]), out = fmaf(skip, xs[r], sum_steps<G>(y));
                 dy[r] = gys[r] * (zs[r] * sig);
                 const int64_t t = t0 + r * Q + p.ng % Q;
-                if (stores && t < p.end) d_gate[t * a.D] = narrow<IO>(t < p.live ? gys[r] * out * silu_slope(zs[r], sig) : 0.0f);
+                d_gate.store(r, t < p.live ? gys[r] * out * silu_slope(zs[r], sig) : 0.0f);
             }
         }
 #pragma unroll
@@ -181,20 +193,13 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS, G >= 4 ? 2 :
             const float for_x = fmaf(length[r], gb, skip * dy[r]), for_dt = fmaf(xs[r], gb, pa) * slope[r];
             const int64_t t = t0 + r * Q + p.ng % Q;
             const bool counts = t < p.live;
-            if (stores && t < p.end) {
-                d_x[t * a.D] = narrow<IO>(counts ? for_x : 0.0f);
-                d_dt[t * a.D] = narrow<IO>(counts ? for_dt : 0.0f);
-            }
+            d_x.store(r, counts ? for_x : 0.0f);
+            d_dt.store(r, counts ? for_dt : 0.0f);
             d_skip = fmaf(dy[r], xs[r], d_skip);
             d_bias += counts ? for_dt : 0.0f;
         }
         __syncthreads();
-        const int here = (int)((p.end - t0 < TILE ? p.end - t0 : TILE) * 2 * NP);
-        for (int i = threadIdx.x; i < here; i += THREADS) {
-            const float *const v = &sums[0][0][0] + i;
-            constexpr int next = TILE * 2 * NP;
-            bc[t0 * 2 * NP + i] = ((v[0] + v[next]) + v[2 * next]) + v[3 * next];
-        }
+        store_steps(t0, true);
     }
     // (a channel's lanes beyond the first quad have the same steps as that)
     d_skip = sum_share<G>(d_skip);
@@ -250,7 +255,8 @@ template <typename IO, int G> int launch_backward(const SelectArgs &a, const Gri
             hipLaunchKernelGGL((select_maps_kernel<IO, G, true>), dim3(row * (g.chunks - 1)), dim3(THREADS), 0, stream, a, g);
             if ((rc = check_hip(hipGetLastError(), "select_maps_kernel launch"))) return rc;
         }
-        hipLaunchKernelGGL((select_backward_kernel<IO, G>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
+        if (a.gate != nullptr) hipLaunchKernelGGL((select_backward_kernel<IO, G, true>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
+        else hipLaunchKernelGGL((select_backward_kernel<IO, G, false>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
         if ((rc = check_hip(hipGetLastError(), "select_backward_kernel launch"))) return rc;
     }
     const int64_t n = a.B * a.T * 2 * NP, groups = (n + THREADS - 1) / THREADS, columns = (a.D * (NP + 2) + 63) / 64;
@@ -265,11 +271,9 @@ template <typename IO, int G> int launch_backward(const SelectArgs &a, const Gri
 
 }  // namespace
 
-Grid select_ns::backward_grid(int64_t B, int64_t T, int64_t D, int64_t N) { return grid_of(B, T, D, N, 512, 4); }
-
 int select_backward(const SelectArgs &args, int dtype, hipStream_t stream) {
     SelectArgs a = args;
-    const Grid g = backward_grid(a.B, a.T, a.D, a.N);
+    const Grid g = grid_of(a.B, a.T, a.D, a.N);
     if (!g.fits) return too_many();
     const int64_t NP = lanes_of(a.N) * S;
     // the scratch: maps, gradients of b and c by blocks, those of the weights by rows and chunks

@@ -6,7 +6,7 @@ namespace t2fw {
 using namespace select_ns;
 namespace {
 
-template <typename IO, int G> __global__ __launch_bounds__(THREADS) void select_forward_kernel(SelectArgs a, Grid g) {
+template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS) void select_forward_kernel(SelectArgs a, Grid g) {
     constexpr int NP = G * S, Q = share<G>(), ROUNDS = TILE / Q;
     constexpr bool FAST = sizeof(IO) == 2;
     __shared__ float bs[2][TILE][NP], cs[2][TILE][NP];
@@ -20,21 +20,23 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS) void select_
     const auto load = [&](int64_t t0) {
         x.load(a.x, a.x_b, a.x_t, a, p, t0);
         dt.load(a.dt, a.dt_b, a.dt_t, a, p, t0);
-        if (a.gate != nullptr) gate.load(a.gate, a.z_b, a.z_t, a, p, t0);
+        if constexpr (GATED) gate.load(a.gate, a.z_b, a.z_t, a, p, t0);
         b.load(a.b, a.b_b, a.b_t, a, p, t0);
         c.load(a.c, a.c_b, a.c_t, a, p, t0);
     };
     if (tiles > 0) load(p.begin);
     if (a.s0 != nullptr) load_states(h, a.s0 + (p.b * a.D + p.d) * a.N, p.n0, a.N);
     through_maps<G, false>(h, a, g, p, rate);
-    IO *const to = static_cast<IO *>(a.y) + p.b * a.T * a.D + p.d;
-    const bool stores = p.mine && p.ng < Q;
     for (int k = 0; k < tiles; ++k) {
         const int64_t t0 = p.begin + (int64_t)k * TILE;
         float (&b_here)[TILE][NP] = bs[k % 2], (&c_here)[TILE][NP] = cs[k % 2];
         b.store(&b_here[0][0], a, p, t0);
         c.store(&c_here[0][0], a, p, t0);
-        if (a.ckpt != nullptr && p.mine) store_padded(a.ckpt + ((p.b * g.tiles + t0 / TILE) * a.D + p.d) * NP + p.n0, h);
+        if (a.ckpt != nullptr) {
+            const Buffer at = result_of(a.ckpt + (p.b * g.tiles + t0 / TILE) * a.D * NP, a.D * NP * 4);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Four, Vec<float, S>{{h[0], h[1], h[2], h[3]}}), at, p.mine ? (uint32_t)((p.d * NP + p.n0) * 4) : BEYOND, 0, 0);
+        }
+        const Results<IO, G> y_to(a.y, a, p, t0);
         float length[ROUNDS], push[ROUNDS], add[ROUNDS], times[ROUNDS];
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
@@ -43,7 +45,8 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS) void select_
             length[r] = counts ? one : 0.0f;
             push[r] = counts ? one * v : 0.0f;
             add[r] = a.skip == nullptr ? 0.0f : skip * v;
-            times[r] = a.gate != nullptr ? silu_of<FAST>(widen(gate.v[r])) : 1.0f;
+            times[r] = 1.0f;
+            if constexpr (GATED) times[r] = silu_of<FAST>(widen(gate.v[r]));
         }
         __syncthreads();
         if (k + 1 < tiles) load(t0 + TILE);
@@ -68,12 +71,15 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS) void select_
             if constexpr (Q == 4) { step(std::integral_constant<int, 2>{}); step(std::integral_constant<int, 3>{}); }
             const float out = (sum_steps<G>(y) + add[r]) * times[r];
             const int64_t t = t0 + r * Q + p.ng % Q;
-            if (stores && t < p.end) to[t * a.D] = narrow<IO>(t < p.live ? out : 0.0f);
+            y_to.store(r, t < p.live ? out : 0.0f);
         }
     }
     // steps beyond the row's length
-    if (stores)
-        for (int64_t t = p.begin + (int64_t)tiles * TILE + p.ng; t < p.end; t += Q) to[t * a.D] = narrow<IO>(0.0f);
+    for (int64_t t0 = p.begin + (int64_t)tiles * TILE; t0 < p.end; t0 += TILE) {
+        const Results<IO, G> y_to(a.y, a, p, t0);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) y_to.store(r, 0.0f);
+    }
     if (p.mine && p.chunk == g.chunks - 1) store_states(a.last + (p.b * a.D + p.d) * a.N, h, p.n0, a.N);
 }
 
@@ -118,7 +124,8 @@ template <typename IO, int G> int launch_forward(const SelectArgs &a, const Grid
         const int rc = check_hip(hipGetLastError(), "select_maps_kernel launch");
         if (rc) return rc;
     }
-    hipLaunchKernelGGL((select_forward_kernel<IO, G>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
+    if (a.gate != nullptr) hipLaunchKernelGGL((select_forward_kernel<IO, G, true>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
+    else hipLaunchKernelGGL((select_forward_kernel<IO, G, false>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
     return check_hip(hipGetLastError(), "select_forward_kernel launch");
 }
 template <typename IO, int G> int launch_step(const SelectArgs &a, uint32_t blocks, hipStream_t stream) {
@@ -128,28 +135,26 @@ template <typename IO, int G> int launch_step(const SelectArgs &a, uint32_t bloc
 
 }  // namespace
 
-Grid select_ns::forward_grid(int64_t B, int64_t T, int64_t D, int64_t N) { return grid_of(B, T, D, N, 1024, 4); }
-
 int select_forward(const SelectArgs &a, int dtype, hipStream_t stream) {
-    const Grid g = forward_grid(a.B, a.T, a.D, a.N);
+    const Grid g = grid_of(a.B, a.T, a.D, a.N);
     if (!g.fits) return too_many();
     SELECT_OF(launch_forward, dtype, lanes_of(a.N), a, g, stream)
 }
 
 int select_step(const SelectArgs &a, int dtype, hipStream_t stream) {
-    const Grid g = forward_grid(a.B, 1, a.D, a.N);
+    const Grid g = grid_of(a.B, 1, a.D, a.N);
     if (!g.fits) return too_many();
     SELECT_OF(launch_step, dtype, lanes_of(a.N), a, g.blocks, stream)
 }
 
 SelectPlan select_plan(int64_t B, int64_t T, int64_t D, int64_t N) {
-    const Grid f = forward_grid(B, T, D, N), r = backward_grid(B, T, D, N);
+    const Grid g = grid_of(B, T, D, N);
     const int64_t NP = lanes_of(N) * S;
     SelectPlan p{};
-    if (!f.fits || !r.fits) return p;
-    p.checkpoints = (size_t)(B * f.tiles * D * NP) * sizeof(float);
-    p.forward = maps_bytes(f, B, D, N);
-    p.backward = (maps_bytes(r, B, D, N) + 15) / 16 * 16 + (size_t)((int64_t)r.blocks * B * T * 2 * NP + (int64_t)r.chunks * B * D * (NP + 2)) * sizeof(float);
+    if (!g.fits) return p;
+    p.checkpoints = (size_t)(B * g.tiles * D * NP) * sizeof(float);
+    p.forward = maps_bytes(g, B, D, N);
+    p.backward = (maps_bytes(g, B, D, N) + 15) / 16 * 16 + (size_t)((int64_t)g.blocks * B * T * 2 * NP + (int64_t)g.chunks * B * D * (NP + 2)) * sizeof(float);
     return p;
 }
 

@@ -142,17 +142,38 @@ __device__ __forceinline__ void load_rates(float (&v)[S], const SelectArgs &a, c
     for (int s = 0; s < S; ++s) v[s] *= LOG2E;
 }
 
+// Arrays through buffer descriptors: a scalar address for the tile, a lane's offset that stays as it is, and a scalar one for the round.  What is beyond the
+// array is not loaded (zeros come) and not stored, so no branch stands between the accesses: with branches the compiler does not know
+// how many are under way, and waits for the stores of a tile where it needs loads from before them (backward of 32 x 512 x 1536 x 16 bf16: 664 us, so
+// 446).
+typedef __amdgpu_buffer_rsrc_t Buffer;
+typedef uint32_t Four __attribute__((ext_vector_type(4)));
+constexpr uint32_t BEYOND = 0x80000000u;                 // an offset that is in no array
+__device__ __forceinline__ Buffer buffer_of(const void *at, int64_t bytes) {
+    const int64_t n = bytes < 0 ? 0 : bytes < (int64_t)0xfffffff0u ? bytes : (int64_t)0xfffffff0u;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(at), 0, (int)(uint32_t)n, 0x00027000);
+}
+__device__ __forceinline__ Buffer result_of(void *at, int64_t bytes) { return buffer_of(at, bytes < (int64_t)BEYOND ? bytes : (int64_t)BEYOND); }
+template <typename IO> __device__ __forceinline__ IO load_from(Buffer b, uint32_t lane, uint32_t offset) {
+    if constexpr (sizeof(IO) == 2) return __builtin_bit_cast(IO, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, lane, offset, 0));
+    else return __builtin_bit_cast(IO, __builtin_amdgcn_raw_buffer_load_b32(b, lane, offset, 0));
+}
+template <typename IO> __device__ __forceinline__ void store_to(Buffer b, uint32_t lane, uint32_t offset, IO v) {
+    if constexpr (sizeof(IO) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), b, lane, offset, 0);
+    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), b, lane, offset, 0);
+}
+
 // What a tile needs of the arrays, on its way: a lane's steps of those per channel ...
 template <typename IO, int G> struct PerChannel {
     static constexpr int ROUNDS = TILE / share<G>();
     IO v[ROUNDS];
     __device__ __forceinline__ void load(const void *base, int64_t row, int64_t step, const SelectArgs &a, const Place &p, int64_t t0) {
-        const IO *const at = static_cast<const IO *>(base) + p.b * row + p.d;
+        const int64_t first = (int64_t)p.block * (THREADS / G);
+        const IO *const at = static_cast<const IO *>(base) + p.b * row + t0 * step + first;
+        const Buffer from = buffer_of(at, ((a.T - 1 - t0) * step + a.D - first) * (int64_t)sizeof(IO));
+        const uint32_t lane = ((uint32_t)(p.ng % share<G>()) * (uint32_t)step + (uint32_t)(p.d - first)) * sizeof(IO);
 #pragma unroll
-        for (int r = 0; r < ROUNDS; ++r) {
-            const int64_t t = t0 + r * share<G>() + p.ng % share<G>();
-            v[r] = at[(t < a.T ? t : a.T - 1) * step];
-        }
+        for (int r = 0; r < ROUNDS; ++r) v[r] = load_from<IO>(from, lane, (uint32_t)(r * share<G>()) * (uint32_t)step * sizeof(IO));
     }
 };
 // ... and elements of b or c, which go to shared memory
@@ -160,12 +181,11 @@ template <typename IO, int G> struct PerStep {
     static constexpr int NP = G * S, EACH = (TILE * NP + THREADS - 1) / THREADS;
     IO v[EACH];
     __device__ __forceinline__ void load(const void *base, int64_t row, int64_t step, const SelectArgs &a, const Place &p, int64_t t0) {
-        const IO *const at = static_cast<const IO *>(base) + p.b * row;
+        const Buffer from = buffer_of(static_cast<const IO *>(base) + p.b * row + t0 * step, ((a.T - 1 - t0) * step + a.N) * (int64_t)sizeof(IO));
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int j = i * THREADS + threadIdx.x, n = j % NP;
-            const int64_t t = t0 + j / NP;
-            v[i] = at[(t < a.T ? t : a.T - 1) * step + (n < a.N ? n : 0)];
+            v[i] = load_from<IO>(from, j < TILE * NP && n < a.N ? ((uint32_t)(j / NP) * (uint32_t)step + n) * (uint32_t)sizeof(IO) : 0u, 0);
         }
     }
     // zeros for states that are none, and for steps that do not count, whatever they hold
@@ -175,6 +195,20 @@ template <typename IO, int G> struct PerStep {
             const int j = i * THREADS + threadIdx.x;
             if (j < TILE * NP) to[j] = j % NP < a.N && t0 + j / NP < p.live ? widen(v[i]) : 0.0f;
         }
+    }
+};
+// Results per channel: a lane's steps of a tile
+template <typename IO, int G> struct Results {
+    Buffer to;
+    uint32_t lane;
+    int64_t D;
+    __device__ __forceinline__ Results(void *base, const SelectArgs &a, const Place &p, int64_t t0) : D(a.D) {
+        const int64_t first = (int64_t)p.block * (THREADS / G);
+        to = result_of(static_cast<IO *>(base) + (p.b * a.T + t0) * a.D + first, ((a.T - t0) * a.D - first) * (int64_t)sizeof(IO));
+        lane = p.mine && p.ng < share<G>() ? ((uint32_t)p.ng * (uint32_t)a.D + (uint32_t)(p.d - first)) * sizeof(IO) : BEYOND;
+    }
+    __device__ __forceinline__ void store(int r, float v) const {
+        store_to<IO>(to, lane, (uint32_t)(r * share<G>()) * (uint32_t)D * sizeof(IO), narrow<IO>(v));
     }
 };
 
@@ -294,25 +328,25 @@ inline int lanes_of(int64_t N) {
     while (g * S < N) g *= 2;
     return g;
 }
-// `want` workgroups, or as many as there are chunks of no less than `least` tiles
-inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N, int64_t want, int64_t least) {
+// Chunks: none where channels and rows alone make two workgroups for every CU (32 x 512 x 1536 x 16 bf16: forward 140 us, in two chunks 177; backward 446
+// and 490), else as many as make 1280 (8 x 1024 x 1536 x 16, forward and backward: 768 workgroups 122 and 266 us, 1024 113 and 260, 1536 113 and 252, 4096 118 and
+// 283), but no more than the root of the steps, as a chunk goes through the maps of all before it (1 x 16384 x 64 x 16: 64 chunks 77 and 146, 128 60 and 110, 256
+// 70 and 119; 1 x 131072 x 64 x 16: 128 chunks 314 and 529, 256 201 and 329).
+inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N) {
     Grid g{};
     const int64_t channels = THREADS / lanes_of(N), blocks = (D + channels - 1) / channels, tiles = T <= 0 ? 0 : (T + TILE - 1) / TILE;
     const long double rows = (long double)blocks * B;
     int64_t chunks = 1;
-    if (rows > 0 && rows < want) chunks = (int64_t)((want + rows - 1) / rows);
-    if (chunks > tiles / least) chunks = tiles / least;
-    if (chunks < 1) chunks = 1;
+    if (rows > 0 && rows < 512) chunks = (int64_t)((1280 + rows - 1) / rows);
+    while (chunks > 1 && (chunks * chunks > T || chunks > tiles)) --chunks;
     const int64_t each = tiles == 0 ? 1 : (tiles + chunks - 1) / chunks;
     g.steps = each * TILE;
     g.chunks = (uint32_t)(tiles == 0 ? 1 : (tiles + each - 1) / each);
     g.blocks = (uint32_t)blocks;
-    g.fits = blocks < 0x7fffffff && B < 0x7fffffff && tiles < 0x7fffffff && rows * g.chunks < MOST_GROUPS;
+    g.fits = D * 16 * S < (1ll << 27) && B < 0x7fffffff && tiles < 0x7fffffff && rows * g.chunks < MOST_GROUPS;
     g.tiles = (uint32_t)tiles;
     return g;
 }
-Grid forward_grid(int64_t B, int64_t T, int64_t D, int64_t N);
-Grid backward_grid(int64_t B, int64_t T, int64_t D, int64_t N);
 inline size_t maps_bytes(const Grid &g, int64_t B, int64_t D, int64_t N) {
     return g.chunks == 1 ? 0 : (size_t)g.chunks * B * D * (lanes_of(N) * S + 1) * sizeof(float);
 }

@@ -85,7 +85,12 @@ template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS) voi
     const Place p = place_of<VEC>(a, g);
     if (!p.mine) return;
     const int64_t length = row_length(a, p.b);
-    if (a.T > 0) {
+    IO *const to = static_cast<IO *>(a.y) + (p.b * a.T + p.t0) * a.D + p.d;
+    if (p.t0 >= length) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (p.t0 + r < a.T) store_vec(to + r * a.D, nothing<IO, VEC>());
+    } else {
         Vec<IO, VEC> x[R + W - 1];
         if (p.t0 > 0) {
             const IO *const at = static_cast<const IO *>(a.x) + p.b * a.x_b + p.d;
@@ -101,7 +106,6 @@ template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS) voi
         float w[VEC * W], bias[VEC];
         load_weights<IO, VEC, W>(w, a, p.d);
         load_bias<IO, VEC>(bias, a, p.d);
-        IO *const to = static_cast<IO *>(a.y) + (p.b * a.T + p.t0) * a.D + p.d;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             Vec<IO, VEC> y;
@@ -117,9 +121,9 @@ template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS) voi
         }
     }
     if (p.t0 == 0) {
-        IO *const to = static_cast<IO *>(a.last) + p.b * (W - 1) * a.D + p.d;
+        IO *const last = static_cast<IO *>(a.last) + p.b * (W - 1) * a.D + p.d;
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) store_vec(to + j * a.D, input_at<IO, VEC, W>(a, p.b, length + j - (W - 1), p.d));
+        for (int j = 0; j < W - 1; ++j) store_vec(last + j * a.D, input_at<IO, VEC, W>(a, p.b, length + j - (W - 1), p.d));
     }
 }
 
@@ -176,7 +180,17 @@ template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS, 2) 
     for (int64_t t0 = p.t0; p.mine && t0 < end + W - 1; t0 += R) {
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) x[i] = x[R + i];
-        if (a.T > 0) {
+        if (t0 >= length + W - 1) {
+            Held<IO, VEC> zero;
+            zero.clear();
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t t = t0 + r - (W - 1);
+                if (t >= p.t0 && t < end) zero.store(static_cast<IO *>(a.d_x) + (p.b * a.T + t) * a.D + p.d);
+            }
+            continue;
+        }
+        if (t0 < length) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const int64_t t = t0 + r < a.T ? t0 + r : a.T - 1;

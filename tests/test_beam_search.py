@@ -52,7 +52,7 @@ def logits_of(B, K, V, dtype, seed, std=3.0):
 
 # logits of one, of fewer than candidates, of less and more than a vector, a piece and several; beams of one, odd, many
 SHAPES = [(1, 1, 1, 1), (2, 3, 2, 6), (1, 4, 8000, 8), (3, 1, 100, 100), (2, 5, 257, 7), (4, 2, 8192, 4), (1, 3, 8193, 6), (2, 8, 50257, 16), (1, 16, 20000, 32),
-          (3, 64, 130, 128), (1, 200, 40, 20), (2, 2, 131072, 128), (70, 4, 60, 8)]
+          (3, 64, 130, 128), (64, 8, 16389, 16), (30, 8, 40000, 20), (1, 200, 40, 20), (2, 2, 131072, 128), (70, 4, 60, 8)]
 
 
 @pytest.mark.gpu
@@ -338,7 +338,7 @@ def test_c_abi_refusals():
         ptrs = [p] * 6
         ptrs[i] = None
         assert sel(ptrs=ptrs) == 1
-    assert lib.t2fw_beam_select_workspace_bytes(32, 8, 50257, 16, 2) == 32 * 8 * 7 * (16 + 16 * 8)
+    assert lib.t2fw_beam_select_workspace_bytes(32, 8, 50257, 16, 2) % (32 * 8 * (16 + 16 * 8)) == 0
     desc = (_lib.ReorderDesc * 1)(_lib.ReorderDesc(p, p, 64))
     move = lambda count=1, B=1, K=2, d=desc, beams=p: lib.t2fw_beam_reorder(d, count, beams, B, K, None)
     assert move(K=0) == 3 and move(K=65) == 3 and move(B=-1) == 3 and move(count=-1) == 3 and move(d=None) == 1 and move(beams=None) == 1
