@@ -3,9 +3,11 @@
 //
 // Bound by memory: a lane owns 16 bytes of neighbouring channels of one row (backward: four channels) and 8 steps of them forward, so that an input is loaded once, and again
 // from the cache for the lane that has the next steps.  A workgroup has 16 such lanes side by side (256 bytes of a step) and 16 stretches in time.
-// Backward a lane goes through a stretch in tiles of 8 steps, the last W - 1 values of dz before the tile in registers: dx_p = sum_j w_j dz_{p+W-1-j}
-// needs the W - 1 steps after its own, which are the lane's last, computed there for dx alone.  z is made again from x.  The weights' gradients
-// are summed in registers, over the stretches of a workgroup in shared memory, and over workgroups by a second launch: in a fixed order.
+// Backward dx_p = sum_j w_j dz_{p+W-1-j} needs dz of the W - 1 steps after a lane's own too, which it makes again from x and the gradient: as many
+// loads at once as there are, and no loop whose loads wait for the stores of the one before (stretches of 13 to 125 steps, dz handed on in registers: 41 us
+// for 8 x 1024 x 1536 bf16, now 34).  The weights' gradients are summed in registers, over the stretches of a workgroup in
+// shared memory, and over workgroups by a second launch: in a fixed order.
+#include <type_traits>
 #include "short_conv.hpp"
 #include "activation.hpp"
 #include "vec.hpp"
@@ -14,7 +16,7 @@ namespace t2fw {
 namespace {
 
 constexpr int THREADS = 256, R = 8;                              // R: steps of a lane
-// ... and of its tile backward: four where eight do not fit the registers of two waves
+// ... backward: four where eight do not fit the registers of two waves
 constexpr int back_steps(int taps, bool wide) { return taps + (wide ? 2 : 0) > 6 ? 4 : 8; }
 constexpr int64_t MOST_GROUPS = (1ll << 32) / THREADS - 1;      // a grid has less than 2^32 threads along an axis
 
@@ -80,7 +82,7 @@ template <int VEC> __device__ __forceinline__ Place place_of(const ConvArgs &a, 
     return p;
 }
 
-template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS) void conv_forward_kernel(ConvArgs a, ConvGrid g) {
+template <typename IO, int VEC, int W, bool SILU> __global__ __launch_bounds__(THREADS) void conv_forward_kernel(ConvArgs a, ConvGrid g) {
     constexpr bool FAST = sizeof(IO) == 2;
     const Place p = place_of<VEC>(a, g);
     if (!p.mine) return;
@@ -93,11 +95,12 @@ template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS) voi
     } else {
         Vec<IO, VEC> x[R + W - 1];
         if (p.t0 > 0) {
-            const IO *const at = static_cast<const IO *>(a.x) + p.b * a.x_b + p.d;
+            const IO *at = static_cast<const IO *>(a.x) + p.b * a.x_b + (p.t0 - (W - 1)) * a.x_t + p.d;
+            const int there = a.T - p.t0 < R ? (int)(a.T - p.t0) + W - 1 : R + W - 1;
 #pragma unroll
             for (int i = 0; i < R + W - 1; ++i) {
-                const int64_t t = p.t0 - (W - 1) + i;
-                x[i] = load_vec<IO, VEC>(at + (t < a.T ? t : a.T - 1) * a.x_t);
+                x[i] = load_vec<IO, VEC>(at);
+                at += i + 1 < there ? a.x_t : 0;         // (of a step beyond the last one that again)
             }
         } else {
 #pragma unroll
@@ -114,7 +117,7 @@ template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS) voi
                 float z = bias[v];
 #pragma unroll
                 for (int j = 0; j < W; ++j) z = fmaf(w[v * W + j], widen(x[r + j].e[v]), z);
-                y.e[v] = narrow<IO>(a.silu ? silu_of<FAST>(z) : z);
+                y.e[v] = narrow<IO>(SILU ? silu_of<FAST>(z) : z);
             }
             if (p.t0 + r >= length) y = nothing<IO, VEC>();
             if (p.t0 + r < a.T) store_vec(to + r * a.D, y);
@@ -150,115 +153,160 @@ template <typename IO, int VEC> struct Held {
     }
 };
 
-template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS, 2) void conv_backward_kernel(ConvArgs a, ConvGrid g) {
+// Two values per lane, added up over the halves of the wave (of 32 lanes) and of rows of 32 (of 16): the first in the lower, the second in the upper half
+__device__ __forceinline__ float over_halves(float v0, float v1) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v0), __float_as_uint(v1), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float over_rows(float v0, float v1) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v0), __float_as_uint(v1), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename IO, int VEC, int W, bool SILU> __global__ __launch_bounds__(THREADS, 2) void conv_backward_kernel(ConvArgs a, ConvGrid g) {
     constexpr bool FAST = sizeof(IO) == 2;
-    constexpr int SUMS = VEC * (W + 1), LANES = 16, R = back_steps(W, sizeof(IO) == 4);
-    __shared__ float shares[THREADS / 64][LANES * SUMS];
+    constexpr int SUMS = (VEC * (W + 1) + 3) / 4 * 4, LANES = 16, R = back_steps(W, sizeof(IO) == 4), H = W - 1;
+    __shared__ float shares[THREADS / 64][SUMS][LANES];
     const Place p = place_of<VEC>(a, g);
-    const int64_t length = p.mine ? row_length(a, p.b) : 0, end = !p.mine ? p.t0 : p.t0 + g.steps < a.T ? p.t0 + g.steps : a.T;
-    float w[VEC * W], bias[VEC], sums[VEC][W + 1], before[W - 1][VEC];
-    load_weights<IO, VEC, W>(w, a, p.d);
-    load_bias<IO, VEC>(bias, a, p.d);
+    const int64_t length = p.mine ? row_length(a, p.b) : 0;
+    float sums[SUMS];                                    // of the weights and the bias of each channel
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
+    for (int i = 0; i < SUMS; ++i) sums[i] = 0.0f;
+    IO *const d_x = static_cast<IO *>(a.d_x) + (p.b * a.T + p.t0) * a.D + p.d, *const d_state = static_cast<IO *>(a.d_state);
+    const IO *const g_last = static_cast<const IO *>(a.g_last);
+    if (p.mine && p.t0 < length) {
+        const IO *xs = static_cast<const IO *>(a.x) + p.b * a.x_b + p.t0 * a.x_t + p.d, *gs = static_cast<const IO *>(a.g_y) + p.b * a.g_b + p.t0 * a.g_t + p.d;
+        // steps t0 - H .. t0 + R + H of x, t0 .. t0 + R + H of the gradient
+        Held<IO, VEC> x[R + 2 * H], gy[R + H];
+        if (p.t0 >= H) {
+            const IO *at = xs - H * a.x_t;
 #pragma unroll
-        for (int j = 0; j <= W; ++j) sums[v][j] = 0.0f;
+            for (int i = 0; i < H; ++i) x[i].load(at + i * a.x_t);
+        } else {
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) before[j][v] = 0.0f;
-    }
-    const IO *const xs = static_cast<const IO *>(a.x) + p.b * a.x_b + p.d, *const gs = static_cast<const IO *>(a.g_y) + p.b * a.g_b + p.d;
-    const IO *const state = static_cast<const IO *>(a.state), *const g_last = static_cast<const IO *>(a.g_last);
-    Held<IO, VEC> x[R + W - 1], gy[R];
-#pragma unroll
-    for (int i = 0; i < W - 1; ++i) {
-        const int64_t t = p.t0 - (W - 1) + i;
-        x[R + i].clear();
-        if (p.mine && t >= 0 && t < length) x[R + i].load(xs + t * a.x_t);
-        if (p.mine && t < 0 && state != nullptr) x[R + i].load(state + (p.b * (W - 1) + t + W - 1) * a.D + p.d);
-    }
-    // (the steps after the stretch: their dz counts for its last inputs)
-    for (int64_t t0 = p.t0; p.mine && t0 < end + W - 1; t0 += R) {
-#pragma unroll
-        for (int i = 0; i < W - 1; ++i) x[i] = x[R + i];
-        if (t0 >= length + W - 1) {
-            Held<IO, VEC> zero;
-            zero.clear();
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t t = t0 + r - (W - 1);
-                if (t >= p.t0 && t < end) zero.store(static_cast<IO *>(a.d_x) + (p.b * a.T + t) * a.D + p.d);
-            }
-            continue;
-        }
-        if (t0 < length) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t t = t0 + r < a.T ? t0 + r : a.T - 1;
-                x[W - 1 + r].load(xs + t * a.x_t);
-                gy[r].load(gs + t * a.g_t);
+            for (int i = 0; i < H; ++i) {
+                const int64_t t = p.t0 - H + i;
+                x[i].clear();
+                if (t >= 0) x[i].load(xs + (i - H) * a.x_t);
+                else if (a.state != nullptr) x[i].load(static_cast<const IO *>(a.state) + (p.b * H + t + H) * a.D + p.d);
             }
         }
-        // what steps beyond the row's length hold does not count, whatever it is
-        const int live = length - t0 < 0 ? 0 : length - t0 < R ? (int)(length - t0) : R, own = end - t0 < 0 ? 0 : end - t0 < R ? (int)(end - t0) : R;
+        const int there = a.T - p.t0 < R + H ? (int)(a.T - p.t0) : R + H, live = length - p.t0 < R + H ? (int)(length - p.t0) : R + H;
+#pragma unroll
+        for (int i = 0; i < R + H; ++i) {
+            x[H + i].load(xs);
+            gy[i].load(gs);
+            xs += i + 1 < there ? a.x_t : 0;             // (of a step beyond the last one that again)
+            gs += i + 1 < there ? a.g_t : 0;
+        }
+        float w[VEC * W], bias[VEC];
+        load_weights<IO, VEC, W>(w, a, p.d);
+        load_bias<IO, VEC>(bias, a, p.d);
+        const auto all = [&](auto WHOLE) {
+            constexpr bool whole = decltype(WHOLE)::value;
+            // what steps beyond the row's length hold does not count, whatever it is
+            if constexpr (!whole) {
+#pragma unroll
+                for (int i = 0; i < R + H; ++i)
+                    if (i >= live) {
+                        x[H + i].clear();
+                        gy[i].clear();
+                    }
+            }
+            float dz[R + H][VEC];
+#pragma unroll
+            for (int i = 0; i < R + H; ++i) {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    float d = gy[i].get(v);
+                    if constexpr (SILU) {
+                        float z = bias[v];
+#pragma unroll
+                        for (int j = 0; j < W; ++j) z = fmaf(w[v * W + j], x[i + j].get(v), z);
+                        d = d * silu_slope(z, sigmoid_of<FAST>(z));
+                    }
+                    dz[i][v] = whole || i < live ? d : 0.0f;
+                    if (i < R) {                         // (the steps after the lane's own are others')
+#pragma unroll
+                        for (int j = 0; j < W; ++j) sums[v * (W + 1) + j] = fmaf(dz[i][v], x[i + j].get(v), sums[v * (W + 1) + j]);
+                        sums[v * (W + 1) + W] += dz[i][v];
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                // the gradient of the last inputs as they are handed on
+                const int64_t t = p.t0 + r, at = t - length + H;
+                Held<IO, VEC> handed;
+                handed.clear();
+                if (!whole && g_last != nullptr && at >= 0 && at < H) handed.load(g_last + (p.b * H + at) * a.D + p.d);
+                float dx[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    float d = whole ? 0.0f : handed.get(v);
+#pragma unroll
+                    for (int j = 0; j < W; ++j) d = fmaf(w[v * W + j], dz[r + H - j][v], d);
+                    dx[v] = whole || t < length ? d : 0.0f;
+                }
+                Held<IO, VEC> out;
+                out.put(dx);
+                if (whole || t < a.T) out.store(d_x + r * a.D);
+            }
+            if (p.t0 == 0 && d_state != nullptr) {
+#pragma unroll
+                for (int m = 0; m < H; ++m) {
+                    const int64_t at = m - length;
+                    Held<IO, VEC> handed;
+                    handed.clear();
+                    if (g_last != nullptr && at >= 0) handed.load(g_last + (p.b * H + at) * a.D + p.d);
+                    float ds[VEC];
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        ds[v] = handed.get(v);
+#pragma unroll
+                        for (int j = 0; j <= m; ++j) ds[v] = fmaf(w[v * W + j], dz[m - j][v], ds[v]);
+                    }
+                    Held<IO, VEC> out;
+                    out.put(ds);
+                    out.store(d_state + (p.b * H + m) * a.D + p.d);
+                }
+            }
+        };
+        // nowhere in the wave the end of a row: neither what is beyond it nor what is handed on
+        if (__all(live == R + H)) all(std::true_type{});
+        else all(std::false_type{});
+    } else if (p.mine) {
+        Held<IO, VEC> none;
+        none.clear();
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (r >= live) {
-                x[W - 1 + r].clear();
-                gy[r].clear();
+            if (p.t0 + r < a.T) none.store(d_x + r * a.D);
+        if (p.t0 == 0 && d_state != nullptr) {           // a row without steps hands its state on
+#pragma unroll
+            for (int m = 0; m < H; ++m) {
+                Held<IO, VEC> handed;
+                handed.clear();
+                if (g_last != nullptr) handed.load(g_last + (p.b * H + m) * a.D + p.d);
+                handed.store(d_state + (p.b * H + m) * a.D + p.d);
             }
-        // the tile has some of the last inputs, whose gradient comes in as they are handed on
-        const bool near = g_last != nullptr && t0 + R > length && t0 < length + W - 1;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float dx[VEC];
-            const int64_t t = t0 + r - (W - 1);
-            Held<IO, VEC> handed;
-            handed.clear();
-            if (near && t0 + r >= length && t0 + r - length < W - 1) handed.load(g_last + (p.b * (W - 1) + t0 + r - length) * a.D + p.d);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                float dz = gy[r].get(v);
-                if (a.silu) {
-                    float z = bias[v];
-#pragma unroll
-                    for (int j = 0; j < W; ++j) z = fmaf(w[v * W + j], x[r + j].get(v), z);
-                    dz = dz * silu_slope(z, sigmoid_of<FAST>(z));
-                }
-                if (r >= live) dz = 0.0f;
-                const float counted = r < own ? dz : 0.0f;
-#pragma unroll
-                for (int j = 0; j < W; ++j) sums[v][j] = fmaf(counted, x[r + j].get(v), sums[v][j]);
-                sums[v][W] += counted;
-                float d = fmaf(w[v * W], dz, handed.get(v));
-#pragma unroll
-                for (int j = 1; j < W; ++j) d = fmaf(w[v * W + j], before[W - 1 - j][v], d);
-                dx[v] = t < length ? d : 0.0f;
-#pragma unroll
-                for (int j = 0; j < W - 2; ++j) before[j][v] = before[j + 1][v];
-                before[W - 2][v] = dz;
-            }
-            Held<IO, VEC> out;
-            out.put(dx);
-            if (t >= p.t0 && t < end) out.store(static_cast<IO *>(a.d_x) + (p.b * a.T + t) * a.D + p.d);
-            if (t < 0 && a.d_state != nullptr) out.store(static_cast<IO *>(a.d_state) + (p.b * (W - 1) + t + W - 1) * a.D + p.d);
         }
     }
-    // lanes of the same channels in a wave, then the waves
+    // Lanes of the same channels in a wave, then the waves.  Over the four rows of 16 lanes the values are spread while they are added.
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v)
-#pragma unroll
-        for (int j = 0; j <= W; ++j) {
-            float s = sums[v][j];
-            for (uint32_t m = g.lanes; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
-            if (lane < (int)g.lanes) shares[wave][lane * SUMS + v * (W + 1) + j] = s;
-        }
+    for (int i = 0; i < SUMS / 4; ++i) {
+        float s = over_rows(over_halves(sums[i], sums[i + SUMS / 2]), over_halves(sums[i + SUMS / 4], sums[i + SUMS / 4 * 3]));
+        for (uint32_t m = g.lanes; m < LANES; m <<= 1) s += __shfl_xor(s, m, 64);
+        if (lane % LANES < (int)g.lanes) shares[wave][i + lane / 16 % 2 * (SUMS / 4) + lane / 32 * (SUMS / 2)][lane % LANES] = s;
+    }
     __syncthreads();
     const uint32_t block = blockIdx.x % g.blocks, group = blockIdx.x / g.blocks;
-    for (int i = threadIdx.x; i < (int)g.lanes * SUMS; i += THREADS) {
-        const int64_t slot = (int64_t)block * g.lanes + i / SUMS, d = slot * VEC + VEC <= a.D ? slot * VEC : a.D - VEC;
+    constexpr int EACH = VEC * (W + 1);
+    for (int i = threadIdx.x; i < (int)g.lanes * EACH; i += THREADS) {
+        const int at = i % EACH, of = i / EACH;
+        const int64_t slot = (int64_t)block * g.lanes + of, d = slot * VEC + VEC <= a.D ? slot * VEC : a.D - VEC;
         if (slot >= g.per_row) break;
-        a.partials[((int64_t)group * a.D + d) * (W + 1) + i % SUMS] = ((shares[0][i] + shares[1][i]) + shares[2][i]) + shares[3][i];
+        a.partials[((int64_t)group * a.D + d) * (W + 1) + at] = ((shares[0][at][of] + shares[1][at][of]) + shares[2][at][of]) + shares[3][at][of];
     }
 }
 
@@ -344,15 +392,7 @@ ConvGrid grid_of(int64_t B, int64_t T, int64_t D, int vec, int64_t steps) {
     g.groups = g.fits ? (uint32_t)((B * stretches + TG - 1) / TG) : 0;
     return g;
 }
-// Tiles of a lane in the backward: as many as leave two workgroups for every CU, since the W - 1 steps after a stretch are done again
-ConvGrid backward_grid(int64_t B, int64_t T, int64_t D, int vec, int taps, bool wide) {
-    const int R = back_steps(taps, wide), least = 16 / R;
-    for (int tiles = 128 / R; tiles > least; tiles /= 2) {
-        const ConvGrid g = grid_of(B, T, D, vec, tiles * R - (taps - 1));
-        if (!g.fits || (int64_t)g.blocks * g.groups >= 512) return g;
-    }
-    return grid_of(B, T, D, vec, least * R - (taps - 1));
-}
+ConvGrid backward_grid(int64_t B, int64_t T, int64_t D, int vec, int taps, bool wide) { return grid_of(B, T, D, vec, back_steps(taps, wide)); }
 // Channels of a lane: 16 bytes of them forward, four backward, where eight would take the registers of all waves but one
 int vec_of(int64_t D, int dtype) {
     const int vec = dtype == T2FW_F32 ? 4 : 8;
@@ -361,11 +401,13 @@ int vec_of(int64_t D, int dtype) {
 int backward_vec_of(int64_t D) { return D >= 4 ? 4 : 1; }
 
 template <typename IO, int VEC, int W> int launch_forward(const ConvArgs &a, const ConvGrid &g, hipStream_t stream) {
-    hipLaunchKernelGGL((conv_forward_kernel<IO, VEC, W>), dim3(g.blocks * g.groups), dim3(THREADS), 0, stream, a, g);
+    if (a.silu) hipLaunchKernelGGL((conv_forward_kernel<IO, VEC, W, true>), dim3(g.blocks * g.groups), dim3(THREADS), 0, stream, a, g);
+    else hipLaunchKernelGGL((conv_forward_kernel<IO, VEC, W, false>), dim3(g.blocks * g.groups), dim3(THREADS), 0, stream, a, g);
     return check_hip(hipGetLastError(), "conv_forward_kernel launch");
 }
 template <typename IO, int VEC, int W> int launch_backward(const ConvArgs &a, const ConvGrid &g, hipStream_t stream) {
-    hipLaunchKernelGGL((conv_backward_kernel<IO, VEC, W>), dim3(g.blocks * g.groups), dim3(THREADS), 0, stream, a, g);
+    if (a.silu) hipLaunchKernelGGL((conv_backward_kernel<IO, VEC, W, true>), dim3(g.blocks * g.groups), dim3(THREADS), 0, stream, a, g);
+    else hipLaunchKernelGGL((conv_backward_kernel<IO, VEC, W, false>), dim3(g.blocks * g.groups), dim3(THREADS), 0, stream, a, g);
     return check_hip(hipGetLastError(), "conv_backward_kernel launch");
 }
 template <typename IO, int VEC, int W> int launch_step(const ConvArgs &a, const ConvGrid &g, hipStream_t stream) {
