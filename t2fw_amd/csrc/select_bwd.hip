@@ -34,6 +34,13 @@ __device__ __forceinline__ float over_eights(float v0, float v1) {
     return threadIdx.x & 8 ? b : a;
 }
 
+// The value of the same lane of the other four in eight
+__device__ __forceinline__ float other_fours(float v) {
+    constexpr int SHL4 = 0x104, SHR4 = 0x114, EVEN = 0x5, ODD = 0xa;
+    const int i = __float_as_int(v), up = __builtin_amdgcn_update_dpp(0, i, SHL4, 0xf, EVEN, true);
+    return __int_as_float(__builtin_amdgcn_update_dpp(up, i, SHR4, 0xf, ODD, false));
+}
+
 // The sums over a wave's channels of a lane's four values for b and four for c, to the wave's place in shared memory
 template <int G> __device__ __forceinline__ void add_channels(float *to, const float (&for_b)[S], const float (&for_c)[S]) {
     constexpr int NP = G * S;
@@ -47,11 +54,12 @@ template <int G> __device__ __forceinline__ void add_channels(float *to, const f
         to[at] = p0;
         to[at + 1] = p1;
     } else {
+        // (lanes that hold the same sum write it to the same place: a choice of lanes would be a branch that no load is brought forward over)
         float v = over_eights(p0, p1);
-        if constexpr (G <= 4) v += dpp_move<DPP_ROW_SHL4>(v);
+        if constexpr (G <= 4) v += other_fours(v);
         if constexpr (G <= 2) v += dpp_move<DPP_QUAD_XOR2>(v);
         if constexpr (G <= 1) v += dpp_move<DPP_QUAD_XOR1>(v);
-        if ((lane & (7 & ~(G - 1))) == 0) to[at + (lane >> 3 & 1)] = v;
+        to[at + (lane >> 3 & 1)] = v;
     }
 }
 
@@ -114,17 +122,16 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, 
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
             const bool counts = p.mine && t0 + r * Q + p.ng % Q < p.live;
-            const auto one = length_of<true>(a, widen(dt.v[r]) + bias);
+            const auto one = length_of<true>(a, dt.get(r) + bias);
             length[r] = counts ? one.dt : 0.0f;
             slope[r] = counts ? one.slope : 0.0f;
-            xs[r] = counts ? widen(x.v[r]) : 0.0f;
-            gys[r] = counts ? widen(gy.v[r]) : 0.0f;
-            zs[r] = GATED && counts ? widen(gate.v[r]) : 0.0f;
+            xs[r] = counts ? x.get(r) : 0.0f;
+            gys[r] = counts ? gy.get(r) : 0.0f;
+            zs[r] = GATED && counts ? gate.get(r) : 0.0f;
         }
 #pragma unroll
         for (int s = 0; s < S; ++s) h0[s] = p.mine ? next_h[s] : 0.0f;
         __syncthreads();
-        if (k > 0) load(t0 - TILE);
         float decay[TILE][S], h[TILE][S], dy[ROUNDS], push[ROUNDS];
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
@@ -163,6 +170,8 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, 
 #pragma unroll
         for (int i = 0; i < ROUNDS; ++i) {
             const int r = ROUNDS - 1 - i;
+            // (when half of the decays and states are done with, whose registers it takes)
+            if (i == ROUNDS / 2) load(k > 0 ? t0 - TILE : t0);
             float by_input[Q], by_decay[Q];
             const auto step = [&](auto J) {
                 constexpr int j = decltype(J)::value;

@@ -41,15 +41,15 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS) 
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
             const bool counts = t0 + r * Q + p.ng % Q < p.live;
-            const float v = widen(x.v[r]), one = length_of<false>(a, widen(dt.v[r]) + bias).dt;
+            const float v = x.get(r), one = length_of<false>(a, dt.get(r) + bias).dt;
             length[r] = counts ? one : 0.0f;
             push[r] = counts ? one * v : 0.0f;
             add[r] = a.skip == nullptr ? 0.0f : skip * v;
             times[r] = 1.0f;
-            if constexpr (GATED) times[r] = silu_of<FAST>(widen(gate.v[r]));
+            if constexpr (GATED) times[r] = silu_of<FAST>(gate.get(r));
         }
         __syncthreads();
-        if (k + 1 < tiles) load(t0 + TILE);
+        load(k + 1 < tiles ? t0 + TILE : t0);
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
             float y[Q];
@@ -92,13 +92,26 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS) void select_
     float y = 0.0f, xv = 0.0f;
     if (mine) {
         float rate[S], h[S], bv[S], cv[S];
-        load_states(rate, a.a + d * a.N, n0, a.N);
-        load_states(h, a.s0 + (b * a.D + d) * a.N, n0, a.N);
         const IO *const br = static_cast<const IO *>(a.b) + b * a.b_b, *const cr = static_cast<const IO *>(a.c) + b * a.c_b;
+        // whole fours of states: one load each, at any address
+        const bool fours = a.N % S == 0;
+        if (fours && n0 < a.N) {
+            load_padded(rate, a.a + d * a.N + n0);
+            load_padded(h, a.s0 + (b * a.D + d) * a.N + n0);
+            const Vec<IO, S> bs = load_vec<IO, S>(br + n0), cs = load_vec<IO, S>(cr + n0);
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            bv[s] = n0 + s < a.N ? widen(br[n0 + s]) : 0.0f;
-            cv[s] = n0 + s < a.N ? widen(cr[n0 + s]) : 0.0f;
+            for (int s = 0; s < S; ++s) {
+                bv[s] = widen(bs.e[s]);
+                cv[s] = widen(cs.e[s]);
+            }
+        } else {
+            load_states(rate, a.a + d * a.N, n0, a.N);
+            load_states(h, a.s0 + (b * a.D + d) * a.N, n0, a.N);
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                bv[s] = n0 + s < a.N ? widen(br[n0 + s]) : 0.0f;
+                cv[s] = n0 + s < a.N ? widen(cr[n0 + s]) : 0.0f;
+            }
         }
         xv = widen(static_cast<const IO *>(a.x)[b * a.x_b + d]);
         const float l = length_of<false>(a, widen(static_cast<const IO *>(a.dt)[b * a.dt_b + d]) + (a.dt_bias == nullptr ? 0.0f : a.dt_bias[d])).dt;
@@ -108,7 +121,8 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS) void select_
             h[s] = fmaf(exp2_of(l * (rate[s] * LOG2E)), h[s], u * bv[s]);
             y = fmaf(cv[s], h[s], y);
         }
-        store_states(a.last + (b * a.D + d) * a.N, h, n0, a.N);
+        if (fours && n0 < a.N) store_padded(a.last + (b * a.D + d) * a.N + n0, h);
+        else store_states(a.last + (b * a.D + d) * a.N, h, n0, a.N);
     }
     y = group_sum(y, G);
     if (!mine || n0 != 0) return;

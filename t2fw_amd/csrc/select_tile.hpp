@@ -154,10 +154,12 @@ __device__ __forceinline__ Buffer buffer_of(const void *at, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(at), 0, (int)(uint32_t)n, 0x00027000);
 }
 __device__ __forceinline__ Buffer result_of(void *at, int64_t bytes) { return buffer_of(at, bytes < (int64_t)BEYOND ? bytes : (int64_t)BEYOND); }
-template <typename IO> __device__ __forceinline__ IO load_from(Buffer b, uint32_t lane, uint32_t offset) {
-    if constexpr (sizeof(IO) == 2) return __builtin_bit_cast(IO, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, lane, offset, 0));
-    else return __builtin_bit_cast(IO, __builtin_amdgcn_raw_buffer_load_b32(b, lane, offset, 0));
+// An element on its way, in 32 bits: two of 16 bits would be put into one register, as soon as they are asked for, which waits for them
+template <typename IO> __device__ __forceinline__ uint32_t load_from(Buffer b, uint32_t lane, uint32_t offset) {
+    if constexpr (sizeof(IO) == 2) return (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, lane, offset, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b32(b, lane, offset, 0);
 }
+template <typename IO> __device__ __forceinline__ float arrived(uint32_t v) { return element_of<IO>(&v, 0); }
 template <typename IO> __device__ __forceinline__ void store_to(Buffer b, uint32_t lane, uint32_t offset, IO v) {
     if constexpr (sizeof(IO) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), b, lane, offset, 0);
     else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), b, lane, offset, 0);
@@ -166,7 +168,8 @@ template <typename IO> __device__ __forceinline__ void store_to(Buffer b, uint32
 // What a tile needs of the arrays, on its way: a lane's steps of those per channel ...
 template <typename IO, int G> struct PerChannel {
     static constexpr int ROUNDS = TILE / share<G>();
-    IO v[ROUNDS];
+    uint32_t v[ROUNDS];
+    __device__ __forceinline__ float get(int r) const { return arrived<IO>(v[r]); }
     __device__ __forceinline__ void load(const void *base, int64_t row, int64_t step, const SelectArgs &a, const Place &p, int64_t t0) {
         const int64_t first = (int64_t)p.block * (THREADS / G);
         const IO *const at = static_cast<const IO *>(base) + p.b * row + t0 * step + first;
@@ -179,7 +182,7 @@ template <typename IO, int G> struct PerChannel {
 // ... and elements of b or c, which go to shared memory
 template <typename IO, int G> struct PerStep {
     static constexpr int NP = G * S, EACH = (TILE * NP + THREADS - 1) / THREADS;
-    IO v[EACH];
+    uint32_t v[EACH];
     __device__ __forceinline__ void load(const void *base, int64_t row, int64_t step, const SelectArgs &a, const Place &p, int64_t t0) {
         const Buffer from = buffer_of(static_cast<const IO *>(base) + p.b * row + t0 * step, ((a.T - 1 - t0) * step + a.N) * (int64_t)sizeof(IO));
 #pragma unroll
@@ -193,7 +196,7 @@ template <typename IO, int G> struct PerStep {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int j = i * THREADS + threadIdx.x;
-            if (j < TILE * NP) to[j] = j % NP < a.N && t0 + j / NP < p.live ? widen(v[i]) : 0.0f;
+            if (j < TILE * NP) to[j] = j % NP < a.N && t0 + j / NP < p.live ? arrived<IO>(v[i]) : 0.0f;
         }
     }
 };
@@ -281,10 +284,10 @@ template <typename IO, int G, bool BACK> __global__ __launch_bounds__(THREADS) v
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r) {
             const bool counts = t0 + r * Q + p.ng % Q < p.live;
-            const float raw = widen(dt.v[r]) + bias, one = length_of<false>(a, raw).dt;
+            const float raw = dt.get(r) + bias, one = length_of<false>(a, raw).dt;
             length[r] = counts ? one : 0.0f;
-            float v = widen(in.v[r]);
-            if (BACK && a.gate != nullptr) v *= silu_of<FAST>(widen(gate.v[r]));
+            float v = in.get(r);
+            if (BACK && a.gate != nullptr) v *= silu_of<FAST>(gate.get(r));
             push[r] = counts ? (BACK ? v : one * v) : 0.0f;
             total += length[r];
         }
