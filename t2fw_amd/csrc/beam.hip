@@ -356,19 +356,19 @@ template <int K, typename Word> int launch_reorder(const ReorderTable &t, const 
 }  // namespace
 
 // Logits of a thread: 64 where there are workgroups enough all the same, as what a workgroup does for its n best takes as long as 30 of a thread's logits;
-// of few logits 8 (a request of 4 x 8000: PIECE_US)
-int beam_each(int64_t rows, int64_t V) {
+// of few logits 8 (4 x 8000 float32: 10 us with 32, 7 so)
+int beam_each(int64_t rows, int64_t V, int64_t n) {
     const auto pieces = [&](int each) { return (V + each * THREADS - 1) / (each * THREADS); };
-    if (rows * pieces(64) >= 512) return 64;
+    if (rows * pieces(64) >= 512 && n <= 96) return 64;            // (the list has to fit 64 KB of shared memory)
     return V <= 64 * THREADS && rows * pieces(32) < 256 ? 8 : 32;
 }
-BeamPieces beam_pieces(int64_t B, int64_t K, int64_t V) {
-    const int64_t most = (int64_t)beam_each(B * K, V) * THREADS, n = (V + most - 1) / most;
+BeamPieces beam_pieces(int64_t B, int64_t K, int64_t V, int64_t n_best) {
+    const int64_t most = (int64_t)beam_each(B * K, V, n_best) * THREADS, n = (V + most - 1) / most;
     return {(int32_t)n, (int32_t)(((V + n - 1) / n + 7) / 8 * 8)};       // of nearly equal size, and no more than `most`, which is whole eights
 }
 
 template <typename IO> int launch_pieces(const BeamArgs &a, unsigned groups, size_t held, hipStream_t stream) {
-    const int each = beam_each(a.B * a.K, a.V);
+    const int each = beam_each(a.B * a.K, a.V, a.n);
     const unsigned list = (unsigned)(each * held * sizeof(uint64_t));
     if (each == 64) hipLaunchKernelGGL((beam_piece_kernel<IO, 64>), dim3(groups), dim3(THREADS), list, stream, a);
     else if (each == 32) hipLaunchKernelGGL((beam_piece_kernel<IO, 32>), dim3(groups), dim3(THREADS), list, stream, a);

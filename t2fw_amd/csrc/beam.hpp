@@ -22,7 +22,7 @@ struct BeamArgs {
 struct BeamPieces {
     int32_t pieces, piece;
 };
-BeamPieces beam_pieces(int64_t B, int64_t K, int64_t V);
+BeamPieces beam_pieces(int64_t B, int64_t K, int64_t V, int64_t n);
 int beam_select(const BeamArgs &a, int dtype, hipStream_t stream);
 
 constexpr int REORDER_TABLE = 96;       // arrays of a launch

@@ -79,7 +79,7 @@ struct BeamLayout {
 };
 BeamLayout beam_layout(int64_t B, int64_t K, int64_t V, int64_t n) {
     BeamLayout l;
-    l.cut = beam_pieces(B, K, V);
+    l.cut = beam_pieces(B, K, V, n);
     l.shares = B * K * l.cut.pieces * 16;
     l.bytes = (size_t)(l.shares + B * K * l.cut.pieces * n * 8);
     return l;

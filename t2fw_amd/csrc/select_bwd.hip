@@ -258,6 +258,8 @@ __global__ __launch_bounds__(THREADS) void select_weights_kernel(SelectArgs a, i
 template <typename IO, int G> int launch_backward(const SelectArgs &a, const Grid &g, hipStream_t stream) {
     constexpr int NP = G * S;
     const unsigned row = (unsigned)(g.blocks * a.B);
+    const int64_t n = a.B * a.T * 2 * NP, groups = (n + THREADS - 1) / THREADS, columns = (a.D * (NP + 2) + 63) / 64;
+    if (groups > MOST_GROUPS || columns > MOST_GROUPS) return too_many();
     int rc;
     if (row > 0) {
         if (g.chunks > 1) {
@@ -268,8 +270,6 @@ template <typename IO, int G> int launch_backward(const SelectArgs &a, const Gri
         else hipLaunchKernelGGL((select_backward_kernel<IO, G, false>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
         if ((rc = check_hip(hipGetLastError(), "select_backward_kernel launch"))) return rc;
     }
-    const int64_t n = a.B * a.T * 2 * NP, groups = (n + THREADS - 1) / THREADS, columns = (a.D * (NP + 2) + 63) / 64;
-    if (groups > MOST_GROUPS || columns > MOST_GROUPS) return too_many();
     if (n > 0) {
         hipLaunchKernelGGL((select_steps_kernel<IO>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a, g.blocks, NP, n);
         if ((rc = check_hip(hipGetLastError(), "select_steps_kernel launch"))) return rc;

@@ -118,7 +118,7 @@ template <typename IO, int G> __global__ __launch_bounds__(THREADS) void select_
         const float u = l * xv;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            h[s] = fmaf(exp2_of(l * (rate[s] * LOG2E)), h[s], u * bv[s]);
+            h[s] = fmaf(exp2_of(l * rate_of(rate[s])), h[s], u * bv[s]);
             y = fmaf(cv[s], h[s], y);
         }
         if (fours && n0 < a.N) store_padded(a.last + (b * a.D + d) * a.N + n0, h);

@@ -135,11 +135,16 @@ __device__ __forceinline__ void load_padded(float (&v)[S], const float *at) {
 }
 __device__ __forceinline__ void store_padded(float *at, const float (&v)[S]) { store_vec(at, Vec<float, S>{{v[0], v[1], v[2], v[3]}}); }
 
-// The decays' exponents per unit of step, for the hardware's exponential, which is that of two
+// The decays' exponents per unit of step, for the hardware's exponential, which is that of two.  Finite, so that a step of no length (one that does not
+// count) leaves every state as it is.
+__device__ __forceinline__ float rate_of(float a) {
+    const float r = a * LOG2E;
+    return r < -3.4028234e38f ? -3.4028234e38f : r;
+}
 __device__ __forceinline__ void load_rates(float (&v)[S], const SelectArgs &a, const Place &p) {
     load_states(v, a.a + p.d * a.N, p.n0, a.N);
 #pragma unroll
-    for (int s = 0; s < S; ++s) v[s] *= LOG2E;
+    for (int s = 0; s < S; ++s) v[s] = rate_of(v[s]);
 }
 
 // Arrays through buffer descriptors: a scalar address for the tile, a lane's offset that stays as it is, and a scalar one for the round.  What is beyond the

@@ -9,7 +9,7 @@ def short_conv(x, weight, bias=None, state=None, lengths=None, silu=False):
     [B, taps - 1, D])``, with gradients.
 
     ``x: [B, T, D]`` (float32, float16 or bfloat16), with its channels next to each other in memory and any strides between rows and steps.
-    ``weight: [D, taps]`` with 2 to 8 taps and ``bias: [D]`` have the type of ``x`` or float32.  ``state: [B, taps - 1, D]``: the inputs before the
+    ``weight: [D, taps]`` with 2 to 8 taps (``weight[:, 0]`` of a depthwise ``Conv1d``) and ``bias: [D]`` have the type of ``x`` or float32.  ``state: [B, taps - 1, D]``: the inputs before the
     first, oldest first (``None``: zeros), of the type of ``x``, as are the last inputs: what the next call takes as its state.  Sums are float32;
     those of the weights' gradient over rows and steps are made in a fixed order.
 

@@ -15,7 +15,8 @@ def selective_scan(x, dt, a, b, c, state=None, skip=None, gate=None, dt_bias=Non
     ``dt``; ``softplus=True``: the step's length is ``log(1 + exp(dt + dt_bias))``, and the gradient that comes back is that of ``dt``.
 
     The decays over the steps of a row are put together by ``exp(a * sum of dt)``, which has to stay finite: where ``dt * a <= 0``, as it
-    is meant, it always does.  States and sums are float32; sums over channels and rows are made in a fixed order.
+    is meant, it always does.  Next to an infinite state or input such a product that is too small for float32 makes NaN, where the recurrence step by step
+    would stay infinite.  States and sums are float32; sums over channels and rows are made in a fixed order.
 
     ``lengths: [B]`` (int32 or int64, on the device), for rows that are padded at their end: steps from ``lengths[b]`` on do not count, whatever
     they hold, NaN included.  Their outputs and gradients are zero, and the last state of the row is that after its last step."""

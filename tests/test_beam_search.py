@@ -52,7 +52,7 @@ def logits_of(B, K, V, dtype, seed, std=3.0):
 
 # logits of one, of fewer than candidates, of less and more than a vector, a piece and several; beams of one, odd, many
 SHAPES = [(1, 1, 1, 1), (2, 3, 2, 6), (1, 4, 8000, 8), (3, 1, 100, 100), (2, 5, 257, 7), (4, 2, 8192, 4), (1, 3, 8193, 6), (2, 8, 50257, 16), (1, 16, 20000, 32),
-          (3, 64, 130, 128), (64, 8, 16389, 16), (30, 8, 40000, 20), (1, 200, 40, 20), (2, 2, 131072, 128), (70, 4, 60, 8)]
+          (3, 64, 130, 128), (64, 8, 16389, 16), (8, 64, 8300, 128), (16, 40, 5000, 96), (30, 8, 40000, 20), (1, 200, 40, 20), (2, 2, 131072, 128), (70, 4, 60, 8)]
 
 
 @pytest.mark.gpu

@@ -307,6 +307,22 @@ def test_long_steps_and_large_numbers():
 
 
 @pytest.mark.gpu
+def test_states_that_forget_at_once_and_steps_that_do_not_count():
+    """a decay rate of minus infinity: what is before a step is gone; steps beyond a row's length leave the state all the same"""
+    import t2fw_amd as t2
+    p, gy, gs = inputs(2, 40, 16, 4, torch.float32, seed=6)
+    p["a"][:, 1] = -float("inf")
+    lengths = torch.tensor([40, 13], device="cuda")
+    out = run(p, lengths, True, gy, gs)
+    assert all(bool(torch.isfinite(v).all()) for v in out.values())
+    dt = torch.nn.functional.softplus(p["dt"][:, :, :] + p["dt_bias"])
+    at = torch.tensor([39, 12], device="cuda")
+    row = torch.arange(2, device="cuda")
+    want = dt[row, at] * p["x"][row, at] * p["b"][row, at, 1:2]
+    assert bool(((out["last"][..., 1] - want).abs() <= 2.0 ** -19 * want.abs()).all())
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """Directional differences of the float64 sum at distance 1e-5: off by h^2 / 6 of the third derivative and by rounding, 1e-7 of the terms here;
     the gradients' own errors are the bounds above, summed along the direction"""
@@ -349,8 +365,7 @@ def test_on_another_stream_and_captured():
         out = t2.selective_scan(*[leaves[n] for n in NAMES[:5]], softplus=True, **{n: leaves[n] for n in NAMES[5:]})
         return out + torch.autograd.grad(out, [leaves[n] for n in NAMES], (gy, gs))
     with torch.cuda.stream(side):
-        eager = step()
-        step()
+        eager = [t.detach() for t in step()]
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     want = run(p, None, True, gy, gs)
