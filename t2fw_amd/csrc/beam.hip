@@ -107,6 +107,18 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
     const int64_t begin = (int64_t)piece * a.piece;
     const int here = a.V - begin < a.piece ? (int)(a.V - begin) : a.piece;
     const IO *const z = static_cast<const IO *>(a.logits) + row * a.V + begin;
+    uint64_t *const to = a.lists + (int64_t)blockIdx.x * a.n;
+    const bool ended = a.finished != nullptr && a.finished[row] != 0;
+    if (ended || !(a.scores[row] > -INFINITY)) {
+        // an ended beam has one candidate, the token for that, one that cannot be has none: then the others by their index
+        const int pad = ended && a.pad >= begin && a.pad < begin + here ? (int)(a.pad - begin) : -1;
+        for (int j = threadIdx.x; j < a.n; j += THREADS) {
+            const int at = pad < 0 ? j : j == 0 ? pad : j <= pad ? j - 1 : j;
+            to[j] = at < here ? packed(at == pad ? 0.0f : -INFINITY, (uint32_t)(begin + at)) : 0;
+        }
+        if (threadIdx.x == 0) static_cast<Share *>(a.partial)[blockIdx.x] = {-INFINITY, 0, 0.0};
+        return;
+    }
     // all loads at once, of what is not there of the first logits; the last vector of the piece, where it is no whole one, by its elements
     Vec<IO, VEC> raw[VECS];
     if (here >= VEC) {
@@ -128,15 +140,6 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
         if (at < here && at + VEC > here) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[i * VEC + e] = at + e < here ? widen(z[at + e]) : -INFINITY;
-        }
-    }
-    const bool ended = a.finished != nullptr && a.finished[row] != 0, never = !(a.scores[row] > -INFINITY);
-    if (ended || never) {
-        // an ended beam has one candidate, the token for that; one that cannot be has none
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int at = (i / VEC * THREADS + threadIdx.x) * VEC + i % VEC;
-            v[i] = ended && begin + at == a.pad ? 0.0f : -INFINITY;
         }
     }
     if (threadIdx.x == 0) found = 0;
@@ -162,24 +165,22 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
     }
     const double all = over_group((double)sum, sums, [](double x, double y) { return x + y; });
     if (threadIdx.x == 0) static_cast<Share *>(a.partial)[blockIdx.x] = {top, 0, all};
+    // Logits of minus infinity and NaN stay out of it: where there are fewer others than wanted, the first of them follow by their index.  (Threads
+    // that hold nothing are told apart by small numbers.)
     const int mine_at = (mine_i / VEC * THREADS + threadIdx.x) * VEC + mine_i % VEC;
-    // (threads that hold nothing are told apart by small numbers)
-    const uint64_t mine = mine_at < here ? packed(mine_z, (uint32_t)(begin + mine_at)) : THREADS - threadIdx.x;
+    const uint64_t mine = mine_z > -INFINITY ? packed(mine_z, (uint32_t)(begin + mine_at)) : THREADS - threadIdx.x;
     const auto more = [](uint64_t x, uint64_t y) { return x > y; };
-    uint64_t limit = nth_best(of_group(mine, a.n, more), best, least, a.n, more);
-    if (limit <= THREADS) limit = THREADS + 1;
-    if (mine >= limit) {
-        const float limit_z = logit_of(limit);
+    const uint64_t limit = nth_best(of_group(mine, a.n, more), best, least, a.n, more);
+    if (mine > THREADS && mine >= limit) {
+        const float limit_z = limit > THREADS ? logit_of(limit) : -INFINITY;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            if (v[i] < limit_z) continue;                // (NaN is not: it counts as the lowest)
-            const int at = (i / VEC * THREADS + threadIdx.x) * VEC + i % VEC;
-            const uint64_t k = at < here ? packed(v[i], (uint32_t)(begin + at)) : 0;
+            if (!(v[i] >= limit_z && v[i] > -INFINITY)) continue;
+            const uint64_t k = packed(v[i], (uint32_t)(begin + (i / VEC * THREADS + threadIdx.x) * VEC + i % VEC));
             if (k >= limit) list[atomicAdd(&found, 1)] = k;
         }
     }
     __syncthreads();
-    uint64_t *const to = a.lists + (int64_t)blockIdx.x * a.n;
     const int m = found;
     for (int j = threadIdx.x; j < m; j += THREADS) {
         const uint64_t k = list[j];
@@ -188,7 +189,17 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
         for (int i = 0; i < m; ++i) place += list[i] > k;
         if (place < a.n) to[place] = k;
     }
-    for (int j = m + threadIdx.x; j < a.n; j += THREADS) to[j] = 0;      // fewer logits than that
+    if (m >= a.n) return;
+    // fewer than n others: of the first 2 n tokens at least n - m are none of them
+    for (int j = threadIdx.x; j < 2 * a.n; j += THREADS) {
+        int place = m + j;
+        for (int i = 0; i < m; ++i) {
+            const uint32_t t = token_of(list[i]) - (uint32_t)begin;
+            place = t == (uint32_t)j ? a.n : place - (t < (uint32_t)j);      // (it has its place, which is below m)
+            if (t == (uint32_t)j) break;
+        }
+        if (place < a.n) to[place] = j < here ? packed(-INFINITY, (uint32_t)(begin + j)) : 0;
+    }
 }
 
 // A request: the n best of its lists, in rounds of ROUND candidates, each with the n best so far

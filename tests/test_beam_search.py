@@ -345,3 +345,22 @@ def test_c_abi_refusals():
     assert move(B=0) == 0 and move(count=0) == 0
     assert move(d=(_lib.ReorderDesc * 1)(_lib.ReorderDesc(None, p, 64))) == 1 and move(d=(_lib.ReorderDesc * 1)(_lib.ReorderDesc(p, p, -1))) == 3
     assert move(B=1 << 30, d=(_lib.ReorderDesc * 1)(_lib.ReorderDesc(p, p, 1 << 20))) == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n", [1, 5, 16, 40, 128])
+def test_few_tokens_that_are_allowed(n, dtype):
+    """fewer than candidates, in one piece or several, among the first tokens or the last: those that cannot be follow by their index"""
+    for V in (300, 9000, 40000):
+        logits, scores = logits_of(3, 2, V, dtype, V + n)
+        allowed = torch.zeros(3, 2, V, dtype=torch.bool, device="cuda")
+        g = torch.Generator(device="cuda").manual_seed(n)
+        for b, k, count, top in ((0, 0, n // 2, V), (0, 1, 1, 20), (1, 0, n + 3, V), (1, 1, n, min(V, 2 * n + 5)), (2, 0, 3, 8), (2, 1, 0, 1)):
+            allowed[b, k, torch.randperm(top, generator=g, device="cuda")[:count]] = True
+        for seed in range(100):
+            logits, scores = logits_of(3, 2, V, dtype, seed)
+            logits = logits.masked_fill(~allowed, float("-inf"))
+            if apart(reference(logits, scores, min(n + 1, 2 * V))[0]):
+                break
+        check(logits, scores, n)
