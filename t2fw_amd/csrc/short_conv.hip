@@ -5,7 +5,7 @@
 // from the cache for the lane that has the next steps.  A workgroup has 16 such lanes side by side (256 bytes of a step) and 16 stretches in time.
 // Backward dx_p = sum_j w_j dz_{p+W-1-j} needs dz of the W - 1 steps after a lane's own too, which it makes again from x and the gradient: as many
 // loads at once as there are, and no loop whose loads wait for the stores of the one before (stretches of 13 to 125 steps, dz handed on in registers: 41 us
-// for 8 x 1024 x 1536 bf16, now 34).  The weights' gradients are summed in registers, over the stretches of a workgroup in
+// for 8 x 1024 x 1536 bf16, now 26).  The weights' gradients are summed in registers, over the stretches of a workgroup in
 // shared memory, and over workgroups by a second launch: in a fixed order.
 #include <type_traits>
 #include "short_conv.hpp"
@@ -17,12 +17,12 @@ namespace {
 
 constexpr int THREADS = 256, R = 8;                              // R: steps of a lane
 // ... backward: four where eight do not fit the registers of two waves
-constexpr int back_steps(int taps, bool wide) { return taps + (wide ? 2 : 0) > 6 ? 4 : 8; }
+constexpr int back_steps(int taps, bool wide) { return taps + (wide ? 3 : 0) > 5 ? 4 : 8; }
 constexpr int64_t MOST_GROUPS = (1ll << 32) / THREADS - 1;      // a grid has less than 2^32 threads along an axis
 
-// Lanes side by side, workgroups side by side, stretches of a row, steps of one, workgroups one after another
+// Lanes side by side, workgroups side by side, stretches of a row, steps of one, workgroups one after another, rounds of stretches of one
 struct ConvGrid {
-    uint32_t lanes, per_row, blocks, stretches, steps, groups;
+    uint32_t lanes, per_row, blocks, stretches, steps, groups, rounds;
     bool fits;
 };
 
@@ -68,11 +68,11 @@ struct Place {
     int64_t d, q, b, t0;
     bool mine;
 };
-template <int VEC> __device__ __forceinline__ Place place_of(const ConvArgs &a, const ConvGrid &g) {
+template <int VEC> __device__ __forceinline__ Place place_of(const ConvArgs &a, const ConvGrid &g, uint32_t round = 0) {
     Place p;
     const uint32_t block = blockIdx.x % g.blocks, group = blockIdx.x / g.blocks, lane = threadIdx.x % g.lanes;
     const uint32_t slot = block * g.lanes + lane;
-    p.q = (int64_t)group * (THREADS / g.lanes) + threadIdx.x / g.lanes;
+    p.q = ((int64_t)group * g.rounds + round) * (THREADS / g.lanes) + threadIdx.x / g.lanes;
     p.mine = slot < g.per_row && p.q < a.B * (int64_t)g.stretches;
     if (!p.mine) p.q = 0;
     p.b = (uint32_t)p.q / g.stretches;
@@ -167,127 +167,147 @@ template <typename IO, int VEC, int W, bool SILU> __global__ __launch_bounds__(T
     constexpr bool FAST = sizeof(IO) == 2;
     constexpr int SUMS = (VEC * (W + 1) + 3) / 4 * 4, LANES = 16, R = back_steps(W, sizeof(IO) == 4), H = W - 1;
     __shared__ float shares[THREADS / 64][SUMS][LANES];
-    const Place p = place_of<VEC>(a, g);
-    const int64_t length = p.mine ? row_length(a, p.b) : 0;
     float sums[SUMS];                                    // of the weights and the bias of each channel
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) sums[i] = 0.0f;
-    IO *const d_x = static_cast<IO *>(a.d_x) + (p.b * a.T + p.t0) * a.D + p.d, *const d_state = static_cast<IO *>(a.d_state);
-    const IO *const g_last = static_cast<const IO *>(a.g_last);
-    if (p.mine && p.t0 < length) {
-        const IO *xs = static_cast<const IO *>(a.x) + p.b * a.x_b + p.t0 * a.x_t + p.d, *gs = static_cast<const IO *>(a.g_y) + p.b * a.g_b + p.t0 * a.g_t + p.d;
-        // steps t0 - H .. t0 + R + H of x, t0 .. t0 + R + H of the gradient
-        Held<IO, VEC> x[R + 2 * H], gy[R + H];
-        if (p.t0 >= H) {
-            const IO *at = xs - H * a.x_t;
-#pragma unroll
-            for (int i = 0; i < H; ++i) x[i].load(at + i * a.x_t);
-        } else {
-#pragma unroll
-            for (int i = 0; i < H; ++i) {
-                const int64_t t = p.t0 - H + i;
-                x[i].clear();
-                if (t >= 0) x[i].load(xs + (i - H) * a.x_t);
-                else if (a.state != nullptr) x[i].load(static_cast<const IO *>(a.state) + (p.b * H + t + H) * a.D + p.d);
-            }
-        }
-        const int there = a.T - p.t0 < R + H ? (int)(a.T - p.t0) : R + H, live = length - p.t0 < R + H ? (int)(length - p.t0) : R + H;
-#pragma unroll
-        for (int i = 0; i < R + H; ++i) {
-            x[H + i].load(xs);
-            gy[i].load(gs);
-            xs += i + 1 < there ? a.x_t : 0;             // (of a step beyond the last one that again)
-            gs += i + 1 < there ? a.g_t : 0;
-        }
-        float w[VEC * W], bias[VEC];
+    float w[VEC * W], bias[VEC];
+    {
+        const Place p = place_of<VEC>(a, g);
         load_weights<IO, VEC, W>(w, a, p.d);
         load_bias<IO, VEC>(bias, a, p.d);
-        const auto all = [&](auto WHOLE) {
-            constexpr bool whole = decltype(WHOLE)::value;
-            // what steps beyond the row's length hold does not count, whatever it is
-            if constexpr (!whole) {
+    }
+    IO *const d_state = static_cast<IO *>(a.d_state);
+    const IO *const g_last = static_cast<const IO *>(a.g_last);
+    for (uint32_t round = 0; round < g.rounds; ++round) {
+        const Place p = place_of<VEC>(a, g, round);
+        const int64_t length = p.mine ? row_length(a, p.b) : 0;
+        IO *const d_x = static_cast<IO *>(a.d_x) + (p.b * a.T + p.t0) * a.D + p.d;
+        if (p.mine && p.t0 < length) {
+            const IO *xs = static_cast<const IO *>(a.x) + p.b * a.x_b + p.t0 * a.x_t + p.d, *gs = static_cast<const IO *>(a.g_y) + p.b * a.g_b + p.t0 * a.g_t + p.d;
+            // steps t0 - H .. t0 + R + H of x, t0 .. t0 + R + H of the gradient
+            Held<IO, VEC> x[R + 2 * H], gy[R + H];
+            if (p.t0 >= H) {
+                const IO *at = xs - H * a.x_t;
 #pragma unroll
-                for (int i = 0; i < R + H; ++i)
-                    if (i >= live) {
-                        x[H + i].clear();
-                        gy[i].clear();
-                    }
+                for (int i = 0; i < H; ++i) x[i].load(at + i * a.x_t);
+            } else {
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    const int64_t t = p.t0 - H + i;
+                    x[i].clear();
+                    if (t >= 0) x[i].load(xs + (i - H) * a.x_t);
+                    else if (a.state != nullptr) x[i].load(static_cast<const IO *>(a.state) + (p.b * H + t + H) * a.D + p.d);
+                }
             }
-            float dz[R + H][VEC];
+            const int there = a.T - p.t0 < R + H ? (int)(a.T - p.t0) : R + H, live = length - p.t0 < R + H ? (int)(length - p.t0) : R + H;
 #pragma unroll
             for (int i = 0; i < R + H; ++i) {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    float d = gy[i].get(v);
-                    if constexpr (SILU) {
-                        float z = bias[v];
-#pragma unroll
-                        for (int j = 0; j < W; ++j) z = fmaf(w[v * W + j], x[i + j].get(v), z);
-                        d = d * silu_slope(z, sigmoid_of<FAST>(z));
-                    }
-                    dz[i][v] = whole || i < live ? d : 0.0f;
-                    if (i < R) {                         // (the steps after the lane's own are others')
-#pragma unroll
-                        for (int j = 0; j < W; ++j) sums[v * (W + 1) + j] = fmaf(dz[i][v], x[i + j].get(v), sums[v * (W + 1) + j]);
-                        sums[v * (W + 1) + W] += dz[i][v];
-                    }
-                }
+                x[H + i].load(xs);
+                gy[i].load(gs);
+                xs += i + 1 < there ? a.x_t : 0;             // (of a step beyond the last one that again)
+                gs += i + 1 < there ? a.g_t : 0;
             }
+            const auto all = [&](auto WHOLE) {
+                constexpr bool whole = decltype(WHOLE)::value;
+                // what steps beyond the row's length hold does not count, whatever it is
+                if constexpr (!whole) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
+                    for (int i = 0; i < R + H; ++i)
+                        if (i >= live) {
+                            x[H + i].clear();
+                            gy[i].clear();
+                        }
+                }
                 // the gradient of the last inputs as they are handed on
-                const int64_t t = p.t0 + r, at = t - length + H;
-                Held<IO, VEC> handed;
-                handed.clear();
-                if (!whole && g_last != nullptr && at >= 0 && at < H) handed.load(g_last + (p.b * H + at) * a.D + p.d);
-                float dx[VEC];
+                Held<IO, VEC> handed[R];
+                if constexpr (!whole) {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    float d = whole ? 0.0f : handed.get(v);
+                    for (int r = 0; r < R; ++r) handed[r].clear();
+                    if (g_last != nullptr && p.t0 + R + H > length) {
+                        const int64_t first = p.t0 - length + H;
 #pragma unroll
-                    for (int j = 0; j < W; ++j) d = fmaf(w[v * W + j], dz[r + H - j][v], d);
-                    dx[v] = whole || t < length ? d : 0.0f;
+                        for (int r = 0; r < R; ++r) {
+                            const int64_t at = first + r;
+                            handed[r].load(g_last + (p.b * H + (at < 0 ? 0 : at < H ? at : H - 1)) * a.D + p.d);
+                            if (at < 0 || at >= H) handed[r].clear();
+                        }
+                    }
                 }
-                Held<IO, VEC> out;
-                out.put(dx);
-                if (whole || t < a.T) out.store(d_x + r * a.D);
-            }
-            if (p.t0 == 0 && d_state != nullptr) {
+                float dz[R + H][VEC];
 #pragma unroll
-                for (int m = 0; m < H; ++m) {
-                    const int64_t at = m - length;
-                    Held<IO, VEC> handed;
-                    handed.clear();
-                    if (g_last != nullptr && at >= 0) handed.load(g_last + (p.b * H + at) * a.D + p.d);
-                    float ds[VEC];
+                for (int i = 0; i < R + H; ++i) {
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
-                        ds[v] = handed.get(v);
+                        float d = gy[i].get(v);
+                        if constexpr (SILU) {
+                            float z = bias[v];
 #pragma unroll
-                        for (int j = 0; j <= m; ++j) ds[v] = fmaf(w[v * W + j], dz[m - j][v], ds[v]);
+                            for (int j = 0; j < W; ++j) z = fmaf(w[v * W + j], x[i + j].get(v), z);
+                            d = d * silu_slope(z, sigmoid_of<FAST>(z));
+                        }
+                        dz[i][v] = whole || i < live ? d : 0.0f;
+                        if (i < R) {                         // (the steps after the lane's own are others')
+#pragma unroll
+                            for (int j = 0; j < W; ++j) sums[v * (W + 1) + j] = fmaf(dz[i][v], x[i + j].get(v), sums[v * (W + 1) + j]);
+                            sums[v * (W + 1) + W] += dz[i][v];
+                        }
+                    }
+                    if (i < H) continue;
+                    // all that counts for the input of W - 1 steps before
+                    const int r = i - H;
+                    const int64_t t = p.t0 + r;
+                    float dx[VEC];
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        float d = 0.0f;
+                        if constexpr (!whole) d = handed[r].get(v);
+#pragma unroll
+                        for (int j = 0; j < W; ++j) d = fmaf(w[v * W + j], dz[i - j][v], d);
+                        dx[v] = whole || t < length ? d : 0.0f;
                     }
                     Held<IO, VEC> out;
-                    out.put(ds);
-                    out.store(d_state + (p.b * H + m) * a.D + p.d);
+                    out.put(dx);
+                    if (whole || t < a.T) out.store(d_x + r * a.D);
+                    // (one step after another: the registers of a step's numbers are free for the next one's)
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
-        };
-        // nowhere in the wave the end of a row: neither what is beyond it nor what is handed on
-        if (__all(live == R + H)) all(std::true_type{});
-        else all(std::false_type{});
-    } else if (p.mine) {
-        Held<IO, VEC> none;
-        none.clear();
+                if (p.t0 == 0 && d_state != nullptr) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (p.t0 + r < a.T) none.store(d_x + r * a.D);
-        if (p.t0 == 0 && d_state != nullptr) {           // a row without steps hands its state on
+                    for (int m = 0; m < H; ++m) {
+                        const int64_t at = m - length;
+                        Held<IO, VEC> handed;
+                        handed.clear();
+                        if (g_last != nullptr && at >= 0) handed.load(g_last + (p.b * H + at) * a.D + p.d);
+                        float ds[VEC];
 #pragma unroll
-            for (int m = 0; m < H; ++m) {
-                Held<IO, VEC> handed;
-                handed.clear();
-                if (g_last != nullptr) handed.load(g_last + (p.b * H + m) * a.D + p.d);
-                handed.store(d_state + (p.b * H + m) * a.D + p.d);
+                        for (int v = 0; v < VEC; ++v) {
+                            ds[v] = handed.get(v);
+#pragma unroll
+                            for (int j = 0; j <= m; ++j) ds[v] = fmaf(w[v * W + j], dz[m - j][v], ds[v]);
+                        }
+                        Held<IO, VEC> out;
+                        out.put(ds);
+                        out.store(d_state + (p.b * H + m) * a.D + p.d);
+                    }
+                }
+            };
+            // nowhere in the wave the end of a row: neither what is beyond it nor what is handed on
+            if (__all(live == R + H)) all(std::true_type{});
+            else all(std::false_type{});
+        } else if (p.mine) {
+            Held<IO, VEC> none;
+            none.clear();
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (p.t0 + r < a.T) none.store(d_x + r * a.D);
+            if (p.t0 == 0 && d_state != nullptr) {           // a row without steps hands its state on
+#pragma unroll
+                for (int m = 0; m < H; ++m) {
+                    Held<IO, VEC> handed;
+                    handed.clear();
+                    if (g_last != nullptr) handed.load(g_last + (p.b * H + m) * a.D + p.d);
+                    handed.store(d_state + (p.b * H + m) * a.D + p.d);
+                }
             }
         }
     }
@@ -377,7 +397,7 @@ template <typename IO, int VEC, int W> __global__ __launch_bounds__(THREADS) voi
     }
 }
 
-ConvGrid grid_of(int64_t B, int64_t T, int64_t D, int vec, int64_t steps) {
+ConvGrid grid_of(int64_t B, int64_t T, int64_t D, int vec, int64_t steps, bool rounds = false) {
     ConvGrid g{};
     const int64_t per_row = (D + vec - 1) / vec;
     g.lanes = 16;
@@ -390,9 +410,17 @@ ConvGrid grid_of(int64_t B, int64_t T, int64_t D, int vec, int64_t steps) {
     g.stretches = (uint32_t)stretches;
     g.steps = (uint32_t)steps;
     g.groups = g.fits ? (uint32_t)((B * stretches + TG - 1) / TG) : 0;
+    // Two workgroups for every CU, which load the weights and add their sums up once (backward, with the second launch: 8 x 1024 x 1536 bf16 34 us with a
+    // workgroup for every 16 stretches, 26 so; 32 x 1024 x 4096 292 and 214)
+    g.rounds = 1;
+    if (rounds && g.groups > 0) {
+        const int64_t n = blocks * g.groups / 512;
+        g.rounds = n < 1 ? 1 : n < 16 ? (uint32_t)n : 16;
+        g.groups = (g.groups + g.rounds - 1) / g.rounds;
+    }
     return g;
 }
-ConvGrid backward_grid(int64_t B, int64_t T, int64_t D, int vec, int taps, bool wide) { return grid_of(B, T, D, vec, back_steps(taps, wide)); }
+ConvGrid backward_grid(int64_t B, int64_t T, int64_t D, int vec, int taps, bool wide) { return grid_of(B, T, D, vec, back_steps(taps, wide), true); }
 // Channels of a lane: 16 bytes of them forward, four backward, where eight would take the registers of all waves but one
 int vec_of(int64_t D, int dtype) {
     const int vec = dtype == T2FW_F32 ? 4 : 8;
