@@ -150,7 +150,7 @@ __device__ __forceinline__ void load_rates(float (&v)[S], const SelectArgs &a, c
 // Arrays through buffer descriptors: a scalar address for the tile, a lane's offset that stays as it is, and a scalar one for the round.  What is beyond the
 // array is not loaded (zeros come) and not stored, so no branch stands between the accesses: with branches the compiler does not know
 // how many are under way, and waits for the stores of a tile where it needs loads from before them (backward of 32 x 512 x 1536 x 16 bf16: 664 us, so
-// 446).
+// 446; 412 with loads held as they come and no branch between the steps).
 typedef __amdgpu_buffer_rsrc_t Buffer;
 typedef uint32_t Four __attribute__((ext_vector_type(4)));
 constexpr uint32_t BEYOND = 0x80000000u;                 // an offset that is in no array
@@ -336,16 +336,16 @@ inline int lanes_of(int64_t N) {
     while (g * S < N) g *= 2;
     return g;
 }
-// Chunks: none where channels and rows alone make two workgroups for every CU (32 x 512 x 1536 x 16 bf16: forward 140 us, in two chunks 177; backward 446
-// and 490), else as many as make 1280 (8 x 1024 x 1536 x 16, forward and backward: 768 workgroups 122 and 266 us, 1024 113 and 260, 1536 113 and 252, 4096 118 and
-// 283), but no more than the root of the steps, as a chunk goes through the maps of all before it (1 x 16384 x 64 x 16: 64 chunks 77 and 146, 128 60 and 110, 256
-// 70 and 119; 1 x 131072 x 64 x 16: 128 chunks 314 and 529, 256 201 and 329).
+// Chunks: none where channels and rows alone make three workgroups for two CUs (T = 1024, D = 1536, N = 16 bf16, forward and step of training: 20 rows, 480
+// workgroups, 184 and 672 us, in two chunks 223 and 788; 16 rows 180 and 658, in four 182 and 638; 14 rows 179 and 655, in six 164 and 571), else as many as make
+// 1536 (8 rows 130 and 474 us, in four chunks 113 and 366, in eight 106 and 348), but no more than the root of the steps, as a chunk goes through the maps of
+// all before it (1 x 16384 x 64 x 16: 64 chunks 69 and 209 us, 128 57 and 161, 256 73 and 183; 1 x 131072 x 64 x 16: 128 chunks 233 and 726, 256 161 and 471).
 inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N) {
     Grid g{};
     const int64_t channels = THREADS / lanes_of(N), blocks = (D + channels - 1) / channels, tiles = T <= 0 ? 0 : (T + TILE - 1) / TILE;
     const long double rows = (long double)blocks * B;
     int64_t chunks = 1;
-    if (rows > 0 && rows < 512) chunks = (int64_t)((1280 + rows - 1) / rows);
+    if (rows > 0 && rows < 384) chunks = (int64_t)((1536 + rows - 1) / rows);
     while (chunks > 1 && (chunks * chunks > T || chunks > tiles)) --chunks;
     const int64_t each = tiles == 0 ? 1 : (tiles + chunks - 1) / chunks;
     g.steps = each * TILE;
