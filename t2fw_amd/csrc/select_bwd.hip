@@ -232,6 +232,7 @@ template <typename IO> __global__ __launch_bounds__(THREADS) void select_steps_k
     const int at = (int)(i - t * 2 * NP), s = at % NP;
     if (s >= a.N) return;
     float v = 0.0f;
+#pragma unroll 8
     for (uint32_t k = 0; k < blocks; ++k) v += a.bc[k * n + i];
     (at < NP ? static_cast<IO *>(a.d_b) : static_cast<IO *>(a.d_c))[t * a.N + s] = narrow<IO>(v);
 }
@@ -242,8 +243,10 @@ __global__ __launch_bounds__(THREADS) void select_weights_kernel(SelectArgs a, i
     const int64_t width = a.D * (NP + 2), i = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
     const int part = threadIdx.x / 64;
     float v = 0.0f;
-    if (i < width)
+    if (i < width) {
+#pragma unroll 8
         for (int64_t r = part; r < rows; r += THREADS / 64) v += a.sums[r * width + i];
+    }
     parts[part][threadIdx.x % 64] = v;
     __syncthreads();
     if (part != 0 || i >= width) return;

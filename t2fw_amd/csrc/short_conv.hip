@@ -341,8 +341,10 @@ template <typename IO> __global__ __launch_bounds__(THREADS) void conv_weights_k
     const int64_t width = a.D * (a.taps + 1), c = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
     const int part = threadIdx.x / 64;
     float s = 0.0f;
-    if (c < width)
+    if (c < width) {
+#pragma unroll 8
         for (int64_t r = part; r < rows; r += THREADS / 64) s += a.partials[r * width + c];
+    }
     parts[part][threadIdx.x % 64] = s;
     __syncthreads();
     if (part != 0 || c >= width) return;
