@@ -297,8 +297,9 @@ void check_select(const SelectInputs &i, int64_t axes) {
     lowp_code(i.x, "x");
     check_rows(i.x, i.x, "x");
     const auto like_x = [&](const Tensor &t, const char *name) {
-        check_rows(t, i.x, name);
+        check_on(t, i.x, name);
         check_sizes(t, i.x.sizes(), name);
+        check_rows(t, i.x, name);
         check_type(t, i.x.scalar_type(), name);
     };
     like_x(i.dt, "dt");

@@ -279,6 +279,9 @@ def bad_calls():
     return {
         "logits are flat": lambda: t2.beam_select(z(6, 8), s),
         "logits apart": lambda: t2.beam_select(z(2, 8, 3).transpose(1, 2), s),
+        "logits are a number": lambda: t2.beam_select(z(), s),
+        "scores are a number": lambda: t2.beam_select(x, z()),
+        "beams are a number": lambda: t2.reorder_beams([t], z(**i64)),
         "logits in 64 bits": lambda: t2.beam_select(x.double(), s),
         "no logits": lambda: t2.beam_select(z(2, 3, 0), s),
         "no beams": lambda: t2.beam_select(z(2, 0, 8), z(2, 0)),

@@ -398,6 +398,12 @@ def bad_calls():
         "x by steps": lambda: scan(x=z(2, 8, 5).transpose(1, 2)),
         "x in 64 bits": lambda: t2.selective_scan(x.double(), x.double(), a, b.double(), b.double()),
         "dt of another shape": lambda: scan(dt=z(2, 5, 7)),
+        "dt is a number": lambda: scan(dt=z()),
+        "gate is a number": lambda: scan(gate=z()),
+        "b is a number": lambda: scan(b=z()),
+        "a is a number": lambda: scan(a=z()),
+        "state is a number": lambda: scan(state=z()),
+        "x is a number": lambda: scan(x=z()),
         "dt of another type": lambda: scan(dt=x.half()),
         "b of another type": lambda: scan(b=b.half()),
         "b of other states": lambda: scan(b=z(2, 5, 3)),

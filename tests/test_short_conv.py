@@ -260,6 +260,10 @@ def bad_calls():
         "x has no channels": lambda: t2.short_conv(z(2, 5, 0), z(0, 4)),
         "x by steps": lambda: t2.short_conv(z(2, 8, 5).transpose(1, 2), w),
         "x in 64 bits": lambda: t2.short_conv(x.double(), w.double()),
+        "x is a number": lambda: t2.short_conv(z(), w),
+        "weight is a number": lambda: t2.short_conv(x, z()),
+        "bias is a number": lambda: t2.short_conv(x, w, z()),
+        "state is a number": lambda: t2.short_conv(x, w, state=z()),
         "one tap": lambda: t2.short_conv(x, z(8, 1)),
         "nine taps": lambda: t2.short_conv(x, z(8, 9)),
         "weight of other channels": lambda: t2.short_conv(x, z(7, 4)),
