@@ -8,7 +8,7 @@ def beam_select(logits, scores, count=None, finished=None, pad=0):
     """The ``count`` best continuations of each request over all its beams and the vocabulary; returns ``(scores [B, count] float32,
     beams [B, count] int64, tokens [B, count] int64)``, best first.
 
-    A continuation of beam ``k`` by token ``v`` has the score ``scores[k] + log_softmax(logits[k])[v]``.  ``logits: [B, K, V]`` float32, float16 or
+    A continuation of beam ``k`` by token ``v`` has the score ``scores[k] + log_softmax(logits[k])[v]``.  ``logits: [B, K, V]``, contiguous, float32, float16 or
     bfloat16, with up to 256 beams; ``scores: [B, K]`` float32; ``count`` is at most 128 (``None``: K).  The first step, when all beams are the same
     prompt: scores of zero for one of them and minus infinity for the others.
 

@@ -88,7 +88,7 @@ int check_beams(int64_t B, int64_t K, int64_t V, int64_t n, int32_t dtype) {
     int rc = check_lowp(dtype, "beam selection");
     if (rc || (rc = check_sizes({B, K, V, BEAM_COUNT}, "beam selection"))) return rc;
     if (K < 1 || K > BEAM_ROWS) return fail(T2FW_ERR_BAD_SHAPE, "beam selection: 1 to %d beams, not %lld", BEAM_ROWS, (long long)K);
-    if (V < 1 || K * V >= 0xffffffffll) return fail(T2FW_ERR_BAD_SHAPE, "beam selection: %lld x %lld candidates", (long long)K, (long long)V);
+    if (V < 1 || K * V > 0x7fffffff) return fail(T2FW_ERR_BAD_SHAPE, "beam selection: %lld x %lld candidates", (long long)K, (long long)V);
     if (n < 1 || n > BEAM_COUNT) return fail(T2FW_ERR_BAD_SHAPE, "beam selection: 1 to %d candidates, not %lld", BEAM_COUNT, (long long)n);
     if (n > K * V) return fail(T2FW_ERR_BAD_SHAPE, "beam selection: %lld of %lld candidates", (long long)n, (long long)(K * V));
     return T2FW_OK;

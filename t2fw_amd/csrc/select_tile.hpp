@@ -351,14 +351,15 @@ inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N) {
     g.steps = each * TILE;
     g.chunks = (uint32_t)(tiles == 0 ? 1 : (tiles + each - 1) / each);
     g.blocks = (uint32_t)blocks;
-    g.fits = D * 16 * S < (1ll << 27) && B < 0x7fffffff && tiles < 0x7fffffff && rows * g.chunks < MOST_GROUPS;
+    g.fits = D < (1 << 21) &&      // (a step of the checkpoints is addressed by 32 bits)
+             B < 0x7fffffff && tiles < 0x7fffffff && rows * g.chunks < MOST_GROUPS;
     g.tiles = (uint32_t)tiles;
     return g;
 }
 inline size_t maps_bytes(const Grid &g, int64_t B, int64_t D, int64_t N) {
     return g.chunks == 1 ? 0 : (size_t)g.chunks * B * D * (lanes_of(N) * S + 1) * sizeof(float);
 }
-inline int too_many() { return fail(T2FW_ERR_BAD_SHAPE, "selective scan: too many workgroups for one launch"); }
+inline int too_many() { return fail(T2FW_ERR_BAD_SHAPE, "selective scan: too many channels, or workgroups for one launch"); }
 
 #define SELECT_LANES(what, IO, lanes, ...)                                  \
     switch (lanes) {                                                        \

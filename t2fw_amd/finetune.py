@@ -218,8 +218,8 @@ def rewards(tokens, vocab):
     return (tokens < vocab // 2).float()
 
 
-def finetune(rounds=10, batch=64, prompt=16, answer=48, vocab=512, width=128, layers=4, steps=2, eight_bit=False, seed=0, selective=False, beams=0,
-             say=print):
+def finetune(rounds=10, batch=64, prompt=16, answer=48, vocab=512, width=128, layers=4, steps=2, eight_bit=False, seed=0, say=print,
+             selective=False, beams=0):
     """The mean reward of each round's answers; with ``beams``, of the best ones that a beam search finds at the end too"""
     model = RecurrentLM(vocab, width, layers, seed=seed, selective=selective).cuda()
     trainer = PolicyTrainer(model)
