@@ -214,3 +214,93 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for w, g in zip(want, got):
             assert all(torch.equal(p, q) for p, q in zip(w, g))
+
+
+class Frame:
+    """arrays with a margin on either side, of NaN (inputs) or of a number that has to stay (results)"""
+    MARGIN = 4096
+
+    def __init__(self):
+        self.kept = []
+
+    def given(self, t):
+        whole = torch.full((t.numel() + 2 * self.MARGIN,), float("nan"), dtype=t.dtype, device="cuda")
+        part = whole[self.MARGIN:self.MARGIN + t.numel()].view(t.shape)
+        part.copy_(t)
+        return part
+
+    def result(self, *shape, dtype=torch.float32):
+        n = torch.Size(shape).numel()
+        whole = torch.full((n + 2 * self.MARGIN,), 77.0, dtype=dtype, device="cuda")
+        self.kept.append((whole, n))
+        return whole[self.MARGIN:self.MARGIN + n].view(shape)
+
+    def check(self):
+        for whole, n in self.kept:
+            assert bool((whole[:self.MARGIN] == 77).all()) and bool((whole[self.MARGIN + n:] == 77).all()), (n, whole.dtype)
+
+
+def pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1, 5, 16), (2, 5, 70, 16), (3, 17, 7, 6), (1, 33, 300, 1), (2, 7, 9, 64), (1, 200, 5, 16), (2, 31, 33, 30)], ids=str)
+def test_nothing_around_the_arrays_of_the_scan(shape, dtype):
+    """neither read into a result nor written"""
+    import t2fw_amd as t2
+    from t2fw_amd import _lib
+    lib, (B, T, D, N), code = _lib.load(), shape, 0 if dtype == torch.float32 else 2
+    NP = max(4, 1 << (N - 1).bit_length())
+    tiles = (T + 15) // 16
+    x, dt, z, gy = (rand(B, T, D, seed=i).to(dtype) for i in range(4))
+    b, c = (rand(B, T, N, seed=4 + i).to(dtype) for i in range(2))
+    a, s0, gs, skip, bias = -rand(D, N).abs(), rand(B, D, N), rand(B, D, N, seed=1), rand(D), rand(D, seed=1)
+    f = Frame()
+    ins = [f.given(t) for t in (x, dt, a, b, c, skip, z, bias)]
+    s0_, gs_, gy_ = f.given(s0), f.given(gs), f.given(gy)
+    y, last, ckpt = f.result(B, T, D, dtype=dtype), f.result(B, D, N), f.result(B, tiles, D, NP)
+    assert lib.t2fw_selective_scan_checkpoint_bytes(B, T, D, N) == ckpt.numel() * 4
+    room = lib.t2fw_selective_scan_workspace_bytes(B, T, D, N)
+    space = f.result((room + 3) // 4)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.t2fw_selective_scan_forward(*map(pointer, ins), s0_.data_ptr(), None, *map(pointer, (y, last, ckpt)), B, T, D, N, None, code, 1, space.data_ptr(), room, stream) == 0
+    room = lib.t2fw_selective_scan_backward_workspace_bytes(B, T, D, N)
+    space = f.result((room + 3) // 4)
+    like = [f.result(B, T, D, dtype=dtype), f.result(B, T, D, dtype=dtype), f.result(D, N), f.result(B, T, N, dtype=dtype), f.result(B, T, N, dtype=dtype), f.result(D),
+            f.result(B, T, D, dtype=dtype), f.result(D), f.result(B, D, N)]
+    assert lib.t2fw_selective_scan_backward(gy_.data_ptr(), gs_.data_ptr(), *map(pointer, ins), None, ckpt.data_ptr(), *map(pointer, like), B, T, D, N, None, code, 1,
+                                            space.data_ptr(), room, stream) == 0
+    torch.cuda.synchronize()
+    f.check()
+    leaves = [t.clone().requires_grad_(True) for t in (x, dt, a, b, c, skip, z, bias, s0)]
+    out = t2.selective_scan(*leaves[:5], skip=leaves[5], gate=leaves[6], dt_bias=leaves[7], state=leaves[8], softplus=True)
+    grads = torch.autograd.grad(out, leaves, (gy, gs))
+    assert torch.equal(out[0], y) and torch.equal(out[1], last)
+    assert all(torch.equal(p, q) for p, q in zip(grads, like))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1, 5, 4), (2, 5, 70, 2), (3, 17, 7, 8), (1, 33, 300, 3), (2, 9, 3, 5), (1, 200, 1, 4), (2, 31, 33, 7)], ids=str)
+def test_nothing_around_the_arrays_of_the_convolution(shape, dtype):
+    import t2fw_amd as t2
+    from t2fw_amd import _lib
+    lib, (B, T, D, taps), code = _lib.load(), shape, 0 if dtype == torch.float32 else 2
+    x, gy = rand(B, T, D).to(dtype), rand(B, T, D, seed=1).to(dtype)
+    w, bias, s0, gs = rand(D, taps).to(dtype), rand(D).to(dtype), rand(B, taps - 1, D).to(dtype), rand(B, taps - 1, D, seed=1).to(dtype)
+    f = Frame()
+    x_, w_, bias_, s0_, gy_, gs_ = map(f.given, (x, w, bias, s0, gy, gs))
+    y, last = f.result(B, T, D, dtype=dtype), f.result(B, taps - 1, D, dtype=dtype)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.t2fw_short_conv_forward(*map(pointer, (x_, w_, bias_, s0_)), None, y.data_ptr(), last.data_ptr(), B, T, D, taps, None, code, 1, stream) == 0
+    room = lib.t2fw_short_conv_backward_workspace_bytes(B, T, D, taps, code)
+    space = f.result((room + 3) // 4)
+    like = [f.result(*t.shape, dtype=dtype) for t in (x, w, bias, s0)]
+    assert lib.t2fw_short_conv_backward(*map(pointer, (gy_, gs_, x_, w_, bias_, s0_)), None, *map(pointer, like), B, T, D, taps, None, code, 1, space.data_ptr(), room, stream) == 0
+    torch.cuda.synchronize()
+    f.check()
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, bias, s0)]
+    out = t2.short_conv(*leaves, silu=True)
+    grads = torch.autograd.grad(out, leaves, (gy, gs))
+    assert torch.equal(out[0], y) and torch.equal(out[1], last)
+    assert all(torch.equal(p, q) for p, q in zip(grads, like))
