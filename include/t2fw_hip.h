@@ -461,8 +461,8 @@ int t2fw_clip_grad_norm_f64(const t2fw_clip_desc *arrays, int64_t count, double 
  * inputs before the first, oldest first, and then x [B, T, D]; y = z, or z sigmoid(z) with T2FW_CONV_SILU.  fp32 / fp16 / bf16; w [D, taps] and bias [D]
  * (or null) of that type, or float with T2FW_CONV_WEIGHT_F32.  `last` [B, taps - 1, D]: the inputs before the next sequence.
  * `lengths` [B] (int32, or int64 with T2FW_CONV_LENGTHS64), or null: steps of row b from lengths[b] on do not count,
- * whatever they hold; y is zero there, and `last` is what precedes them.  `strides`: elements between rows and steps of x, or null for a dense array; the channels of a
- * step are next to each other.
+ * whatever they hold; y is zero there, and `last` is what precedes them.  `strides`: elements between rows and steps of x, or null for a dense array;
+ * the channels of a step are next to each other.
  */
 #define T2FW_CONV_SILU 1
 #define T2FW_CONV_LENGTHS64 2
@@ -487,10 +487,10 @@ int t2fw_short_conv_step(const void *x, const void *w, const void *bias, const v
  * Selective state space scan: h_t = exp(dt_t a) h_{t-1} + dt_t x_t b_t for each channel and its N (1 to 64) states, y_t = <c_t, h_t> + skip x_t, times
  * z sigmoid(z) of the gate z where there is one.  x, dt, gate (or null), y [B, T, D], b, c [B, T, N] fp32 / fp16 / bf16; a [D, N], skip, dt_bias [D]
  * (or null), s0 (null: zeros), last [B, D, N] float.  dt_bias is added to dt, and T2FW_SELECT_SOFTPLUS takes log(1 + e^dt) of that.  `lengths`: as for
- * t2fw_gated_scan_forward (T2FW_SELECT_LENGTHS64).  `strides`: elements between rows and steps of x, dt, b, c and gate (ten numbers; gate's are not looked at without one), or
- * null for dense arrays; the channels (states) of a step are next to each other, and 16 steps within 4 GB.  The products of a channel's decays over the steps of a row have to
- * stay finite (of dt a <= 0 they always do).  `ckpt`: t2fw_selective_scan_checkpoint_bytes for the backward call, or null.  The workspaces need no
- * initialisation and are not read across calls.
+ * t2fw_gated_scan_forward (T2FW_SELECT_LENGTHS64).  `strides`: elements between rows and steps of x, dt, b, c and gate (ten numbers; gate's are not
+ * looked at without one), or null for dense arrays; the channels (states) of a step are next to each other, and 16 steps within 4 GB.  The products
+ * of a channel's decays over the steps of a row have to stay finite (of dt a <= 0 they always do).  `ckpt`: t2fw_selective_scan_checkpoint_bytes for
+ * the backward call, or null.  The workspaces need no initialisation and are not read across calls.
  */
 #define T2FW_SELECT_SOFTPLUS 1
 #define T2FW_SELECT_LENGTHS64 2
@@ -503,8 +503,8 @@ int t2fw_selective_scan_forward(const void *x, const void *dt, const float *a, c
                                 void *workspace, size_t workspace_bytes, void *stream);
 /*
  * Gradients from those of y and of `last` (g_last, or null): d_x, d_dt, d_b, d_c, d_gate (null without a gate) dense and in the tensors' type, d_a,
- * d_skip, d_bias and d_s0 (the last three null where they are not wanted) float.  strides: as above, then g_y's two.  Sums over channels, rows and chunks are made in float, in
- * a fixed order.
+ * d_skip, d_bias and d_s0 (the last three null where they are not wanted) float.  strides: as above, then g_y's two.  Sums over channels, rows and
+ * chunks are made in float, in a fixed order.
  */
 size_t t2fw_selective_scan_backward_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t N);
 int t2fw_selective_scan_backward(const void *g_y, const float *g_last, const void *x, const void *dt, const float *a,
@@ -523,10 +523,10 @@ int t2fw_selective_scan_step(const void *x, const void *dt, const float *a, cons
 
 /*
  * The n (1 to 128) best of the K V candidates of each of B requests, best first: candidate (k, v) has the score scores[k] + log softmax(logits[k])[v].
- * logits [B, K, V] fp32 / fp16 / bf16, K at most 256; scores [B, K] float; results [B, n].  Of equal scores the lower k V + v is the better one; scores are compared in double, with sums of
- * float exponentials.  `finished` [B, K] bytes, or null: a beam that has ended has one candidate, the token `pad`, with its own score.  A
- * candidate that cannot be (a logit of minus infinity, a score of minus infinity or NaN, another token of an ended beam, a beam with a NaN or plus infinity among
- * its logits) has a score of minus infinity; which tokens of a beam with NaN come is not said.
+ * logits [B, K, V] fp32 / fp16 / bf16, K at most 256; scores [B, K] float; results [B, n].  Of equal scores the lower k V + v is the better one;
+ * scores are compared in double, with sums of float exponentials.  `finished` [B, K] bytes, or null: a beam that has ended has one candidate, the
+ * token `pad`, with its own score.  A candidate that cannot be (a logit of minus infinity, a score of minus infinity or NaN, another token of an
+ * ended beam, a beam with a NaN or plus infinity among its logits) has a score of minus infinity; which tokens of a beam with NaN come is not said.
  */
 size_t t2fw_beam_select_workspace_bytes(int64_t B, int64_t K, int64_t V, int64_t n, int32_t dtype);
 int t2fw_beam_select(const void *logits, const float *scores, const void *finished,

@@ -1,8 +1,9 @@
 // The causal convolution of W = 2 to 8 taps per channel, z_t = bias + sum_j w_j xs_{t+j} with xs the W - 1 inputs before the sequence (the state)
 // and its own, y = z or z sigmoid(z); what is before a selective scan.
 //
-// Bound by memory (1 x 32749 x 1021 float32 forward 50 us, 5.3 TB/s; 32 x 1024 x 4096 bf16 122 us forward, 4.4 TB/s, backward 208, 3.9): a lane owns 16 bytes of neighbouring channels of one row (backward: four channels) and 8 steps of them forward, so that an input is loaded once, and again
-// from the cache for the lane that has the next steps.  A workgroup has 16 such lanes side by side (256 bytes of a step) and 16 stretches in time.
+// Bound by memory (1 x 32749 x 1021 float32 forward 50 us, 5.3 TB/s; 32 x 1024 x 4096 bf16 122 us forward, 4.4 TB/s, backward 208, 3.9): a lane owns
+// 16 bytes of neighbouring channels of one row (backward: four channels) and 8 steps of them forward, so that an input is loaded once, and again from
+// the cache for the lane that has the next steps.  A workgroup has 16 such lanes side by side (256 bytes of a step) and 16 stretches in time.
 // Backward dx_p = sum_j w_j dz_{p+W-1-j} needs dz of the W - 1 steps after a lane's own too, which it makes again from x and the gradient: as many
 // loads at once as there are, and no loop whose loads wait for the stores of the one before (stretches of 13 to 125 steps, dz handed on in registers: 41 us
 // for 8 x 1024 x 1536 bf16, now 26).  The weights' gradients are summed in registers, over the stretches of a workgroup in

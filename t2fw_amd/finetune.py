@@ -5,8 +5,9 @@
     python -m t2fw_amd.finetune --selective --beams 4 # selective state space layers; the last answers by beam search
 
 The layers alternate between the decay rule (``LFWHeadsFunction``, a 64 x 64 state per head) and the recurrence with a vector for its
-state (``gated_scan``), or, with ``--selective``, the selective state space scan behind its convolution (``short_conv``, ``selective_scan``).  Each is a residual branch: ``residual_rms_norm`` adds the branch before to a float32 stream and normalises it,
-a projection makes the recurrence's inputs, another its output.
+state (``gated_scan``), or, with ``--selective``, the selective state space scan behind its convolution (``short_conv``, ``selective_scan``).  Each is
+a residual branch: ``residual_rms_norm`` adds the branch before to a float32 stream and normalises it, a projection makes the recurrence's inputs,
+another its output.
 
 * Training: logits of whole sequences, ``policy_loss`` on the answers' tokens, backward, ``clip_grad_norm`` of the 16-bit gradients into
   float32 ones, a gradient step on float32 parameters.

@@ -9,9 +9,9 @@ def short_conv(x, weight, bias=None, state=None, lengths=None, silu=False):
     [B, taps - 1, D])``, with gradients.
 
     ``x: [B, T, D]`` (float32, float16 or bfloat16), with its channels next to each other in memory and any strides between rows and steps.
-    ``weight: [D, taps]`` with 2 to 8 taps (``weight[:, 0]`` of a depthwise ``Conv1d``) and ``bias: [D]`` have the type of ``x`` or float32.  ``state: [B, taps - 1, D]``: the inputs before the
-    first, oldest first (``None``: zeros), of the type of ``x``, as are the last inputs: what the next call takes as its state.  Sums are float32;
-    those of the weights' gradient over rows and steps are made in a fixed order.
+    ``weight: [D, taps]`` with 2 to 8 taps (``weight[:, 0]`` of a depthwise ``Conv1d``) and ``bias: [D]`` have the type of ``x`` or float32.
+    ``state: [B, taps - 1, D]``: the inputs before the first, oldest first (``None``: zeros), of the type of ``x``, as are the last inputs: what the
+    next call takes as its state.  Sums are float32; those of the weights' gradient over rows and steps are made in a fixed order.
 
     ``lengths: [B]`` (int32 or int64, on the device), for rows that are padded at their end: steps from ``lengths[b]`` on do not count, whatever
     they hold, NaN included.  Their outputs and gradients are zero, and the last inputs of the row are those before its end."""
