@@ -89,8 +89,7 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, 
         for (int s = 0; s < S; ++s) next_h[s] = v.e[s];
     };
     if (tiles > 0) load(p.begin + (int64_t)(tiles - 1) * TILE);
-    if (a.g_state != nullptr) load_states(adj, a.g_state + (p.b * a.D + p.d) * a.N, p.n0, a.N);
-    through_maps<G, true>(adj, a, g, p, rate);
+    at_chunk<G, true>(adj, a, g, p, rate);
     // sums over the block's channels, of the tile
     const auto store_steps = [&](int64_t t0, bool some) {
         constexpr int ALL = TILE * 2 * NP;
@@ -267,7 +266,7 @@ template <typename IO, int G> int launch_backward(const SelectArgs &a, const Gri
     if (row > 0) {
         if (g.chunks > 1) {
             hipLaunchKernelGGL((select_maps_kernel<IO, G, true>), dim3(row * (g.chunks - 1)), dim3(THREADS), 0, stream, a, g);
-            if ((rc = check_hip(hipGetLastError(), "select_maps_kernel launch"))) return rc;
+            if ((rc = check_hip(hipGetLastError(), "select_maps_kernel launch")) || (rc = launch_join<G, true>(a, g, stream))) return rc;
         }
         if (a.gate != nullptr) hipLaunchKernelGGL((select_backward_kernel<IO, G, true>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
         else hipLaunchKernelGGL((select_backward_kernel<IO, G, false>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);

@@ -25,8 +25,7 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS) 
         c.load(a.c, a.c_b, a.c_t, a, p, t0);
     };
     if (tiles > 0) load(p.begin);
-    if (a.s0 != nullptr) load_states(h, a.s0 + (p.b * a.D + p.d) * a.N, p.n0, a.N);
-    through_maps<G, false>(h, a, g, p, rate);
+    at_chunk<G, false>(h, a, g, p, rate);
     for (int k = 0; k < tiles; ++k) {
         const int64_t t0 = p.begin + (int64_t)k * TILE;
         float (&b_here)[TILE][NP] = bs[k % 2], (&c_here)[TILE][NP] = cs[k % 2];
@@ -135,8 +134,8 @@ template <typename IO, int G> int launch_forward(const SelectArgs &a, const Grid
     const unsigned row = (unsigned)(g.blocks * a.B);
     if (g.chunks > 1) {
         hipLaunchKernelGGL((select_maps_kernel<IO, G, false>), dim3(row * (g.chunks - 1)), dim3(THREADS), 0, stream, a, g);
-        const int rc = check_hip(hipGetLastError(), "select_maps_kernel launch");
-        if (rc) return rc;
+        int rc = check_hip(hipGetLastError(), "select_maps_kernel launch");
+        if (rc || (rc = launch_join<G, false>(a, g, stream))) return rc;
     }
     if (a.gate != nullptr) hipLaunchKernelGGL((select_forward_kernel<IO, G, true>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);
     else hipLaunchKernelGGL((select_forward_kernel<IO, G, false>), dim3(row * g.chunks), dim3(THREADS), 0, stream, a, g);

@@ -10,7 +10,8 @@
 //
 // A stretch of steps is an affine map of the state before it, h -> exp(a sum dt) h + S: its decay needs no more than the sum of its steps' lengths.  So a
 // sequence is cut in chunks where there are too few channels for the chip: one launch for the chunks' maps, and another in which a
-// chunk puts those before it together and goes through its steps.  It costs a chunk's decays twice.
+// chunk puts those before it together and goes through its steps; of many chunks a launch between them puts the maps together.  It costs a chunk's
+// decays twice.
 //
 // Bound by the vector units: a state and step is a product, an exponential (which takes two instructions' time), a product and two
 // multiply-adds forward.
@@ -30,6 +31,7 @@ constexpr int64_t MOST_GROUPS = (1ll << 32) / THREADS - 1;      // a grid has le
 struct Grid {
     uint32_t blocks, chunks, tiles;      // tiles: of a whole row
     int64_t steps;
+    bool joined;                         // many chunks: the states at their starts are made by a launch of their own
     bool fits;
 };
 
@@ -243,6 +245,90 @@ template <int G, bool BACK> __device__ __forceinline__ void through_maps(float (
     }
 }
 
+// The state (BACK: the adjoint) at a chunk's start (end)
+template <int G, bool BACK> __device__ __forceinline__ void at_chunk(float (&h)[S], const SelectArgs &a, const Grid &g, const Place &p, const float (&rate)[S]) {
+    if (g.joined) {
+        load_padded(h, a.maps + (((int64_t)p.chunk * a.B + p.b) * a.D + p.d) * (G * S) + p.n0);
+        return;
+    }
+    const float *const first = BACK ? a.g_state : a.s0;
+    if (first != nullptr) load_states(h, first + (p.b * a.D + p.d) * a.N, p.n0, a.N);
+    through_maps<G, BACK>(h, a, g, p, rate);
+}
+
+// ... of all chunks, in place of their maps, where a chunk that goes through all the maps before it takes longer than the launch (forward and step of
+// training in us, without it and with it: 8 x 1024 x 64 x 16 in 32 chunks 18, 50 and 19, 53; 8 x 2048 x 256 x 16 in 64 63, 192 and 59, 178; 1 x 16384
+// x 64 x 16 in 512 120, 264 and 27, 78; 1 x 131072 x 64 x 16 in 1024 258, 652 and 91, 290).  JOIN_LANES lanes side by side in a workgroup, the chunks
+// of each cut in JOIN_PARTS parts.  A thread puts the maps of its part together, the parts before it are put together in shared memory, in steps of
+// twice as many, and it goes through its maps again.
+constexpr int JOIN_LANES = 4, JOIN_PARTS = THREADS / JOIN_LANES;
+template <int G, bool BACK> __global__ __launch_bounds__(THREADS) void select_join_kernel(SelectArgs a, Grid g) {
+    constexpr int NP = G * S, AHEAD = 8;
+    __shared__ float maps[2][S + 1][THREADS];
+    const int part = threadIdx.x / JOIN_LANES;
+    const int64_t lanes = a.B * a.D * G, unit = (int64_t)blockIdx.x * JOIN_LANES + threadIdx.x % JOIN_LANES;
+    const bool mine = unit < lanes;
+    const int64_t row = (mine ? unit : lanes - 1) / G, d = row % a.D;        // (row and channel)
+    const int n0 = (int)((mine ? unit : lanes - 1) % G) * S;
+    float *const states = a.maps + row * NP + n0;
+    const float *const lengths = a.maps + (int64_t)g.chunks * a.B * a.D * NP + row;
+    float rate[S], h[S] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f;
+    load_states(rate, a.a + d * a.N, n0, a.N);
+#pragma unroll
+    for (int s = 0; s < S; ++s) rate[s] = rate_of(rate[s]);
+    // chunks in the order in which they follow; the last one's map is not needed
+    const int chunks = (int)g.chunks, each = (chunks + JOIN_PARTS - 1) / JOIN_PARTS, begin = part * each, end = begin + each < chunks ? begin + each : chunks;
+    const auto walk = [&](bool again) {
+        for (int i = begin; i < end; i += AHEAD) {
+            float v[AHEAD][S], sum[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int j = i + u < chunks - 1 ? i + u : chunks - 2;
+                const int64_t at = (int64_t)(BACK ? chunks - 1 - j : j) * a.B * a.D;
+                load_padded(v[u], states + at * NP);
+                sum[u] = lengths[at];
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (i + u >= end) break;
+                if (again && mine) store_padded(states + (int64_t)(BACK ? chunks - 1 - i - u : i + u) * a.B * a.D * NP, h);
+                if (i + u == chunks - 1) break;
+#pragma unroll
+                for (int s = 0; s < S; ++s) h[s] = fmaf(exp2_of(rate[s] * sum[u]), h[s], v[u][s]);
+                total += sum[u];
+            }
+        }
+    };
+    walk(false);
+    int k = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) maps[0][s][threadIdx.x] = h[s];
+    maps[0][S][threadIdx.x] = total;
+    __syncthreads();
+    for (int m = JOIN_LANES; m < THREADS; m *= 2, k ^= 1) {
+        if ((int)threadIdx.x >= m) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) h[s] = fmaf(exp2_of(rate[s] * total), maps[k][s][threadIdx.x - m], h[s]);
+            total += maps[k][S][threadIdx.x - m];
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) maps[k ^ 1][s][threadIdx.x] = h[s];
+        maps[k ^ 1][S][threadIdx.x] = total;
+        __syncthreads();
+    }
+    // what is before the thread's part, on the state that is given
+    const float *const given = BACK ? a.g_state : a.s0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) h[s] = 0.0f;
+    if (given != nullptr) load_states(h, given + row * a.N, n0, a.N);
+    if (part > 0) {
+        total = maps[k][S][threadIdx.x - JOIN_LANES];
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[s] = fmaf(exp2_of(rate[s] * total), h[s], maps[k][s][threadIdx.x - JOIN_LANES]);
+    }
+    walk(true);
+}
+
 // A step's length, and its product with the input
 template <bool SLOPE> struct StepLength {
     float dt, slope;
@@ -336,21 +422,36 @@ inline int lanes_of(int64_t N) {
     while (g * S < N) g *= 2;
     return g;
 }
-// Chunks: none where channels and rows alone make three workgroups for two CUs (T = 1024, D = 1536, N = 16 bf16, forward and step of training: 20 rows, 480
-// workgroups, 184 and 672 us, in two chunks 223 and 788; 16 rows 180 and 658, in four 182 and 638; 14 rows 179 and 655, in six 164 and 571), else as many as make
-// 1536 (8 rows 130 and 474 us, in four chunks 113 and 366, in eight 106 and 348), but no more than the root of the steps, as a chunk goes through the maps of
-// all before it (1 x 16384 x 64 x 16: 64 chunks 69 and 209 us, 128 57 and 161, 256 73 and 183; 1 x 131072 x 64 x 16: 128 chunks 233 and 726, 256 161 and 471).
+// Chunks: the vector units of a CU are shared by its workgroups, so the time goes with the workgroups of the fullest CU times a chunk's tiles; half a
+// workgroup and half a tile more stand for latencies that few workgroups do not hide, and for what a chunk takes whatever its length.  The maps cost
+// 0.45 of the rest.  (D = 1536, N = 16 bf16, forward and step of training in us: 18 x 1024, 432 workgroups, whole 184 and 671, in two chunks 222 and 776;
+// 14 x 1024 whole 182 and 661, in six 168 and 563; 8 x 1024 whole 134 and 490, in four 114 and 361, in eight 107 and 342, in 32 128 and 420; 8 x 128 whole
+// 22 and 78, in four 23 and 74; 1 x 256 whole 37 and 129, in 16 15 and 41.  D = 64: 1 x 32 whole 8.6 and 27, in two 11 and 27.)
+inline int64_t cost_of(int64_t rows, int64_t chunks, int64_t each) {
+    const int64_t fullest = (rows * chunks + 255) / 256;
+    return (2 * fullest + 1) * (2 * each + 1) * (chunks > 1 ? 29 : 20);
+}
 inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N) {
     Grid g{};
     const int64_t channels = THREADS / lanes_of(N), blocks = (D + channels - 1) / channels, tiles = T <= 0 ? 0 : (T + TILE - 1) / TILE;
     const long double rows = (long double)blocks * B;
-    int64_t chunks = 1;
-    if (rows > 0 && rows < 384) chunks = (int64_t)((1536 + rows - 1) / rows);
-    while (chunks > 1 && (chunks * chunks > T || chunks > tiles)) --chunks;
-    const int64_t each = tiles == 0 ? 1 : (tiles + chunks - 1) / chunks;
+    int64_t each = tiles == 0 ? 1 : tiles;
+    if (rows > 0 && rows < 512 && tiles > 2) {
+        const int64_t n = (int64_t)rows;
+        int64_t least = cost_of(n, 1, each);
+        for (int64_t full = 1; full <= 8; ++full) {
+            const int64_t most = full * 256 / n, chunks = most < tiles ? most : tiles;
+            if (chunks < 2) continue;
+            const int64_t some = (tiles + chunks - 1) / chunks, cost = cost_of(n, (tiles + some - 1) / some, some);
+            if (cost > least) continue;
+            least = cost;
+            each = some;
+        }
+    }
     g.steps = each * TILE;
     g.chunks = (uint32_t)(tiles == 0 ? 1 : (tiles + each - 1) / each);
     g.blocks = (uint32_t)blocks;
+    g.joined = g.chunks > 48;
     g.fits = D < (1 << 21) &&      // (a step of the checkpoints is addressed by 32 bits)
              B < 0x7fffffff && tiles < 0x7fffffff && rows * g.chunks < MOST_GROUPS;
     g.tiles = (uint32_t)tiles;
@@ -358,6 +459,12 @@ inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N) {
 }
 inline size_t maps_bytes(const Grid &g, int64_t B, int64_t D, int64_t N) {
     return g.chunks == 1 ? 0 : (size_t)g.chunks * B * D * (lanes_of(N) * S + 1) * sizeof(float);
+}
+template <int G, bool BACK> int launch_join(const SelectArgs &a, const Grid &g, hipStream_t stream) {
+    if (!g.joined) return T2FW_OK;
+    const int64_t groups = (a.B * a.D * G + JOIN_LANES - 1) / JOIN_LANES;
+    hipLaunchKernelGGL((select_join_kernel<G, BACK>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a, g);
+    return check_hip(hipGetLastError(), "select_join_kernel launch");
 }
 inline int too_many() { return fail(T2FW_ERR_BAD_SHAPE, "selective scan: too many channels, or workgroups for one launch"); }
 

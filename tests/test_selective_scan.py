@@ -5,6 +5,7 @@ Bounds, u = 2^-24; M and GM are the recurrence and its adjoint of absolute value
   by twice the rounding of dt + bias; without the softplus by that alone.
 * A decay exp(dt a): the length's error times |a|, three roundings of the exponent, 2^-22 |dt a|, and the exponential's own 2^-22 and a product's rounding, 2^-21.
   Over chunks the exponent is a times a sum of lengths, in four shares of at most T / 4 terms each: T 2^-25 |dt a| more for every step.
+  (Of more than 48 chunks, T / 16 at most, the sums are put together by chunks / 64 + 7 additions, which with a chunk's own T / 4 / 48 are fewer still.)
 * A state: E_t = decay E_{t-1} + (its error) decay M_{t-1} + (the input's error) + 2 u M_t.  The adjoint obeys the same.
 * A sum of n products of such numbers: the products' errors, and (n + 4) u of the sum of absolute values, in any order.
 * The gate's sigmoid: 2^-20 (16-bit tensors, |z| < 40) or 2^-21; its slope that times 1 + |z|.
@@ -214,6 +215,27 @@ def test_many_chunks_and_many_rows(shape, dtype):
     lengths = torch.randint(0, shape[1] + 1, (shape[0],), generator=torch.Generator().manual_seed(1))
     lengths[0] = shape[1] - 3
     compare(p, lengths.cuda(), True, gy, gs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 6, 16, 30, 64])
+def test_chunks_by_the_hundred(N):
+    """their maps put together by a launch of its own: for every number of lanes, with rows that end in the first chunk, before it, and in the last one"""
+    B, T, D = 4, 1100, 9
+    p, gy, gs = inputs(B, T, D, N, torch.float32, seed=N, long=True)
+    compare(p, torch.tensor([T - 1, 0, 7, 530]).cuda(), True, gy, gs)
+    got = run(p, None, True, gy, gs)
+    alone = [run({n: None if t is None else t[b:b + 1].contiguous() if n in ("x", "dt", "b", "c", "state", "gate") else t for n, t in p.items()}, None, True,
+                 gy[b:b + 1].contiguous(), gs[b:b + 1].contiguous()) for b in range(B)]
+    # (rows alone are cut in other chunks)
+    ref = reference(p, None, True, gy, gs)
+    for n in ("y", "last", "d_x", "d_state"):
+        check(n, got[n], ref[n])
+        check(n, torch.cat([o[n] for o in alone]), ref[n])
+    p["state"] = None
+    got, ref = run(p, None, True, gy, torch.zeros_like(gs)), reference(p, None, True, gy, torch.zeros_like(gs))
+    for n in ("y", "last", "d_x", "d_a"):
+        check(n, got[n], ref[n])
 
 
 @pytest.mark.gpu
