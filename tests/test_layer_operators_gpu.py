@@ -1,5 +1,7 @@
 """short_conv, selective_scan, beam_select and reorder_beams as calls: other ways to differentiate and transform them, hooks on what their nodes save, memory
 that does not hold its values as they are, arrays whose offsets pass 32 bits, streams side by side.  What they do not have is refused."""
+import gc
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -129,7 +131,19 @@ def test_inputs_that_want_no_gradient():
             assert torch.equal(got, want[i]), (name, i)
 
 
-def test_offsets_past_32_bits():
+@pytest.fixture
+def large():
+    gc.collect()                                         # (tensors in cycles that earlier tests have left)
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()                             # (what the tests after this hold would be parts of these blocks)
+
+
+def test_offsets_past_32_bits(large):
     """rows of 2^31 elements and more apart, in one array of 8.6 GB: the same results as from the rows brought together"""
     import t2fw_amd as t2
     B, T, D, N = 2, 60, 40, 6
@@ -169,7 +183,7 @@ def both_train(t2, u, w, a, state, D, N):
     return t2.short_conv(x, w, silu=True) + t2.selective_scan(x, dt, a, b, c, state=state, gate=z, softplus=True)
 
 
-def test_large_arrays_of_beams():
+def test_large_arrays_of_beams(large):
     import t2fw_amd as t2
     V = 131072
     logits = torch.empty(1100, 16, V, dtype=torch.bfloat16, device="cuda").normal_()
