@@ -443,7 +443,7 @@ inline Grid grid_of(int64_t B, int64_t T, int64_t D, int64_t N) {
             const int64_t most = full * 256 / n, chunks = most < tiles ? most : tiles;
             if (chunks < 2) continue;
             const int64_t some = (tiles + chunks - 1) / chunks, cost = cost_of(n, (tiles + some - 1) / some, some);
-            if (cost > least) continue;
+            if (cost >= least) continue;              // (of equal ones the fewer: 8 x 4096 x 256 x 16 in 32 81 and 256, in 64 91 and 285)
             least = cost;
             each = some;
         }
