@@ -261,9 +261,8 @@ template <int G, bool BACK> __device__ __forceinline__ void at_chunk(float (&h)[
 // x 64 x 16 in 512 120, 264 and 27, 78; 1 x 131072 x 64 x 16 in 1024 258, 652 and 91, 290).  JOIN_LANES lanes side by side in a workgroup, the chunks
 // of each cut in JOIN_PARTS parts.  A thread puts the maps of its part together, the parts before it are put together in shared memory, in steps of
 // twice as many, and it goes through its maps again.
-constexpr int JOIN_LANES = 4, JOIN_PARTS = THREADS / JOIN_LANES;
-template <int G, bool BACK> __global__ __launch_bounds__(THREADS) void select_join_kernel(SelectArgs a, Grid g) {
-    constexpr int NP = G * S, AHEAD = 8;
+template <int G, bool BACK, int JOIN_LANES> __global__ __launch_bounds__(THREADS) void select_join_kernel(SelectArgs a, Grid g) {
+    constexpr int NP = G * S, AHEAD = 8, JOIN_PARTS = THREADS / JOIN_LANES;
     __shared__ float maps[2][S + 1][THREADS];
     const int part = threadIdx.x / JOIN_LANES;
     const int64_t lanes = a.B * a.D * G, unit = (int64_t)blockIdx.x * JOIN_LANES + threadIdx.x % JOIN_LANES;
@@ -462,8 +461,11 @@ inline size_t maps_bytes(const Grid &g, int64_t B, int64_t D, int64_t N) {
 }
 template <int G, bool BACK> int launch_join(const SelectArgs &a, const Grid &g, hipStream_t stream) {
     if (!g.joined) return T2FW_OK;
-    const int64_t groups = (a.B * a.D * G + JOIN_LANES - 1) / JOIN_LANES;
-    hipLaunchKernelGGL((select_join_kernel<G, BACK>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a, g);
+    const int64_t lanes = a.B * a.D * G;
+    // few parts where lanes alone make a workgroup for every CU (64 chunks of 1536 x 16 states 12.2 us in 64 parts, 7.3 in 16), else many (64 chunks of 64 x 16
+    // states, with the scan, 15 us in 16, 14 in 64)
+    if (g.chunks <= 128 && lanes >= 16 * 256) hipLaunchKernelGGL((select_join_kernel<G, BACK, 16>), dim3((unsigned)((lanes + 15) / 16)), dim3(THREADS), 0, stream, a, g);
+    else hipLaunchKernelGGL((select_join_kernel<G, BACK, 4>), dim3((unsigned)((lanes + 3) / 4)), dim3(THREADS), 0, stream, a, g);
     return check_hip(hipGetLastError(), "select_join_kernel launch");
 }
 inline int too_many() { return fail(T2FW_ERR_BAD_SHAPE, "selective scan: too many channels, or workgroups for one launch"); }

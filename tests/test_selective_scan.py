@@ -209,7 +209,7 @@ def test_lengths_as_given_and_nothing_that_may_be_missing(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
-@pytest.mark.parametrize("shape", [(1, 3000, 12, 16), (3, 1100, 40, 16), (40, 40, 300, 16)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 3000, 12, 16), (3, 1100, 40, 16), (40, 40, 300, 16), (1, 1000, 1030, 14)], ids=str)
 def test_many_chunks_and_many_rows(shape, dtype):
     p, gy, gs = inputs(*shape, dtype, seed=7, long=True)
     lengths = torch.randint(0, shape[1] + 1, (shape[0],), generator=torch.Generator().manual_seed(1))
