@@ -79,18 +79,23 @@ template <typename Key, typename Above> __device__ __forceinline__ Key of_group(
     }
     return mine;
 }
+// How many of m numbers are above one: `per` (1, 2 or 4) threads side by side share them out, and all have the answer.  A loop of 64 took 1 us of the second launch.
+template <typename Key, typename Above> __device__ __forceinline__ int count_above(const Key *all, int m, const Key &one, int per, Above above) {
+    int place = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x % per; i < m; i += per) place += above(all[i], one);
+    if (per > 1) place += __shfl_xor(place, 1, 64);
+    if (per > 2) place += __shfl_xor(place, 2, 64);
+    return place;
+}
+__device__ __forceinline__ int threads_for(int m) { return m <= THREADS / 4 ? 4 : m <= THREADS / 2 ? 2 : 1; }
 // The n-th largest of the groups' best, `mine`: all are distinct
 template <typename Key, typename Above> __device__ __forceinline__ Key nth_best(const Key &mine, Key (&best)[THREADS], Key &least, int n, Above above) {
     const int groups = groups_of(n), per = THREADS / groups;
     if (threadIdx.x % per == 0) best[threadIdx.x / per] = mine;
     __syncthreads();
-    if ((int)threadIdx.x < groups) {                     // (of 64 groups: one wave)
-        const Key one = best[threadIdx.x];
-        int place = 0;
-#pragma unroll 16
-        for (int i = 0; i < groups; ++i) place += above(best[i], one);
-        if (place == n - 1) least = one;
-    }
+    const Key one = best[threadIdx.x / per];
+    if (count_above(best, groups, one, per, above) == n - 1) least = one;      // (of each of its threads)
     __syncthreads();
     return least;
 }
@@ -182,11 +187,10 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
     }
     __syncthreads();
     const int m = found;
-    for (int j = threadIdx.x; j < m; j += THREADS) {
+    const int per = threads_for(m);
+    for (int j = threadIdx.x / per; j < m; j += THREADS / per) {
         const uint64_t k = list[j];
-        int place = 0;
-#pragma unroll 8
-        for (int i = 0; i < m; ++i) place += list[i] > k;
+        const int place = count_above(list, m, k, per, more);
         if (place < a.n) to[place] = k;
     }
     if (m >= a.n) return;
@@ -284,11 +288,10 @@ __global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lan
         }
         __syncthreads();
         const int m = found;
-        for (int j = threadIdx.x; j < m; j += THREADS) {
+        const int per = threads_for(m);
+        for (int j = threadIdx.x / per; j < m; j += THREADS / per) {
             const Candidate one = list[j];
-            int place = 0;
-#pragma unroll 4
-            for (int i = 0; i < m; ++i) place += list[i].above(one);
+            const int place = count_above(list, m, one, per, more);
             if (place < a.n) kept[place] = one;
         }
         __syncthreads();
