@@ -10,6 +10,7 @@
 //
 // Reordering.  A thread has the same 16 bytes of all beams of a request, loads those that move, and stores them when all of them are there: in place
 // without a copy, and a beam that goes on from itself is neither read nor written.  One launch for up to 96 arrays.
+#include <type_traits>
 #include "beam.hpp"
 #include "vec.hpp"
 
@@ -37,6 +38,26 @@ __device__ __forceinline__ uint64_t packed(float z, uint32_t v) { return (uint64
 __device__ __forceinline__ float logit_of(uint64_t p) { return number((uint32_t)(p >> 32)); }
 __device__ __forceinline__ uint32_t token_of(uint64_t p) { return 0xffffffffu - (uint32_t)p; }
 
+// A logit and its place in the piece, of 2^14 at most: 16 bits of both are enough for 16-bit logits.  All keys are larger than THREADS.
+template <typename IO> struct Piece {
+    typedef uint32_t Key;
+    static __device__ __forceinline__ Key key(float z, uint32_t v) {
+        const uint32_t u = __builtin_bit_cast(uint16_t, narrow<IO>(z + 0.0f));
+        return (u & 0x8000u ? ~u << 16 : (u | 0x8000u) << 16) | (0xffffu - v);
+    }
+    static __device__ __forceinline__ float logit(Key k) {
+        const uint16_t u = (uint16_t)(k >> 16);
+        return widen(__builtin_bit_cast(IO, (uint16_t)(u & 0x8000u ? u & 0x7fffu : ~u)));
+    }
+    static __device__ __forceinline__ uint32_t place(Key k) { return 0xffffu - (k & 0xffffu); }
+};
+template <> struct Piece<float> {
+    typedef uint64_t Key;
+    static __device__ __forceinline__ Key key(float z, uint32_t v) { return packed(z, v); }
+    static __device__ __forceinline__ float logit(Key k) { return logit_of(k); }
+    static __device__ __forceinline__ uint32_t place(Key k) { return token_of(k); }
+};
+
 // A candidate of a request: its score, and its place among the K V
 struct Candidate {
     uint64_t key;
@@ -56,6 +77,7 @@ template <typename T, typename Op> __device__ __forceinline__ T over_group(T v, 
     return v;
 }
 
+__device__ __forceinline__ uint32_t shuffled(uint32_t v, int m) { return __shfl_xor(v, m, 64); }
 __device__ __forceinline__ uint64_t shuffled(uint64_t v, int m) { return __shfl_xor(v, m, 64); }
 __device__ __forceinline__ Candidate shuffled(const Candidate &v, int m) { return {__shfl_xor(v.key, m, 64), __shfl_xor(v.at, m, 64)}; }
 
@@ -104,9 +126,12 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
     constexpr int VEC = 16 / sizeof(IO), VECS = EACH / VEC;
     __shared__ float tops[THREADS / 64];
     __shared__ double sums[THREADS / 64];
-    __shared__ uint64_t best[THREADS], least;
+    typedef Piece<IO> Of;
+    typedef typename Of::Key Key;
+    __shared__ Key best[THREADS], least;
     __shared__ int found;
-    extern __shared__ uint64_t list[];                    // what the groups of threads that are not below the n-th hold
+    extern __shared__ uint64_t memory[];
+    Key *const list = reinterpret_cast<Key *>(memory);    // what the groups of threads that are not below the n-th hold
     const int64_t row = blockIdx.x / a.pieces;
     const int piece = blockIdx.x % a.pieces;
     const int64_t begin = (int64_t)piece * a.piece;
@@ -125,19 +150,24 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
         return;
     }
     // all loads at once, of what is not there of the first logits; the last vector of the piece, where it is no whole one, by its elements
-    Vec<IO, VEC> raw[VECS];
+    constexpr uint32_t NONE = sizeof(IO) == 4 ? 0xff800000u : std::is_same<IO, _Float16>::value ? 0xfc00fc00u : 0xff80ff80u;      // minus infinity
+    uint32_t raw[VECS][4];
     if (here >= VEC) {
 #pragma unroll
         for (int i = 0; i < VECS; ++i) {
             const int at = (i * THREADS + threadIdx.x) * VEC;
-            raw[i] = load_vec<IO, VEC>(z + (at + VEC <= here ? at : 0));
+            const Vec<IO, VEC> one = load_vec<IO, VEC>(z + (at + VEC <= here ? at : 0));
+            __builtin_memcpy(raw[i], &one, 16);
         }
     }
     float v[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int at = (i / VEC * THREADS + threadIdx.x) * VEC;
-        v[i] = at + VEC <= here ? widen(raw[i / VEC].e[i % VEC]) : -INFINITY;
+    for (int i = 0; i < VECS; ++i) {
+        const bool whole = (int)(i * THREADS + threadIdx.x) * VEC + VEC <= here;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) raw[i][w] = whole ? raw[i][w] : NONE;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[i * VEC + e] = element_of<IO>(raw[i], e);
     }
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
@@ -152,53 +182,66 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
     float mine_z = -INFINITY;
     int mine_i = 0;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const bool more = v[i] > mine_z;
-        mine_z = more ? v[i] : mine_z;
-        mine_i = more ? i : mine_i;
-    }
+    for (int i = 0; i < EACH; ++i) mine_z = fmaxf(mine_z, v[i]);
+#pragma unroll
+    for (int i = EACH - 1; i >= 0; --i) mine_i = v[i] == mine_z ? i : mine_i;
     const float top = over_group(mine_z, tops, [](float x, float y) { return fmaxf(x, y); });
     // Exponentials by the hardware, as powers of two: off by 2^-22, and by |z - top| 2^-23 for the exponent's rounding where e^(z - top) is the smaller.  Of
     // nothing above minus infinity the sum is zero, or NaN where there is one, which the largest does not show.
-    float sum = 0.0f;
-    if (top > -INFINITY) {
+    // The difference and the product in one: what rounding the largest's product leaves is in all terms alike, and comes out of their sum again.
+    constexpr float LOG2E = 1.44269504088896340736f;
+    const float scaled = top * LOG2E, back = fabsf(top) < 0x1p20f ? fmaf(top, LOG2E, -scaled) : 0.0f;
+    float parts[4] = {0.0f, 0.0f, 0.0f, 0.0f};           // (four sums: fewer roundings one after another)
+    if (__builtin_amdgcn_readfirstlane(fabsf(top) < 0x1p20f)) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) sum += __builtin_amdgcn_exp2f((v[i] - top) * 1.44269504088896340736f);
+        for (int i = 0; i < EACH; ++i) parts[i % 4] += __builtin_amdgcn_exp2f(fmaf(v[i], LOG2E, -scaled));
+    } else if (top > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) parts[i % 4] += __builtin_amdgcn_exp2f((v[i] - top) * LOG2E);
     } else {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) sum += v[i] == v[i] ? 0.0f : v[i];
+        for (int i = 0; i < EACH; ++i) parts[i % 4] += v[i] == v[i] ? 0.0f : v[i];
     }
+    const float sum = (parts[0] + parts[1]) + (parts[2] + parts[3]);
     const double all = over_group((double)sum, sums, [](double x, double y) { return x + y; });
-    if (threadIdx.x == 0) static_cast<Share *>(a.partial)[blockIdx.x] = {top, 0, all};
+    if (threadIdx.x == 0) static_cast<Share *>(a.partial)[blockIdx.x] = {top, 0, all * __builtin_amdgcn_exp2f(-back)};
     // Logits of minus infinity and NaN stay out of it: where there are fewer others than wanted, the first of them follow by their index.  (Threads
     // that hold nothing are told apart by small numbers.)
     const int mine_at = (mine_i / VEC * THREADS + threadIdx.x) * VEC + mine_i % VEC;
-    const uint64_t mine = mine_z > -INFINITY ? packed(mine_z, (uint32_t)(begin + mine_at)) : THREADS - threadIdx.x;
-    const auto more = [](uint64_t x, uint64_t y) { return x > y; };
-    const uint64_t limit = nth_best(of_group(mine, a.n, more), best, least, a.n, more);
+    const Key mine = mine_z > -INFINITY ? Of::key(mine_z, (uint32_t)mine_at) : THREADS - threadIdx.x;
+    const auto more = [](Key x, Key y) { return x > y; };
+    const Key limit = nth_best(of_group(mine, a.n, more), best, least, a.n, more);
     if (mine > THREADS && mine >= limit) {
-        const float limit_z = limit > THREADS ? logit_of(limit) : -INFINITY;
+        // (a branch for eight: most threads have one that counts)
+        const float limit_z = limit > THREADS ? Of::logit(limit) : -3.4028234e38f;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            if (!(v[i] >= limit_z && v[i] > -INFINITY)) continue;
-            const uint64_t k = packed(v[i], (uint32_t)(begin + (i / VEC * THREADS + threadIdx.x) * VEC + i % VEC));
-            if (k >= limit) list[atomicAdd(&found, 1)] = k;
+        for (int i = 0; i < EACH; i += 8) {
+            float most = v[i];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) most = fmaxf(most, v[i + e]);
+            if (!(most >= limit_z)) continue;
+#pragma unroll
+            for (int e = i; e < i + 8; ++e) {
+                if (!(v[e] >= limit_z)) continue;
+                const Key k = Of::key(v[e], (uint32_t)((e / VEC * THREADS + threadIdx.x) * VEC + e % VEC));
+                if (k >= limit) list[atomicAdd(&found, 1)] = k;
+            }
         }
     }
     __syncthreads();
     const int m = found;
     const int per = threads_for(m);
     for (int j = threadIdx.x / per; j < m; j += THREADS / per) {
-        const uint64_t k = list[j];
+        const Key k = list[j];
         const int place = count_above(list, m, k, per, more);
-        if (place < a.n) to[place] = k;
+        if (place < a.n) to[place] = packed(Of::logit(k), (uint32_t)begin + Of::place(k));
     }
     if (m >= a.n) return;
     // fewer than n others: of the first 2 n tokens at least n - m are none of them
     for (int j = threadIdx.x; j < 2 * a.n; j += THREADS) {
         int place = m + j;
         for (int i = 0; i < m; ++i) {
-            const uint32_t t = token_of(list[i]) - (uint32_t)begin;
+            const uint32_t t = Of::place(list[i]);
             place = t == (uint32_t)j ? a.n : place - (t < (uint32_t)j);      // (it has its place, which is below m)
             if (t == (uint32_t)j) break;
         }
@@ -206,9 +249,10 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
     }
 }
 
-// A request: the n best of its lists, in rounds of ROUND candidates, each with the n best so far
-constexpr int HOLD = 4, ROUND = THREADS * HOLD;
-__global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lanes) {
+// A request: the n best of its lists, in rounds of up to 256 HOLD candidates, each with the n best so far.  A thread has some that follow each other in a
+// list, so that the lists' first ones are with many threads: their n-th best is no worse than few others (64 requests, 16 x 131072 logits, 32 candidates: with
+// the same places of several lists to a thread 33 us, so 21).
+template <int HOLD> __global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lanes) {
     __shared__ double sums[BEAM_ROWS];                    // logarithms of the sums; the largest logits stay apart
     __shared__ float tops[BEAM_ROWS], scores[BEAM_ROWS];
     __shared__ bool ended[BEAM_ROWS];
@@ -218,12 +262,13 @@ __global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lan
     Candidate *const kept = reinterpret_cast<Candidate *>(memory), *const list = kept + a.n;
     const int64_t b = blockIdx.x;
     const uint32_t per_beam = (uint32_t)a.pieces * a.n, total = (uint32_t)a.K * per_beam;
+    const uint32_t each = total < THREADS * HOLD ? (total + THREADS - 1) / THREADS : HOLD;
     uint64_t p[HOLD];
     const auto load = [&](uint32_t from) {
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
-            const uint32_t j = from + i * THREADS + threadIdx.x;
-            p[i] = j < total ? a.lists[b * total + j] : 0;
+            const uint32_t j = from + threadIdx.x * each + i;
+            p[i] = (uint32_t)i < each && j < total ? a.lists[b * total + j] : 0;
         }
     };
     load(0);
@@ -255,7 +300,7 @@ __global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lan
     }
     for (int j = threadIdx.x; j < a.n; j += THREADS) kept[j] = {0, 0xffffffffu - j};
     __syncthreads();
-    for (uint32_t from = 0; from < total; from += ROUND) {
+    for (uint32_t from = 0; from < total; from += THREADS * each) {
         if (from > 0) load(from);
         if (threadIdx.x == 0) found = 0;
         // those of the rounds before are with the first n threads; threads that hold nothing are told apart by their places
@@ -267,7 +312,7 @@ __global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lan
         at[HOLD] = mine.at;
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
-            const uint32_t j = from + i * THREADS + threadIdx.x, k = p[i] != 0 ? j / per_beam : 0;
+            const uint32_t k = p[i] != 0 ? (from + threadIdx.x * each + i) / per_beam : 0;
             const float score = scores[k], z = logit_of(p[i]);
             double s = -(double)INFINITY;
             if (ended[k]) s = z == 0.0f && token_of(p[i]) == (uint32_t)a.pad ? (double)score : s;
@@ -383,7 +428,7 @@ BeamPieces beam_pieces(int64_t B, int64_t K, int64_t V, int64_t n_best) {
 
 template <typename IO> int launch_pieces(const BeamArgs &a, unsigned groups, size_t held, hipStream_t stream) {
     const int each = beam_each(a.B * a.K, a.V, a.n);
-    const unsigned list = (unsigned)(each * held * sizeof(uint64_t));
+    const unsigned list = (unsigned)(each * held * sizeof(typename Piece<IO>::Key));
     if (each == 64) hipLaunchKernelGGL((beam_piece_kernel<IO, 64>), dim3(groups), dim3(THREADS), list, stream, a);
     else if (each == 32) hipLaunchKernelGGL((beam_piece_kernel<IO, 32>), dim3(groups), dim3(THREADS), list, stream, a);
     else hipLaunchKernelGGL((beam_piece_kernel<IO, 8>), dim3(groups), dim3(THREADS), list, stream, a);
@@ -395,13 +440,15 @@ int beam_select(const BeamArgs &a, int dtype, hipStream_t stream) {
     if (groups > MOST_GROUPS || a.B > MOST_GROUPS) return fail(T2FW_ERR_BAD_SHAPE, "beam selection: too many workgroups for one launch");
     // threads of the n groups that are not below the n-th
     const int held = a.n * (THREADS / groups_of(a.n));
-    const unsigned merge = (unsigned)(((HOLD + 1) * held + a.n) * sizeof(Candidate));
+    const int hold = (int64_t)a.K * a.pieces * a.n <= 4 * THREADS ? 4 : 16;
+    const unsigned merge = (unsigned)(((hold + 1) * held + a.n) * sizeof(Candidate));
     int lanes = 1;
     while (lanes < a.pieces && lanes < 64) lanes *= 2;
     const int rc = dtype == T2FW_F32 ? launch_pieces<float>(a, (unsigned)groups, held, stream) : dtype == T2FW_F16 ? launch_pieces<_Float16>(a, (unsigned)groups, held, stream) :
                    launch_pieces<__bf16>(a, (unsigned)groups, held, stream);
     if (rc) return rc;
-    hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes);
+    if (hold == 4) hipLaunchKernelGGL(beam_merge_kernel<4>, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes);
+    else hipLaunchKernelGGL(beam_merge_kernel<16>, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes);
     return check_hip(hipGetLastError(), "beam_merge_kernel launch");
 }
 

@@ -1,8 +1,8 @@
 """beam_select against the scores in float64, sorted; reorder_beams against indexing.
 
 A score is off by the logarithm of a sum of float32 exponentials: each off by 2^-22 (the exponential's unit, and its argument's rounding at arguments
-that count, 2^-24 |z - top| e^(z - top) < 2^-25), partial sums of 32 of them by 31 u: 2^-19 of the sum in all, which is 2^-19 in its logarithm.  What is returned is rounded to
-float32.  Which candidates come, and in what order, is exact wherever no two scores are nearer than that: the tests' inputs hold scores apart, or equal."""
+that count, 2^-24 |z - top| e^(z - top) < 2^-25), partial sums of 64 of them in four shares by 17 u, and a factor that is off by 2^-22 like them: 25.5 u of
+the sum in all, less than 2^-19, which is 2^-19 in its logarithm.  What is returned is rounded to float32.  Which candidates come, and in what order, is exact wherever no two scores are nearer than that: the tests' inputs hold scores apart, or equal."""
 import pytest
 import torch
 
@@ -65,6 +65,21 @@ def test_best_of_all(shape, dtype):
         if apart(reference(logits, scores, min(n + 1, K * V))[0]):
             return check(logits, scores, n)
     pytest.fail("no such draw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("middle,std", [(1e3, 3.0), (-9e5, 3.0), (1048575.0, 3.0), (1e6, 1e5), (-3e7, 50.0), (0.0, 1e7)])
+def test_large_logits(middle, std):
+    """on either side of where the exponents are taken another way; B K V such that a thread has 8, 32 and 64 logits"""
+    for B, K, V in ((1, 3, 5000), (8, 8, 40000), (64, 8, 16400)):
+        for seed in range(100):
+            logits, scores = logits_of(B, K, V, torch.float32, seed, std)
+            logits += middle
+            if apart(reference(logits, scores, 9)[0]):
+                check(logits, scores, 8)
+                break
+        else:
+            pytest.fail("no such draw")
 
 
 @pytest.mark.gpu
