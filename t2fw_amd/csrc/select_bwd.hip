@@ -91,17 +91,17 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, 
     if (tiles > 0) load(p.begin + (int64_t)(tiles - 1) * TILE);
     at_chunk<G, true>(adj, a, g, p, rate);
     // sums over the block's channels, of the tile
-    const auto store_steps = [&](int64_t t0, bool some) {
+    const auto store_steps = [&](int64_t t0) {
         constexpr int ALL = TILE * 2 * NP;
         const Buffer to = result_of(a.bc + (((int64_t)p.block * a.B + p.b) * a.T + t0) * 2 * NP, (a.T - t0) * 2 * NP * 4);
 #pragma unroll
         for (int i = 0; i < ALL; i += THREADS) {
             const int at = i + threadIdx.x, from = at < ALL ? at : 0;
             const float *const v = &sums[0][0][0] + from;
-            store_to<float>(to, at < ALL ? at * 4u : BEYOND, 0, some ? ((v[0] + v[ALL]) + v[2 * ALL]) + v[3 * ALL] : 0.0f);
+            store_to<float>(to, at < ALL ? at * 4u : BEYOND, 0, ((v[0] + v[ALL]) + v[2 * ALL]) + v[3 * ALL]);
         }
     };
-    // steps beyond the row's length
+    // steps beyond the row's length (those of b and c: select_steps_kernel)
     for (int64_t t0 = p.begin + (int64_t)tiles * TILE; t0 < p.end; t0 += TILE) {
         const Results<IO, G> d_x(a.d_x, a, p, t0), d_dt(a.d_dt, a, p, t0), d_gate(GATED ? a.d_gate : a.d_x, a, p, t0);
 #pragma unroll
@@ -110,7 +110,6 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, 
             d_dt.store(r, 0.0f);
             if constexpr (GATED) d_gate.store(r, 0.0f);
         }
-        store_steps(t0, false);
     }
     for (int k = tiles - 1; k >= 0; --k) {
         const int64_t t0 = p.begin + (int64_t)k * TILE;
@@ -207,7 +206,7 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, 
             d_bias += counts ? for_dt : 0.0f;
         }
         __syncthreads();
-        store_steps(t0, true);
+        store_steps(t0);
     }
     // (a channel's lanes beyond the first quad have the same steps as that)
     d_skip = sum_share<G>(d_skip);
@@ -223,16 +222,20 @@ template <typename IO, int G, bool GATED> __global__ __launch_bounds__(THREADS, 
     }
 }
 
-// Gradients of b and c: sums over the blocks of channels
+// Gradients of b and c: sums over the blocks of channels; zeros for steps that do not count, of which the blocks have left nothing, or, next to a state that is
+// not finite, products of it with zero
 template <typename IO> __global__ __launch_bounds__(THREADS) void select_steps_kernel(SelectArgs a, uint32_t blocks, int NP, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
     if (i >= n) return;
     const int64_t t = i / (2 * NP);
     const int at = (int)(i - t * 2 * NP), s = at % NP;
     if (s >= a.N) return;
+    const int64_t row = a.lengths == nullptr ? 0 : t / a.T;
     float v = 0.0f;
+    if (a.lengths == nullptr || t - row * a.T < row_length(a, row)) {
 #pragma unroll 8
-    for (uint32_t k = 0; k < blocks; ++k) v += a.bc[k * n + i];
+        for (uint32_t k = 0; k < blocks; ++k) v += a.bc[k * n + i];
+    }
     (at < NP ? static_cast<IO *>(a.d_b) : static_cast<IO *>(a.d_c))[t * a.N + s] = narrow<IO>(v);
 }
 
