@@ -70,12 +70,16 @@ template <int G> __device__ __forceinline__ float sum_share(float v) { return gr
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // log(1 + e^v) = max(v, 0) + log(1 + e), e = e^-|v|, and log(1 + e) = 2 artanh(r), r = e / (2 + e) <= 1/3: r + r^3 / 3 + ..., its seven terms off by 2^-26
-// of it.  Relative accuracy for steps of any length, which a logarithm of a sum does not have.
+// of it.  What the exponent's rounding leaves, up to 2^-18 of e at |v| = 80, is multiplied in: e^-|v| = 2^n e^(-|v| - n log 2) for n next to -|v| log2(e).  A
+// step is off by 2^-20 of its length for v > -86; below that e comes to the smallest numbers, and is zero from -88 on.  (Four instructions: forward of
+// 8 x 1024 x 1536 x 16 bf16 109 us without them, 111 so; of 4 x 1024 x 3000 x 4, where a lane makes every step of its channel, 57 and 59.)
 struct Softplus {
     float value, slope;
 };
 template <bool SLOPE> __device__ __forceinline__ Softplus softplus_of(float v) {
-    const float e = exp2_of(-fabsf(v) * LOG2E), r = e * __builtin_amdgcn_rcpf(2.0f + e), q = r * r;
+    constexpr float LN2 = 0.69314718055994530942f;
+    const float m = fmaxf(-fabsf(v), -128.0f), n = m * LOG2E, about = exp2_of(n);
+    const float e = fmaf(about, fmaf(-n, LN2, m), about), r = e * __builtin_amdgcn_rcpf(2.0f + e), q = r * r;
     float p = 1.0f / 13.0f;
     p = fmaf(p, q, 1.0f / 11.0f);
     p = fmaf(p, q, 1.0f / 9.0f);
@@ -84,7 +88,7 @@ template <bool SLOPE> __device__ __forceinline__ Softplus softplus_of(float v) {
     p = fmaf(p, q, 1.0f / 3.0f);
     p = fmaf(p * q, r, r);
     Softplus s;
-    s.value = fmaf(2.0f, p, fmaxf(v, 0.0f));
+    s.value = fmaf(2.0f, p, v < 0.0f ? 0.0f : v);        // (NaN stays)
     s.slope = SLOPE ? (v >= 0.0f ? 1.0f : e) * __builtin_amdgcn_rcpf(1.0f + e) : 0.0f;
     return s;
 }
