@@ -523,10 +523,11 @@ int t2fw_selective_scan_step(const void *x, const void *dt, const float *a, cons
 
 /*
  * The n (1 to 128) best of the K V candidates of each of B requests, best first: candidate (k, v) has the score scores[k] + log softmax(logits[k])[v].
- * logits [B, K, V] fp32 / fp16 / bf16, K at most 256; scores [B, K] float; results [B, n].  Of equal scores the lower k V + v is the better one;
- * scores are compared in double, with sums of float exponentials.  `finished` [B, K] bytes, or null: a beam that has ended has one candidate, the
- * token `pad`, with its own score.  A candidate that cannot be (a logit of minus infinity, a score of minus infinity or NaN, another token of an
- * ended beam, a beam with a NaN or plus infinity among its logits) has a score of minus infinity; which tokens of a beam with NaN come is not said.
+ * logits [B, K, V] fp32 / fp16 / bf16, K at most 256; scores [B, K] float; results [B, n].  Scores are compared in double, with sums of float
+ * exponentials; of equal ones the lower beam is better, within a beam the larger logit, then the lower token.  `finished` [B, K] bytes, or null: a beam
+ * that has ended has one candidate, the token `pad`, with its own score.  A candidate that cannot be (a logit of minus infinity, a score of minus infinity
+ * or NaN, another token of an ended beam, a beam with a NaN or plus infinity among its logits) has a score of minus infinity and comes after the others, by
+ * its place k V + v; which tokens of a beam with NaN or plus infinity come is not said.
  */
 size_t t2fw_beam_select_workspace_bytes(int64_t B, int64_t K, int64_t V, int64_t n, int32_t dtype);
 int t2fw_beam_select(const void *logits, const float *scores, const void *finished,

@@ -9,12 +9,15 @@ def beam_select(logits, scores, count=None, finished=None, pad=0):
     beams [B, count] int64, tokens [B, count] int64)``, best first.
 
     A continuation of beam ``k`` by token ``v`` has the score ``scores[k] + log_softmax(logits[k])[v]``.
-    ``logits: [B, K, V]``, contiguous, float32, float16 or bfloat16, with up to 256 beams; ``scores: [B, K]`` float32; ``count`` is at most 128 (``None``: K).  The first step, when all beams are the same
-    prompt: scores of zero for one of them and minus infinity for the others.
+    ``logits: [B, K, V]``, contiguous, float32, float16 or bfloat16, with up to 256 beams; ``scores: [B, K]`` float32; ``count`` is at most 128
+    (``None``: K).  The first step, when all beams are the same prompt: scores of zero for one of them and minus infinity for the others.
 
-    ``finished: [B, K]`` bool: a beam that has ended goes on with the token ``pad`` alone, at its own score.  Of equal scores the lower ``k V + v``
-    comes first; they are compared in float64, from sums of float32 exponentials.  What cannot be (logits or scores of minus infinity, other tokens of an
-    ended beam, a beam with NaN or plus infinity among its logits) has a score of minus infinity and comes last, of a beam with NaN in no order that is promised.
+    ``finished: [B, K]`` bool: a beam that has ended goes on with the token ``pad`` alone, at its own score.  Scores are compared in float64, from sums of
+    float32 exponentials (off by up to 2^-19: candidates of different beams nearer than twice that may change places).  Of equal scores the lower beam comes first,
+    within a beam the larger logit, then the lower token: next to a score of -1e30, say, all tokens' scores are equal, and they still come by their logits.
+
+    What cannot be (logits or scores of minus infinity, other tokens of an ended beam, a beam with NaN or plus infinity among its logits) has a
+    score of minus infinity and comes last, by its index ``k V + v``; of a beam with NaN or plus infinity in no order that is promised.
     No gradients."""
     return _lib.host().beam_select(logits, scores, count, finished, pad, _stream(logits, "logits"))
 

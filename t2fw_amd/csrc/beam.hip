@@ -2,11 +2,11 @@
 //
 // Selection.  A candidate (k, v) has the score score_k + z_kv - lse_k.  Within a beam the logit alone orders candidates, so a workgroup reads a
 // piece of 2048 to 16384 logits of one beam once, for its part of the log-sum-exp and for its n best; a second launch puts the parts together, in
-// double, and takes the n best of all lists.  No two candidates are equal: of equal scores the lower index is the better one.
+// double, and takes the n best of all lists.  No two candidates are equal: of equal scores the lower beam, the larger logit and the lower token are better.
 //   The n best of what 256 threads hold: n of the threads' largest are no smaller than the n-th largest of those, so nothing smaller can be among the n
 //   best.  What is not smaller (most often little more than n, at most what n threads hold) goes to a list, where each counts those above it: its place.
 //   The order in which the list is filled does not matter.
-// Bound by memory for many logits, by latency for few: loads, three barriers, two launches.
+// Bound by memory for many logits, by latency for few: loads, five barriers a launch, two launches.
 //
 // Reordering.  A thread has the same 16 bytes of all beams of a request, loads those that move, and stores them when all of them are there: in place
 // without a copy, and a beam that goes on from itself is neither read nor written.  One launch for up to 96 arrays.
@@ -58,11 +58,21 @@ template <> struct Piece<float> {
     static __device__ __forceinline__ uint32_t place(Key k) { return token_of(k); }
 };
 
-// A candidate of a request: its score, and its place among the K V
+// A candidate of a request: its score, and what decides between equal ones, from the upper bits on: its beam (the lower is better), its logit and its token.
+// Scores of one beam may be equal where its logits are not, as the sum next to a large score has no room for what sets them apart: the logit counts
+// then, as in the choice of a piece's best.  Beams and tokens have 32 bits together.
 struct Candidate {
-    uint64_t key;
-    uint32_t at;
-    __device__ __forceinline__ bool above(const Candidate &o) const { return key > o.key || (key == o.key && at < o.at); }
+    uint64_t key, next;
+    __device__ __forceinline__ bool above(const Candidate &o) const { return key > o.key || (key == o.key && next > o.next); }
+};
+struct Ties {
+    int bits;                                             // of a token
+    __device__ __forceinline__ uint32_t tokens() const { return (1u << bits) - 1; }
+    __device__ __forceinline__ uint64_t next(uint32_t k, uint32_t z, uint32_t v) const {
+        return ~(uint64_t)k << (32 + bits) | (uint64_t)z << bits | (~v & tokens());
+    }
+    __device__ __forceinline__ uint32_t beam(uint64_t next) const { return (uint32_t)(~next >> (32 + bits)); }
+    __device__ __forceinline__ uint32_t token(uint64_t next) const { return ~(uint32_t)next & tokens(); }
 };
 
 // ---- sums over a workgroup ----------------------------------------------------------------------------------------
@@ -79,7 +89,7 @@ template <typename T, typename Op> __device__ __forceinline__ T over_group(T v, 
 
 __device__ __forceinline__ uint32_t shuffled(uint32_t v, int m) { return __shfl_xor(v, m, 64); }
 __device__ __forceinline__ uint64_t shuffled(uint64_t v, int m) { return __shfl_xor(v, m, 64); }
-__device__ __forceinline__ Candidate shuffled(const Candidate &v, int m) { return {__shfl_xor(v.key, m, 64), __shfl_xor(v.at, m, 64)}; }
+__device__ __forceinline__ Candidate shuffled(const Candidate &v, int m) { return {__shfl_xor(v.key, m, 64), __shfl_xor(v.next, m, 64)}; }
 
 struct Share {
     float top;
@@ -252,7 +262,7 @@ template <typename IO, int EACH> __global__ __launch_bounds__(THREADS) void beam
 // A request: the n best of its lists, in rounds of up to 256 HOLD candidates, each with the n best so far.  A thread has some that follow each other in a
 // list, so that the lists' first ones are with many threads: their n-th best is no worse than few others (64 requests, 16 x 131072 logits, 32 candidates: with
 // the same places of several lists to a thread 33 us, so 21).
-template <int HOLD> __global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lanes) {
+template <int HOLD> __global__ __launch_bounds__(THREADS) void beam_merge_kernel(BeamArgs a, int lanes, Ties ties) {
     __shared__ double sums[BEAM_ROWS];                    // logarithms of the sums; the largest logits stay apart
     __shared__ float tops[BEAM_ROWS], scores[BEAM_ROWS];
     __shared__ bool ended[BEAM_ROWS];
@@ -298,18 +308,15 @@ template <int HOLD> __global__ __launch_bounds__(THREADS) void beam_merge_kernel
             ended[k] = a.finished != nullptr && a.finished[b * a.K + k] != 0;
         }
     }
-    for (int j = threadIdx.x; j < a.n; j += THREADS) kept[j] = {0, 0xffffffffu - j};
+    for (int j = threadIdx.x; j < a.n; j += THREADS) kept[j] = {0, (uint64_t)(THREADS + j)};
     __syncthreads();
     for (uint32_t from = 0; from < total; from += THREADS * each) {
         if (from > 0) load(from);
         if (threadIdx.x == 0) found = 0;
         // those of the rounds before are with the first n threads; threads that hold nothing are told apart by their places
-        uint64_t key[HOLD + 1];
-        uint32_t at[HOLD + 1];
-        Candidate mine{0, 0xfffffeffu - threadIdx.x};
+        Candidate all[HOLD + 1], mine{0, threadIdx.x};
         if ((int)threadIdx.x < a.n) mine = kept[threadIdx.x];
-        key[HOLD] = mine.key;
-        at[HOLD] = mine.at;
+        all[HOLD] = mine;
 #pragma unroll
         for (int i = 0; i < HOLD; ++i) {
             const uint32_t k = p[i] != 0 ? (from + threadIdx.x * each + i) / per_beam : 0;
@@ -317,19 +324,15 @@ template <int HOLD> __global__ __launch_bounds__(THREADS) void beam_merge_kernel
             double s = -(double)INFINITY;
             if (ended[k]) s = z == 0.0f && token_of(p[i]) == (uint32_t)a.pad ? (double)score : s;
             else if (z > -INFINITY && score > -INFINITY) s = (double)score + (((double)z - (double)tops[k]) - sums[k]);
-            key[i] = p[i] != 0 ? ordered(s) : 0;
-            at[i] = p[i] != 0 ? k * (uint32_t)a.V + token_of(p[i]) : 0;
-            const Candidate one{key[i], at[i]};
-            if (key[i] != 0 && one.above(mine)) mine = one;
+            all[i] = {p[i] != 0 ? ordered(s) : 0, ties.next(k, s > -(double)INFINITY ? ordered(z) : 0, token_of(p[i]))};
+            if (all[i].key != 0 && all[i].above(mine)) mine = all[i];
         }
         const auto more = [](const Candidate &x, const Candidate &y) { return x.above(y); };
         const Candidate limit = nth_best(of_group(mine, a.n, more), best, least, a.n, more);
         if (!limit.above(mine)) {
 #pragma unroll
-            for (int i = 0; i <= HOLD; ++i) {
-                const Candidate one{key[i], at[i]};
-                if (one.key != 0 && !limit.above(one)) list[atomicAdd(&found, 1)] = one;
-            }
+            for (int i = 0; i <= HOLD; ++i)
+                if (all[i].key != 0 && !limit.above(all[i])) list[atomicAdd(&found, 1)] = all[i];
         }
         __syncthreads();
         const int m = found;
@@ -344,8 +347,8 @@ template <int HOLD> __global__ __launch_bounds__(THREADS) void beam_merge_kernel
     for (int j = threadIdx.x; j < a.n; j += THREADS) {
         const Candidate one = kept[j];
         a.out_scores[b * a.n + j] = (float)number(one.key);
-        a.out_beams[b * a.n + j] = one.at / (uint32_t)a.V;
-        a.out_tokens[b * a.n + j] = one.at % (uint32_t)a.V;
+        a.out_beams[b * a.n + j] = ties.beam(one.next);
+        a.out_tokens[b * a.n + j] = ties.token(one.next);
     }
 }
 
@@ -442,13 +445,15 @@ int beam_select(const BeamArgs &a, int dtype, hipStream_t stream) {
     const int held = a.n * (THREADS / groups_of(a.n));
     const int hold = (int64_t)a.K * a.pieces * a.n <= 4 * THREADS ? 4 : 16;
     const unsigned merge = (unsigned)(((hold + 1) * held + a.n) * sizeof(Candidate));
+    Ties ties{0};
+    while (1ll << ties.bits < a.V) ++ties.bits;
     int lanes = 1;
     while (lanes < a.pieces && lanes < 64) lanes *= 2;
     const int rc = dtype == T2FW_F32 ? launch_pieces<float>(a, (unsigned)groups, held, stream) : dtype == T2FW_F16 ? launch_pieces<_Float16>(a, (unsigned)groups, held, stream) :
                    launch_pieces<__bf16>(a, (unsigned)groups, held, stream);
     if (rc) return rc;
-    if (hold == 4) hipLaunchKernelGGL(beam_merge_kernel<4>, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes);
-    else hipLaunchKernelGGL(beam_merge_kernel<16>, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes);
+    if (hold == 4) hipLaunchKernelGGL(beam_merge_kernel<4>, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes, ties);
+    else hipLaunchKernelGGL(beam_merge_kernel<16>, dim3((unsigned)a.B), dim3(THREADS), merge, stream, a, lanes, ties);
     return check_hip(hipGetLastError(), "beam_merge_kernel launch");
 }
 
