@@ -227,9 +227,10 @@ def finetune(rounds=10, batch=64, prompt=16, answer=48, vocab=512, width=128, la
     reference = RecurrentLM(vocab, width, layers, seed=seed, selective=selective).cuda()
     at_start = PolicyTrainer(reference)
     g = torch.Generator(device="cuda").manual_seed(seed)
-    history = []
+    history, asked = [], None
+    prompts = lambda: torch.randint(0, vocab, (batch, prompt), generator=g, device="cuda")
     for r in range(rounds):
-        asked = torch.randint(0, vocab, (batch, prompt), generator=g, device="cuda")
+        asked = prompts()
         tokens, _ = model.generate(asked, answer, generator=g, eight_bit=eight_bit)
         reward = rewards(tokens[:, 1:], vocab)
         old, ref = trainer.log_probabilities(tokens), at_start.log_probabilities(tokens)
@@ -241,6 +242,7 @@ def finetune(rounds=10, batch=64, prompt=16, answer=48, vocab=512, width=128, la
         history.append(float(mean))
         say("round %3d  reward %.3f  loss %+.4f  gradient norm %.3f" % (r, history[-1], float(loss), float(norm)))
     if beams:
+        asked = prompts() if asked is None else asked                    # (those of the last round)
         tokens, scores = model.beam_search(asked, answer, beams=beams, eight_bit=eight_bit)
         history.append(float(rewards(tokens[:, 0, prompt:], vocab).mean()))
         say("beam search of %d: reward %.3f  log probability %.2f" % (beams, history[-1], float(scores[:, 0].mean())))

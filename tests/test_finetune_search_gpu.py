@@ -1,0 +1,19 @@
+"""What a beam search of the small model starts from."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_search_without_rounds_of_training():
+    from t2fw_amd.finetune import finetune
+    said = []
+    history = finetune(rounds=0, batch=4, prompt=3, answer=5, vocab=40, width=64, layers=2, beams=3, selective=True, say=said.append)
+    assert len(history) == len(said) == 1 and 0.0 <= history[0] <= 1.0 and "beam search of 3" in said[0]
+    assert finetune(rounds=0, batch=4, vocab=40, width=64, layers=2, say=said.append) == [] and len(said) == 1
+
+
+def test_the_search_follows_the_last_rounds_prompts():
+    """the generator's draws are those of a training without a search"""
+    from t2fw_amd.finetune import finetune
+    options = dict(rounds=2, batch=4, prompt=3, answer=5, vocab=40, width=64, layers=2, say=lambda s: None)
+    assert finetune(beams=2, **options)[:2] == finetune(**options)
