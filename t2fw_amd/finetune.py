@@ -162,6 +162,8 @@ class RecurrentLM(torch.nn.Module):
         """[B, T] tokens -> ([B, beams, T + steps] tokens, their answers' log probabilities [B, beams] float32), best first.  An answer ends at the
         token ``end`` (``None``: nowhere) and is filled up with it."""
         B, T = prompt.shape
+        if T < 1:
+            raise ValueError("a search goes on from at least one token")
         step, states = self._stepper(B * beams, eight_bit)
         tokens = torch.zeros(B * beams, T + steps, dtype=torch.int64, device=prompt.device)
         tokens[:, :T] = prompt.repeat_interleave(beams, dim=0)

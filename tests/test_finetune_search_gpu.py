@@ -1,5 +1,6 @@
 """What a beam search of the small model starts from."""
 import pytest
+import torch
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +18,12 @@ def test_the_search_follows_the_last_rounds_prompts():
     from t2fw_amd.finetune import finetune
     options = dict(rounds=2, batch=4, prompt=3, answer=5, vocab=40, width=64, layers=2, say=lambda s: None)
     assert finetune(beams=2, **options)[:2] == finetune(**options)
+
+
+def test_a_search_needs_a_prompt():
+    from t2fw_amd.finetune import RecurrentLM
+    model = RecurrentLM(vocab=40, width=64, layers=2).cuda()
+    with pytest.raises(ValueError, match="at least one token"):
+        model.beam_search(torch.zeros(2, 0, dtype=torch.int64, device="cuda"), 3, beams=2)
+    tokens, scores = model.beam_search(torch.zeros(2, 1, dtype=torch.int64, device="cuda"), 3, beams=2)
+    assert tokens.shape == (2, 2, 4) and bool(torch.isfinite(scores).all())
