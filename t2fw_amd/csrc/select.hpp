@@ -17,10 +17,11 @@ struct SelectArgs {
     void *y;                            // [B, T, D] dense
     float *last;                        // [B, D, N]
     float *ckpt;                        // state before every tile [B, tiles, D, padded N], or null
-    float *maps;                        // scratch: the chunks' maps [B, chunks, D, padded N + 1]
+    float *maps;                        // scratch: the chunks' maps [chunks, B, D, padded N], and the sums of their steps' lengths [chunks, B, D]
     void *d_x, *d_dt, *d_b, *d_c, *d_gate;
     float *d_a, *d_skip, *d_bias, *d_s0;     // d_skip, d_bias, d_s0 may be null
-    float *bc, *sums;                   // scratch: gradients of b and c by blocks of channels; of a, skip and dt_bias by rows and chunks
+    float *bc, *sums;                   // scratch: gradients of b and c by blocks of channels (G^2 / 8 bytes a channel and step, of G lanes a channel: 2 for 16
+                                        // states, 32 for 64); of a, skip and dt_bias by rows and chunks
     int64_t B, T, D, N;
     // strides of rows and steps, in elements
     int64_t x_b, x_t, dt_b, dt_t, b_b, b_t, c_b, c_t, z_b, z_t, g_b, g_t;

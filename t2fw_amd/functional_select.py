@@ -16,7 +16,11 @@ def selective_scan(x, dt, a, b, c, state=None, skip=None, gate=None, dt_bias=Non
 
     The decays over the steps of a row are put together by ``exp(a * sum of dt)``, which has to stay finite: where ``dt * a <= 0``, as it
     is meant, it always does.  Next to an infinite state or input such a product that is too small for float32 makes NaN, where the recurrence step by step
-    would stay infinite.  States and sums are float32; sums over channels and rows are made in a fixed order.
+    would stay infinite.  States and sums are float32; sums over channels and rows are made in a fixed order.  A decay is off by its exponent's three
+    roundings, 2^-22 of ``dt a``, and by 2^-22; a step by the softplus by 2^-20 of its length.
+
+    For the gradients the forward keeps a state every 16 steps (N / 4 bytes a channel and step), and the backward takes scratch for those of ``b`` and ``c``: per channel
+    and step 2 bytes with 9 to 16 states, 8 with 17 to 32, 32 with more.
 
     ``lengths: [B]`` (int32 or int64, on the device), for rows that are padded at their end: steps from ``lengths[b]`` on do not count, whatever
     they hold, NaN included.  Their outputs and gradients are zero, and the last state of the row is that after its last step."""
